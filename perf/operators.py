@@ -108,7 +108,7 @@ def prepare(case, seed):
 def _quantize(x):
     """Whole numbers -127..127 per row and the row's scale; in 64 bits, where 127 x / max next to a half decides."""
     most = x.float().abs().amax(-1, keepdim=True)
-    return torch.round(127.0 * x.double() / most.double()), most / 127.0
+    return torch.round(127.0 * x.double() / most.double()), (most.double() / 127.0).float()
 
 
 def _linear8(x, w, scale, bias, dtype):

@@ -18,7 +18,7 @@ FL_ACT = {"swish_clamp": 0, "gelu_tanh": 1, "relu2": 2, "relu": 3, "silu": 4}
 FL_ROT_SCALE = {"yarn": 0, "bands": 1}
 FL_ROUTER = {"softmax": 0, "sigmoid_groups": 1, "softmax_groups": 2}
 FL_FFN = {"none": 0, "dense": 1, "moe": 2}
-FL_DTYPE_F32, FL_DTYPE_BF16, FL_DTYPE_F16 = 0, 1, 2
+FL_DTYPE_F32, FL_DTYPE_BF16, FL_DTYPE_F16, FL_DTYPE_I8 = 0, 1, 2, 3
 
 
 class FlConfig(C.Structure):
@@ -65,7 +65,7 @@ class FastllmError(RuntimeError):
 
 
 # every symbol include/fastllm_b200.h declares: name -> (restype, argtypes)
-_VP, _I, _U64, _SZ = C.c_void_p, C.c_int, C.c_uint64, C.c_size_t
+_VP, _I, _U64, _SZ, _I64 = C.c_void_p, C.c_int, C.c_uint64, C.c_size_t, C.c_int64
 SYMBOLS = {
     "fl_init": (_I, [_I]),
     "fl_last_error": (C.c_char_p, []),
@@ -103,6 +103,10 @@ SYMBOLS = {
     "fl_cache_slot_len": (_I, [_VP, _I, C.POINTER(_I)]),
     "fl_cache_moe_routing": (_I, [_VP, _I, _VP, _VP]),
     "fl_forward_sample_device": (_I, [_VP, _VP, _VP, _I, _I, _SZ, _VP, C.POINTER(C.c_uint32)]),
+    "fl_quantize_rows": (_I, [_VP, _I, _I64, _I64, _I64, _VP, _I64, _VP, _VP]),
+    "fl_linear8_workspace": (_I, [_I64, _I64, _I, C.POINTER(_SZ)]),
+    "fl_linear8": (_I, [_VP, _I, _I64, _VP, _VP, _I64, _VP, _VP, _I64, _I64, _I64, _VP, _I, _I64, _VP, _SZ, _VP]),
+    "fl_logprobs": (_I, [_VP, _I, _I64, _I64, _I64, _VP, _I, _I64, C.c_double, _I, _VP, _VP, _VP, _VP, _VP, _VP]),
     "fl_embed": (_I, [_VP, _VP, _VP, _I, _I, _VP]),
     "fl_embed_timed": (_I, [_VP, _VP, _VP, _I, _I, _VP, _I, C.POINTER(C.c_float)]),
     "fl_comm_unique_id": (_I, [_VP]),

@@ -27,6 +27,11 @@ Profiler g_prof;
 NcclApi g_nccl;
 PeerComm g_peer;
 static std::atomic<int> g_device{-1};
+int bound_device() {
+    const int dev = g_device.load();
+    FL_CHECK(dev >= 0, FL_ERR_STATE, "fl_init has not been called");
+    return dev;
+}
 
 static inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
@@ -1687,19 +1692,6 @@ static void run_forward_slots(fl_cache& c, const int* slots, const uint32_t* ids
 // ------------------------------------------------------------------------------------------------------------------
 using namespace fl;
 
-#define FL_API_BEGIN try {
-#define FL_API_END                                                 \
-    return FL_OK;                                                  \
-    }                                                              \
-    catch (const fl::Error& e) {                                   \
-        fl::g_last_error = e.what();                               \
-        return e.code;                                             \
-    }                                                              \
-    catch (const std::exception& e) {                              \
-        fl::g_last_error = std::string("internal: ") + e.what();   \
-        return FL_ERR_INVALID;                                     \
-    }
-
 static void check_peer_error() {
     if (!g_peer.ready) return;
     int err = 0;
@@ -1717,9 +1709,7 @@ void step_check(fl_cache& c) {
 }  // namespace fl
 
 static void use_device() {
-    const int dev = g_device.load();
-    FL_CHECK(dev >= 0, FL_ERR_STATE, "fl_init has not been called");
-    FL_CUDA(cudaSetDevice(dev));   // no thread-affine state: callers may hop OS threads between calls
+    FL_CUDA(cudaSetDevice(bound_device()));   // no thread-affine state: callers may hop OS threads between calls
 }
 
 extern "C" {

@@ -31,6 +31,21 @@ struct Profiler {
     std::vector<ProfEntry> entries;
 };
 extern Profiler g_prof;
+int bound_device();             // the device of fl_init; throws before it
+
+// what stands around the body of every entry point
+#define FL_API_BEGIN try {
+#define FL_API_END                                                 \
+    return FL_OK;                                                  \
+    }                                                              \
+    catch (const fl::Error& e) {                                   \
+        fl::g_last_error = e.what();                               \
+        return e.code;                                             \
+    }                                                              \
+    catch (const std::exception& e) {                              \
+        fl::g_last_error = std::string("internal: ") + e.what();   \
+        return FL_ERR_INVALID;                                     \
+    }
 
 inline bool env_flag(const char* name) {
     const char* v = std::getenv(name);

@@ -90,7 +90,7 @@ typedef enum fl_arch {
                               beside a shared expert; hashed bigram rows in the embedding, per-layer token vectors, looped layers */
 } fl_arch;
 
-typedef enum fl_dtype { FL_DTYPE_F32 = 0, FL_DTYPE_BF16 = 1, FL_DTYPE_F16 = 2 } fl_dtype;
+typedef enum fl_dtype { FL_DTYPE_F32 = 0, FL_DTYPE_BF16 = 1, FL_DTYPE_F16 = 2, FL_DTYPE_I8 = 3 /* operators only */ } fl_dtype;
 
 /* Mirrors the fields the reference adapters read from config.json
  * (llama.rs:17-29, mistral.rs:78-91, models/config.rs:5-18, models/embeddings.rs:46-54). */
@@ -380,6 +380,36 @@ FL_EXPORT int fl_forward_sample(fl_model* m, fl_cache* c, const uint32_t* ids, i
  * within ~1e-6 (relative) of a boundary between two tokens may pick the neighbour.  The parity path is fl_forward_sample. */
 FL_EXPORT int fl_forward_sample_device(fl_model* m, fl_cache* c, const uint32_t* ids, int b, int t, size_t rope_offset, fl_sampler* s,
                                        uint32_t* next_id);
+
+/* ---- operators on device memory (no reference counterpart) ---------------------------------------
+ * Pointers are memory of the device that fl_init bound, strides are counted in elements between rows, the last dimension is dense.
+ * `stream` is a cudaStream_t (NULL: the default stream).  A call checks its arguments on the host, launches on that stream and returns:
+ * it neither allocates nor waits, keeps nothing of its arguments, may be captured into a CUDA graph, and runs beside other calls on
+ * other streams as long as they do not share a workspace or an output.  Calls of zero rows do nothing.
+ *
+ * fl_quantize_rows: rows of f32, bf16 or f16 [rows, cols] as whole numbers of 8 bits and a scale: with a = max |x| of the row,
+ * scale = a / 127 and q = 127 x / a to the nearest whole number, halves to the even one (of the exact quotient).  A row of zeros has
+ * scale 0; a row with a NaN or an infinity q = 0 and scale NaN.  cols <= 131071. */
+FL_EXPORT int fl_quantize_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale, void* stream);
+/* Matrix product in 8-bit integers with a scale per token and per channel:
+ *     y[r, i] = (sum over j of q[r, j] * w[i, j]) * x_scale[r] * w_scale[i] (+ bias[i]),    r < rows, i < n, j < k
+ * The sum is exact (32-bit integers, k <= 131071); the scales and the f32 bias are applied in f32 and the result is rounded once to y's
+ * type (f32, bf16, f16).  x: f32, bf16 or f16 rows, which the call rounds as fl_quantize_rows does (x_scale NULL), or rows that are 8-bit
+ * already (FL_DTYPE_I8) with their x_scale [rows].  w [n, k] with w_scale [n]: an 8-bit checkpoint's, or fl_quantize_rows of a weight.
+ * 8-bit rows start on 16-byte borders (pointer and row stride); what lies between a row's end and the next row is not read.
+ * workspace: fl_linear8_workspace bytes on a 256-byte border (none for FL_DTYPE_I8), free again when the call's work on the stream is done. */
+FL_EXPORT int fl_linear8_workspace(int64_t rows, int64_t k, int x_dtype, size_t* bytes);
+FL_EXPORT int fl_linear8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
+                         int64_t rows, int64_t n, int64_t k, void* y, int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
+/* Log probabilities over logits [rows, vocab] (f32, bf16, f16), z = logits / temperature:
+ *     logsumexp = log sum exp z,   logprob[r, j] = z[tokens[r, j]] - logsumexp,   entropy = -sum p log p,
+ * and the `top` (0 to 32) largest logits of a row in falling order, the lowest index first among equals: top_ids, top_logprobs [rows, top].
+ * tokens [rows, given] (dense) are 32- or 64-bit integers (token_bytes 4 or 8); a negative one is padding with logprob 0, one past the vocabulary
+ * gets NaN.  A logit of -infinity has probability 0.  A row of nothing but those has logsumexp and logprobs of -infinity and entropy 0; a
+ * row with a NaN or +infinity has no probabilities: its numbers are NaN and its top_ids -1.  logsumexp and entropy may be NULL, and so may
+ * tokens and logprob with given = 0.  vocab <= 2^20. */
+FL_EXPORT int fl_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void* tokens, int token_bytes, int64_t given,
+                          double temperature, int top, float* logprob, float* logsumexp, float* entropy, int32_t* top_ids, float* top_logprobs, void* stream);
 
 /* ---- embeddings (BERT family) ------------------------------------------------------------------ */
 /* ids/mask: host u32 [b, t]; mask may be NULL (all ones).  out: host f32 [b, hidden], mean-pooled and L2-normalised. */

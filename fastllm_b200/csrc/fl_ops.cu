@@ -2,6 +2,7 @@
 #include <cmath>
 
 #include "../../include/fastllm_b200.h"
+#include "bert_model.cuh"
 #include "linear8.cuh"
 #include "logprobs.cuh"
 #include "runtime.cuh"
@@ -39,15 +40,117 @@ constexpr int64_t kLinear8MaxK = 131071;        // 128 * 128 * k stays below 2^3
 static int64_t padded_k(int64_t k) { return (k + 15) / 16 * 16; }
 static size_t quantized_bytes(int64_t rows, int64_t k) { return ((size_t)rows * padded_k(k) + 255) / 256 * 256; }
 
-static void quantize_rows(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, int64_t cols_q, float* scale) {
-    auto go = [&](auto* p) {
-        using T = std::remove_pointer_t<decltype(p)>;
-        launch(lc, "quantize_rows", rows * cols * (sizeof(T) + 1), quantize_rows_kernel<T>, dim3((unsigned)rows), dim3(256), 0, static_cast<const T*>(x), (long long)ldx,
-               (int)cols, q, (long long)ldq, (int)cols_q, scale);
+// Launch of an operator's kernel in clusters of `cluster` blocks; pdl: it may start under the kernel before it, which this call launched too
+// (never under a caller's).
+template <typename... KArgs, typename... Args>
+static void launch_op(LaunchCtx& lc, const char* tag, uint64_t bytes, void (*kern)(KArgs...), dim3 grid, int threads, size_t smem, int cluster, bool pdl, Args&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = lc.stream;
+    cudaLaunchAttribute attr[2];
+    const bool prof = g_prof.on && !lc.capturing;
+    if (pdl && !prof) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = cluster; attr[cfg.numAttrs].val.clusterDim.y = 1; attr[cfg.numAttrs++].val.clusterDim.z = 1;
+    }
+    cfg.attrs = attr;
+    ProfEntry pe;
+    if (prof) {
+        pe.tag = tag;
+        pe.bytes = bytes;
+        FL_CUDA(cudaEventCreate(&pe.e0));
+        FL_CUDA(cudaEventCreate(&pe.e1));
+        FL_CUDA(cudaEventRecord(pe.e0, lc.stream));
+    }
+    FL_CUDA(cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...));
+    if (prof) {
+        FL_CUDA(cudaEventRecord(pe.e1, lc.stream));
+        g_prof.entries.push_back(pe);
+    }
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+}
+
+// What the operators keep for the process: one page-locked word that a kernel sets when a wait inside it ran out; the next call reports it.
+static int* g_op_failed = nullptr;
+static int g_pair_clusters = 0;                 // pairs of SMs that can be resident at once
+
+template <int BN>
+static void few_attr() {
+    FL_CUDA(cudaFuncSetAttribute(linear8_few_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L8Few<BN>::kSmem));
+}
+// One-time set-up, with fl_init: also loads the kernels, so that a caller's first call may be one inside a graph capture.
+void ops_init() {
+    if (g_op_failed != nullptr) return;
+    few_attr<16>(); few_attr<32>(); few_attr<64>(); few_attr<128>(); few_attr<256>();
+    FL_CUDA(cudaFuncSetAttribute(linear8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL8PairSmem));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(kNumSMs); cfg.blockDim = dim3(kL8PairThreads); cfg.dynamicSmemBytes = kL8PairSmem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    FL_CUDA(cudaOccupancyMaxActiveClusters(&g_pair_clusters, linear8_pair_kernel, &cfg));
+    int* p = nullptr;
+    FL_CUDA(cudaMallocHost(&p, sizeof(int)));
+    *p = 0;
+    g_op_failed = p;
+}
+static void check_op_failed() {
+    FL_CHECK(*reinterpret_cast<volatile int*>(g_op_failed) == 0, FL_ERR_CUDA, "a wait inside an operator's kernel ran out in an earlier call: its results are not valid");
+}
+
+template <typename T>
+static void quantize_rows_t(LaunchCtx& lc, const void* x, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, int64_t cols_q, float* scale) {
+    constexpr int V = 16 / sizeof(T);
+    const uint64_t bytes = rows * cols * (sizeof(T) + 1);
+    auto go = [&](auto kern) {
+        launch_op(lc, "quantize_rows", bytes, kern, dim3((unsigned)rows), 256, 0, 1, false, static_cast<const T*>(x), (long long)ldx, (int)cols, q, (long long)ldq,
+                  (int)cols_q, scale);
     };
-    if (dtype == FL_DTYPE_F32) go((float*)nullptr);
-    else if (dtype == FL_DTYPE_BF16) go((__nv_bfloat16*)nullptr);
-    else go((__half*)nullptr);
+    const bool vec = aligned(x, 16) && aligned(q, V) && (rows == 1 || (ldx % V == 0 && ldq % V == 0));
+    const int64_t vecs = (cols_q + V - 1) / V;
+    if (!vec || vecs > 8 * 256) go(quantize_rows_kernel<T, 0>);
+    else if (vecs <= 256) go(quantize_rows_kernel<T, 1>);
+    else if (vecs <= 2 * 256) go(quantize_rows_kernel<T, 2>);
+    else if (vecs <= 4 * 256) go(quantize_rows_kernel<T, 4>);
+    else go(quantize_rows_kernel<T, 8>);
+}
+static void quantize_rows(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, int64_t cols_q, float* scale) {
+    if (dtype == FL_DTYPE_F32) quantize_rows_t<float>(lc, x, rows, cols, ldx, q, ldq, cols_q, scale);
+    else if (dtype == FL_DTYPE_BF16) quantize_rows_t<__nv_bfloat16>(lc, x, rows, cols, ldx, q, ldq, cols_q, scale);
+    else quantize_rows_t<__half>(lc, x, rows, cols, ldx, q, ldq, cols_q, scale);
+}
+
+template <int BN>
+static void launch_few(LaunchCtx& lc, uint64_t bytes, const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, const Linear8Args& g, bool pdl) {
+    const int tiles = (g.n + 127) / 128 * ((g.rows + BN - 1) / BN), nk = (g.k + kL8BK - 1) / kL8BK;
+    int S = 1;
+    while (S < 8 && 2 * S * tiles <= L8Few<BN>::kPerSm * kNumSMs && nk >= 8 * S) S *= 2;
+    const CUtensorMap tw = make_tmap_i8(w, g.n, g.k, ldw, 128), tx = make_tmap_i8(x, g.rows, g.k, ldx, BN);
+    launch_op(lc, "linear8", bytes, linear8_few_kernel<BN>, dim3((unsigned)((g.n + 127) / 128 * S), (unsigned)((g.rows + BN - 1) / BN)), L8Few<BN>::kThreads, L8Few<BN>::kSmem, S, pdl,
+              tw, tx, g, S);
+}
+static bool launch_pair(LaunchCtx& lc, uint64_t bytes, const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, const Linear8Args& g, bool pdl) {
+    if (g_pair_clusters < 1) return false;
+    const int size = g.y_dtype == FL_DTYPE_F32 ? 4 : 2;
+    const bool whole = aligned(g.y, 32) && g.ldy * size % 32 == 0;
+    const int mp = (g.rows + 255) / 256, clusters = std::min(g_pair_clusters, kNumSMs / 2);
+    int bn = 256;
+    long long best = -1;
+    for (int b : {256, 192, 128}) {             // the width whose waves of tiles cost least
+        const long long waves = ((long long)mp * ((g.n + b - 1) / b) + clusters - 1) / clusters;
+        if (best < 0 || waves * b < best) { best = waves * b; bn = b; }
+    }
+    const long long tiles = (long long)mp * ((g.n + bn - 1) / bn);
+    const CUtensorMap tx = make_tmap_i8(x, g.rows, g.k, ldx, 128), tw = make_tmap_i8(w, g.n, g.k, ldw, bn / 2);
+    launch_op(lc, "linear8", bytes, linear8_pair_kernel, dim3((unsigned)(2 * std::min<long long>(tiles, clusters))), kL8PairThreads, kL8PairSmem, 1, pdl, tx, tw, g, bn, whole);
+    return true;
 }
 
 }  // namespace fl
@@ -100,23 +203,24 @@ FL_EXPORT int fl_linear8(const void* x, int x_dtype, int64_t ldx, const float* x
              "linear8: the workspace is smaller than fl_linear8_workspace asks for, or not on a 256-byte border");
     DeviceScope dev;
     LaunchCtx lc = op_ctx(stream);
-    Linear8Args g{};
-    if (given) {
-        g.xq = static_cast<const int8_t*>(x); g.ldq = ldx; g.xs = x_scale;
-    } else {
-        int8_t* q = static_cast<int8_t*>(workspace);
-        float* s = reinterpret_cast<float*>(q + quantized_bytes(rows, k));
-        quantize_rows(lc, x, x_dtype, rows, k, ldx, q, padded_k(k), padded_k(k), s);
-        g.xq = q; g.ldq = padded_k(k); g.xs = s;
+    check_op_failed();
+    const int8_t* q = static_cast<const int8_t*>(x);
+    int64_t ldq = rows == 1 ? padded_k(k) : ldx;
+    Linear8Args g{(int)rows, (int)n, (int)k, x_scale, w_scale, bias, y, ldy, y_dtype, g_op_failed};
+    if (!given) {
+        int8_t* to = static_cast<int8_t*>(workspace);
+        float* s = reinterpret_cast<float*>(to + quantized_bytes(rows, k));
+        quantize_rows(lc, x, x_dtype, rows, k, ldx, to, padded_k(k), padded_k(k), s);
+        q = to; ldq = padded_k(k); g.xs = s;
     }
-    g.w = w; g.ldw = ldw; g.ws = w_scale; g.bias = bias; g.y = y; g.ldy = ldy;
-    g.rows = (int)rows; g.n = (int)n; g.k = (int)k;
-    const dim3 grid((unsigned)((n + 63) / 64), (unsigned)((rows + 63) / 64));
-    FL_CHECK(grid.y <= 65535, FL_ERR_INVALID, "linear8: too many rows");
+    if (n == 1) ldw = padded_k(k);
     const uint64_t bytes = (uint64_t)n * k + (uint64_t)rows * (k + n * dtype_size(y_dtype));
-    if (y_dtype == FL_DTYPE_F32) launch(lc, "linear8", bytes, linear8_kernel<float>, grid, dim3(256), 0, g);
-    else if (y_dtype == FL_DTYPE_BF16) launch(lc, "linear8", bytes, linear8_kernel<__nv_bfloat16>, grid, dim3(256), 0, g);
-    else launch(lc, "linear8", bytes, linear8_kernel<__half>, grid, dim3(256), 0, g);
+    if (rows > 256 && launch_pair(lc, bytes, q, ldq, w, ldw, g, !given)) return FL_OK;
+    if (rows <= 16) launch_few<16>(lc, bytes, q, ldq, w, ldw, g, !given);
+    else if (rows <= 32) launch_few<32>(lc, bytes, q, ldq, w, ldw, g, !given);
+    else if (rows <= 64) launch_few<64>(lc, bytes, q, ldq, w, ldw, g, !given);
+    else if (rows <= 128) launch_few<128>(lc, bytes, q, ldq, w, ldw, g, !given);
+    else launch_few<256>(lc, bytes, q, ldq, w, ldw, g, !given);
     FL_API_END
 }
 

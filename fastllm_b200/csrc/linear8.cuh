@@ -4,7 +4,7 @@
 #pragma once
 #include <cuda_fp16.h>
 
-#include "common.cuh"
+#include "gemm_pair.cuh"
 
 namespace fl {
 
@@ -44,65 +44,427 @@ struct RowScale {
 // larger for every NaN than for an infinity, and for that than for any number
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// A block per row; columns [cols, cols_q) of q are filled with zeros.
-template <typename T>
+// A block per row; columns [cols, cols_q) of q are filled with zeros.  kVecs > 0: the row starts on 16-byte borders on both sides (8 for q) and has at
+// most 256 * kVecs vectors of 16 bytes, which stay in registers between the maximum and the rounding; 0: any row, read twice.
+template <typename T, int kVecs>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, long long ldx, int cols, int8_t* __restrict__ q, long long ldq, int cols_q,
                                                             float* __restrict__ scale) {
+    constexpr int V = 16 / sizeof(T);
     __shared__ uint32_t part[8];
     const T* xr = x + (long long)blockIdx.x * ldx;
     int8_t* qr = q + (long long)blockIdx.x * ldq;
+    pdl_launch_dependents();
     uint32_t m = 0;
-    for (int i = threadIdx.x; i < cols; i += 256) m = max(m, abs_bits(to_f32(xr[i])));
+    uint4 held[kVecs > 0 ? kVecs : 1];
+    if constexpr (kVecs > 0) {
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) {
+            const int at = (threadIdx.x + 256 * u) * V;
+            held[u] = make_uint4(0, 0, 0, 0);
+            if (at + V <= cols) {
+                held[u] = __ldg(reinterpret_cast<const uint4*>(xr + at));
+            } else if (at < cols) {
+                T* e = reinterpret_cast<T*>(&held[u]);
+                for (int j = 0; j < V; ++j)
+                    if (at + j < cols) e[j] = xr[at + j];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) {
+            const T* e = reinterpret_cast<const T*>(&held[u]);
+#pragma unroll
+            for (int j = 0; j < V; ++j) m = max(m, abs_bits(to_f32(e[j])));
+        }
+    } else {
+        for (int i = threadIdx.x; i < cols; i += 256) m = max(m, abs_bits(to_f32(xr[i])));
+    }
     m = __reduce_max_sync(0xFFFFFFFFu, m);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
     __syncthreads();
+#pragma unroll
     for (int i = 0; i < 8; ++i) m = max(m, part[i]);
     const RowScale rs(m);
-    for (int i = threadIdx.x; i < cols_q; i += 256) qr[i] = i < cols ? (int8_t)rs(to_f32(xr[i])) : (int8_t)0;
+    if constexpr (kVecs > 0) {
+#pragma unroll
+        for (int u = 0; u < kVecs; ++u) {
+            const int at = (threadIdx.x + 256 * u) * V;
+            if (at >= cols_q) break;
+            const T* e = reinterpret_cast<const T*>(&held[u]);
+            uint32_t w[V / 4];
+#pragma unroll
+            for (int i = 0; i < V / 4; ++i) {
+                w[i] = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[i] |= (uint32_t)(uint8_t)(int8_t)rs(to_f32(e[4 * i + j])) << (8 * j);
+            }
+            if (at + V <= cols_q) {
+                if constexpr (V == 8) *reinterpret_cast<uint2*>(qr + at) = make_uint2(w[0], w[1]);
+                else *reinterpret_cast<uint32_t*>(qr + at) = w[0];
+            } else {
+                for (int j = 0; at + j < cols_q; ++j) qr[at + j] = (int8_t)(w[j / 4] >> (8 * (j % 4)));
+            }
+        }
+    } else {
+        for (int i = threadIdx.x; i < cols_q; i += 256) qr[i] = i < cols ? (int8_t)rs(to_f32(xr[i])) : (int8_t)0;
+    }
     if (threadIdx.x == 0) scale[blockIdx.x] = rs.scale;
 }
 
 struct Linear8Args {
-    const int8_t* xq; long long ldq; const float* xs;       // [rows, k], [rows]
-    const int8_t* w; long long ldw; const float* ws;        // [n, k], [n]
-    const float* bias;                                      // [n] or null
-    void* y; long long ldy;
     int rows, n, k;
+    const float* xs;                                        // [rows]
+    const float* ws;                                        // [n]
+    const float* bias;                                      // [n] or null
+    void* y; long long ldy; int y_dtype;                    // fl_dtype
+    int* failed;                                            // set when a wait ran out
 };
 
-// 64 x 64 outputs per block, four products of 8 bits per instruction
-template <typename T>
-__global__ void __launch_bounds__(256) linear8_kernel(const Linear8Args g) {
-    __shared__ int sx[64][17], sw[64][17];
-    const int n0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
-    const int tn = threadIdx.x & 15, tr = threadIdx.x >> 4;
-    int acc[4][4] = {};
-    auto word = [&](const int8_t* row, int k) {             // four values from column k on, zeros past the end
-        uint32_t v = 0;
-        for (int j = 0; j < 4; ++j)
-            if (k + j < g.k) v |= (uint32_t)(uint8_t)row[k + j] << (8 * j);
-        return (int)v;
-    };
-    for (int k0 = 0; k0 < g.k; k0 += 64) {
-        for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-            const int row = i >> 4, c = i & 15;
-            sx[row][c] = r0 + row < g.rows ? word(g.xq + (long long)(r0 + row) * g.ldq, k0 + 4 * c) : 0;
-            sw[row][c] = n0 + row < g.n ? word(g.w + (long long)(n0 + row) * g.ldw, k0 + 4 * c) : 0;
-        }
-        __syncthreads();
-        for (int c = 0; c < 16; ++c)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(sx[tr + 16 * i][c], sw[tn + 16 * j][c], acc[i][j]);
-        __syncthreads();
+constexpr int kL8BK = 128;                                  // 128 values = 128 bytes = one swizzle row
+constexpr uint32_t kL8WBytes = 128 * kL8BK;                 // a box of 128 weight rows
+
+// Instruction descriptor, kind::i8: D = s32 (bits 4-5 = 2), A = B = signed (bits 7-9 = 1, 10-12 = 1), both K-major, N>>3 at 17, M>>4 at 24.
+__host__ __device__ constexpr uint32_t umma_idesc_i8(int M, int N) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// whole warps, one elected lane issues (see uniform_warp)
+__device__ __forceinline__ void umma_i8_warp(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p, e;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "elect.sync _|e, 0xFFFFFFFF;\n"
+        "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_i8_pair_warp(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p, e;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "elect.sync _|e, 0xFFFFFFFF;\n"
+        "@e tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void l8_store(const Linear8Args& g, long long at, float v) {
+    if (g.y_dtype == 0) reinterpret_cast<float*>(g.y)[at] = v;
+    else if (g.y_dtype == 1) reinterpret_cast<__nv_bfloat16*>(g.y)[at] = from_f32<__nv_bfloat16>(v);
+    else reinterpret_cast<__half*>(g.y)[at] = from_f32<__half>(v);
+}
+// A wait ran out: report it and leave the copies in flight time to land; the block goes on to its end.
+__device__ __forceinline__ void l8_give_up(int* failed) {
+    if ((threadIdx.x & 31) == 0) *failed = 1;
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------------------------------
+// The weights are the 128-row operand and nearly all the traffic, BN activation rows the other one; a cluster of S blocks cuts K of one tile, and
+// its blocks add up each other's parts through shared memory: whole numbers, so the order does not matter, and no workspace.
+template <int BN> struct L8Few {
+    static constexpr uint32_t kX = BN * kL8BK, kStage = kL8WBytes + kX;
+    static constexpr int kPerSm = BN <= 128 ? 2 : 1;                                   // blocks that an SM holds
+    static constexpr uint32_t kRing = kPerSm == 2 ? 108 * 1024 : 208 * 1024;
+    static constexpr int kStages = kRing / kStage < 8 ? kRing / kStage : 8;
+    static constexpr size_t kSmem = (size_t)kStages * kStage + 1024;
+    static constexpr int kThreads = 192;
+    static constexpr uint32_t kTmem = BN < 32 ? 32 : BN;
+    static_assert(kStages * kStage >= (uint32_t)BN * 512, "the parts of a tile fit the ring");
+};
+
+template <int BN>
+__global__ void __launch_bounds__(L8Few<BN>::kThreads, L8Few<BN>::kPerSm)
+linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Linear8Args g, const int S) {
+    using L = L8Few<BN>;
+    constexpr int kStages = L::kStages;
+    extern __shared__ uint8_t gsm_raw[];
+    uint8_t* gsm = gsm_raw + ((1024u - (smem_u32(gsm_raw) & 1023u)) & 1023u);          // (the same offset in all blocks of a cluster)
+    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], done;
+    __shared__ uint32_t tmem_base_s;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    const int s = S == 1 ? 0 : (int)cluster_rank();
+    const int n0 = blockIdx.x / S * 128, r0 = blockIdx.y * BN;
+    const int nk = (g.k + kL8BK - 1) / kL8BK, kb0 = (int)((long long)s * nk / S), kb1 = (int)((long long)(s + 1) * nk / S);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        mbar_init(&done, 1);
+        mbar_fence_init();
     }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int r = r0 + tr + 16 * i, n = n0 + tn + 16 * j;
-            if (r >= g.rows || n >= g.n) continue;
-            float v = (float)acc[i][j] * g.xs[r] * g.ws[n];
-            if (g.bias) v += g.bias[n];
-            reinterpret_cast<T*>(g.y)[(long long)r * g.ldy + n] = from_f32<T>(v);
+    if (warp == 1) tmem_alloc(&tmem_base_s, L::kTmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_s;
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            auto weights = [&](int kb, int st) {
+                mbar_expect_tx(&full[st], L::kStage);
+                tma_load_2d(gsm + st * L::kStage, &tmW, kb * kL8BK, n0, &full[st]);
+            };
+            auto rows = [&](int kb, int st) { tma_load_2d(gsm + st * L::kStage + kL8WBytes, &tmX, kb * kL8BK, r0, &full[st]); };
+            // the weights do not depend on the kernel that rounds the rows: a ring-full of them is requested ahead of the wait
+            const int pre = min(kb1, kb0 + kStages);
+            for (int kb = kb0; kb < pre; ++kb) weights(kb, kb - kb0);
+            pdl_wait();
+            asm volatile("fence.proxy.async;" ::: "memory");                           // the rows were written through the generic proxy
+            for (int kb = kb0; kb < pre; ++kb) rows(kb, kb - kb0);
+            int st = 0;
+            uint32_t ph = 0;
+            for (int kb = pre; kb < kb1; ++kb) {
+                if (!(ok = mbar_wait_bounded(&empty[st], ph, kMbarTries))) break;
+                weights(kb, st);
+                rows(kb, st);
+                if (++st == kStages) { st = 0; ph ^= 1; }
+            }
         }
+    } else if (warp == 1) {
+        constexpr uint32_t idesc = umma_idesc_i8(128, BN);
+        const uint64_t base = umma_smem_desc_sw128(gsm);
+        int st = 0;
+        uint32_t ph = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            if (ok) ok = mbar_wait_bounded(&full[st], ph, kMbarTries);
+            __syncwarp();
+            tc_fence_after();
+            const uint64_t a = base + (uint64_t)(st * (L::kStage >> 4)), b = a + (kL8WBytes >> 4);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) umma_i8_warp(tmem, a + 2 * q, b + 2 * q, idesc, ((kb - kb0) | q) ? 1u : 0u);
+            umma_commit_warp(&empty[st]);
+            if (++st == kStages) { st = 0; ph ^= 1; }
+        }
+        umma_commit_warp(&done);
+    }
+    const int row = (warp & 3) * 32 + lane;                                            // accumulator row = weight row of the tile (epilogue warps)
+    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const int n = n0 + row;
+    if (warp >= 2) {
+        pdl_wait();                                                                    // (the rows' scales)
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&done, 0, kMbarTries));
+        tc_fence_after();
+    }
+    const float wsn = warp >= 2 && n < g.n ? g.ws[n] : 0.f, bn = warp >= 2 && g.bias != nullptr && n < g.n ? g.bias[n] : 0.f;
+    auto store = [&](int c, int sum) {                                                 // for a fixed column the 32 lanes write 32 neighbours of one row
+        const int r = r0 + c;
+        if (r >= g.rows || n >= g.n) return;
+        float v = (float)sum * g.xs[r] * wsn;
+        if (g.bias != nullptr) v += bn;
+        l8_store(g, (long long)r * g.ldy + n, v);
+    };
+    if (S == 1) {
+        if (warp >= 2 && ok) {
+#pragma unroll 1
+            for (int c = 0; c < BN && r0 + c < g.rows; c += 16) {
+                uint32_t v[16];
+                tmem_ld16(at + (uint32_t)c, v);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) store(c + j, (int)v[j]);
+            }
+        }
+    } else {
+        const int per = BN / S;                                                        // columns that one block of the cluster adds up and writes
+        __syncwarp();
+        cluster_sync_all();                                                            // every block's products are done: the rings are free
+        if (warp >= 2) {
+            const uint32_t base = smem_u32(gsm) + (uint32_t)(s * per * 128 + row) * 4;
+#pragma unroll 1
+            for (int c = 0; c < BN && r0 + c < g.rows; c += 16) {
+                uint32_t v[16];
+                tmem_ld16(at + (uint32_t)c, v);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int owner = (c + j) / per;
+                    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(mapa_u32(base + (uint32_t)((c + j) - owner * per) * 512, owner)), "r"(v[j]) : "memory");
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();
+        if (warp >= 2 && ok) {
+            const int* part = reinterpret_cast<const int*>(gsm) + row;
+            for (int c = 0; c < per && r0 + s * per + c < g.rows; ++c) {
+                int sum = 0;
+                for (int t = 0; t < S; ++t) sum += part[(t * per + c) * 128];
+                store(s * per + c, sum);
+            }
+        }
+    }
+    if (!ok) l8_give_up(g.failed);
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, L::kTmem);
+    }
+}
+
+// ---- many rows ----------------------------------------------------------------------------------------------------------------------
+// Pairs of SMs on 256 x bn tiles (tcgen05.mma.cta_group::2): each holds its 128 activation rows and half of the weight tile.
+constexpr int kL8PairStages = 6, kL8PairEpi = 16, kL8PairThreads = 64 + 32 * kL8PairEpi;
+constexpr uint32_t kL8PairStage = 2 * kL8WBytes;
+constexpr size_t kL8PairSmem = (size_t)kL8PairStages * kL8PairStage + 1024;
+
+// 16 outputs of one row; whole: 32-byte stores are allowed
+__device__ __forceinline__ void l8_store16(const Linear8Args& g, int row, int col, const float (&v)[16], bool whole) {
+    if (whole && col + 16 <= g.n) {
+        if (g.y_dtype == 0) {
+            float* o = reinterpret_cast<float*>(g.y) + (long long)row * g.ldy + col;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(v[8 * h + j]);
+                st_global_32b(o + 8 * h, w);
+            }
+        } else {
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (g.y_dtype == 1) {
+                    w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
+                } else {
+                    const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+                    w[j] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+            }
+            st_global_32b(reinterpret_cast<uint16_t*>(g.y) + (long long)row * g.ldy + col, w);
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+        if (col + j < g.n) l8_store(g, (long long)row * g.ldy + col + j, v[j]);
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kL8PairThreads, 1)
+linear8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const Linear8Args g, const int bn, const bool whole) {
+    extern __shared__ uint8_t gsm_raw[];
+    uint8_t* gsm = gsm_raw + ((1024u - (smem_u32(gsm_raw) & 1023u)) & 1023u);          // (the same offset in both CTAs)
+    __shared__ __align__(8) uint64_t full[kL8PairStages], empty[kL8PairStages], acc_full[2], acc_empty[2];
+    __shared__ uint32_t tmem_base_s;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int cl = blockIdx.x >> 1, G = gridDim.x >> 1;
+    const int nk = (g.k + kL8BK - 1) / kL8BK, mp = (g.rows + 255) / 256, nt = (g.n + bn - 1) / bn, T = mp * nt;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kL8PairStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 2 * kL8PairEpi); }
+        mbar_fence_init();
+        tma_prefetch_desc(&tmX);
+        tma_prefetch_desc(&tmW);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_base_s;
+    // 8 pair rows share a weight tile before the walk moves on (see kGemmRasterRows)
+    auto place = [&](int tile, int& m, int& n) {
+        constexpr int RM = kGemmRasterRows / 2;
+        const int per = RM * nt, first = tile / per * RM, local = tile % per, cnt = min(RM, mp - first);
+        m = (first + local % cnt) * 256 + (int)rank * 128;
+        n = local / cnt * bn;
+    };
+    const uint32_t tx = 2 * (kL8WBytes + (uint32_t)bn / 2 * kL8BK);                    // bytes of a stage in both CTAs
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            pdl_wait();
+            asm volatile("fence.proxy.async;" ::: "memory");
+            int st = 0;
+            uint32_t ph = 1;
+            for (int tile = cl; ok && tile < T; tile += G) {
+                int m0, n0;
+                place(tile, m0, n0);
+                for (int kb = 0; kb < nk; ++kb) {
+                    if (!(ok = pair_wait(&empty[st], ph))) break;
+                    if (rank == 0) mbar_expect_tx(&full[st], tx);                      // both CTAs' loads complete on the first one's barrier
+                    const uint32_t bar = mapa_u32(smem_u32(&full[st]), 0), sa = smem_u32(gsm) + st * kL8PairStage;
+                    tma_load_2d_pair(sa, &tmX, kb * kL8BK, m0, bar);
+                    tma_load_2d_pair(sa + kL8WBytes, &tmW, kb * kL8BK, n0 + (int)rank * (bn >> 1), bar);
+                    if (++st == kL8PairStages) { st = 0; ph ^= 1; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {
+            const uint32_t idesc = umma_idesc_i8(256, bn);
+            const uint64_t base = umma_smem_desc_sw128(gsm);
+            int st = 0;
+            uint32_t ph = 0, seg = 0;
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                if (ok) ok = pair_wait(bar, parity);
+                __syncwarp();
+                tc_fence_after();
+            };
+            for (int tile = cl; tile < T; tile += G, ++seg) {
+                const uint32_t as = seg & 1, tacc = tmem_base + as * 256;
+                wait(&acc_empty[as], ((seg >> 1) & 1) ^ 1);
+                for (int kb = 0; kb < nk; ++kb) {
+                    wait(&full[st], ph);
+                    const uint64_t a = base + (uint64_t)(st * (kL8PairStage >> 4)), b = a + (kL8WBytes >> 4);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) umma_i8_pair_warp(tacc, a + 2 * q, b + 2 * q, idesc, (kb | q) ? 1u : 0u);
+                    umma_commit_pair_warp(&empty[st]);
+                    if (++st == kL8PairStages) { st = 0; ph ^= 1; }
+                }
+                umma_commit_pair_warp(&acc_full[as]);
+            }
+        }
+    } else {
+        const int q = warp & 3, cs = (warp - 2) >> 2, cols = bn >> 2;                  // TMEM lane quarter (hardware rule); a quarter of the columns
+        uint32_t seg = 0;
+        pdl_wait();                                                                    // (the rows' scales)
+        for (int tile = cl; tile < T; tile += G, ++seg) {
+            int m0, n0;
+            place(tile, m0, n0);
+            const uint32_t as = seg & 1;
+            if (ok) ok = __all_sync(0xFFFFFFFFu, pair_wait(&acc_full[as], (seg >> 1) & 1));
+            tc_fence_after();
+            const uint32_t at = tmem_base + as * 256 + ((uint32_t)(q * 32) << 16);
+            const int row = m0 + q * 32 + lane;
+            const float xs = row < g.rows ? g.xs[row] : 0.f;
+            if (ok) {
+#pragma unroll 1
+                for (int c = cs * cols; c < (cs + 1) * cols && n0 + c < g.n; c += 16) {
+                    uint32_t a[16];
+                    float v[16];
+                    tmem_ld16(at + (uint32_t)c, a);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const int n = min(n0 + c + j, g.n - 1);
+                        v[j] = (float)(int)a[j] * xs * __ldg(g.ws + n);
+                        if (g.bias != nullptr) v[j] += __ldg(g.bias + n);
+                    }
+                    if (row < g.rows) l8_store16(g, row, n0 + c, v, whole);
+                    __syncwarp();
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[as]), 0));
+        }
+    }
+    if (!ok) l8_give_up(g.failed);
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();          // the other CTA's products read this one's shared memory, its epilogue arrives on this one's barriers
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
+    }
 }
 
 }  // namespace fl

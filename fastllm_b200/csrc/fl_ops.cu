@@ -89,6 +89,9 @@ void ops_init() {
     if (g_op_failed != nullptr) return;
     few_attr<16>(); few_attr<32>(); few_attr<64>(); few_attr<128>(); few_attr<256>();
     FL_CUDA(cudaFuncSetAttribute(linear8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL8PairSmem));
+    auto wide = [](auto kern) { FL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)); };
+    wide(logprobs_kernel<float, false>); wide(logprobs_kernel<__nv_bfloat16, false>); wide(logprobs_kernel<__half, false>);
+    wide(logprobs_kernel<float, true>); wide(logprobs_kernel<__nv_bfloat16, true>); wide(logprobs_kernel<__half, true>);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(kNumSMs); cfg.blockDim = dim3(kL8PairThreads); cfg.dynamicSmemBytes = kL8PairSmem;
     cudaLaunchAttribute at[1];
@@ -151,6 +154,21 @@ static bool launch_pair(LaunchCtx& lc, uint64_t bytes, const int8_t* x, int64_t 
     const CUtensorMap tx = make_tmap_i8(x, g.rows, g.k, ldx, 128), tw = make_tmap_i8(w, g.n, g.k, ldw, bn / 2);
     launch_op(lc, "linear8", bytes, linear8_pair_kernel, dim3((unsigned)(2 * std::min<long long>(tiles, clusters))), kL8PairThreads, kL8PairSmem, 1, pdl, tx, tw, g, bn, whole);
     return true;
+}
+
+// Blocks per row: as many as the chip holds (four per SM) over the rows, while every warp still has a chunk of two; the cluster of 16 is not portable
+// to every chip, but B200 has it.
+template <typename T>
+static void run_logprobs(LaunchCtx& lc, const LogprobArgs& a) {
+    const int chunks = (a.vocab + 2 * LpRow<T>::N - 1 + LpRow<T>::kChunk - 1) / LpRow<T>::kChunk;
+    int C = 1;
+    while (C < kLpMaxCluster && (long long)a.rows * 2 * C <= 4 * kNumSMs && chunks >= 2 * C * (kLpThreads / 32)) C *= 2;
+    const uint64_t bytes = (uint64_t)a.rows * a.vocab * sizeof(T);
+    const dim3 grid((unsigned)((long long)a.rows * C));
+    if (a.top > 0)
+        launch_op(lc, "logprobs", bytes, logprobs_kernel<T, true>, grid, kLpThreads, (size_t)((chunks + C - 1) / C + 1) * 4, C, false, a, C);
+    else
+        launch_op(lc, "logprobs", bytes, logprobs_kernel<T, false>, grid, kLpThreads, 0, C, false, a, C);
 }
 
 }  // namespace fl
@@ -240,12 +258,12 @@ FL_EXPORT int fl_logprobs(const void* logits, int dtype, int64_t rows, int64_t v
                  aligned(top_ids, 4) && aligned(top_logprobs, 4), FL_ERR_INVALID, "logprobs: a pointer is not aligned to its type");
     DeviceScope dev;
     LaunchCtx lc = op_ctx(stream);
-    const LogprobArgs a{logits, ld, (int)rows, (int)vocab, inv_t, tokens, (int)given, token_bytes == 8, top, given ? logprob : nullptr, logsumexp, entropy, top_ids, top_logprobs};
-    const uint64_t bytes = (uint64_t)rows * vocab * dtype_size(dtype);
-    const dim3 grid((unsigned)rows);
-    if (dtype == FL_DTYPE_F32) launch(lc, "logprobs", bytes, logprobs_kernel<float>, grid, dim3(256), 0, a);
-    else if (dtype == FL_DTYPE_BF16) launch(lc, "logprobs", bytes, logprobs_kernel<__nv_bfloat16>, grid, dim3(256), 0, a);
-    else launch(lc, "logprobs", bytes, logprobs_kernel<__half>, grid, dim3(256), 0, a);
+    const float c = (float)(1.4426950408889634 / temperature);
+    FL_CHECK(std::isfinite(c) && c > 0, FL_ERR_INVALID, "logprobs: the temperature is a positive number");
+    const LogprobArgs a{logits, ld, (int)rows, (int)vocab, inv_t, c, tokens, (int)given, token_bytes == 8, top, given ? logprob : nullptr, logsumexp, entropy, top_ids, top_logprobs};
+    if (dtype == FL_DTYPE_F32) run_logprobs<float>(lc, a);
+    else if (dtype == FL_DTYPE_BF16) run_logprobs<__nv_bfloat16>(lc, a);
+    else run_logprobs<__half>(lc, a);
     FL_API_END
 }
 

@@ -1,5 +1,15 @@
 // Log probabilities over a vocabulary: z = x / T, logZ = log sum exp z, lp(t) = z_t - logZ, H = logZ - sum p z, and the largest logits with
 // theirs, the lowest index first among equals.
+//
+// One pass over the logits.  A thread keeps a reference r near its running maximum and adds up e = 2^(c x - r) and e (c x - r), c = log2(e) / T; sums with
+// different references are brought to the largest one and joined.  The reference moves when a maximum is 2^16 above it, so the exponentials
+// stay far from overflow and the loop is nearly free of rescaling.  A row belongs to a cluster of C blocks (C = 1 when there are many rows), whose results
+// meet in the first block's shared memory: no workspace, no atomics, the same bits every time.
+//
+// Alternatives: the row lies in chunks of 512 bytes (one load of a warp), whose maxima are kept.  The K-th largest of a block's 256 thread maxima
+// is a lower bound for its K-th largest logit, since K threads hold one at least as large.  Only chunks that reach the bound are read again (from L2),
+// only logits that reach it are ranked: about K + K^2 / 512 of them where the order is random.  Where equal logits leave more than the tables hold, the K
+// best chunks by (maximum, lower index) are taken instead: a logit outside them is behind K others, one per chunk; then K rounds pick one each.
 #pragma once
 #include "linear8.cuh"
 
@@ -7,11 +17,13 @@ namespace fl {
 
 constexpr int kLpMaxTop = 32;
 constexpr int kLpMaxVocab = 1 << 20;
+constexpr int kLpThreads = 256, kLpMaxCluster = 16;
+constexpr int kLpList = 96, kLpCand = 256;          // chunks that are read again, logits that are ranked
 
 struct LogprobArgs {
     const void* x; long long ld;                // [rows, vocab]
     int rows, vocab;
-    float inv_t;
+    float inv_t, c;                             // 1 / T, log2(e) / T
     const void* tokens; int given, wide;        // [rows, given] int32, or int64 (wide)
     int top;
     float *logprob, *logsumexp, *entropy;       // [rows, given], [rows], [rows]; null = not wanted
@@ -23,70 +35,433 @@ __device__ __forceinline__ uint32_t ordered_bits(float v) {
     const uint32_t b = __float_as_uint(v + 0.f);
     return (b >> 31) ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ unsigned long long order_key(float v, int i) { return (unsigned long long)ordered_bits(v) << 32 | (uint32_t)~i; }
+__device__ __forceinline__ float from_ordered(uint32_t o) { return __uint_as_float((o >> 31) ? o & 0x7FFFFFFFu : ~o); }
+__device__ __forceinline__ unsigned long long order_key(uint32_t ordered, int i) { return (unsigned long long)ordered << 32 | (uint32_t)~i; }
 
-// A block per row: one walk for the maximum, one for the sums, one per alternative.
-template <typename T>
-__global__ void __launch_bounds__(256) logprobs_kernel(const LogprobArgs a) {
-    __shared__ float red[3][8];
-    __shared__ unsigned long long best[8];
-    const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const T* x = reinterpret_cast<const T*>(a.x) + (long long)row * a.ld;
-    auto z = [&](int i) { return to_f32(x[i]) * a.inv_t; };
-    float m = -INFINITY;
-    for (int i = tid; i < a.vocab; i += 256) m = fmaxf(m, z(i));
-    m = warp_max(m);
-    if (lane == 0) red[0][warp] = m;
-    __syncthreads();
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, red[0][i]);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float s = 0.f, t = 0.f;
-    for (int i = tid; i < a.vocab; i += 256) {
-        const float d = z(i) - ref, e = expf(d);
-        s += e;
-        if (e > 0.f) t += e * d;
+__device__ __forceinline__ float ex2(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// two f32 at once
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// 16 bytes of logits.  low: what -infinity is raised to before the sums, so that e (c x - r) is 0 and not 0 times infinity (NaN stays NaN); a row whose
+// maximum lies below `far` is summed by another loop.
+template <typename T> struct LpVec;
+template <> struct LpVec<float> {
+    static constexpr int N = 4;
+    static constexpr float kLow = -1e30f, kFar = -1e29f;
+    static __device__ __forceinline__ float max_of(const uint4& v) {
+        return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
     }
-    s = warp_sum(s);
-    t = warp_sum(t);
-    if (lane == 0) { red[1][warp] = s; red[2][warp] = t; }
+    static __device__ __forceinline__ float raise(uint32_t w) {
+        float r;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(w)), "f"(kLow));
+        return r;
+    }
+    template <typename F> static __device__ __forceinline__ void pairs(const uint4& v, F&& f) {
+        f(raise(v.x), raise(v.y));
+        f(raise(v.z), raise(v.w));
+    }
+    static __device__ __forceinline__ float at(const uint4& v, int j) { return __uint_as_float(j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w); }
+};
+template <> struct LpVec<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static constexpr float kLow = -1e30f, kFar = -1e29f;
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ float max_of(const uint4& v) {
+        const uint32_t m = max2(max2(v.x, v.y), max2(v.z, v.w));
+        return fmaxf(bf16lo(m), bf16hi(m));
+    }
+    template <typename F> static __device__ __forceinline__ void pairs(const uint4& v, F&& f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+            asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(w) : "r"(w), "r"(0xF14AF14Au));     // (-1.0002e30)
+            f(bf16lo(w), bf16hi(w));
+        }
+    }
+    static __device__ __forceinline__ float at(const uint4& v, int j) {
+        const uint32_t w = j < 2 ? v.x : j < 4 ? v.y : j < 6 ? v.z : v.w;
+        return (j & 1) ? bf16hi(w) : bf16lo(w);
+    }
+};
+template <> struct LpVec<__half> {
+    static constexpr int N = 8;
+    static constexpr float kLow = -65504.f, kFar = -30000.f;
+    static __device__ __forceinline__ float2 two(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        uint32_t r;
+        asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ float max_of(const uint4& v) {
+        const float2 m = two(max2(max2(v.x, v.y), max2(v.z, v.w)));
+        return fmaxf(m.x, m.y);
+    }
+    template <typename F> static __device__ __forceinline__ void pairs(const uint4& v, F&& f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+            asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(w) : "r"(w), "r"(0xFBFFFBFFu));      // (-65504)
+            const float2 p = two(w);
+            f(p.x, p.y);
+        }
+    }
+    static __device__ __forceinline__ float at(const uint4& v, int j) {
+        const float2 p = two(j < 2 ? v.x : j < 4 ? v.y : j < 6 ? v.z : v.w);
+        return (j & 1) ? p.y : p.x;
+    }
+};
+
+// A row in chunks of 32 vectors of 16 bytes, from the last 16-byte border at or before its start on; chunks that reach over an end are read value by value.
+template <typename T> struct LpRow {
+    static constexpr int N = LpVec<T>::N, kChunk = 32 * N;
+    const T* x;
+    int vocab, skip, chunks;                    // values between that border and the row; chunks of the row
+    __device__ LpRow(const LogprobArgs& a, int row) : x(reinterpret_cast<const T*>(a.x) + (long long)row * a.ld), vocab(a.vocab) {
+        skip = (int)(reinterpret_cast<uintptr_t>(x) & 15) / (int)sizeof(T);
+        chunks = (skip + vocab + kChunk - 1) / kChunk;
+    }
+    __device__ __forceinline__ int first(int chunk, int lane) const { return chunk * kChunk + lane * N - skip; }        // index of the lane's first value
+    // -infinity outside the row
+    __device__ __forceinline__ uint4 load(int chunk, int lane) const {
+        const int i0 = first(chunk, lane);
+        if (i0 >= 0 && i0 + N <= vocab) return ldg_stream(reinterpret_cast<const uint4*>(x + i0));
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = sizeof(T) == 4 ? 0xFF800000u : sizeof(T) == 2 && std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            if (i0 + j < 0 || i0 + j >= vocab) continue;
+            if constexpr (sizeof(T) == 4) {
+                w[j] = __float_as_uint(x[i0 + j]);
+            } else {
+                const uint32_t h = reinterpret_cast<const uint16_t*>(x)[i0 + j];
+                w[j / 2] = (j & 1) ? (w[j / 2] & 0xFFFFu) | h << 16 : (w[j / 2] & 0xFFFF0000u) | h;
+            }
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+struct __align__(16) LpPart { float m, r, s, t; };     // largest x; reference; sum of e; sum of e (c x - r)
+__device__ __forceinline__ LpPart lp_join(const LpPart& a, const LpPart& b) {
+    const float r = fmaxf(a.r, b.r), fa = ex2(a.r - r), fb = ex2(b.r - r);
+    return LpPart{fmaxf(a.m, b.m), r, a.s * fa + b.s * fb, (a.t + a.s * (a.r - r)) * fa + (b.t + b.s * (b.r - r)) * fb};
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobArgs a, const int C) {
+    constexpr int kWarps = kLpThreads / 32, U = 4;
+    extern __shared__ uint32_t chunk_max[];                     // TOP: ordered maxima of this block's chunks
+    __shared__ LpPart part[kWarps], parts[kLpMaxCluster];
+    __shared__ uint32_t sup[TOP ? kLpThreads : 1];
+    __shared__ unsigned long long cand[TOP ? kLpCand : 1], best[TOP ? kLpMaxCluster * kLpMaxTop : 1], round_best[TOP ? kWarps : 1];
+    __shared__ int list[TOP ? kLpList : 1];
+    __shared__ int n_list, n_cand;
+    __shared__ uint32_t bound;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = C == 1 ? 0 : (int)cluster_rank(), row = blockIdx.x / C;
+    const LpRow<T> x(a, row);
+    const int ch0 = (int)((long long)rank * x.chunks / C), ch1 = (int)((long long)(rank + 1) * x.chunks / C);
+    const float c = a.c, nan = __uint_as_float(0x7FFFFFFFu);
+    if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // (that the first block has started, before anyone writes to it)
+    if (tid == 0) { n_list = 0; n_cand = 0; }
+
+    // the given tokens' logits, on their way while the row is read
+    long long token = -1;
+    float token_x = 0.f;
+    const bool mine = rank == 0 && tid < a.given;
+    auto token_at = [&](int j) {
+        const long long at = (long long)row * a.given + j;
+        return a.wide ? reinterpret_cast<const long long*>(a.tokens)[at] : (long long)reinterpret_cast<const int*>(a.tokens)[at];
+    };
+    if (mine) {
+        token = token_at(tid);
+        if (token >= 0 && token < a.vocab) token_x = to_f32(x.x[token]);
+    }
+
+    LpPart p{-INFINITY, 0.9f * LpVec<T>::kLow * c, 0.f, 0.f};   // (well above what -infinity is raised to, below every other value of a row that is not `far`)
+    uint64_t s2 = pack2(0.f, 0.f), t2 = s2;
+    const uint64_t c2 = pack2(c, c);
+    for (int ch = ch0 + warp; ch < ch1; ch += kWarps * U) {
+        uint4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (ch + u * kWarps < ch1) v[u] = x.load(ch + u * kWarps, lane);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (ch + u * kWarps >= ch1) break;
+            const float m = LpVec<T>::max_of(v[u]);
+            p.m = fmaxf(p.m, m);
+            if (TOP) {
+                const uint32_t o = __reduce_max_sync(0xFFFFFFFFu, ordered_bits(m));
+                if (lane == 0) chunk_max[ch + u * kWarps - ch0] = o;
+            }
+            if (m * c > p.r + 16.f) {
+                const float r = m * c, f = ex2(p.r - r);
+                float sa, sb, ta, tb;
+                unpack2(s2, sa, sb);
+                unpack2(t2, ta, tb);
+                s2 = pack2(sa * f, sb * f);
+                t2 = pack2((ta + sa * (p.r - r)) * f, (tb + sb * (p.r - r)) * f);
+                p.r = r;
+            }
+            const uint64_t r2 = pack2(-p.r, -p.r);
+            LpVec<T>::pairs(v[u], [&](float va, float vb) {
+                const uint64_t d = fma2(pack2(va, vb), c2, r2);
+                float da, db;
+                unpack2(d, da, db);
+                const uint64_t e = pack2(ex2(da), ex2(db));
+                s2 = add2(s2, e);
+                t2 = fma2(e, d, t2);
+            });
+        }
+    }
+    {
+        float sa, sb, ta, tb;
+        unpack2(s2, sa, sb);
+        unpack2(t2, ta, tb);
+        p.s = sa + sb;
+        p.t = ta + tb;
+    }
+    if (TOP) sup[tid] = p.m == -INFINITY ? 0u : ordered_bits(p.m);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const LpPart q{__shfl_xor_sync(0xFFFFFFFFu, p.m, o), __shfl_xor_sync(0xFFFFFFFFu, p.r, o), __shfl_xor_sync(0xFFFFFFFFu, p.s, o), __shfl_xor_sync(0xFFFFFFFFu, p.t, o)};
+        p = lane & o ? lp_join(q, p) : lp_join(p, q);           // (the same order in both lanes: the same bits)
+    }
+    if (lane == 0) part[warp] = p;
     __syncthreads();
-    s = t = 0.f;
-    for (int i = 0; i < 8; ++i) { s += red[1][i]; t += red[2][i]; }
-    const bool none = m == -INFINITY && s == 0.f, bad = !(s == s) || m == INFINITY;
-    const float nan = __uint_as_float(0x7FFFFFFFu);
-    const float log_s = logf(s);
-    const float log_z = bad ? nan : (none ? -INFINITY : ref + log_s);
-    auto lp = [&](float zi) { return bad ? nan : (none || zi == -INFINITY ? -INFINITY : (zi - ref) - log_s); };
+    if (warp == 0) {
+        p = part[0];
+        for (int i = 1; i < kWarps; ++i) p = lp_join(p, part[i]);
+    }
+
+    // ---- this block's K best logits, largest first ----
+    unsigned long long* mine_best = best + rank * kLpMaxTop;    // (in the first block's table, this block's place)
+    if (TOP) {
+        const int K = a.top, n = ch1 - ch0;
+        for (int i = tid; i < kLpMaxTop; i += kLpThreads) mine_best[i] = 0;
+        if (warp == 0) {                                        // the largest bound that K threads reach, or one that a few more do
+            uint32_t v[kWarps], hi = 0;
+#pragma unroll
+            for (int i = 0; i < kWarps; ++i) { v[i] = sup[lane + 32 * i]; hi = max(hi, v[i]); }
+            hi = __reduce_max_sync(0xFFFFFFFFu, hi) + 1;
+            uint32_t lo = 0;
+            while (hi - lo > 1) {
+                const uint32_t mid = lo + (hi - lo) / 2;
+                int k = 0;
+#pragma unroll
+                for (int i = 0; i < kWarps; ++i) k += v[i] >= mid;
+                k = __reduce_add_sync(0xFFFFFFFFu, k);
+                if (k >= K) {
+                    lo = mid;
+                    if (k <= K + 8) break;
+                } else {
+                    hi = mid;
+                }
+            }
+            if (lane == 0) bound = lo;
+        }
+        __syncthreads();
+        const uint32_t least = bound;
+        for (int i = tid; i < n; i += kLpThreads)
+            if (chunk_max[i] >= least) {
+                const int at = atomicAdd(&n_list, 1);
+                if (at < kLpList) list[at] = ch0 + i;
+            }
+        __syncthreads();
+        bool fits = n_list <= kLpList;
+        if (fits) {
+            for (int i = warp; i < n_list; i += kWarps) {
+                const uint4 v = x.load(list[i], lane);
+                const int i0 = x.first(list[i], lane);
+#pragma unroll
+                for (int j = 0; j < LpVec<T>::N; ++j) {
+                    const uint32_t o = ordered_bits(LpVec<T>::at(v, j));
+                    if (o >= least && i0 + j >= 0 && i0 + j < a.vocab) {
+                        const int at = atomicAdd(&n_cand, 1);
+                        if (at < kLpCand) cand[at] = order_key(o, i0 + j);
+                    }
+                }
+            }
+            __syncthreads();
+            fits = n_cand <= kLpCand;
+        }
+        if (fits) {
+            for (int i = tid; i < n_cand; i += kLpThreads) {
+                const unsigned long long key = cand[i];
+                int before = 0;
+                for (int j = 0; j < n_cand; ++j) before += cand[j] > key;
+                if (before < K) mine_best[before] = key;
+            }
+        } else {
+            // the K-th best chunk by (maximum, lower index), then K rounds over the chunks up to it
+            __shared__ unsigned long long chunk_bound;
+            __syncthreads();                                    // (everyone has seen that the tables did not do)
+            if (warp == 0) {
+                unsigned long long lo = 0, hi = ~0ull;          // K chunks reach lo (or all do), fewer reach hi
+                while (hi - lo > 1) {
+                    const unsigned long long mid = lo + (hi - lo) / 2;
+                    int k = 0;
+                    for (int i = lane; i < n; i += 32) k += order_key(chunk_max[i], i) >= mid;
+                    k = __reduce_add_sync(0xFFFFFFFFu, k);
+                    if (k >= K) lo = mid; else hi = mid;
+                    if (k == K) break;
+                }
+                if (lane == 0) { chunk_bound = lo; n_list = 0; }
+            }
+            __syncthreads();
+            for (int i = tid; i < n; i += kLpThreads)
+                if (order_key(chunk_max[i], i) >= chunk_bound) list[atomicAdd(&n_list, 1)] = ch0 + i;       // (K of them at most: keys are distinct)
+            __syncthreads();
+            const int held = n_list;
+            unsigned long long last = ~0ull;
+            for (int k = 0; k < K; ++k) {
+                unsigned long long b = 0;
+                for (int i = warp; i < held; i += kWarps) {
+                    const uint4 v = x.load(list[i], lane);
+                    const int i0 = x.first(list[i], lane);
+#pragma unroll
+                    for (int j = 0; j < LpVec<T>::N; ++j) {
+                        const unsigned long long key = order_key(ordered_bits(LpVec<T>::at(v, j)), i0 + j);
+                        if (i0 + j >= 0 && i0 + j < a.vocab && key < last && key > b) b = key;
+                    }
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    const unsigned long long q = __shfl_xor_sync(0xFFFFFFFFu, b, o);
+                    b = q > b ? q : b;
+                }
+                if (lane == 0) round_best[warp] = b;
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < kWarps; ++i) b = round_best[i] > b ? round_best[i] : b;
+                __syncthreads();
+                if (tid == 0) mine_best[k] = b;
+                last = b;
+                if (b == 0) break;
+            }
+        }
+        __syncthreads();
+    }
+
+    // ---- the cluster's results meet in its first block ----
+    if (C > 1) {
+        asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (rank != 0) {
+            if (TOP && tid < a.top)
+                asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(mapa_u32(smem_u32(mine_best + tid), 0)), "l"(mine_best[tid]) : "memory");
+            if (tid == 0) {
+                const uint32_t to = mapa_u32(smem_u32(&parts[rank]), 0);
+                asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to), "f"(p.m), "f"(p.r), "f"(p.s), "f"(p.t) : "memory");
+            }
+            __syncwarp();
+            asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+            return;
+        }
+        if (tid == 0) parts[0] = p;
+        __syncwarp();
+        cluster_sync_all();
+        p = parts[0];
+        for (int i = 1; i < C; ++i) p = lp_join(p, parts[i]);
+    } else {
+        if (tid == 0) parts[0] = p;
+        __syncthreads();
+        p = parts[0];
+    }
+
+    // ---- the row's numbers, the same in all threads ----
+    // Rows far from 0 (c x near the end of the range, or a maximum near what -infinity was raised to): summed once more, about the maximum itself.
+    // So are temperatures at which the raised -infinity would not vanish, or overflows.
+    const bool far = p.m > -INFINITY && p.m < INFINITY && (fabsf(p.m) * c > 1e37f || p.m < LpVec<T>::kFar || c > 1e6f || c * (LpVec<T>::kFar - LpVec<T>::kLow) < 1000.f);
+    const bool none = p.m == -INFINITY && p.s == p.s;
+    float log_s, entropy;                                       // log of the sum about the maximum
+    bool bad;
+    if (far) {
+        float s = 0.f, t = 0.f;
+        for (int i = tid; i < a.vocab; i += kLpThreads) {
+            const float d = (to_f32(x.x[i]) - p.m) * a.inv_t, e = expf(d);
+            s += e;
+            if (e > 0.f) t += e * d;
+        }
+        s = warp_sum(s);
+        t = warp_sum(t);
+        if (lane == 0) part[warp] = LpPart{0.f, 0.f, s, t};
+        __syncthreads();
+        s = t = 0.f;
+        for (int i = 0; i < kWarps; ++i) { s += part[i].s; t += part[i].t; }
+        bad = !(s <= 3.4e38f);
+        log_s = logf(s);
+        entropy = log_s - t / s;
+    } else {
+        constexpr float ln2 = 0.693147180559945309f;
+        bad = !(p.s <= 3.4e38f);
+        const float l = log2f(p.s);
+        log_s = ln2 * (l + fmaf(-p.m, c, p.r));
+        entropy = ln2 * (l - p.t / p.s);
+    }
+    const float log_z = fmaf(p.m, a.inv_t, log_s);
+    auto lp = [&](float v) { return bad ? nan : (none || v == -INFINITY ? -INFINITY : fmaf(v - p.m, a.inv_t, -log_s)); };
     if (tid == 0) {
-        if (a.logsumexp) a.logsumexp[row] = log_z;
-        if (a.entropy) a.entropy[row] = bad ? nan : (none ? 0.f : log_s - t / s);
+        if (a.logsumexp) a.logsumexp[row] = bad ? nan : (none ? -INFINITY : log_z);
+        if (a.entropy) a.entropy[row] = bad ? nan : (none ? 0.f : entropy);
     }
-    if (a.logprob)
-        for (int j = tid; j < a.given; j += 256) {
-            const long long at = (long long)row * a.given + j;
-            const long long k = a.wide ? reinterpret_cast<const long long*>(a.tokens)[at] : reinterpret_cast<const int*>(a.tokens)[at];
-            a.logprob[at] = k < 0 ? 0.f : (k >= a.vocab ? nan : lp(z((int)k)));
+    for (int j = tid; j < a.given; j += kLpThreads) {
+        if (j >= kLpThreads) {
+            token = token_at(j);
+            token_x = token >= 0 && token < a.vocab ? to_f32(x.x[token]) : 0.f;
         }
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < a.top; ++k) {
-        unsigned long long b = 0;
-        for (int i = tid; i < a.vocab && !bad; i += 256) {
-            const unsigned long long key = order_key(to_f32(x[i]), i);
-            if (key < last && key > b) b = key;
+        a.logprob[(long long)row * a.given + j] = token < 0 ? 0.f : (token >= a.vocab ? nan : lp(token_x));
+    }
+    if (TOP) {
+        // lists of falling keys: a key's place is its own plus the keys of the other lists before it
+        for (int i = tid; i < C * kLpMaxTop; i += kLpThreads) {
+            const int own = i / kLpMaxTop, at = i % kLpMaxTop;
+            if (at >= a.top) continue;
+            const unsigned long long key = best[i];
+            if (key == 0) continue;
+            int place = at;
+            for (int o = 0; o < C; ++o) {
+                if (o == own) continue;
+                int lo = 0, hi = a.top;
+                while (lo < hi) {
+                    const int mid = (lo + hi) / 2;
+                    if (best[o * kLpMaxTop + mid] > key) lo = mid + 1; else hi = mid;
+                }
+                place += lo;
+            }
+            if (place < a.top) {
+                const long long to = (long long)row * a.top + place;
+                a.top_ids[to] = bad ? -1 : (int)~(uint32_t)key;
+                a.top_logprobs[to] = lp(from_ordered((uint32_t)(key >> 32)));
+            }
         }
-        for (int o = 16; o > 0; o >>= 1) {
-            const unsigned long long other = __shfl_xor_sync(0xFFFFFFFFu, b, o);
-            b = other > b ? other : b;
-        }
-        if (lane == 0) best[warp] = b;
-        __syncthreads();
-        for (int i = 0; i < 8; ++i) b = best[i] > b ? best[i] : b;
-        __syncthreads();
-        last = b;
-        if (tid == 0) {
-            const int id = bad ? -1 : (int)~(uint32_t)b;
-            a.top_ids[(long long)row * a.top + k] = id;
-            a.top_logprobs[(long long)row * a.top + k] = bad ? nan : lp(z(id));
+        if (bad && tid < a.top) {                               // (keys of NaN are no order)
+            a.top_ids[(long long)row * a.top + tid] = -1;
+            a.top_logprobs[(long long)row * a.top + tid] = nan;
         }
     }
 }

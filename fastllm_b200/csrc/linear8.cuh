@@ -20,40 +20,56 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 // x * (127 / a) in f32 is off by at most 127 * 2^-23 = 1.5e-5, so only quotients that lie within 1e-4 of a half need the exact sign of
 // 254 x - (2 low + 1) a, which 64 bits hold without rounding.
 struct RowScale {
-    float a, mul, up;       // max |x| times `up`; 127 / a; a power of two that keeps 127 / a finite for the smallest rows
+    float a, mul, up;       // max |x|; 127 / a (0: all q are 0); 1, or a power of two that keeps 127 / (a up) finite in the smallest rows
     float scale;            // a / 127; NaN for a row with a NaN or an infinity
     __device__ explicit RowScale(uint32_t max_bits) {
-        const float most = __uint_as_float(max_bits);
+        a = __uint_as_float(max_bits);
         const bool bad = max_bits >= 0x7F800000u;
-        up = most < 1e-30f ? 0x1p96f : 1.f;
-        a = most * up;
-        mul = bad || most == 0.f ? 0.f : 127.f / a;
-        scale = bad ? __uint_as_float(0x7FFFFFFFu) : most / 127.f;
+        up = a < 1e-30f ? 0x1p96f : 1.f;
+        mul = bad || a == 0.f ? 0.f : 127.f / (a * up);
+        scale = bad ? __uint_as_float(0x7FFFFFFFu) : a / 127.f;
     }
-    __device__ int operator()(float x) const {
-        if (mul == 0.f) return 0;
-        x *= up;
-        const float v = x * mul, n = rintf(v);
-        if (fabsf(v - n) < 0.4999f) return (int)n;
-        const float low = floorf(v);
+    static __device__ __noinline__ uint32_t exact(float x, float mul, float a) {
+        const float low = floorf(x * mul);
         const double over = fma(254.0, (double)x, -(2.0 * (double)low + 1.0) * (double)a);
         const int l = (int)low;
-        return over > 0.0 ? l + 1 : (over < 0.0 ? l : l + (l & 1));
+        return (uint32_t)(over > 0.0 ? l + 1 : (over < 0.0 ? l : l + (l & 1)));
+    }
+    // four values, packed.  1.5 * 2^23 leaves the nearest whole number in the sum's low bits.
+    __device__ __forceinline__ uint32_t four(float x0, float x1, float x2, float x3) const {
+        constexpr float kBig = 12582912.f;
+        if (mul == 0.f) return 0u;                                  // (the same for the whole row)
+        const float x[4] = {x0, x1, x2, x3};
+        float far = up != 1.f ? 1.f : 0.f;
+        uint32_t b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float t = fmaf(x[i], mul, kBig);
+            b[i] = __float_as_uint(t);
+            far = fmaxf(far, fabsf(fmaf(x[i], mul, kBig - t)));
+        }
+        if (far > 0.4999f) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] = exact(x[i] * up, mul, a * up);
+        }
+        return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     }
 };
 // larger for every NaN than for an infinity, and for that than for any number
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// A block per row; columns [cols, cols_q) of q are filled with zeros.  kVecs > 0: the row starts on 16-byte borders on both sides (8 for q) and has at
+// A block per row; columns [cols, cols_q) of q are filled with zeros, and so are the `zeros` words that the kernel behind counts in.  kVecs > 0: the row starts on 16-byte borders on both sides (8 for q) and has at
 // most 256 * kVecs vectors of 16 bytes, which stay in registers between the maximum and the rounding; 0: any row, read twice.
 template <typename T, int kVecs>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, long long ldx, int cols, int8_t* __restrict__ q, long long ldq, int cols_q,
-                                                            float* __restrict__ scale) {
+                                                            float* __restrict__ scale, int* __restrict__ zero, int zeros) {
     constexpr int V = 16 / sizeof(T);
     __shared__ uint32_t part[8];
     const T* xr = x + (long long)blockIdx.x * ldx;
     int8_t* qr = q + (long long)blockIdx.x * ldq;
     pdl_launch_dependents();
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i < zeros; i += 256) zero[i] = 0;
     uint32_t m = 0;
     uint4 held[kVecs > 0 ? kVecs : 1];
     if constexpr (kVecs > 0) {
@@ -71,9 +87,16 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
         }
 #pragma unroll
         for (int u = 0; u < kVecs; ++u) {
-            const T* e = reinterpret_cast<const T*>(&held[u]);
-#pragma unroll
-            for (int j = 0; j < V; ++j) m = max(m, abs_bits(to_f32(e[j])));
+            if constexpr (sizeof(T) == 4) {
+                m = max(max(m, max(held[u].x & 0x7FFFFFFFu, held[u].y & 0x7FFFFFFFu)), max(held[u].z & 0x7FFFFFFFu, held[u].w & 0x7FFFFFFFu));
+            } else {                                            // two magnitudes at once: their bits are in the order of their sizes
+                const uint32_t w = __vmaxu2(__vmaxu2(held[u].x & 0x7FFF7FFFu, held[u].y & 0x7FFF7FFFu), __vmaxu2(held[u].z & 0x7FFF7FFFu, held[u].w & 0x7FFF7FFFu));
+                m = __vmaxu2(m, w);
+            }
+        }
+        if constexpr (sizeof(T) == 2) {
+            const uint16_t h = (uint16_t)max(m & 0xFFFFu, m >> 16);
+            m = abs_bits(to_f32(*reinterpret_cast<const T*>(&h)));
         }
     } else {
         for (int i = threadIdx.x; i < cols; i += 256) m = max(m, abs_bits(to_f32(xr[i])));
@@ -92,11 +115,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
             const T* e = reinterpret_cast<const T*>(&held[u]);
             uint32_t w[V / 4];
 #pragma unroll
-            for (int i = 0; i < V / 4; ++i) {
-                w[i] = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) w[i] |= (uint32_t)(uint8_t)(int8_t)rs(to_f32(e[4 * i + j])) << (8 * j);
-            }
+            for (int i = 0; i < V / 4; ++i) w[i] = rs.four(to_f32(e[4 * i]), to_f32(e[4 * i + 1]), to_f32(e[4 * i + 2]), to_f32(e[4 * i + 3]));
             if (at + V <= cols_q) {
                 if constexpr (V == 8) *reinterpret_cast<uint2*>(qr + at) = make_uint2(w[0], w[1]);
                 else *reinterpret_cast<uint32_t*>(qr + at) = w[0];
@@ -105,7 +124,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
             }
         }
     } else {
-        for (int i = threadIdx.x; i < cols_q; i += 256) qr[i] = i < cols ? (int8_t)rs(to_f32(xr[i])) : (int8_t)0;
+        for (int i = threadIdx.x; i < cols_q; i += 256) qr[i] = i < cols ? (int8_t)rs.four(to_f32(xr[i]), 0.f, 0.f, 0.f) : (int8_t)0;
     }
     if (threadIdx.x == 0) scale[blockIdx.x] = rs.scale;
 }
@@ -149,10 +168,46 @@ __device__ __forceinline__ void umma_i8_pair_warp(uint32_t tmem_d, uint64_t ades
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void l8_store(const Linear8Args& g, long long at, float v) {
-    if (g.y_dtype == 0) reinterpret_cast<float*>(g.y)[at] = v;
-    else if (g.y_dtype == 1) reinterpret_cast<__nv_bfloat16*>(g.y)[at] = from_f32<__nv_bfloat16>(v);
-    else reinterpret_cast<__half*>(g.y)[at] = from_f32<__half>(v);
+// Results of one weight row n (a lane each) and 16 activation rows r, r + 1, ..: for a fixed row the 32 lanes write 32 neighbours.  16-bit results go in twos
+// where rows start on even places (`twos`): neighbouring lanes exchange a value, even lanes write row r + j and odd ones r + j + 1.
+__device__ __forceinline__ void l8_store16(const Linear8Args& g, int r, int n, float wsn, float bn, const int (&sum)[16], bool twos) {
+    const int lane = threadIdx.x & 31;
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        v[j] = (float)sum[j] * __ldg(g.xs + min(r + j, g.rows - 1)) * wsn;
+        if (g.bias != nullptr) v[j] += bn;
+    }
+    if (g.y_dtype == 0) {
+        float* o = reinterpret_cast<float*>(g.y) + (long long)r * g.ldy + n;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (r + j < g.rows && n < g.n) o[j * g.ldy] = v[j];
+        return;
+    }
+    auto half = [&](float a, float b) {
+        if (g.y_dtype == 1) return pack_bf16x2(a, b);
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    };
+    uint16_t* o = reinterpret_cast<uint16_t*>(g.y) + (long long)r * g.ldy + n;
+    if (twos) {
+        const bool odd = lane & 1;
+        o -= odd;
+#pragma unroll
+        for (int j = 0; j < 16; j += 2) {
+            const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[j] : v[j + 1], 1);
+            const uint32_t w = odd ? half(got, v[j + 1]) : half(v[j], got);
+            if (r + j + odd < g.rows && n < g.n) *reinterpret_cast<uint32_t*>(o + (j + odd) * g.ldy) = w;      // (g.n is even: both or none)
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+        const uint32_t w = half(v[j], v[j + 1]);
+        if (r + j < g.rows && n < g.n) o[j * g.ldy] = (uint16_t)w;
+        if (r + j + 1 < g.rows && n < g.n) o[(j + 1) * g.ldy] = (uint16_t)(w >> 16);
+    }
 }
 // A wait ran out: report it and leave the copies in flight time to land; the block goes on to its end.
 __device__ __forceinline__ void l8_give_up(int* failed) {
@@ -176,7 +231,7 @@ template <int BN> struct L8Few {
 
 template <int BN>
 __global__ void __launch_bounds__(L8Few<BN>::kThreads, L8Few<BN>::kPerSm)
-linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Linear8Args g, const int S) {
+linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Linear8Args g, const int S, const bool twos) {
     using L = L8Few<BN>;
     constexpr int kStages = L::kStages;
     extern __shared__ uint8_t gsm_raw[];
@@ -248,21 +303,16 @@ linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         tc_fence_after();
     }
     const float wsn = warp >= 2 && n < g.n ? g.ws[n] : 0.f, bn = warp >= 2 && g.bias != nullptr && n < g.n ? g.bias[n] : 0.f;
-    auto store = [&](int c, int sum) {                                                 // for a fixed column the 32 lanes write 32 neighbours of one row
-        const int r = r0 + c;
-        if (r >= g.rows || n >= g.n) return;
-        float v = (float)sum * g.xs[r] * wsn;
-        if (g.bias != nullptr) v += bn;
-        l8_store(g, (long long)r * g.ldy + n, v);
-    };
     if (S == 1) {
         if (warp >= 2 && ok) {
 #pragma unroll 1
             for (int c = 0; c < BN && r0 + c < g.rows; c += 16) {
                 uint32_t v[16];
+                int sum[16];
                 tmem_ld16(at + (uint32_t)c, v);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) store(c + j, (int)v[j]);
+                for (int j = 0; j < 16; ++j) sum[j] = (int)v[j];
+                l8_store16(g, r0 + c, n, wsn, bn, sum, twos);
             }
         }
     } else {
@@ -286,10 +336,17 @@ linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         cluster_sync_all();
         if (warp >= 2 && ok) {
             const int* part = reinterpret_cast<const int*>(gsm) + row;
-            for (int c = 0; c < per && r0 + s * per + c < g.rows; ++c) {
+            for (int c = 0; c < per && r0 + s * per + c < g.rows; ++c) {               // (few columns: BN / S)
                 int sum = 0;
                 for (int t = 0; t < S; ++t) sum += part[(t * per + c) * 128];
-                store(s * per + c, sum);
+                const int r = r0 + s * per + c;
+                if (n >= g.n) continue;
+                float v = (float)sum * g.xs[r] * wsn;
+                if (g.bias != nullptr) v += bn;
+                const long long at_y = (long long)r * g.ldy + n;
+                if (g.y_dtype == 0) reinterpret_cast<float*>(g.y)[at_y] = v;
+                else if (g.y_dtype == 1) reinterpret_cast<__nv_bfloat16*>(g.y)[at_y] = from_f32<__nv_bfloat16>(v);
+                else reinterpret_cast<__half*>(g.y)[at_y] = from_f32<__half>(v);
             }
         }
     }
@@ -304,53 +361,32 @@ linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
 }
 
 // ---- many rows ----------------------------------------------------------------------------------------------------------------------
-// Pairs of SMs on 256 x bn tiles (tcgen05.mma.cta_group::2): each holds its 128 activation rows and half of the weight tile.
+// Pairs of SMs on tiles of 256 weight rows x bn activation rows (tcgen05.mma.cta_group::2): each holds its 128 weight rows and half of the activation
+// tile.  bn is any multiple of 32, so that a row count is cut without much padding.  Tiles that do not fill a wave are cut along K, evenly over all
+// pairs: a part of a tile goes to the workspace, the last of its parts to arrive adds the others to its own and writes the results (nobody
+// waits for anybody, and the order does not matter for whole numbers).
 constexpr int kL8PairStages = 6, kL8PairEpi = 16, kL8PairThreads = 64 + 32 * kL8PairEpi;
 constexpr uint32_t kL8PairStage = 2 * kL8WBytes;
 constexpr size_t kL8PairSmem = (size_t)kL8PairStages * kL8PairStage + 1024;
 
-// 16 outputs of one row; whole: 32-byte stores are allowed
-__device__ __forceinline__ void l8_store16(const Linear8Args& g, int row, int col, const float (&v)[16], bool whole) {
-    if (whole && col + 16 <= g.n) {
-        if (g.y_dtype == 0) {
-            float* o = reinterpret_cast<float*>(g.y) + (long long)row * g.ldy + col;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t w[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = __float_as_uint(v[8 * h + j]);
-                st_global_32b(o + 8 * h, w);
-            }
-        } else {
-            uint32_t w[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (g.y_dtype == 1) {
-                    w[j] = pack_bf16x2(v[2 * j], v[2 * j + 1]);
-                } else {
-                    const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-                    w[j] = *reinterpret_cast<const uint32_t*>(&h);
-                }
-            }
-            st_global_32b(reinterpret_cast<uint16_t*>(g.y) + (long long)row * g.ldy + col, w);
-        }
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-        if (col + j < g.n) l8_store(g, (long long)row * g.ldy + col + j, v[j]);
-}
+struct L8Pair {
+    int bn, nk, mt, nt;         // activation rows of a tile; k blocks; weight and activation tiles
+    int clusters, full, L;      // pairs at work; whole tiles per pair; then k blocks per pair of the tiles that are left
+    int* parts;                 // [cluster][first | second tile of its range][CTA][bn][128]
+    int* tickets;               // [2 * tiles left], zero
+};
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kL8PairThreads, 1)
-linear8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const Linear8Args g, const int bn, const bool whole) {
+linear8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Linear8Args g, const L8Pair p, const bool twos) {
     extern __shared__ uint8_t gsm_raw[];
     uint8_t* gsm = gsm_raw + ((1024u - (smem_u32(gsm_raw) & 1023u)) & 1023u);          // (the same offset in both CTAs)
     __shared__ __align__(8) uint64_t full[kL8PairStages], empty[kL8PairStages], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_base_s;
+    __shared__ int s_last;
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
-    const int cl = blockIdx.x >> 1, G = gridDim.x >> 1;
-    const int nk = (g.k + kL8BK - 1) / kL8BK, mp = (g.rows + 255) / 256, nt = (g.n + bn - 1) / bn, T = mp * nt;
+    const int cl = blockIdx.x >> 1, G = gridDim.x >> 1, nk = p.nk, T = p.mt * p.nt, bn = p.bn;
+    const int left0 = p.full * G, units = (T - left0) * nk;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kL8PairStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
@@ -368,12 +404,29 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_s;
-    // 8 pair rows share a weight tile before the walk moves on (see kGemmRasterRows)
-    auto place = [&](int tile, int& m, int& n) {
+
+    // This pair's work in order: whole tiles cl, cl + G, ..., then its run of k blocks of the tiles that are left.
+    // -> false at the end; tile, [kb0, kb1)
+    struct Walk { int seg = 0, u = 0; };
+    const int u1 = min((cl + 1) * p.L, units);
+    auto next = [&](Walk& w, int& tile, int& kb0, int& kb1) {
+        if (w.seg < p.full) {
+            tile = cl + w.seg * G; kb0 = 0; kb1 = nk;
+        } else {
+            if (w.seg == p.full) w.u = cl * p.L;
+            if (w.u >= u1) return false;
+            tile = left0 + w.u / nk; kb0 = w.u % nk; kb1 = min(nk, kb0 + u1 - w.u);
+            w.u += kb1 - kb0;
+        }
+        ++w.seg;
+        return true;
+    };
+    // 8 activation tiles share a weight tile before the walk moves on (see kGemmRasterRows)
+    auto place = [&](int tile, int& n, int& r) {
         constexpr int RM = kGemmRasterRows / 2;
-        const int per = RM * nt, first = tile / per * RM, local = tile % per, cnt = min(RM, mp - first);
-        m = (first + local % cnt) * 256 + (int)rank * 128;
-        n = local / cnt * bn;
+        const int per = RM * p.mt, first = tile / per * RM, local = tile % per, cnt = min(RM, p.nt - first);
+        r = (first + local % cnt) * bn;
+        n = local / cnt * 256 + (int)rank * 128;
     };
     const uint32_t tx = 2 * (kL8WBytes + (uint32_t)bn / 2 * kL8BK);                    // bytes of a stage in both CTAs
     bool ok = true;
@@ -382,17 +435,18 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
         if (lane == 0) {
             pdl_wait();
             asm volatile("fence.proxy.async;" ::: "memory");
-            int st = 0;
+            Walk w;
+            int tile, kb0, kb1, st = 0;
             uint32_t ph = 1;
-            for (int tile = cl; ok && tile < T; tile += G) {
-                int m0, n0;
-                place(tile, m0, n0);
-                for (int kb = 0; kb < nk; ++kb) {
+            while (ok && next(w, tile, kb0, kb1)) {
+                int n0, r0;
+                place(tile, n0, r0);
+                for (int kb = kb0; kb < kb1; ++kb) {
                     if (!(ok = pair_wait(&empty[st], ph))) break;
                     if (rank == 0) mbar_expect_tx(&full[st], tx);                      // both CTAs' loads complete on the first one's barrier
                     const uint32_t bar = mapa_u32(smem_u32(&full[st]), 0), sa = smem_u32(gsm) + st * kL8PairStage;
-                    tma_load_2d_pair(sa, &tmX, kb * kL8BK, m0, bar);
-                    tma_load_2d_pair(sa + kL8WBytes, &tmW, kb * kL8BK, n0 + (int)rank * (bn >> 1), bar);
+                    tma_load_2d_pair(sa, &tmW, kb * kL8BK, n0, bar);
+                    tma_load_2d_pair(sa + kL8WBytes, &tmX, kb * kL8BK, r0 + (int)rank * (bn >> 1), bar);
                     if (++st == kL8PairStages) { st = 0; ph ^= 1; }
                 }
             }
@@ -401,54 +455,85 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_consta
         if (rank == 0) {
             const uint32_t idesc = umma_idesc_i8(256, bn);
             const uint64_t base = umma_smem_desc_sw128(gsm);
-            int st = 0;
+            Walk w;
+            int tile, kb0, kb1, st = 0;
             uint32_t ph = 0, seg = 0;
             auto wait = [&](uint64_t* bar, uint32_t parity) {
                 if (ok) ok = pair_wait(bar, parity);
                 __syncwarp();
                 tc_fence_after();
             };
-            for (int tile = cl; tile < T; tile += G, ++seg) {
+            while (next(w, tile, kb0, kb1)) {
                 const uint32_t as = seg & 1, tacc = tmem_base + as * 256;
                 wait(&acc_empty[as], ((seg >> 1) & 1) ^ 1);
-                for (int kb = 0; kb < nk; ++kb) {
+                for (int kb = kb0; kb < kb1; ++kb) {
                     wait(&full[st], ph);
                     const uint64_t a = base + (uint64_t)(st * (kL8PairStage >> 4)), b = a + (kL8WBytes >> 4);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) umma_i8_pair_warp(tacc, a + 2 * q, b + 2 * q, idesc, (kb | q) ? 1u : 0u);
+                    for (int q = 0; q < 4; ++q) umma_i8_pair_warp(tacc, a + 2 * q, b + 2 * q, idesc, ((kb - kb0) | q) ? 1u : 0u);
                     umma_commit_pair_warp(&empty[st]);
                     if (++st == kL8PairStages) { st = 0; ph ^= 1; }
                 }
                 umma_commit_pair_warp(&acc_full[as]);
+                ++seg;
             }
         }
     } else {
-        const int q = warp & 3, cs = (warp - 2) >> 2, cols = bn >> 2;                  // TMEM lane quarter (hardware rule); a quarter of the columns
+        const int q = warp & 3, cs = (warp - 2) >> 2, lrow = q * 32 + lane;            // TMEM lane quarter (hardware rule); every fourth run of 16 columns
+        Walk w;
+        int tile, kb0, kb1;
         uint32_t seg = 0;
         pdl_wait();                                                                    // (the rows' scales)
-        for (int tile = cl; tile < T; tile += G, ++seg) {
-            int m0, n0;
-            place(tile, m0, n0);
+        while (next(w, tile, kb0, kb1)) {                                              // (to the end even behind a wait that ran out: the warps meet at barriers)
+            int n0, r0;
+            place(tile, n0, r0);
             const uint32_t as = seg & 1;
             if (ok) ok = __all_sync(0xFFFFFFFFu, pair_wait(&acc_full[as], (seg >> 1) & 1));
+            ++seg;
             tc_fence_after();
             const uint32_t at = tmem_base + as * 256 + ((uint32_t)(q * 32) << 16);
-            const int row = m0 + q * 32 + lane;
-            const float xs = row < g.rows ? g.xs[row] : 0.f;
-            if (ok) {
+            const int n = n0 + lrow, last_col = min(bn, g.rows - r0);
+            const bool whole = kb0 == 0 && kb1 == nk;
+            const int left = tile - left0;                                             // (of a tile that is left)
+            auto part_of = [&](int c) { return p.parts + (size_t)((c * 2 + left - c * p.L / nk) * 2 + (int)rank) * bn * 128 + lrow; };
+            bool store = whole;
+            int c0 = 0, c1 = -1;
+            if (!whole) {
+                c0 = left * nk / p.L; c1 = ((left + 1) * nk - 1) / p.L;
+                int* part = part_of(cl);
 #pragma unroll 1
-                for (int c = cs * cols; c < (cs + 1) * cols && n0 + c < g.n; c += 16) {
-                    uint32_t a[16];
-                    float v[16];
-                    tmem_ld16(at + (uint32_t)c, a);
+                for (int c = cs * 16; ok && c < last_col; c += 64) {
+                    uint32_t v[16];
+                    tmem_ld16(at + (uint32_t)c, v);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int n = min(n0 + c + j, g.n - 1);
-                        v[j] = (float)(int)a[j] * xs * __ldg(g.ws + n);
-                        if (g.bias != nullptr) v[j] += __ldg(g.bias + n);
+                    for (int j = 0; j < 16; ++j) part[(size_t)(c + j) * 128] = (int)v[j];
+                }
+                __threadfence();
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * kL8PairEpi) : "memory");
+                if (threadIdx.x == 64 && ok) {
+                    __threadfence();
+                    s_last = atomicAdd(p.tickets + 2 * left + (int)rank, 1) == c1 - c0;
+                    __threadfence();
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * kL8PairEpi) : "memory");
+                store = s_last != 0;
+            }
+            if (store && ok) {
+                const float wsn = n < g.n ? __ldg(g.ws + n) : 0.f, bias = g.bias != nullptr && n < g.n ? __ldg(g.bias + n) : 0.f;
+#pragma unroll 1
+                for (int c = cs * 16; c < last_col; c += 64) {
+                    uint32_t v[16];
+                    int sum[16];
+                    tmem_ld16(at + (uint32_t)c, v);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) sum[j] = (int)v[j];
+                    for (int o = c0; o <= c1; ++o) {
+                        if (o == cl) continue;
+                        const int* part = part_of(o) + (size_t)c * 128;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) sum[j] += __ldcg(part + j * 128);
                     }
-                    if (row < g.rows) l8_store16(g, row, n0 + c, v, whole);
-                    __syncwarp();
+                    l8_store16(g, r0 + c, n, wsn, bias, sum, twos);
                 }
             }
             tc_fence_before();

@@ -17,7 +17,7 @@ namespace fl {
 
 constexpr int kLpMaxTop = 32;
 constexpr int kLpMaxVocab = 1 << 20;
-constexpr int kLpThreads = 256, kLpMaxCluster = 16;
+constexpr int kLpMaxCluster = 16;
 constexpr int kLpList = 96, kLpCand = 256;          // chunks that are read again, logits that are ranked
 
 struct LogprobArgs {
@@ -166,18 +166,49 @@ template <typename T> struct LpRow {
 };
 
 struct __align__(16) LpPart { float m, r, s, t; };     // largest x; reference; sum of e; sum of e (c x - r)
-__device__ __forceinline__ LpPart lp_join(const LpPart& a, const LpPart& b) {
-    const float r = fmaxf(a.r, b.r), fa = ex2(a.r - r), fb = ex2(b.r - r);
-    return LpPart{fmaxf(a.m, b.m), r, a.s * fa + b.s * fb, (a.t + a.s * (a.r - r)) * fa + (b.t + b.s * (b.r - r)) * fb};
+// n of them as one, about the largest reference
+__device__ __forceinline__ LpPart lp_join(const LpPart* part, int n) {
+    LpPart p = part[0];
+    for (int i = 1; i < n; ++i) { p.m = fmaxf(p.m, part[i].m); p.r = fmaxf(p.r, part[i].r); }
+    p.s = p.t = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        const LpPart q = part[i];
+        const float f = ex2(q.r - p.r);
+        p.s += q.s * f;
+        p.t += (q.t + q.s * (q.r - p.r)) * f;
+    }
+    return p;
+}
+__device__ __forceinline__ LpPart lp_join_warp(LpPart p) {
+    const float r = warp_max(p.r), f = ex2(p.r - r);
+    p.t = warp_sum((p.t + p.s * (p.r - r)) * f);
+    p.s = warp_sum(p.s * f);
+    p.r = r;
+    p.m = warp_max(p.m);
+    return p;
+}
+// how many of the keys lie before `key`; n a multiple of 8 (zeros fill it up)
+__device__ __forceinline__ int lp_place(const unsigned long long* keys, int n, unsigned long long key) {
+    int before = 0;
+    for (int j = 0; j < n; j += 8) {
+        ulonglong2 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const ulonglong2*>(keys + j + 2 * i);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) before += (v[i].x > key) + (v[i].y > key);
+    }
+    return before;
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobArgs a, const int C) {
-    constexpr int kWarps = kLpThreads / 32, U = 4;
+template <typename T, bool TOP, int kThreads>
+__global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a, const int C) {
+    constexpr int kWarps = kThreads / 32, U = 4;
     extern __shared__ uint32_t chunk_max[];                     // TOP: ordered maxima of this block's chunks
     __shared__ LpPart part[kWarps], parts[kLpMaxCluster];
-    __shared__ uint32_t sup[TOP ? kLpThreads : 1];
-    __shared__ unsigned long long cand[TOP ? kLpCand : 1], best[TOP ? kLpMaxCluster * kLpMaxTop : 1], round_best[TOP ? kWarps : 1];
+    __shared__ uint32_t sup[TOP ? kThreads : 1];
+    __shared__ __align__(16) unsigned long long cand[TOP ? kLpCand : 1], best[TOP ? kLpMaxCluster * kLpMaxTop : 1];
+    __shared__ unsigned long long round_best[TOP ? kWarps : 1];
     __shared__ int list[TOP ? kLpList : 1];
     __shared__ int n_list, n_cand;
     __shared__ uint32_t bound;
@@ -247,47 +278,42 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobArgs 
         p.t = ta + tb;
     }
     if (TOP) sup[tid] = p.m == -INFINITY ? 0u : ordered_bits(p.m);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const LpPart q{__shfl_xor_sync(0xFFFFFFFFu, p.m, o), __shfl_xor_sync(0xFFFFFFFFu, p.r, o), __shfl_xor_sync(0xFFFFFFFFu, p.s, o), __shfl_xor_sync(0xFFFFFFFFu, p.t, o)};
-        p = lane & o ? lp_join(q, p) : lp_join(p, q);           // (the same order in both lanes: the same bits)
-    }
+    p = lp_join_warp(p);
     if (lane == 0) part[warp] = p;
     __syncthreads();
-    if (warp == 0) {
-        p = part[0];
-        for (int i = 1; i < kWarps; ++i) p = lp_join(p, part[i]);
-    }
 
     // ---- this block's K best logits, largest first ----
-    unsigned long long* mine_best = best + rank * kLpMaxTop;    // (in the first block's table, this block's place)
+    const int K = a.top;
+    unsigned long long* mine_best = best + rank * K;            // (in the first block's table, this block's place)
     if (TOP) {
-        const int K = a.top, n = ch1 - ch0;
-        for (int i = tid; i < kLpMaxTop; i += kLpThreads) mine_best[i] = 0;
-        if (warp == 0) {                                        // the largest bound that K threads reach, or one that a few more do
-            uint32_t v[kWarps], hi = 0;
+        const int n = ch1 - ch0;
+        for (int i = tid; i < K; i += kThreads) mine_best[i] = 0;
+        if (warp == 0) {                                        // the K-th largest thread maximum: the lanes' sorted shares, K times the largest head
+            uint32_t v[kWarps];
 #pragma unroll
-            for (int i = 0; i < kWarps; ++i) { v[i] = sup[lane + 32 * i]; hi = max(hi, v[i]); }
-            hi = __reduce_max_sync(0xFFFFFFFFu, hi) + 1;
-            uint32_t lo = 0;
-            while (hi - lo > 1) {
-                const uint32_t mid = lo + (hi - lo) / 2;
-                int k = 0;
+            for (int i = 0; i < kWarps; ++i) v[i] = sup[lane + 32 * i];
 #pragma unroll
-                for (int i = 0; i < kWarps; ++i) k += v[i] >= mid;
-                k = __reduce_add_sync(0xFFFFFFFFu, k);
-                if (k >= K) {
-                    lo = mid;
-                    if (k <= K + 8) break;
-                } else {
-                    hi = mid;
+            for (int i = 0; i < kWarps - 1; ++i)
+#pragma unroll
+                for (int j = 0; j < kWarps - 1 - i; ++j) {
+                    const uint32_t x0 = max(v[j], v[j + 1]), x1 = min(v[j], v[j + 1]);
+                    v[j] = x0; v[j + 1] = x1;
+                }
+            uint32_t least = 0;
+            for (int k = 0; k < K; ++k) {
+                least = __reduce_max_sync(0xFFFFFFFFu, v[0]);
+                const uint32_t who = __ballot_sync(0xFFFFFFFFu, v[0] == least);
+                if (lane == __ffs(who) - 1) {
+#pragma unroll
+                    for (int i = 0; i < kWarps - 1; ++i) v[i] = v[i + 1];
+                    v[kWarps - 1] = 0;
                 }
             }
-            if (lane == 0) bound = lo;
+            if (lane == 0) bound = least;
         }
         __syncthreads();
         const uint32_t least = bound;
-        for (int i = tid; i < n; i += kLpThreads)
+        for (int i = tid; i < n; i += kThreads)
             if (chunk_max[i] >= least) {
                 const int at = atomicAdd(&n_list, 1);
                 if (at < kLpList) list[at] = ch0 + i;
@@ -295,15 +321,22 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobArgs 
         __syncthreads();
         bool fits = n_list <= kLpList;
         if (fits) {
-            for (int i = warp; i < n_list; i += kWarps) {
-                const uint4 v = x.load(list[i], lane);
-                const int i0 = x.first(list[i], lane);
+            for (int i = warp; i < n_list; i += 4 * kWarps) {
+                uint4 v[4];
 #pragma unroll
-                for (int j = 0; j < LpVec<T>::N; ++j) {
-                    const uint32_t o = ordered_bits(LpVec<T>::at(v, j));
-                    if (o >= least && i0 + j >= 0 && i0 + j < a.vocab) {
-                        const int at = atomicAdd(&n_cand, 1);
-                        if (at < kLpCand) cand[at] = order_key(o, i0 + j);
+                for (int u = 0; u < 4; ++u)
+                    if (i + u * kWarps < n_list) v[u] = x.load(list[i + u * kWarps], lane);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (i + u * kWarps >= n_list) break;
+                    const int i0 = x.first(list[i + u * kWarps], lane);
+                    if (ordered_bits(LpVec<T>::max_of(v[u])) < least) continue;
+                    for (int j = 0; j < LpVec<T>::N; ++j) {
+                        const uint32_t o = ordered_bits(LpVec<T>::at(v[u], j));
+                        if (o >= least && i0 + j >= 0 && i0 + j < a.vocab) {
+                            const int at = atomicAdd(&n_cand, 1);
+                            if (at < kLpCand) cand[at] = order_key(o, i0 + j);
+                        }
                     }
                 }
             }
@@ -311,11 +344,12 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobArgs 
             fits = n_cand <= kLpCand;
         }
         if (fits) {
-            for (int i = tid; i < n_cand; i += kLpThreads) {
-                const unsigned long long key = cand[i];
-                int before = 0;
-                for (int j = 0; j < n_cand; ++j) before += cand[j] > key;
-                if (before < K) mine_best[before] = key;
+            const int held = n_cand, even = (held + 7) / 8 * 8;
+            if (tid < even - held) cand[held + tid] = 0;
+            __syncthreads();
+            for (int i = tid; i < held; i += kThreads) {
+                const int at = lp_place(cand, even, cand[i]);
+                if (at < K) mine_best[at] = cand[i];
             }
         } else {
             // the K-th best chunk by (maximum, lower index), then K rounds over the chunks up to it
@@ -334,7 +368,7 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobArgs 
                 if (lane == 0) { chunk_bound = lo; n_list = 0; }
             }
             __syncthreads();
-            for (int i = tid; i < n; i += kLpThreads)
+            for (int i = tid; i < n; i += kThreads)
                 if (order_key(chunk_max[i], i) >= chunk_bound) list[atomicAdd(&n_list, 1)] = ch0 + i;       // (K of them at most: keys are distinct)
             __syncthreads();
             const int held = n_list;
@@ -372,7 +406,8 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobArgs 
     if (C > 1) {
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (rank != 0) {
-            if (TOP && tid < a.top)
+            p = lp_join(part, kWarps);
+            if (TOP && tid < K)
                 asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(mapa_u32(smem_u32(mine_best + tid), 0)), "l"(mine_best[tid]) : "memory");
             if (tid == 0) {
                 const uint32_t to = mapa_u32(smem_u32(&parts[rank]), 0);
@@ -382,15 +417,15 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobArgs 
             asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
             return;
         }
-        if (tid == 0) parts[0] = p;
+        if (warp == 0) {
+            p = lp_join(part, kWarps);
+            if (lane == 0) parts[0] = p;
+        }
         __syncwarp();
         cluster_sync_all();
-        p = parts[0];
-        for (int i = 1; i < C; ++i) p = lp_join(p, parts[i]);
+        p = lp_join(parts, C);
     } else {
-        if (tid == 0) parts[0] = p;
-        __syncthreads();
-        p = parts[0];
+        p = lp_join(part, kWarps);
     }
 
     // ---- the row's numbers, the same in all threads ----
@@ -402,7 +437,7 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobArgs 
     bool bad;
     if (far) {
         float s = 0.f, t = 0.f;
-        for (int i = tid; i < a.vocab; i += kLpThreads) {
+        for (int i = tid; i < a.vocab; i += kThreads) {
             const float d = (to_f32(x.x[i]) - p.m) * a.inv_t, e = expf(d);
             s += e;
             if (e > 0.f) t += e * d;
@@ -429,32 +464,25 @@ __global__ void __launch_bounds__(kLpThreads) logprobs_kernel(const LogprobArgs 
         if (a.logsumexp) a.logsumexp[row] = bad ? nan : (none ? -INFINITY : log_z);
         if (a.entropy) a.entropy[row] = bad ? nan : (none ? 0.f : entropy);
     }
-    for (int j = tid; j < a.given; j += kLpThreads) {
-        if (j >= kLpThreads) {
+    for (int j = tid; j < a.given; j += kThreads) {
+        if (j >= kThreads) {
             token = token_at(j);
             token_x = token >= 0 && token < a.vocab ? to_f32(x.x[token]) : 0.f;
         }
         a.logprob[(long long)row * a.given + j] = token < 0 ? 0.f : (token >= a.vocab ? nan : lp(token_x));
     }
     if (TOP) {
-        // lists of falling keys: a key's place is its own plus the keys of the other lists before it
-        for (int i = tid; i < C * kLpMaxTop; i += kLpThreads) {
-            const int own = i / kLpMaxTop, at = i % kLpMaxTop;
-            if (at >= a.top) continue;
+        const int all = C * K, even = (all + 7) / 8 * 8;
+        if (C > 1) {
+            if (tid < even - all) best[all + tid] = 0;
+            __syncthreads();
+        }
+        for (int i = tid; i < all; i += kThreads) {
             const unsigned long long key = best[i];
             if (key == 0) continue;
-            int place = at;
-            for (int o = 0; o < C; ++o) {
-                if (o == own) continue;
-                int lo = 0, hi = a.top;
-                while (lo < hi) {
-                    const int mid = (lo + hi) / 2;
-                    if (best[o * kLpMaxTop + mid] > key) lo = mid + 1; else hi = mid;
-                }
-                place += lo;
-            }
-            if (place < a.top) {
-                const long long to = (long long)row * a.top + place;
+            const int place = C == 1 ? i : lp_place(best, even, key);
+            if (place < K) {
+                const long long to = (long long)row * K + place;
                 a.top_ids[to] = bad ? -1 : (int)~(uint32_t)key;
                 a.top_logprobs[to] = lp(from_ordered((uint32_t)(key >> 32)));
             }

@@ -10,6 +10,7 @@ No autograd: results do not require gradients.
 """
 from __future__ import annotations
 
+import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
@@ -17,8 +18,13 @@ import torch
 from . import _lib
 from ._lib import FastllmError
 
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)      # (without the Stream object around it)
+_bound = [None]             # the device of the last call
 _FLOATS = {torch.float32: _lib.FL_DTYPE_F32, torch.bfloat16: _lib.FL_DTYPE_BF16, torch.float16: _lib.FL_DTYPE_F16}
+_TYPES = {**_FLOATS, torch.int8: _lib.FL_DTYPE_I8}
+_TOKENS = {torch.int32: 4, torch.int64: 8}
 MAX_TOP = 32
+_FEW_ROWS = 128
 
 
 def _refuse(msg: str):
@@ -27,10 +33,13 @@ def _refuse(msg: str):
 
 def _device(t: torch.Tensor, what: str) -> int:
     """the tensor's device, which is (or becomes) the one this process is bound to"""
-    if t.device.type != "cuda":
-        _refuse(f"{what}: tensors live on the GPU (there is no CPU fallback), got one on {t.device}")
-    _lib.init(t.device.index)
-    return t.device.index
+    dev = t.get_device()
+    if dev != _bound[0]:
+        if dev < 0:
+            _refuse(f"{what}: tensors live on the GPU (there is no CPU fallback), got one on {t.device}")
+        _lib.init(dev)
+        _bound[0] = dev
+    return dev
 
 
 def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -49,17 +58,18 @@ def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
         _refuse(f"{what}: the leading dimensions do not have one row stride")
 
 
-def _same(device: torch.device, what: str, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            _refuse(f"{what}: {name} lives on {t.device}, the first tensor on {device}")
+def _same(dev: int, t: Optional[torch.Tensor], what: str, name: str):
+    if t is not None and t.get_device() != dev:
+        _refuse(f"{what}: {name} lives on {t.device}, the first tensor on cuda:{dev}")
 
 
-def _vector(t: Optional[torch.Tensor], n: int, what: str, name: str):
+def _vector(t: Optional[torch.Tensor], n: int, dev: int, what: str, name: str):
     if t is None:
         return None
     if t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
         _refuse(f"{what}: {name} is a dense f32 tensor of {n} entries, got {t.dtype} {tuple(t.shape)}")
+    if t.get_device() != dev:
+        _same(dev, t, what, name)
     return t.data_ptr()
 
 
@@ -75,7 +85,7 @@ def quantize_rows(x: torch.Tensor):
     q = torch.empty((rows, step), dtype=torch.int8, device=x.device)
     scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     _lib.check(_lib.load().fl_quantize_rows(x2.data_ptr(), _FLOATS[x.dtype], rows, cols, x2.stride(0), q.data_ptr(), step, scale.data_ptr(),
-                                            torch.cuda.current_stream(dev).cuda_stream))
+                                            _stream(dev)))
     q = q[:, :cols]
     return (q if x.ndim == 2 else q.unflatten(0, x.shape[:-1]) if x.ndim > 2 else q[0]), scale
 
@@ -88,7 +98,7 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, b
     weight int8 [n, k] with rows on 16-byte borders, weight_scale f32 [n], bias f32 [n] or None.  out_dtype: f32 / bf16 / f16 (default: x's
     type, f32 for int8 rows); out: where the result goes, [..., n] with a dense last dimension, not overlapping an input."""
     what = "linear8"
-    x_type = _lib.FL_DTYPE_I8 if x.dtype == torch.int8 else _FLOATS.get(x.dtype)
+    x_type = _TYPES.get(x.dtype)
     if x_type is None:
         _refuse(f"{what}: activations are f32, bf16, f16 or int8, got {x.dtype}")
     if weight.dtype != torch.int8 or weight.ndim != 2:
@@ -96,25 +106,46 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, b
     dev = _device(x, what)
     x2 = x if x.ndim == 2 and x.stride(1) == 1 else _rows(x, what)
     rows, k = x2.shape
-    n = weight.shape[0]
-    if weight.shape[1] != k or (k > 1 and weight.stride(1) != 1):
+    n, wk = weight.shape
+    ldw, w_step = weight.stride()
+    if wk != k or (k > 1 and w_step != 1):
         _refuse(f"{what}: the weight is [n, {k}] with a dense last dimension, got {tuple(weight.shape)}")
-    _same(x.device, what, weight=weight, weight_scale=weight_scale, bias=bias, x_scale=x_scale, out=out)
+    if weight.get_device() != dev:
+        _same(dev, weight, what, "the weight")
+    ws_ptr = _vector(weight_scale, n, dev, what, "weight_scale")
+    xs_ptr = None if x_scale is None else _vector(x_scale, rows, dev, what, "x_scale")
+    bias_ptr = None if bias is None else _vector(bias, n, dev, what, "bias")
     if out is not None:
         if out.shape != x.shape[:-1] + (n,) or (out_dtype is not None and out.dtype != out_dtype):
             _refuse(f"{what}: out is {tuple(x.shape[:-1] + (n,))}, got {tuple(out.shape)} {out.dtype}")
-        y2 = _rows(out, what)
+        _same(dev, out, what, "out")
+        out_dtype = out.dtype
+    elif out_dtype is None:
+        out_dtype = torch.float32 if x_type == _lib.FL_DTYPE_I8 else x.dtype
+    y_type = _FLOATS.get(out_dtype)
+    if y_type is None:
+        _refuse(f"{what}: results are f32, bf16 or f16, got {out_dtype}")
+    if out is None:
+        y2 = x.new_empty((rows, n), dtype=out_dtype)
+        out, ldy = (y2 if x.ndim == 2 else y2.view(x.shape[:-1] + (n,))), n
     else:
-        out = torch.empty(x.shape[:-1] + (n,), dtype=out_dtype or (torch.float32 if x_type == _lib.FL_DTYPE_I8 else x.dtype), device=x.device)
-        y2 = out if out.ndim == 2 else out.view(rows, n)
-    if out.dtype not in _FLOATS:
-        _refuse(f"{what}: results are f32, bf16 or f16, got {out.dtype}")
-    step = (k + 15) // 16 * 16
-    room = 0 if x_type == _lib.FL_DTYPE_I8 else (rows * step + 255) // 256 * 256 + 4 * rows       # (fl_linear8_workspace's rule)
-    ws = torch.empty(room, dtype=torch.uint8, device=x.device) if room else None
-    _lib.check(_lib.load().fl_linear8(x2.data_ptr(), x_type, x2.stride(0), _vector(x_scale, rows, what, "x_scale"), weight.data_ptr(), weight.stride(0),
-                                      _vector(weight_scale, n, what, "weight_scale"), _vector(bias, n, what, "bias"), rows, n, k, y2.data_ptr(), _FLOATS[out.dtype],
-                                      y2.stride(0), ws.data_ptr() if room else None, room, torch.cuda.current_stream(dev).cuda_stream))
+        y2 = _rows(out, what)
+        ldy = y2.stride(0)
+    lib = _lib.load()
+    if rows > _FEW_ROWS:
+        size = C.c_size_t()
+        _lib.check(lib.fl_linear8_workspace(rows, n, k, x_type, C.byref(size)))
+        room = size.value
+    else:                       # (what it answers for few rows)
+        room = 0 if x_type == _lib.FL_DTYPE_I8 else (rows * ((k + 15) // 16 * 16) + 255) // 256 * 256 + (4 * rows + 255) // 256 * 256
+    work = work_ptr = None
+    if room:
+        work = x.new_empty(room, dtype=torch.uint8)
+        work_ptr = work.data_ptr()
+    rc = lib.fl_linear8(x2.data_ptr(), x_type, x2.stride(0), xs_ptr, weight.data_ptr(), ldw, ws_ptr, bias_ptr, rows, n, k, y2.data_ptr(), y_type, ldy, work_ptr, room,
+                        _stream(dev))
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -138,10 +169,12 @@ def logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: i
     x = logits if logits.ndim == 2 and logits.stride(1) == 1 else _rows(logits, what)
     rows, vocab = x.shape
     lead = logits.shape[:-1]
-    given, lp, tok, width = 0, None, None, 4
+    given, tok, tok_ptr, width = 0, None, None, 4
     if tokens is not None:
-        _same(logits.device, what, tokens=tokens)
-        if tokens.dtype not in (torch.int32, torch.int64):
+        if tokens.get_device() != dev:
+            _same(dev, tokens, what, "tokens")
+        width = _TOKENS.get(tokens.dtype)
+        if width is None:
             _refuse(f"{what}: tokens are int32 or int64, got {tokens.dtype}")
         if tokens.shape == lead:
             given = 1
@@ -149,16 +182,23 @@ def logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: i
             given = tokens.shape[-1]
         else:
             _refuse(f"{what}: tokens are {tuple(lead)} or {tuple(lead)} + (m,), got {tuple(tokens.shape)}")
-        tok = tokens.contiguous()
-        width = 4 if tok.dtype == torch.int32 else 8
-        lp = torch.empty(tokens.shape, dtype=torch.float32, device=logits.device)
-    lse = torch.empty(lead, dtype=torch.float32, device=logits.device)
-    ent = torch.empty(lead, dtype=torch.float32, device=logits.device)
-    ids = tlp = None
-    if top > 0:
-        ids = torch.empty(lead + (top,), dtype=torch.int32, device=logits.device)
-        tlp = torch.empty(lead + (top,), dtype=torch.float32, device=logits.device)
-    _lib.check(_lib.load().fl_logprobs(x.data_ptr(), _FLOATS[logits.dtype], rows, vocab, x.stride(0), tok.data_ptr() if given else None, width, given, temperature, top,
-                                       lp.data_ptr() if given else None, lse.data_ptr(), ent.data_ptr(), ids.data_ptr() if top > 0 else None,
-                                       tlp.data_ptr() if top > 0 else None, torch.cuda.current_stream(dev).cuda_stream))
-    return LogProbs(lp, lse, ent, ids, tlp)
+        tok = tokens if tokens.is_contiguous() else tokens.contiguous()
+        tok_ptr = tok.data_ptr()
+    if not 0 <= top <= MAX_TOP:
+        _refuse(f"{what}: from 0 to {MAX_TOP} alternatives, got {top}")
+    # all results in one piece of memory: an allocation each would take as long as the launch
+    mem = x.new_empty(rows * (given + 2 + 2 * top), dtype=torch.float32)
+    at, step = mem.data_ptr(), 4 * rows
+    rc = _lib.load().fl_logprobs(x.data_ptr(), _FLOATS[logits.dtype], rows, vocab, x.stride(0), tok_ptr if given else None, width, given, temperature, top,
+                                 at + 2 * step if given else None, at, at + step, at + (2 + given) * step if top else None, at + (2 + given + top) * step if top else None,
+                                 _stream(dev))
+    if rc:
+        _lib.check(rc)
+
+    def part(first, cols, shape, kind=None):
+        t = mem if kind is None else mem.view(kind)
+        t = t.as_strided((rows, cols) if len(shape) == 2 else (rows * cols,), (cols, 1) if len(shape) == 2 else (1,), first * rows)
+        return t if len(shape) in (1, 2) and t.shape == shape else t.view(shape)
+
+    return LogProbs(None if tok is None else part(2, given, tokens.shape), part(0, 1, lead), part(1, 1, lead),
+                    part(2 + given, top, lead + (top,), torch.int32) if top else None, part(2 + given + top, top, lead + (top,)) if top else None)

@@ -40,44 +40,35 @@ constexpr int64_t kLinear8MaxK = 131071;        // 128 * 128 * k stays below 2^3
 static int64_t padded_k(int64_t k) { return (k + 15) / 16 * 16; }
 static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// How a product of more than kL8FewRows rows goes over the pairs of SMs.  A k block of a tile takes the tensor cores 2 bn clocks and the way of its operands
-// from L2 (16 KB + 64 bn bytes per SM, at about 56 bytes a clock) longer than that, so wide tiles are the faster ones where they fit the row
-// count.  Cutting the tiles that are left costs about 16 k blocks (their parts' way through the workspace).
-constexpr int kL8FewRows = 128, kL8CutCost = 16;
+// How a product of more than kL8FewRows rows goes over the pairs of SMs: the tile width whose waves cost least, by what a k block takes (see
+// linear8_pair_kernel).  Cutting the tiles of a last wave along K was measured and lost everywhere (1531 x 14336 x 4096 68 -> 78 us, 777 x 4096 x 32000 86 ->
+// 96): the parts' way through the workspace takes longer than the idle pairs would.
+constexpr int kL8FewRows = 128;
 static L8Pair pair_plan8(int64_t rows, int64_t n, int64_t k, int clusters) {
     L8Pair best{};
     double cost = -1;
-    for (int bn = 256; bn >= 64; bn -= 32) {
+    for (int bn = 512; bn >= 64; bn -= bn > 256 ? 64 : 32) {
         L8Pair p{};
         p.bn = bn;
         p.nk = (int)((k + kL8BK - 1) / kL8BK);
         p.mt = (int)((n + 255) / 256);
         p.nt = (int)((rows + bn - 1) / bn);
-        const long long T = (long long)p.mt * p.nt;
-        const double block = std::max(2.0 * bn, (16384.0 + 64.0 * bn) / 56.0);
-        p.full = (int)(T / clusters);
-        const int left = (int)(T % clusters);
-        const int L = std::max((left * p.nk + clusters - 1) / clusters, 1);
-        const bool cut = left > 0 && L + kL8CutCost < p.nk;
-        p.L = cut ? L : p.nk;
-        p.clusters = p.full > 0 ? clusters : (left * p.nk + p.L - 1) / p.L;
-        const double blocks = (double)p.full * p.nk + (left == 0 ? 0 : cut ? L + kL8CutCost : p.nk);
-        if (cost < 0 || blocks * block < cost) { cost = blocks * block; best = p; }
+        p.stages = (int)std::min<uint32_t>(kL8PairMaxStages, kL8PairRing / (kL8WBytes + (uint32_t)bn * (kL8BK / 2)));
+        const double block = std::max(1.38 * bn, (16384.0 + 64.0 * bn) / 90.0), tail = bn > 256 ? 13.0 * bn : 0.0;      // ns; results that no product hides
+        const double waves = (double)(((long long)p.mt * p.nt + clusters - 1) / clusters);
+        const double c = waves * (p.nk * block + tail);
+        if (cost < 0 || c < cost) { cost = c; best = p; }
     }
     return best;
 }
-static size_t pair_parts_bytes(const L8Pair& p) { return p.L == p.nk ? 0 : (size_t)p.clusters * 2 * 2 * p.bn * 128 * 4; }
-static int pair_tickets(const L8Pair& p) { return p.L == p.nk ? 0 : 2 * (int)((long long)p.mt * p.nt - (long long)p.full * p.clusters); }
 
-// A call's workspace: rounded rows and their scales (activations that are not 8-bit), counters and parts of shared tiles
-struct L8Room { size_t q = 0, scale = 0, tickets = 0, parts = 0, all = 0; };
-static L8Room linear8_room(int64_t rows, int64_t n, int64_t k, bool given, const L8Pair* p) {
+// A call's workspace: rounded rows and their scales (none for activations that are 8-bit already)
+struct L8Room { size_t scale = 0, all = 0; };
+static L8Room linear8_room(int64_t rows, int64_t k, bool given) {
     L8Room r;
-    size_t at = 0;
-    auto take = [&](size_t bytes) { const size_t here = at; at += up256(bytes); return here; };
-    if (!given) { r.q = take((size_t)rows * padded_k(k)); r.scale = take((size_t)rows * 4); }
-    if (p != nullptr) { r.tickets = take((size_t)pair_tickets(*p) * 4); r.parts = take(pair_parts_bytes(*p)); }
-    r.all = at;
+    if (given) return r;
+    r.scale = up256((size_t)rows * padded_k(k));
+    r.all = r.scale + (size_t)rows * 4;
     return r;
 }
 
@@ -148,20 +139,17 @@ void ops_init() {
     *p = 0;
     g_op_failed = p;
 }
-// (asked for ahead of fl_init, as by fl_linear8_workspace on a machine without a GPU: a whole chip's)
-static int op_pairs() { return g_pair_clusters > 0 ? g_pair_clusters : kNumSMs / 2; }
 static void check_op_failed() {
     FL_CHECK(*reinterpret_cast<volatile int*>(g_op_failed) == 0, FL_ERR_CUDA, "a wait inside an operator's kernel ran out in an earlier call: its results are not valid");
 }
 
 template <typename T>
-static void quantize_rows_t(LaunchCtx& lc, const void* x, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, int64_t cols_q, float* scale, int* zero,
-                            int zeros) {
+static void quantize_rows_t(LaunchCtx& lc, const void* x, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, int64_t cols_q, float* scale) {
     constexpr int V = 16 / sizeof(T);
     const uint64_t bytes = rows * cols * (sizeof(T) + 1);
     auto go = [&](auto kern) {
         launch_op(lc, "quantize_rows", bytes, kern, dim3((unsigned)rows), 256, 0, 1, false, static_cast<const T*>(x), (long long)ldx, (int)cols, q, (long long)ldq,
-                  (int)cols_q, scale, zero, zeros);
+                  (int)cols_q, scale);
     };
     const bool vec = aligned(x, 16) && aligned(q, V) && (rows == 1 || (ldx % V == 0 && ldq % V == 0));
     const int64_t vecs = (cols_q + V - 1) / V;
@@ -171,15 +159,11 @@ static void quantize_rows_t(LaunchCtx& lc, const void* x, int64_t rows, int64_t 
     else if (vecs <= 4 * 256) go(quantize_rows_kernel<T, 4>);
     else go(quantize_rows_kernel<T, 8>);
 }
-static void quantize_rows(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, int64_t cols_q, float* scale,
-                          int* zero = nullptr, int zeros = 0) {
-    if (dtype == FL_DTYPE_F32) quantize_rows_t<float>(lc, x, rows, cols, ldx, q, ldq, cols_q, scale, zero, zeros);
-    else if (dtype == FL_DTYPE_BF16) quantize_rows_t<__nv_bfloat16>(lc, x, rows, cols, ldx, q, ldq, cols_q, scale, zero, zeros);
-    else quantize_rows_t<__half>(lc, x, rows, cols, ldx, q, ldq, cols_q, scale, zero, zeros);
+static void quantize_rows(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, int64_t cols_q, float* scale) {
+    if (dtype == FL_DTYPE_F32) quantize_rows_t<float>(lc, x, rows, cols, ldx, q, ldq, cols_q, scale);
+    else if (dtype == FL_DTYPE_BF16) quantize_rows_t<__nv_bfloat16>(lc, x, rows, cols, ldx, q, ldq, cols_q, scale);
+    else quantize_rows_t<__half>(lc, x, rows, cols, ldx, q, ldq, cols_q, scale);
 }
-
-// 16-bit results may be written in twos
-static bool even_rows(const Linear8Args& g) { return g.n % 2 == 0 && g.ldy % 2 == 0 && aligned(g.y, 4); }
 
 template <int BN>
 static void launch_few(LaunchCtx& lc, uint64_t bytes, const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, const Linear8Args& g, bool pdl) {
@@ -187,11 +171,13 @@ static void launch_few(LaunchCtx& lc, uint64_t bytes, const int8_t* x, int64_t l
     int S = 1;
     while (S < 8 && 2 * S * tiles <= L8Few<BN>::kPerSm * kNumSMs && nk >= 8 * S) S *= 2;
     const CUtensorMap tw = make_tmap_i8(w, g.n, g.k, ldw, 128), tx = make_tmap_i8(x, g.rows, g.k, ldx, BN);
-    launch_op(lc, "linear8", bytes, linear8_few_kernel<BN>, dim3((unsigned)(tiles * S)), L8Few<BN>::kThreads, L8Few<BN>::kSmem, S, pdl, tw, tx, g, S, even_rows(g));
+    launch_op(lc, "linear8", bytes, linear8_few_kernel<BN>, dim3((unsigned)(tiles * S)), L8Few<BN>::kThreads, L8Few<BN>::kSmem, S, pdl, tw, tx, g, S);
 }
-static void launch_pair(LaunchCtx& lc, uint64_t bytes, const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, const Linear8Args& g, const L8Pair& p, bool pdl) {
-    const CUtensorMap tx = make_tmap_i8(x, g.rows, g.k, ldx, p.bn / 2), tw = make_tmap_i8(w, g.n, g.k, ldw, 128);
-    launch_op(lc, "linear8", bytes, linear8_pair_kernel, dim3((unsigned)(2 * p.clusters)), kL8PairThreads, kL8PairSmem, 1, pdl, tw, tx, g, p, even_rows(g));
+static void launch_pair(LaunchCtx& lc, uint64_t bytes, const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, const Linear8Args& g, bool pdl) {
+    const L8Pair p = pair_plan8(g.rows, g.n, g.k, g_pair_clusters);
+    const CUtensorMap tx = make_tmap_i8(x, g.rows, g.k, ldx, p.bn / (p.bn > 256 ? 4 : 2)), tw = make_tmap_i8(w, g.n, g.k, ldw, 128);
+    const long long clusters = std::min<long long>(g_pair_clusters, (long long)p.mt * p.nt);
+    launch_op(lc, "linear8", bytes, linear8_pair_kernel, dim3((unsigned)(2 * clusters)), kL8PairThreads, kL8PairSmem, 1, pdl, tw, tx, g, p);
 }
 
 // Blocks per row: as many as the chip holds (four per SM) over the rows, while every warp still has a chunk of two; the cluster of 16 is not portable
@@ -229,15 +215,12 @@ FL_EXPORT int fl_quantize_rows(const void* x, int dtype, int64_t rows, int64_t c
     FL_API_END
 }
 
-FL_EXPORT int fl_linear8_workspace(int64_t rows, int64_t n, int64_t k, int x_dtype, size_t* bytes) {
+FL_EXPORT int fl_linear8_workspace(int64_t rows, int64_t k, int x_dtype, size_t* bytes) {
     FL_API_BEGIN
     FL_CHECK(bytes, FL_ERR_INVALID, "NULL argument");
     FL_CHECK(is_float(x_dtype) || x_dtype == FL_DTYPE_I8, FL_ERR_INVALID, "linear8: activations are f32, bf16, f16 or i8");
-    FL_CHECK(rows >= 0 && rows <= kMaxRows && n >= 1 && n <= kMaxRows && k >= 1 && k <= kLinear8MaxK, FL_ERR_INVALID,
-             "linear8: rows from 0 to 2^30, n from 1 to 2^30, k from 1 to 131071");
-    const bool pairs = rows > kL8FewRows;
-    const L8Pair p = pairs ? pair_plan8(rows, n, k, op_pairs()) : L8Pair{};
-    *bytes = linear8_room(rows, n, k, x_dtype == FL_DTYPE_I8, pairs ? &p : nullptr).all;
+    FL_CHECK(rows >= 0 && rows <= kMaxRows && k >= 1 && k <= kLinear8MaxK, FL_ERR_INVALID, "linear8: rows from 0 to 2^30, k from 1 to 131071");
+    *bytes = linear8_room(rows, k, x_dtype == FL_DTYPE_I8).all;
     FL_API_END
 }
 
@@ -258,9 +241,7 @@ FL_EXPORT int fl_linear8(const void* x, int x_dtype, int64_t ldx, const float* x
     FL_CHECK(aligned(x, dtype_size(x_dtype)) && aligned(y, dtype_size(y_dtype)) && aligned(w_scale, 4) && aligned(x_scale, 4) && aligned(bias, 4), FL_ERR_INVALID,
              "linear8: a pointer is not aligned to its type");
     FL_CHECK(rows <= ((int64_t)1 << 40) / n, FL_ERR_INVALID, "linear8: more than 2^40 results");
-    const bool pairs = rows > kL8FewRows;
-    L8Pair plan = pairs ? pair_plan8(rows, n, k, op_pairs()) : L8Pair{};
-    const L8Room room = linear8_room(rows, n, k, given, pairs ? &plan : nullptr);
+    const L8Room room = linear8_room(rows, k, given);
     FL_CHECK(room.all == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= room.all), FL_ERR_INVALID,
              "linear8: the workspace is smaller than fl_linear8_workspace asks for, or not on a 256-byte border");
     DeviceScope dev;
@@ -270,20 +251,15 @@ FL_EXPORT int fl_linear8(const void* x, int x_dtype, int64_t ldx, const float* x
     int64_t ldq = rows == 1 ? padded_k(k) : ldx;
     Linear8Args g{(int)rows, (int)n, (int)k, x_scale, w_scale, bias, y, ldy, y_dtype, g_op_failed};
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    const int zeros = pairs ? pair_tickets(plan) : 0;
-    plan.tickets = reinterpret_cast<int*>(ws + room.tickets);
-    plan.parts = reinterpret_cast<int*>(ws + room.parts);
     if (!given) {
-        int8_t* to = reinterpret_cast<int8_t*>(ws + room.q);
+        int8_t* to = reinterpret_cast<int8_t*>(ws);
         float* s = reinterpret_cast<float*>(ws + room.scale);
-        quantize_rows(lc, x, x_dtype, rows, k, ldx, to, padded_k(k), padded_k(k), s, plan.tickets, zeros);
+        quantize_rows(lc, x, x_dtype, rows, k, ldx, to, padded_k(k), padded_k(k), s);
         q = to; ldq = padded_k(k); g.xs = s;
-    } else if (zeros > 0) {
-        FL_CUDA(cudaMemsetAsync(plan.tickets, 0, (size_t)zeros * 4, lc.stream));
     }
     if (n == 1) ldw = padded_k(k);
     const uint64_t bytes = (uint64_t)n * k + (uint64_t)rows * (k + n * dtype_size(y_dtype));
-    if (pairs) launch_pair(lc, bytes, q, ldq, w, ldw, g, plan, !given);
+    if (rows > kL8FewRows) launch_pair(lc, bytes, q, ldq, w, ldw, g, !given);
     else if (rows <= 16) launch_few<16>(lc, bytes, q, ldq, w, ldw, g, !given);
     else if (rows <= 32) launch_few<32>(lc, bytes, q, ldq, w, ldw, g, !given);
     else if (rows <= 64) launch_few<64>(lc, bytes, q, ldq, w, ldw, g, !given);

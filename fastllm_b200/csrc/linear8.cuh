@@ -58,18 +58,16 @@ struct RowScale {
 // larger for every NaN than for an infinity, and for that than for any number
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// A block per row; columns [cols, cols_q) of q are filled with zeros, and so are the `zeros` words that the kernel behind counts in.  kVecs > 0: the row starts on 16-byte borders on both sides (8 for q) and has at
+// A block per row; columns [cols, cols_q) of q are filled with zeros.  kVecs > 0: the row starts on 16-byte borders on both sides (8 for q) and has at
 // most 256 * kVecs vectors of 16 bytes, which stay in registers between the maximum and the rounding; 0: any row, read twice.
 template <typename T, int kVecs>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, long long ldx, int cols, int8_t* __restrict__ q, long long ldq, int cols_q,
-                                                            float* __restrict__ scale, int* __restrict__ zero, int zeros) {
+                                                            float* __restrict__ scale) {
     constexpr int V = 16 / sizeof(T);
     __shared__ uint32_t part[8];
     const T* xr = x + (long long)blockIdx.x * ldx;
     int8_t* qr = q + (long long)blockIdx.x * ldq;
     pdl_launch_dependents();
-    if (blockIdx.x == 0)
-        for (int i = threadIdx.x; i < zeros; i += 256) zero[i] = 0;
     uint32_t m = 0;
     uint4 held[kVecs > 0 ? kVecs : 1];
     if constexpr (kVecs > 0) {
@@ -168,21 +166,35 @@ __device__ __forceinline__ void umma_i8_pair_warp(uint32_t tmem_d, uint64_t ades
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// Results of one weight row n (a lane each) and 16 activation rows r, r + 1, ..: for a fixed row the 32 lanes write 32 neighbours.  16-bit results go in twos
-// where rows start on even places (`twos`): neighbouring lanes exchange a value, even lanes write row r + j and odd ones r + j + 1.
-__device__ __forceinline__ void l8_store16(const Linear8Args& g, int r, int n, float wsn, float bn, const int (&sum)[16], bool twos) {
-    const int lane = threadIdx.x & 31;
+// Results of one weight row n (a lane each) and 16 activation rows r, r + 1, .. with the scales xs (shared memory, 16-byte border): for a fixed row the 32
+// lanes write 32 neighbours.  (16-bit results in twos, after an exchange between neighbouring lanes, took as long or longer: 64 x 152064 20 -> 26 us.)
+__device__ __forceinline__ void l8_store16(const Linear8Args& g, int r, int n, const float* xs, float wsn, float bn, const uint32_t (&sum)[16]) {
     float v[16];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-        v[j] = (float)sum[j] * __ldg(g.xs + min(r + j, g.rows - 1)) * wsn;
-        if (g.bias != nullptr) v[j] += bn;
+    for (int j = 0; j < 16; j += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(xs + j);
+        v[j] = (float)(int)sum[j] * x.x * wsn;
+        v[j + 1] = (float)(int)sum[j + 1] * x.y * wsn;
+        v[j + 2] = (float)(int)sum[j + 2] * x.z * wsn;
+        v[j + 3] = (float)(int)sum[j + 3] * x.w * wsn;
     }
+    if (g.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] += bn;
+    }
+    const int rows = n < g.n ? min(g.rows - r, 16) : 0;
     if (g.y_dtype == 0) {
         float* o = reinterpret_cast<float*>(g.y) + (long long)r * g.ldy + n;
+        if (rows == 16) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (r + j < g.rows && n < g.n) o[j * g.ldy] = v[j];
+            for (int j = 0; j < 16; ++j) { *o = v[j]; o += g.ldy; }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                if (j < rows) *o = v[j];
+                o += g.ldy;
+            }
+        }
         return;
     }
     auto half = [&](float a, float b) {
@@ -191,22 +203,12 @@ __device__ __forceinline__ void l8_store16(const Linear8Args& g, int r, int n, f
         return *reinterpret_cast<const uint32_t*>(&h);
     };
     uint16_t* o = reinterpret_cast<uint16_t*>(g.y) + (long long)r * g.ldy + n;
-    if (twos) {
-        const bool odd = lane & 1;
-        o -= odd;
-#pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-            const float got = __shfl_xor_sync(0xFFFFFFFFu, odd ? v[j] : v[j + 1], 1);
-            const uint32_t w = odd ? half(got, v[j + 1]) : half(v[j], got);
-            if (r + j + odd < g.rows && n < g.n) *reinterpret_cast<uint32_t*>(o + (j + odd) * g.ldy) = w;      // (g.n is even: both or none)
-        }
-        return;
-    }
 #pragma unroll
     for (int j = 0; j < 16; j += 2) {
         const uint32_t w = half(v[j], v[j + 1]);
-        if (r + j < g.rows && n < g.n) o[j * g.ldy] = (uint16_t)w;
-        if (r + j + 1 < g.rows && n < g.n) o[(j + 1) * g.ldy] = (uint16_t)(w >> 16);
+        if (j < rows) o[0] = (uint16_t)w;
+        if (j + 1 < rows) o[g.ldy] = (uint16_t)(w >> 16);
+        o += 2 * g.ldy;
     }
 }
 // A wait ran out: report it and leave the copies in flight time to land; the block goes on to its end.
@@ -231,12 +233,13 @@ template <int BN> struct L8Few {
 
 template <int BN>
 __global__ void __launch_bounds__(L8Few<BN>::kThreads, L8Few<BN>::kPerSm)
-linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Linear8Args g, const int S, const bool twos) {
+linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Linear8Args g, const int S) {
     using L = L8Few<BN>;
     constexpr int kStages = L::kStages;
     extern __shared__ uint8_t gsm_raw[];
     uint8_t* gsm = gsm_raw + ((1024u - (smem_u32(gsm_raw) & 1023u)) & 1023u);          // (the same offset in all blocks of a cluster)
     __shared__ __align__(8) uint64_t full[kStages], empty[kStages], done;
+    __shared__ __align__(16) float xs[4][BN];                                          // the rows' scales, a copy for each epilogue warp
     __shared__ uint32_t tmem_base_s;
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const int s = S == 1 ? 0 : (int)cluster_rank();
@@ -298,7 +301,9 @@ linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const int n = n0 + row;
     if (warp >= 2) {
-        pdl_wait();                                                                    // (the rows' scales)
+        pdl_wait();
+        for (int i = lane; i < BN; i += 32) xs[warp - 2][i] = r0 + i < g.rows ? g.xs[r0 + i] : 0.f;
+        __syncwarp();
         ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&done, 0, kMbarTries));
         tc_fence_after();
     }
@@ -308,11 +313,8 @@ linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
 #pragma unroll 1
             for (int c = 0; c < BN && r0 + c < g.rows; c += 16) {
                 uint32_t v[16];
-                int sum[16];
                 tmem_ld16(at + (uint32_t)c, v);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) sum[j] = (int)v[j];
-                l8_store16(g, r0 + c, n, wsn, bn, sum, twos);
+                l8_store16(g, r0 + c, n, xs[warp - 2] + c, wsn, bn, v);
             }
         }
     } else {
@@ -341,7 +343,7 @@ linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                 for (int t = 0; t < S; ++t) sum += part[(t * per + c) * 128];
                 const int r = r0 + s * per + c;
                 if (n >= g.n) continue;
-                float v = (float)sum * g.xs[r] * wsn;
+                float v = (float)sum * xs[warp - 2][s * per + c] * wsn;
                 if (g.bias != nullptr) v += bn;
                 const long long at_y = (long long)r * g.ldy + n;
                 if (g.y_dtype == 0) reinterpret_cast<float*>(g.y)[at_y] = v;
@@ -362,34 +364,34 @@ linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
 
 // ---- many rows ----------------------------------------------------------------------------------------------------------------------
 // Pairs of SMs on tiles of 256 weight rows x bn activation rows (tcgen05.mma.cta_group::2): each holds its 128 weight rows and half of the activation
-// tile.  bn is any multiple of 32, so that a row count is cut without much padding.  Tiles that do not fill a wave are cut along K, evenly over all
-// pairs: a part of a tile goes to the workspace, the last of its parts to arrive adds the others to its own and writes the results (nobody
-// waits for anybody, and the order does not matter for whole numbers).
-constexpr int kL8PairStages = 6, kL8PairEpi = 16, kL8PairThreads = 64 + 32 * kL8PairEpi;
-constexpr uint32_t kL8PairStage = 2 * kL8WBytes;
-constexpr size_t kL8PairSmem = (size_t)kL8PairStages * kL8PairStage + 1024;
+// tile, 16 KB + 64 bn bytes per k block of 128.  What bounds it: the operands' way from L2, about 90 bytes a nanosecond and SM (a k block took 268 ns at bn =
+// 128, 294 at 160, 364 at 256; the tensor cores need about 1.05 bn).  So tiles are as wide as the row count allows, up to 512: two products of bn / 2 then, in
+// the two halves of the accumulators, which tiles of up to 256 use in turn.
+constexpr int kL8PairEpi = 16, kL8PairThreads = 64 + 32 * kL8PairEpi, kL8PairMaxStages = 8;
+constexpr uint32_t kL8PairRing = 200 * 1024;
+constexpr size_t kL8PairSmem = kL8PairRing + 1024;
 
 struct L8Pair {
-    int bn, nk, mt, nt;         // activation rows of a tile; k blocks; weight and activation tiles
-    int clusters, full, L;      // pairs at work; whole tiles per pair; then k blocks per pair of the tiles that are left
-    int* parts;                 // [cluster][first | second tile of its range][CTA][bn][128]
-    int* tickets;               // [2 * tiles left], zero
+    int bn;                     // activation rows of a tile: a multiple of 32, above 256 of 64
+    int nk, mt, nt;             // k blocks; weight and activation tiles
+    int stages;
 };
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kL8PairThreads, 1)
-linear8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Linear8Args g, const L8Pair p, const bool twos) {
+linear8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Linear8Args g, const L8Pair p) {
     extern __shared__ uint8_t gsm_raw[];
     uint8_t* gsm = gsm_raw + ((1024u - (smem_u32(gsm_raw) & 1023u)) & 1023u);          // (the same offset in both CTAs)
-    __shared__ __align__(8) uint64_t full[kL8PairStages], empty[kL8PairStages], acc_full[2], acc_empty[2];
+    __shared__ __align__(8) uint64_t full[kL8PairMaxStages], empty[kL8PairMaxStages], acc_full[2], acc_empty[2];
+    __shared__ __align__(16) float xs[kL8PairEpi][64];                                 // the scales of the rows that an epilogue warp writes
     __shared__ uint32_t tmem_base_s;
-    __shared__ int s_last;
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
     const int cl = blockIdx.x >> 1, G = gridDim.x >> 1, nk = p.nk, T = p.mt * p.nt, bn = p.bn;
-    const int left0 = p.full * G, units = (T - left0) * nk;
+    const int parts = bn > 256 ? 2 : 1, pn = bn / parts;                               // products of a tile, their activation rows
+    const uint32_t stage = kL8WBytes + (uint32_t)bn * (kL8BK / 2);
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kL8PairStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < p.stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
         for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 2 * kL8PairEpi); }
         mbar_fence_init();
         tma_prefetch_desc(&tmX);
@@ -404,23 +406,6 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_s;
-
-    // This pair's work in order: whole tiles cl, cl + G, ..., then its run of k blocks of the tiles that are left.
-    // -> false at the end; tile, [kb0, kb1)
-    struct Walk { int seg = 0, u = 0; };
-    const int u1 = min((cl + 1) * p.L, units);
-    auto next = [&](Walk& w, int& tile, int& kb0, int& kb1) {
-        if (w.seg < p.full) {
-            tile = cl + w.seg * G; kb0 = 0; kb1 = nk;
-        } else {
-            if (w.seg == p.full) w.u = cl * p.L;
-            if (w.u >= u1) return false;
-            tile = left0 + w.u / nk; kb0 = w.u % nk; kb1 = min(nk, kb0 + u1 - w.u);
-            w.u += kb1 - kb0;
-        }
-        ++w.seg;
-        return true;
-    };
     // 8 activation tiles share a weight tile before the walk moves on (see kGemmRasterRows)
     auto place = [&](int tile, int& n, int& r) {
         constexpr int RM = kGemmRasterRows / 2;
@@ -428,117 +413,92 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
         r = (first + local % cnt) * bn;
         n = local / cnt * 256 + (int)rank * 128;
     };
-    const uint32_t tx = 2 * (kL8WBytes + (uint32_t)bn / 2 * kL8BK);                    // bytes of a stage in both CTAs
     bool ok = true;
 
     if (warp == 0) {
         if (lane == 0) {
             pdl_wait();
             asm volatile("fence.proxy.async;" ::: "memory");
-            Walk w;
-            int tile, kb0, kb1, st = 0;
+            int st = 0;
             uint32_t ph = 1;
-            while (ok && next(w, tile, kb0, kb1)) {
+            for (int tile = cl; ok && tile < T; tile += G) {
                 int n0, r0;
                 place(tile, n0, r0);
-                for (int kb = kb0; kb < kb1; ++kb) {
+                r0 += (int)rank * (pn >> 1);
+                for (int kb = 0; kb < nk; ++kb) {
                     if (!(ok = pair_wait(&empty[st], ph))) break;
-                    if (rank == 0) mbar_expect_tx(&full[st], tx);                      // both CTAs' loads complete on the first one's barrier
-                    const uint32_t bar = mapa_u32(smem_u32(&full[st]), 0), sa = smem_u32(gsm) + st * kL8PairStage;
+                    if (rank == 0) mbar_expect_tx(&full[st], 2 * stage);               // both CTAs' loads complete on the first one's barrier
+                    const uint32_t bar = mapa_u32(smem_u32(&full[st]), 0), sa = smem_u32(gsm) + st * stage;
                     tma_load_2d_pair(sa, &tmW, kb * kL8BK, n0, bar);
-                    tma_load_2d_pair(sa + kL8WBytes, &tmX, kb * kL8BK, r0 + (int)rank * (bn >> 1), bar);
-                    if (++st == kL8PairStages) { st = 0; ph ^= 1; }
+                    tma_load_2d_pair(sa + kL8WBytes, &tmX, kb * kL8BK, r0, bar);
+                    if (parts == 2) tma_load_2d_pair(sa + kL8WBytes + (uint32_t)pn * (kL8BK / 2), &tmX, kb * kL8BK, r0 + pn, bar);
+                    if (++st == p.stages) { st = 0; ph ^= 1; }
                 }
             }
         }
     } else if (warp == 1) {
         if (rank == 0) {
-            const uint32_t idesc = umma_idesc_i8(256, bn);
+            const uint32_t idesc = umma_idesc_i8(256, pn), second = ((uint32_t)pn * (kL8BK / 2)) >> 4;
             const uint64_t base = umma_smem_desc_sw128(gsm);
-            Walk w;
-            int tile, kb0, kb1, st = 0;
+            int st = 0;
             uint32_t ph = 0, seg = 0;
             auto wait = [&](uint64_t* bar, uint32_t parity) {
                 if (ok) ok = pair_wait(bar, parity);
                 __syncwarp();
                 tc_fence_after();
             };
-            while (next(w, tile, kb0, kb1)) {
-                const uint32_t as = seg & 1, tacc = tmem_base + as * 256;
-                wait(&acc_empty[as], ((seg >> 1) & 1) ^ 1);
-                for (int kb = kb0; kb < kb1; ++kb) {
+            for (int tile = cl; tile < T; tile += G, ++seg) {
+                const uint32_t as = parts == 2 ? 0 : seg & 1, uses = parts == 2 ? seg : seg >> 1, tacc = tmem_base + as * 256;
+                wait(&acc_empty[as], (uses & 1) ^ 1);
+                if (parts == 2) wait(&acc_empty[1], (uses & 1) ^ 1);
+                for (int kb = 0; kb < nk; ++kb) {
                     wait(&full[st], ph);
-                    const uint64_t a = base + (uint64_t)(st * (kL8PairStage >> 4)), b = a + (kL8WBytes >> 4);
+                    const uint64_t a = base + (uint64_t)(st * (stage >> 4)), b = a + (kL8WBytes >> 4);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) umma_i8_pair_warp(tacc, a + 2 * q, b + 2 * q, idesc, ((kb - kb0) | q) ? 1u : 0u);
+                    for (int q = 0; q < 4; ++q) umma_i8_pair_warp(tacc, a + 2 * q, b + 2 * q, idesc, (kb | q) ? 1u : 0u);
+                    if (parts == 2) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) umma_i8_pair_warp(tacc + 256, a + 2 * q, b + second + 2 * q, idesc, (kb | q) ? 1u : 0u);
+                    }
                     umma_commit_pair_warp(&empty[st]);
-                    if (++st == kL8PairStages) { st = 0; ph ^= 1; }
+                    if (++st == p.stages) { st = 0; ph ^= 1; }
                 }
                 umma_commit_pair_warp(&acc_full[as]);
-                ++seg;
+                if (parts == 2) umma_commit_pair_warp(&acc_full[1]);
             }
         }
     } else {
-        const int q = warp & 3, cs = (warp - 2) >> 2, lrow = q * 32 + lane;            // TMEM lane quarter (hardware rule); every fourth run of 16 columns
-        Walk w;
-        int tile, kb0, kb1;
+        const int q = warp & 3, cs = (warp - 2) >> 2;                                  // TMEM lane quarter (hardware rule); every fourth run of 16 columns
         uint32_t seg = 0;
         pdl_wait();                                                                    // (the rows' scales)
-        while (next(w, tile, kb0, kb1)) {                                              // (to the end even behind a wait that ran out: the warps meet at barriers)
+        for (int tile = cl; tile < T; tile += G, ++seg) {
             int n0, r0;
             place(tile, n0, r0);
-            const uint32_t as = seg & 1;
-            if (ok) ok = __all_sync(0xFFFFFFFFu, pair_wait(&acc_full[as], (seg >> 1) & 1));
-            ++seg;
-            tc_fence_after();
-            const uint32_t at = tmem_base + as * 256 + ((uint32_t)(q * 32) << 16);
-            const int n = n0 + lrow, last_col = min(bn, g.rows - r0);
-            const bool whole = kb0 == 0 && kb1 == nk;
-            const int left = tile - left0;                                             // (of a tile that is left)
-            auto part_of = [&](int c) { return p.parts + (size_t)((c * 2 + left - c * p.L / nk) * 2 + (int)rank) * bn * 128 + lrow; };
-            bool store = whole;
-            int c0 = 0, c1 = -1;
-            if (!whole) {
-                c0 = left * nk / p.L; c1 = ((left + 1) * nk - 1) / p.L;
-                int* part = part_of(cl);
+            const int n = n0 + q * 32 + lane;
+            const float wsn = n < g.n ? __ldg(g.ws + n) : 0.f, bias = g.bias != nullptr && n < g.n ? __ldg(g.bias + n) : 0.f;
+            for (int h = 0; h < parts; ++h, r0 += pn) {
+                const uint32_t as = parts == 2 ? (uint32_t)h : seg & 1, uses = parts == 2 ? seg : seg >> 1;
+                float* own = xs[warp - 2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {                                          // run i of 16 columns: (cs + 4 i) 16 on; on its way while the products are
+                    const int r = r0 + (cs + 4 * (2 * i + (lane >> 4))) * 16 + (lane & 15);
+                    own[32 * i + lane] = r < g.rows ? __ldg(g.xs + r) : 0.f;
+                }
+                __syncwarp();
+                if (ok) ok = __all_sync(0xFFFFFFFFu, pair_wait(&acc_full[as], uses & 1));
+                tc_fence_after();
+                const uint32_t at = tmem_base + as * 256 + ((uint32_t)(q * 32) << 16);
+                const int last_col = min(pn, g.rows - r0);
 #pragma unroll 1
                 for (int c = cs * 16; ok && c < last_col; c += 64) {
                     uint32_t v[16];
                     tmem_ld16(at + (uint32_t)c, v);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) part[(size_t)(c + j) * 128] = (int)v[j];
+                    l8_store16(g, r0 + c, n, own + (c >> 6) * 16, wsn, bias, v);
                 }
-                __threadfence();
-                asm volatile("bar.sync 1, %0;" ::"n"(32 * kL8PairEpi) : "memory");
-                if (threadIdx.x == 64 && ok) {
-                    __threadfence();
-                    s_last = atomicAdd(p.tickets + 2 * left + (int)rank, 1) == c1 - c0;
-                    __threadfence();
-                }
-                asm volatile("bar.sync 1, %0;" ::"n"(32 * kL8PairEpi) : "memory");
-                store = s_last != 0;
+                tc_fence_before();
+                __syncwarp();                                                          // (and everyone is done with the scales)
+                if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[as]), 0));
             }
-            if (store && ok) {
-                const float wsn = n < g.n ? __ldg(g.ws + n) : 0.f, bias = g.bias != nullptr && n < g.n ? __ldg(g.bias + n) : 0.f;
-#pragma unroll 1
-                for (int c = cs * 16; c < last_col; c += 64) {
-                    uint32_t v[16];
-                    int sum[16];
-                    tmem_ld16(at + (uint32_t)c, v);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) sum[j] = (int)v[j];
-                    for (int o = c0; o <= c1; ++o) {
-                        if (o == cl) continue;
-                        const int* part = part_of(o) + (size_t)c * 128;
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) sum[j] += __ldcg(part + j * 128);
-                    }
-                    l8_store16(g, r0 + c, n, wsn, bias, sum, twos);
-                }
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[as]), 0));
         }
     }
     if (!ok) l8_give_up(g.failed);

@@ -10,7 +10,6 @@ No autograd: results do not require gradients.
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
@@ -24,7 +23,6 @@ _FLOATS = {torch.float32: _lib.FL_DTYPE_F32, torch.bfloat16: _lib.FL_DTYPE_BF16,
 _TYPES = {**_FLOATS, torch.int8: _lib.FL_DTYPE_I8}
 _TOKENS = {torch.int32: 4, torch.int64: 8}
 MAX_TOP = 32
-_FEW_ROWS = 128
 
 
 def _refuse(msg: str):
@@ -132,12 +130,7 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, b
         y2 = _rows(out, what)
         ldy = y2.stride(0)
     lib = _lib.load()
-    if rows > _FEW_ROWS:
-        size = C.c_size_t()
-        _lib.check(lib.fl_linear8_workspace(rows, n, k, x_type, C.byref(size)))
-        room = size.value
-    else:                       # (what it answers for few rows)
-        room = 0 if x_type == _lib.FL_DTYPE_I8 else (rows * ((k + 15) // 16 * 16) + 255) // 256 * 256 + (4 * rows + 255) // 256 * 256
+    room = 0 if x_type == _lib.FL_DTYPE_I8 else (rows * ((k + 15) // 16 * 16) + 255) // 256 * 256 + 4 * rows       # (fl_linear8_workspace's rule)
     work = work_ptr = None
     if room:
         work = x.new_empty(room, dtype=torch.uint8)

@@ -55,7 +55,7 @@ class FlStackConfig(C.Structure):
                 ("tied_head", C.c_int32), ("loop_start", C.c_int32), ("loop_stop", C.c_int32), ("loop_times", C.c_int32),
                 ("loop_reinject", C.c_int32), ("loop_step", C.c_int32), ("norm_tanh", C.c_int32), ("parallel_sub", C.c_int32),
                 ("token_side", C.c_int32), ("bigram_buckets", C.c_int32), ("logit_scale", C.c_float), ("bigram_mul_prev", C.c_int64),
-                ("bigram_mul_cur", C.c_int64), ("reserved", C.c_int32 * 2)]
+                ("bigram_mul_cur", C.c_int64), ("head_bits", C.c_int32), ("reserved", C.c_int32 * 1)]
 
 
 class FastllmError(RuntimeError):
@@ -101,6 +101,7 @@ SYMBOLS = {
     "fl_forward_slots": (_I, [_VP, _VP, _VP, _VP, _I, _I, _VP, _VP]),
     "fl_cache_slot_reset": (_I, [_VP, _I]),
     "fl_cache_slot_len": (_I, [_VP, _I, C.POINTER(_I)]),
+    "fl_cache_logprobs": (_I, [_VP, _I, _VP, _I, C.c_double, _I, _VP, _VP, _VP, _VP, _VP]),
     "fl_cache_moe_routing": (_I, [_VP, _I, _VP, _VP]),
     "fl_forward_sample_device": (_I, [_VP, _VP, _VP, _I, _I, _SZ, _VP, C.POINTER(C.c_uint32)]),
     "fl_quantize_rows": (_I, [_VP, _I, _I64, _I64, _I64, _VP, _I64, _VP, _VP]),

@@ -4,6 +4,7 @@
 #include <cmath>
 #include <map>
 
+#include "ops.hpp"
 #include "layered_model.cuh"
 #include "layered_ops.cuh"
 #include "chunk_scan.cuh"
@@ -157,6 +158,8 @@ void layered_build(LayeredModel& m, const fl_layer_desc* descs) {
              "layered models: unknown arch");
     FL_CHECK(c.vocab >= 1 && c.width >= 1 && c.n_layers >= 1 && c.n_layers <= 4096, FL_ERR_INVALID, "layered models: sizes must be positive");
     FL_CHECK(c.compute_dtype == FL_DTYPE_BF16 || c.compute_dtype == FL_DTYPE_F32, FL_ERR_INVALID, "compute_dtype must be bf16 or f32");
+    FL_CHECK(c.head_bits == 0 || c.head_bits == 16 || (c.head_bits == 8 && c.compute_dtype == FL_DTYPE_BF16 && c.width <= 131071), FL_ERR_INVALID,
+             "head_bits is 16, or 8 in the serving precision (bf16)");
     FL_CHECK(!(c.no_pre_norm && c.no_post_norm), FL_ERR_INVALID, "a stack norms its sublayers' inputs, their outputs, or both");
     FL_CHECK(c.max_positions >= 0 && c.canon_taps >= 0 && c.canon_taps <= kMaxTaps, FL_ERR_INVALID, "bad position table / input convolution size");
     FL_CHECK(c.no_post_norm || !(c.gated_residual || c.depth_avg), FL_ERR_UNSUPPORTED,
@@ -703,6 +706,7 @@ void layered_finalize(LayeredModel& m) {
             }
         }
         map(m.head, m.V, m.W, m.tm_head, m.tc_head);
+        if (m.cfg.head_bits == 8) m.tc_head = false;
     }
     // the norms behind a sublayer park a row in shared memory: above the default 48 KB the kernels are told so once
     if ((!m.cfg.no_post_norm || m.cfg.token_side > 0) && (size_t)m.W * 4 > 48 * 1024) {
@@ -711,6 +715,15 @@ void layered_finalize(LayeredModel& m) {
         FL_CUDA(cudaFuncSetAttribute(ly_post_norm_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, m.W * 4));
         FL_CUDA(cudaFuncSetAttribute(ly_sum_norm_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, m.W * 4));
         FL_CUDA(cudaFuncSetAttribute(ly_sum_norm_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, m.W * 4));
+    }
+    if (m.cfg.head_bits == 8) {
+        const int64_t ld = padded8(m.W);
+        m.head8.alloc((size_t)m.V * ld);
+        m.head8_scale.alloc(m.V);
+        LaunchCtx lc;
+        op_quantize_rows(lc, m.head, FL_DTYPE_BF16, m.V, m.W, m.W, m.head8.p, ld, m.head8_scale.p);
+        FL_CUDA(cudaStreamSynchronize(lc.stream));
+        m.weight_bytes -= (uint64_t)m.V * m.W;          // (a byte a weight instead of two)
     }
     m.finalized = true;
 }
@@ -952,10 +965,11 @@ static void ensure_ws(fl_cache& c, size_t T, size_t n_want) {
         drop_graphs(c);
         const size_t N = std::max<size_t>(n_want, 2 * y.want_cap);
         y.hf.alloc(N * m.W); y.logits.alloc(N * m.V);
-        if (y.h_logits.n < N * m.V) y.h_logits.alloc(N * m.V);
+        if (m.cfg.head_bits == 8) y.head8_ws.alloc(linear8_workspace((int64_t)N, m.W));
         if (!m.f32) { y.hf_hi.alloc(N * m.W); y.hf_lo.alloc(N * m.W); }
         y.want_cap = N;
     }
+    if (!c.keep_logits && y.h_logits.n < y.want_cap * m.V) y.h_logits.alloc(y.want_cap * m.V);
 }
 
 // GEMMs that are not gemm_tc_kernel's: f32 FMA where they stand in for it on shapes outside its tiles (serving precision), the f64 tensor pipe in
@@ -1500,6 +1514,7 @@ void layered_forward(fl_cache& c, const int* slots, const int* counts, int n, co
     FL_CHECK(need_pages <= y.pool.pages_free(), FL_ERR_STATE, "cache page pool exhausted");
     for (long long i = 0; i < T; ++i) FL_CHECK(ids[i] < (uint32_t)m.V, FL_ERR_INVALID, "token id out of range");
     for (int k = 0; k < n_want; ++k) FL_CHECK(want[k] >= 0 && want[k] < T, FL_ERR_INVALID, "wanted row out of range");
+    c.logit_rows = 0;
     ensure_ws(c, (size_t)T, (size_t)n_want);
     reserve_portions(c, slots, counts, n);
     c.may_fail = false;
@@ -1584,6 +1599,7 @@ void layered_forward(fl_cache& c, const int* slots, const int* counts, int n, co
         r += counts[i];
         y.slot_last[slots[i]] = (int)ids[r - 1];
     }
+    c.logit_rows = n_want;
 }
 
 // One mixer over all rows of the step (`pass`: which pass of a loop, 0 elsewhere -- its own cache and state): reads its columns of the projected buffer y.proj (row stride lw.n_in; `in`: the same as
@@ -2089,7 +2105,10 @@ static void enqueue_step(fl_cache& c, LaunchCtx& lc, const StepTab& st, const in
         launch(lc, "final_norm", 0, ly_final_norm_kernel, dim3(n_want), dim3(nthr), 0, (const float*)y.x.p, st.want, norm_of(m.final_norm, m.final_bias, m.final_alpha),
                eps, W, m.cfg.logit_scale != 0.f ? m.cfg.logit_scale : 1.f, y.hf.p,
                m.tc_head ? y.hf_hi.p : (uint16_t*)nullptr, y.hf_lo.p);
-        gemm_tc_or_exact(c, lc, "gemm_head", y.hf.p, m.tc_head ? y.hf_hi.p : nullptr, y.hf_lo.p, m.head, m.tm_head, m.tc_head, m.V, W, y.logits.p, n_want);
+        if (m.cfg.head_bits == 8)
+            op_linear8(lc, y.hf.p, m.head8.p, m.head8_scale.p, n_want, m.V, W, y.logits.p, y.head8_ws.p);
+        else
+            gemm_tc_or_exact(c, lc, "gemm_head", y.hf.p, m.tc_head ? y.hf_hi.p : nullptr, y.hf_lo.p, m.head, m.tm_head, m.tc_head, m.V, W, y.logits.p, n_want);
         if (m.cfg.logit_softcap > 0.f) {
             const size_t nl = (size_t)n_want * m.V;
             launch(lc, "logit_cap", 0, ly_softcap_kernel, dim3((unsigned)std::min<size_t>(4 * kNumSMs, (nl + 255) / 256)), dim3(256), 0, y.logits.p, nl,

@@ -16,6 +16,7 @@
 #include "elementwise.cuh"
 #include "gemv.cuh"
 #include "model.cuh"
+#include "ops.hpp"
 #include "sampler.hpp"
 #include "synth.cuh"
 
@@ -1609,6 +1610,7 @@ static void check_call(fl_cache& c, const uint32_t* ids, int b, int t, size_t ro
 
 static void run_forward(fl_cache& c, const uint32_t* ids, int b, int t, size_t rope_offset) {
     check_call(c, ids, b, t, rope_offset, 0);
+    c.logit_rows = 0;
     c.may_fail = false;
     step_pairs(c, c.w->dense_ok ? (size_t)b * t : 0);
     if ((b * t >= 3 || c.w->cfg.arch == FL_ARCH_MIXTRAL) && c.w->dense_ok) ensure_dense_ws(c, b * t);
@@ -1632,6 +1634,7 @@ static void run_forward(fl_cache& c, const uint32_t* ids, int b, int t, size_t r
         enqueue_forward(c, lc, b, t, false);
     }
     c.kv_len += t;
+    c.logit_rows = b;
 }
 
 // Ragged forward (continuous batching): batch row i is the sequence in cache slot slots[i], which holds slot_len[slots[i]]
@@ -1657,6 +1660,7 @@ static void run_forward_slots(fl_cache& c, const int* slots, const uint32_t* ids
     }
     for (int i = 0; i < n * t; ++i) FL_CHECK(ids[i] < (uint32_t)w.Vfull, FL_ERR_INVALID, "token id out of range");
     c.may_fail = false;
+    c.logit_rows = 0;
     step_pairs(c, (size_t)n * t);
     ensure_dense_ws(c, n * t);
     c.dw.route_rows = n * t;
@@ -1683,6 +1687,7 @@ static void run_forward_slots(fl_cache& c, const int* slots, const uint32_t* ids
         enqueue_forward_dense(c, lc, n, t, false);
     }
     for (int i = 0; i < n; ++i) c.slot_len[slots[i]] += t;
+    c.logit_rows = n;
 }
 
 }  // namespace fl
@@ -1929,6 +1934,11 @@ static bool page_locked(const float* p, size_t n) {
 // through a page-locked one.  Either way nothing there changes unless the step was good -- or gave up on a copy of a block's own (the serial
 // recurrences): such a step is not waited for beforehand, its numbers may be there when the call returns the error.
 static void logits_to_host(fl_cache& c, float* host, size_t n) {
+    if (host == nullptr) {          // they stay on the device (fl_cache_logprobs)
+        FL_CUDA(cudaStreamSynchronize(c.stream));
+        step_check(c);
+        return;
+    }
     const float* dev = c.ly ? c.ly->logits.p : c.logits.p;
     if (page_locked(host, n)) {
         const bool before = c.may_fail || g_peer.ready;
@@ -1959,6 +1969,7 @@ static void layered_uniform(fl_cache& c, const int* slots, const uint32_t* ids, 
         FL_CHECK((size_t)c.slot_len[sl[i]] == off, FL_ERR_INVALID, "position offset differs from the tokens the sequence already holds");
         want[i] = i * t + t - 1;
     }
+    c.keep_logits = logits_host == nullptr;
     layered_forward(c, sl.data(), cnt.data(), n, ids, want.data(), n);
     logits_to_host(c, logits_host, (size_t)n * c.lm->V);
 }
@@ -2010,6 +2021,49 @@ FL_EXPORT int fl_cache_slot_len(fl_cache* c, int slot, int* out) {
     FL_CHECK(c && out, FL_ERR_INVALID, "NULL argument");
     FL_CHECK(slot >= 0 && slot < c->max_batch, FL_ERR_INVALID, "slot index out of range");
     *out = c->slot_len[slot];
+    FL_API_END
+}
+
+FL_EXPORT int fl_cache_logprobs(fl_cache* c, int rows, const int32_t* tokens, int given, double temperature, int top, float* logprob, float* logsumexp,
+                                float* entropy, int32_t* top_ids, float* top_logprobs) {
+    FL_API_BEGIN
+    FL_CHECK(c != nullptr, FL_ERR_INVALID, "NULL argument");
+    FL_CHECK(rows >= 0 && given >= 0 && top >= 0 && (given == 0 || tokens != nullptr || rows == 0), FL_ERR_INVALID, "bad argument");
+    FL_CHECK(!c->poisoned, FL_ERR_CUDA, "cache poisoned by an earlier CUDA error");
+    FL_CHECK(rows <= c->logit_rows, FL_ERR_STATE, "the last forward on this cache left logits of " + std::to_string(c->logit_rows) + " rows");
+    const size_t V = c->ly ? c->lm->V : c->w->Vfull;
+    FL_CHECK(given <= (1 << 20) && top <= 32 && (size_t)top <= V, FL_ERR_INVALID, "from 0 to 32 alternatives, no more than the vocabulary has, and at most 2^20 given tokens a row");
+    if (rows == 0) return FL_OK;
+    use_device();
+    try {
+        const size_t n = (size_t)rows * 4, tok = n * given, res = n * (given + 2 + 2 * (size_t)top);
+        if (c->lp_dev.n < tok + res) {
+            FL_CUDA(cudaStreamSynchronize(c->stream));
+            c->lp_dev.alloc(tok + res);
+            c->lp_host.alloc(tok + res);
+        }
+        if (tok > 0) {
+            std::memcpy(c->lp_host.p, tokens, tok);
+            FL_CUDA(cudaMemcpyAsync(c->lp_dev.p, c->lp_host.p, tok, cudaMemcpyHostToDevice, c->stream));
+        }
+        auto at = [&](uint8_t* base, size_t words) { return reinterpret_cast<float*>(base + tok + n * words); };
+        uint8_t* d = c->lp_dev.p;
+        LaunchCtx lc;
+        lc.stream = c->stream;
+        op_logprobs(lc, c->ly ? c->ly->logits.p : c->logits.p, rows, V, reinterpret_cast<const int32_t*>(d), given, temperature, top, at(d, 2), at(d, 0), at(d, 1),
+                    reinterpret_cast<int32_t*>(at(d, 2 + given)), at(d, 2 + given + top));
+        uint8_t* h = c->lp_host.p;
+        FL_CUDA(cudaMemcpyAsync(h + tok, d + tok, res, cudaMemcpyDeviceToHost, c->stream));
+        FL_CUDA(cudaStreamSynchronize(c->stream));
+        if (logsumexp) std::memcpy(logsumexp, at(h, 0), n);
+        if (entropy) std::memcpy(entropy, at(h, 1), n);
+        if (logprob) std::memcpy(logprob, at(h, 2), n * given);
+        if (top_ids) std::memcpy(top_ids, at(h, 2 + given), n * top);
+        if (top_logprobs) std::memcpy(top_logprobs, at(h, 2 + given + top), n * top);
+    } catch (const fl::Error& e) {
+        if (e.code == FL_ERR_CUDA) c->poisoned = true;
+        throw;
+    }
     FL_API_END
 }
 
@@ -2065,7 +2119,7 @@ FL_EXPORT int fl_cache_destroy(fl_cache* c) {
 
 FL_EXPORT int fl_forward(fl_model* m, fl_cache* c, const uint32_t* ids, int b, int t, size_t rope_offset, float* logits_host) {
     FL_API_BEGIN
-    FL_CHECK(m && c && logits_host, FL_ERR_INVALID, "NULL argument");
+    FL_CHECK(m && c, FL_ERR_INVALID, "NULL argument");
     if (m->lay != nullptr) {
         FL_CHECK(m->lay.get() == c->lm.get(), FL_ERR_INVALID, "cache belongs to a different model");
         use_device();
@@ -2117,6 +2171,7 @@ FL_EXPORT int fl_decode_greedy_loop(fl_model* m, fl_cache* c, const uint32_t* fi
     use_device();
     try {
         check_call(*c, first_ids, b, 1, rope_offset, steps - 1);
+        c->logit_rows = 0;
         step_pairs(*c, c->w->dense_ok ? (size_t)b : 0);
         if ((b >= 3 || c->w->cfg.arch == FL_ARCH_MIXTRAL) && c->w->dense_ok) ensure_dense_ws(*c, b);
         if (c->trace_cap < (size_t)steps * b) {
@@ -2261,7 +2316,7 @@ FL_EXPORT int fl_forward_sample(fl_model* m, fl_cache* c, const uint32_t* ids, i
 FL_EXPORT int fl_forward_slots(fl_model* m, fl_cache* c, const int* slots, const uint32_t* ids, int n, int t, const size_t* rope_offsets,
                                float* logits_host) {
     FL_API_BEGIN
-    FL_CHECK(m && c && logits_host, FL_ERR_INVALID, "NULL argument");
+    FL_CHECK(m && c, FL_ERR_INVALID, "NULL argument");
     if (m->lay != nullptr) {
         FL_CHECK(m->lay.get() == c->lm.get(), FL_ERR_INVALID, "cache belongs to a different model");
         FL_CHECK(slots && rope_offsets, FL_ERR_INVALID, "NULL argument");
@@ -2293,9 +2348,9 @@ FL_EXPORT int fl_forward_ragged(fl_model* m, fl_cache* c, const int* slots, cons
     FL_CHECK(m && c, FL_ERR_INVALID, "NULL argument");
     FL_CHECK(m->lay != nullptr && c->ly != nullptr, FL_ERR_UNSUPPORTED, "mixed batches of unequal portions are offered for layered models only");
     FL_CHECK(m->lay.get() == c->lm.get(), FL_ERR_INVALID, "cache belongs to a different model");
-    FL_CHECK(n_want == 0 || logits_host != nullptr, FL_ERR_INVALID, "NULL argument");
     use_device();
     try {
+        c->keep_logits = logits_host == nullptr;
         layered_forward(*c, slots, counts, n, ids, want, n_want);
         if (n_want > 0) logits_to_host(*c, logits_host, (size_t)n_want * m->lay->V);
         else layered_finish(*c);

@@ -5,7 +5,7 @@
 #include "bert_model.cuh"
 #include "linear8.cuh"
 #include "logprobs.cuh"
-#include "runtime.cuh"
+#include "ops.hpp"
 
 namespace fl {
 
@@ -23,11 +23,9 @@ static LaunchCtx op_ctx(void* stream) {
     LaunchCtx lc;
     lc.stream = static_cast<cudaStream_t>(stream);
     lc.pdl = false;
-    if (g_prof.on) {                        // (no events inside a caller's capture)
-        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-        FL_CUDA(cudaStreamIsCapturing(lc.stream, &st));
-        lc.capturing = st != cudaStreamCaptureStatusNone;
-    }
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    FL_CUDA(cudaStreamIsCapturing(lc.stream, &st));
+    lc.capturing = st != cudaStreamCaptureStatusNone;       // (no events inside a caller's capture, and nothing launched)
     return lc;
 }
 static size_t dtype_size(int dtype) { return dtype == FL_DTYPE_F32 ? 4 : dtype == FL_DTYPE_I8 ? 1 : 2; }
@@ -37,7 +35,6 @@ static bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_
 constexpr int64_t kMaxRows = (int64_t)1 << 30;
 constexpr int64_t kLinear8MaxK = 131071;        // 128 * 128 * k stays below 2^31
 
-static int64_t padded_k(int64_t k) { return (k + 15) / 16 * 16; }
 static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // How a product of more than kL8FewRows rows goes over the pairs of SMs: the tile width whose waves cost least, by what a k block takes (see
@@ -67,7 +64,7 @@ struct L8Room { size_t scale = 0, all = 0; };
 static L8Room linear8_room(int64_t rows, int64_t k, bool given) {
     L8Room r;
     if (given) return r;
-    r.scale = up256((size_t)rows * padded_k(k));
+    r.scale = up256((size_t)rows * padded8(k));
     r.all = r.scale + (size_t)rows * 4;
     return r;
 }
@@ -105,7 +102,8 @@ static void launch_op(LaunchCtx& lc, const char* tag, uint64_t bytes, void (*ker
         FL_CUDA(cudaEventRecord(pe.e1, lc.stream));
         g_prof.entries.push_back(pe);
     }
-    g_launches.fetch_add(1, std::memory_order_relaxed);
+    if (lc.capturing) lc.captured++;
+    else g_launches.fetch_add(1, std::memory_order_relaxed);
 }
 
 // What the operators keep for the process: one page-locked word that a kernel sets when a wait inside it ran out; the next call reports it.
@@ -180,6 +178,27 @@ static void launch_pair(LaunchCtx& lc, uint64_t bytes, const int8_t* x, int64_t 
     launch_op(lc, "linear8", bytes, linear8_pair_kernel, dim3((unsigned)(2 * clusters)), kL8PairThreads, kL8PairSmem, 1, pdl, tw, tx, g, p);
 }
 
+static void run_linear8(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
+                        int64_t rows, int64_t n, int64_t k, void* y, int y_dtype, int64_t ldy, void* workspace) {
+    const bool given = x_dtype == FL_DTYPE_I8;
+    const int8_t* q = static_cast<const int8_t*>(x);
+    int64_t ldq = rows == 1 ? padded8(k) : ldx;
+    Linear8Args g{(int)rows, (int)n, (int)k, x_scale, w_scale, bias, y, ldy, y_dtype, g_op_failed};
+    if (!given) {
+        int8_t* to = static_cast<int8_t*>(workspace);
+        float* s = reinterpret_cast<float*>(to + linear8_room(rows, k, false).scale);
+        quantize_rows(lc, x, x_dtype, rows, k, ldx, to, padded8(k), padded8(k), s);
+        q = to; ldq = padded8(k); g.xs = s;
+    }
+    if (n == 1) ldw = padded8(k);
+    const uint64_t bytes = (uint64_t)n * k + (uint64_t)rows * (k + n * dtype_size(y_dtype));
+    if (rows > kL8FewRows) launch_pair(lc, bytes, q, ldq, w, ldw, g, !given);
+    else if (rows <= 16) launch_few<16>(lc, bytes, q, ldq, w, ldw, g, !given);
+    else if (rows <= 32) launch_few<32>(lc, bytes, q, ldq, w, ldw, g, !given);
+    else if (rows <= 64) launch_few<64>(lc, bytes, q, ldq, w, ldw, g, !given);
+    else launch_few<128>(lc, bytes, q, ldq, w, ldw, g, !given);
+}
+
 // Blocks per row: as many as the chip holds (four per SM) over the rows, while every warp still has a chunk of two; the cluster of 16 is not portable
 // to every chip, but B200 has it.
 template <typename T>
@@ -193,6 +212,34 @@ static void run_logprobs(LaunchCtx& lc, const LogprobArgs& a) {
     auto go = [&](auto kern, int threads) { launch_op(lc, "logprobs", bytes, kern, grid, threads, smem, C, false, a, C); };
     if (C == 1) a.top > 0 ? go(logprobs_kernel<T, true, 128>, 128) : go(logprobs_kernel<T, false, 128>, 128);
     else a.top > 0 ? go(logprobs_kernel<T, true, 256>, 256) : go(logprobs_kernel<T, false, 256>, 256);
+}
+
+template <typename T>
+static void run_logprobs(LaunchCtx& lc, LogprobArgs a, double temperature) {
+    a.inv_t = (float)(1.0 / temperature);
+    a.c = (float)(1.4426950408889634 / temperature);
+    run_logprobs<T>(lc, a);
+}
+static void check_temperature(double temperature) {
+    const float inv_t = (float)(1.0 / temperature), c = (float)(1.4426950408889634 / temperature);
+    FL_CHECK(temperature > 0 && std::isfinite(temperature) && std::isfinite(c) && inv_t > 0, FL_ERR_INVALID, "logprobs: the temperature is a positive number");
+}
+
+size_t linear8_workspace(int64_t rows, int64_t k) { return linear8_room(rows, k, false).all; }
+void op_quantize_rows(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale) {
+    quantize_rows(lc, x, dtype, rows, cols, ldx, q, ldq, ldq, scale);
+}
+void op_linear8(LaunchCtx& lc, const float* x, const int8_t* w, const float* w_scale, int64_t rows, int64_t n, int64_t k, float* y, void* workspace) {
+    check_op_failed();
+    run_linear8(lc, x, FL_DTYPE_F32, k, nullptr, w, padded8(k), w_scale, nullptr, rows, n, k, y, FL_DTYPE_F32, n, workspace);
+}
+void op_logprobs(LaunchCtx& lc, const float* logits, int64_t rows, int64_t vocab, const int32_t* tokens, int64_t given, double temperature, int top, float* logprob,
+                 float* logsumexp, float* entropy, int32_t* top_ids, float* top_logprobs) {
+    FL_CHECK(vocab <= kLpMaxVocab, FL_ERR_UNSUPPORTED, "logprobs: a vocabulary of at most 2^20");
+    FL_CHECK(top >= 0 && top <= kLpMaxTop && top <= vocab, FL_ERR_INVALID, "logprobs: from 0 to 32 alternatives, and no more than the vocabulary has");
+    check_temperature(temperature);
+    run_logprobs<float>(lc, LogprobArgs{logits, vocab, (int)rows, (int)vocab, 1.f, 1.f, tokens, (int)given, 0, top, given ? logprob : nullptr, logsumexp, entropy, top_ids,
+                                        top_logprobs}, temperature);
 }
 
 }  // namespace fl
@@ -247,23 +294,7 @@ FL_EXPORT int fl_linear8(const void* x, int x_dtype, int64_t ldx, const float* x
     DeviceScope dev;
     LaunchCtx lc = op_ctx(stream);
     check_op_failed();
-    const int8_t* q = static_cast<const int8_t*>(x);
-    int64_t ldq = rows == 1 ? padded_k(k) : ldx;
-    Linear8Args g{(int)rows, (int)n, (int)k, x_scale, w_scale, bias, y, ldy, y_dtype, g_op_failed};
-    uint8_t* ws = static_cast<uint8_t*>(workspace);
-    if (!given) {
-        int8_t* to = reinterpret_cast<int8_t*>(ws);
-        float* s = reinterpret_cast<float*>(ws + room.scale);
-        quantize_rows(lc, x, x_dtype, rows, k, ldx, to, padded_k(k), padded_k(k), s);
-        q = to; ldq = padded_k(k); g.xs = s;
-    }
-    if (n == 1) ldw = padded_k(k);
-    const uint64_t bytes = (uint64_t)n * k + (uint64_t)rows * (k + n * dtype_size(y_dtype));
-    if (rows > kL8FewRows) launch_pair(lc, bytes, q, ldq, w, ldw, g, !given);
-    else if (rows <= 16) launch_few<16>(lc, bytes, q, ldq, w, ldw, g, !given);
-    else if (rows <= 32) launch_few<32>(lc, bytes, q, ldq, w, ldw, g, !given);
-    else if (rows <= 64) launch_few<64>(lc, bytes, q, ldq, w, ldw, g, !given);
-    else launch_few<128>(lc, bytes, q, ldq, w, ldw, g, !given);
+    run_linear8(lc, x, x_dtype, ldx, x_scale, w, ldw, w_scale, bias, rows, n, k, y, y_dtype, ldy, workspace);
     FL_API_END
 }
 
@@ -275,20 +306,17 @@ FL_EXPORT int fl_logprobs(const void* logits, int dtype, int64_t rows, int64_t v
     FL_CHECK(rows <= 1 || ld >= vocab, FL_ERR_INVALID, "logprobs: the row stride is smaller than the vocabulary");
     FL_CHECK(given >= 0 && given <= kLpMaxVocab && (given == 0 || token_bytes == 4 || token_bytes == 8), FL_ERR_INVALID, "logprobs: given tokens are 32- or 64-bit integers");
     FL_CHECK(top >= 0 && top <= kLpMaxTop && top <= vocab, FL_ERR_INVALID, "logprobs: from 0 to 32 alternatives, and no more than the vocabulary has");
-    const float inv_t = (float)(1.0 / temperature);
-    FL_CHECK(temperature > 0 && std::isfinite(temperature) && std::isfinite(inv_t) && inv_t > 0, FL_ERR_INVALID, "logprobs: the temperature is a positive number");
+    check_temperature(temperature);
     if (rows == 0) return FL_OK;
     FL_CHECK(logits && (given == 0 || (tokens && logprob)) && (top == 0 || (top_ids && top_logprobs)), FL_ERR_INVALID, "NULL argument");
     FL_CHECK(aligned(logits, dtype_size(dtype)) && (given == 0 || aligned(tokens, token_bytes)) && aligned(logprob, 4) && aligned(logsumexp, 4) && aligned(entropy, 4) &&
                  aligned(top_ids, 4) && aligned(top_logprobs, 4), FL_ERR_INVALID, "logprobs: a pointer is not aligned to its type");
     DeviceScope dev;
     LaunchCtx lc = op_ctx(stream);
-    const float c = (float)(1.4426950408889634 / temperature);
-    FL_CHECK(std::isfinite(c) && c > 0, FL_ERR_INVALID, "logprobs: the temperature is a positive number");
-    const LogprobArgs a{logits, ld, (int)rows, (int)vocab, inv_t, c, tokens, (int)given, token_bytes == 8, top, given ? logprob : nullptr, logsumexp, entropy, top_ids, top_logprobs};
-    if (dtype == FL_DTYPE_F32) run_logprobs<float>(lc, a);
-    else if (dtype == FL_DTYPE_BF16) run_logprobs<__nv_bfloat16>(lc, a);
-    else run_logprobs<__half>(lc, a);
+    const LogprobArgs a{logits, ld, (int)rows, (int)vocab, 1.f, 1.f, tokens, (int)given, token_bytes == 8, top, given ? logprob : nullptr, logsumexp, entropy, top_ids, top_logprobs};
+    if (dtype == FL_DTYPE_F32) run_logprobs<float>(lc, a, temperature);
+    else if (dtype == FL_DTYPE_BF16) run_logprobs<__nv_bfloat16>(lc, a, temperature);
+    else run_logprobs<__half>(lc, a, temperature);
     FL_API_END
 }
 

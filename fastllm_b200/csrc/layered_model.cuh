@@ -124,6 +124,8 @@ struct LayeredModel {
     float *final_norm = nullptr, *final_bias = nullptr, *final_alpha = nullptr;
     CUtensorMap tm_head{};
     bool tc_head = false;
+    DevBuf<int8_t> head8;               // head_bits = 8: [V, padded8(W)] and a scale per row
+    DevBuf<float> head8_scale;
     std::set<std::string> have;
     std::vector<std::string> expected;
     int ignored = 0;
@@ -153,6 +155,7 @@ struct LayeredCache {
     size_t tab_cap = 0;
     // workspace for `rows` tokens of a step
     size_t rows = 0, want_cap = 0;
+    DevBuf<uint8_t> head8_ws;           // head_bits = 8: the wanted rows, rounded
     DevBuf<float> x, h, y, proj, la, u, go, qa, ol, gu, act, eo, sh_gu, sh_act, sh_o, route_w, sgate, hf, logits;
     DevBuf<float> hc, gz, y2, xs;       // convolved sublayer input; gate pre-activations; the second mixer's projected output;
                                         // xs [L + 1][rows][W]: the embedding output and every layer's own result (depth average); a

@@ -171,6 +171,10 @@ struct fl_cache {
     fl::PinnedBuf<int> step_failed;  // one word: a wait inside a kernel ran out (see step_check)
     bool may_fail = false;           // the step launched kernels that report there
     bool poisoned = false;
+    int logit_rows = 0;              // rows of the last forward's logits (fl_cache_logprobs); 0: none
+    bool keep_logits = false;        // the forward at hand leaves them on the device
+    fl::DevBuf<uint8_t> lp_dev;      // fl_cache_logprobs: tokens and results
+    fl::HostBuf<uint8_t> lp_host;
 };
 
 namespace fl {

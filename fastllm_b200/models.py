@@ -18,6 +18,7 @@ from __future__ import annotations
 import ctypes as C
 import json
 from dataclasses import dataclass
+from typing import NamedTuple, Optional
 
 import numpy as np
 
@@ -189,6 +190,15 @@ class _ResultPool:
         self.free.clear()
 
 
+class LogProbs(NamedTuple):
+    """What DeviceCache.logprobs returns, host arrays: per row of the last forward's logits."""
+    logprob: Optional[np.ndarray]           # f32, as tokens; None without tokens
+    logsumexp: np.ndarray                   # f32 [rows]
+    entropy: np.ndarray                     # f32 [rows]
+    top_ids: np.ndarray                     # int32 [rows, top]
+    top_logprobs: np.ndarray                # f32 [rows, top]
+
+
 class DeviceCache:
     """fl_cache*: paged KV cache + per-cache stream/workspaces.  The logits arrays that its calls return may lie over page-locked memory of the
     cache's pool (see _ResultPool): they are the caller's like any array and outlive the cache, but do not own their memory, so that
@@ -209,10 +219,11 @@ class DeviceCache:
         self.results = _ResultPool(self.lib)
         self.results.reserve((max_batch, self.vocab))
 
-    def forward_ragged(self, slots, token_lists, want=None) -> np.ndarray:
+    def forward_ragged(self, slots, token_lists, want=None, fetch: bool = True):
         """One step of a mixed batch (layered models): sequence i lives in slot slots[i] and is fed token_lists[i] (a portion of its
         prompt, or one decoded token) after what the slot already holds.  want: per sequence the places inside its portion whose
-        logits are asked for (None = the last token of every portion).  -> f32 [sum of wanted places, vocab], sequence-major."""
+        logits are asked for (None = the last token of every portion).  -> f32 [sum of wanted places, vocab], sequence-major; fetch=False:
+        they stay on the device (logprobs), -> None."""
         n = len(slots)
         counts = np.asarray([len(t) for t in token_lists], dtype=np.int32)
         if len(token_lists) != n or (counts < 1).any():
@@ -230,11 +241,31 @@ class DeviceCache:
                     rows.append(int(starts[i]) + int(p))
         rows = np.asarray(rows, dtype=np.int32)
         sl = np.ascontiguousarray(slots, dtype=np.int32)
-        out = self.results.empty((len(rows), self.vocab))
+        out = self.results.empty((len(rows), self.vocab)) if fetch else None
         _lib.check(self.lib.fl_forward_ragged(self.model.h, self.h, sl.ctypes.data_as(C.c_void_p), counts.ctypes.data_as(C.c_void_p), n,
                                               ids.ctypes.data_as(C.c_void_p), rows.ctypes.data_as(C.c_void_p), len(rows),
-                                              out.ctypes.data_as(C.c_void_p)))
+                                              out.ctypes.data_as(C.c_void_p) if fetch else None))
         return out
+
+    def logprobs(self, tokens=None, top: int = 0, temperature: float = 1.0, rows: int | None = None) -> LogProbs:
+        """Log probabilities over the logits of the last forward on this cache, which are still on the device (fl_cache_logprobs): of
+        `tokens` ([rows] or [rows, m]; negative ones are padding with 0), and of the `top` most likely alternatives.  rows: the first
+        that many rows of that forward (default: as tokens has)."""
+        tok = None if tokens is None else np.ascontiguousarray(tokens, dtype=np.int32)
+        if tok is not None and tok.ndim not in (1, 2):
+            raise FastllmError(-1, f"tokens are [rows] or [rows, m], got shape {tok.shape}")
+        n = rows if rows is not None else (0 if tok is None else tok.shape[0])
+        if tok is not None and tok.shape[0] != n:
+            raise FastllmError(-1, f"{tok.shape[0]} rows of tokens for {n} rows of logits")
+        given = 0 if tok is None else (1 if tok.ndim == 1 else tok.shape[1])
+        if n < 0 or top < 0:
+            raise FastllmError(-1, "a number of rows or alternatives is negative")
+        lp = None if tok is None else np.empty(tok.shape, dtype=np.float32)
+        r = LogProbs(lp, np.empty(n, np.float32), np.empty(n, np.float32), np.empty((n, top), np.int32), np.empty((n, top), np.float32))
+        ptr = lambda a: None if a is None or a.size == 0 else a.ctypes.data_as(C.c_void_p)  # noqa: E731
+        _lib.check(self.lib.fl_cache_logprobs(self.h, n, ptr(tok), given, float(temperature), top, ptr(lp), ptr(r.logsumexp), ptr(r.entropy), ptr(r.top_ids),
+                                              ptr(r.top_logprobs)))
+        return r
 
     def pool_stats(self):
         """-> (pages of the pool, pages free)"""
@@ -673,9 +704,10 @@ class _LayeredBase(_CausalBase):
         raise NotImplementedError
 
     @classmethod
-    def initialize_model(cls, config: dict, tensors, dtype="bf16", device: int = 0, *, random_seed=None, std: float = 0.02, **hints):
+    def initialize_model(cls, config: dict, tensors, dtype="bf16", device: int = 0, *, random_seed=None, std: float = 0.02, head_bits: int = 16, **hints):
         """tensors: dict or iterable of (name, array) (f32 / f16 / uint16 bf16 bits), or None for synthetic weights.  dtype "bf16":
-        the serving precision; "f32": every product and the cache in true 32-bit."""
+        the serving precision; "f32": every product and the cache in true 32-bit.  head_bits = 8 (serving precision): the output
+        projection is a product in 8-bit integers with a scale per vocabulary row and per token."""
         if dtype not in ("bf16", "bfloat16", "f32", "float32"):
             raise FastllmError(-1, f"unsupported dtype {dtype!r}")
         items, shapes = None, {}
@@ -689,6 +721,7 @@ class _LayeredBase(_CausalBase):
         sc.compute_dtype = _lib.FL_DTYPE_F32 if dtype in ("f32", "float32") else _lib.FL_DTYPE_BF16
         sc.norm_plain, sc.no_pre_norm, sc.no_post_norm = int(cls.norm_plain), int(cls.no_pre_norm), int(cls.no_post_norm)
         cls.stack_options(config, sc)
+        sc.head_bits = int(head_bits)
         dev = DeviceModel(sc, device, layers=cls.layer_descs(config, shapes, **hints))
         if items is None:
             dev.random_init(0 if random_seed is None else random_seed, std)
@@ -1063,15 +1096,18 @@ def model_class_for(config: dict):
     raise FastllmError(-5, f"no registered model supports {names}")
 
 
-def load_model(model_dir: str, dtype: str = "bf16", device: int = 0):
-    """config.json + safetensors of a folder -> (adapter instance, cache handle), the class chosen by the registry."""
+def load_model(model_dir: str, dtype: str = "bf16", device: int = 0, head_bits: int = 16):
+    """config.json + safetensors of a folder -> (adapter instance, cache handle), the class chosen by the registry.  head_bits: see
+    _LayeredBase.initialize_model."""
     import os
     from . import safetensors_io
     with open(os.path.join(model_dir, "config.json")) as f:
         config = json.load(f)
     cls = model_class_for(config)
     if issubclass(cls, _LayeredBase):
-        return cls.initialize_model(config, safetensors_io.iter_tensors(model_dir, copy=True), dtype, device)
+        return cls.initialize_model(config, safetensors_io.iter_tensors(model_dir, copy=True), dtype, device, head_bits=head_bits)
+    if head_bits != 16:
+        raise FastllmError(-5, "an 8-bit output projection is offered for layered models only")
     cf = ConfigFile(config["hidden_size"], config["intermediate_size"], config["vocab_size"], config["num_hidden_layers"],
                     config["num_attention_heads"], config.get("num_key_value_heads"), config.get("rms_norm_eps", 1e-5),
                     config.get("rope_theta"), config.get("max_position_embeddings"), config.get("sliding_window"),
@@ -1232,10 +1268,28 @@ class ContinuousBatcher:
             self.cache = DeviceCache(model.dev, max_batch, model._capacity())
         self.steps = 0          # ragged decode forwards issued (tests / stats)
 
-    def generate(self, prompts, max_tokens: int, temperature: float = 0.0):
-        """-> one id list per prompt, in request order."""
+    def generate(self, prompts, max_tokens: int, temperature: float = 0.0, logprobs: int | None = None):
+        """-> one id list per prompt, in request order.  logprobs = K (0 to 32): -> (id lists, per prompt and token a dict with the token's
+        "logprob" and "top", the K most likely (id, logprob) pairs), from the distribution at temperature 1 on the device."""
+        self._told = None if logprobs is None else [[] for _ in prompts]
+        out = self._generate(prompts, max_tokens, temperature, logprobs)
+        told, self._told = self._told, None
+        return out if logprobs is None else (out, told)
+
+    def _tell(self, picked, rows: int, top):
+        """picked: (row of the last forward, request, token) of the tokens that were emitted"""
+        if self._told is None or not picked:
+            return
+        tokens = np.full(rows, -1, dtype=np.int32)
+        for row, _, tok in picked:
+            tokens[row] = tok
+        lp = self.cache.logprobs(tokens, top)
+        for row, req, _ in picked:
+            self._told[req].append({"logprob": float(lp.logprob[row]), "top": [(int(i), float(v)) for i, v in zip(lp.top_ids[row], lp.top_logprobs[row])]})
+
+    def _generate(self, prompts, max_tokens: int, temperature: float, logprobs):
         if self.prefill_chunk and hasattr(self.cache, "forward_ragged"):
-            return self._generate_mixed(prompts, max_tokens, temperature)
+            return self._generate_mixed(prompts, max_tokens, temperature, logprobs)
         out = [[] for _ in prompts]
         waiting = list(range(len(prompts)))[::-1]
         free = list(range(self.max_batch))[::-1]
@@ -1243,13 +1297,16 @@ class ContinuousBatcher:
         if max_tokens <= 0:
             return out
 
-        def take(logits_row, req, slot, state):
+        picked = []             # what was emitted of the last forward
+
+        def take(logits_row, req, slot, state, row=0):
             """sample -> EOS / budget -> either keep the slot running or free it"""
             tok = state[2].sample(logits_row)
             if self.eos_token_id is not None and tok == self.eos_token_id:
                 done = True
             else:
                 out[req].append(tok)
+                picked.append((row, req, tok))
                 state[3] = tok
                 done = len(out[req]) >= max_tokens
             if done:
@@ -1265,21 +1322,25 @@ class ContinuousBatcher:
                 ids = np.asarray(prompts[req], dtype=np.uint32).reshape(1, -1)
                 logits = self.cache.forward_slots([slot], ids, [0])
                 state = [req, 1 if self.position_per_call else ids.shape[1], LogitsProcessor(0, float(np.float32(temperature))), 0]
+                picked.clear()
                 take(np.asarray(logits)[0].reshape(-1), req, slot, state)
+                self._tell(picked, 1, logprobs)
             if not running:
                 continue
             slots = sorted(running)
             ids = np.array([[running[s][3]] for s in slots], dtype=np.uint32)
             logits = np.asarray(self.cache.forward_slots(slots, ids, [running[s][1] for s in slots]))
             self.steps += 1
+            picked.clear()
             for i, s in enumerate(slots):
                 st = running[s]
                 st[1] += 1
-                take(logits[i].reshape(-1), st[0], s, st)
+                take(logits[i].reshape(-1), st[0], s, st, i)
+            self._tell(picked, len(slots), logprobs)
         return out
 
 
-    def _generate_mixed(self, prompts, max_tokens: int, temperature: float):
+    def _generate_mixed(self, prompts, max_tokens: int, temperature: float, logprobs=None):
         """Mixed steps: a request takes a free slot as soon as there is one; each step carries, per running request, either the next
         portion of its prompt (at most prefill_chunk tokens) or its one new token.  Sampling, EOS and the token budget are those of
         generate(); a finished request gives its slot (pages and state) back."""
@@ -1308,7 +1369,7 @@ class ContinuousBatcher:
                     want.append([0])
             logits = np.asarray(self.cache.forward_ragged(slots, toks, want))
             self.steps += 1
-            row = 0
+            row, picked = 0, []
             for s, w in zip(slots, want):
                 if not w:
                     continue
@@ -1319,13 +1380,67 @@ class ContinuousBatcher:
                     done = True
                 else:
                     out[st[0]].append(tok)
+                    picked.append((row - 1, st[0], tok))
                     st[3] = tok
                     done = len(out[st[0]]) >= max_tokens
                 if done:
                     running.pop(s)
                     self.cache.slot_reset(s)
                     free.append(s)
+            self._tell(picked, row, logprobs)
         return out
+
+
+class Scored(NamedTuple):
+    """One text's scores: entry i is about token i + 1, given the tokens up to i."""
+    logprobs: np.ndarray            # f32 [n - 1]
+    entropy: np.ndarray             # f32 [n - 1]
+    top_ids: np.ndarray             # int32 [n - 1, top]
+    top_logprobs: np.ndarray        # f32 [n - 1, top]
+
+    @property
+    def total(self) -> float:
+        return float(np.sum(self.logprobs, dtype=np.float64))
+
+
+def score(model, texts, top: int = 0, cache: DeviceCache | None = None, portion: int = 512) -> list:
+    """Log probabilities of given texts (token id lists) under a layered model -> one Scored per text.  Up to the cache's slots of texts are
+    read side by side, at most `portion` tokens a step; logits stay on the device, where they become log probabilities."""
+    if cache is None:
+        if not hasattr(model, "new_device_cache"):
+            raise FastllmError(-5, "scoring wants the logits of every position: mixed-batch steps, offered for layered models only")
+        cache = model.new_device_cache(max(1, min(len(texts), 8)), max([64] + [len(t) for t in texts]))
+    if portion < cache.max_batch:
+        raise FastllmError(-1, "a step brings at least one token of every text that is being read")
+    parts = [[] for _ in texts]
+    waiting = [i for i, t in enumerate(texts) if len(t) > 1][::-1]
+    free, running = list(range(cache.max_batch))[::-1], {}      # slot -> [text, tokens fed]
+    while waiting or running:
+        while waiting and free:
+            running[free.pop()] = [waiting.pop(), 0]
+        slots, toks, want, given = sorted(running), [], [], []
+        room = portion
+        for k, s in enumerate(slots):
+            t, fed = running[s]
+            part = [int(x) for x in texts[t][fed:fed + max(1, room - (len(slots) - 1 - k))][:len(texts[t]) - 1 - fed]]      # (the last token is only asked for)
+            room -= len(part)
+            toks.append(part)
+            want.append(range(len(part)))
+            given.extend(int(x) for x in texts[t][fed + 1:fed + 1 + len(part)])
+        cache.forward_ragged(slots, toks, want, fetch=False)
+        lp, row = cache.logprobs(np.asarray(given, dtype=np.int32), top), 0
+        for s, part in zip(slots, toks):
+            t = running[s][0]
+            at = slice(row, row + len(part))
+            parts[t].append((lp.logprob[at], lp.entropy[at], lp.top_ids[at], lp.top_logprobs[at]))
+            row += len(part)
+            running[s][1] += len(part)
+            if running[s][1] >= len(texts[t]) - 1:
+                running.pop(s)
+                cache.slot_reset(s)
+                free.append(s)
+    none = (np.empty(0, np.float32), np.empty(0, np.float32), np.empty((0, top), np.int32), np.empty((0, top), np.float32))
+    return [Scored(*(np.concatenate(c) for c in zip(*(p or [none])))) for p in parts]
 
 
 # --------------------------------------------------------------------------------------------------------------------

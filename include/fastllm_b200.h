@@ -275,7 +275,9 @@ typedef struct fl_stack_config {
                                           the embedding, the last row for a sequence's first token; the previous token is kept per slot */
     float logit_scale;                 /* != 0: logits are multiplied by this (before a cap) */
     int64_t bigram_mul_prev, bigram_mul_cur;
-    int32_t reserved[2];
+    int32_t head_bits;                 /* 8: the output projection is a product in 8-bit integers (fl_linear8): the matrix is rounded per vocabulary row when
+                                          the model is finalized, the final norm's rows per call; 0 or 16: as the other matrices.  Needs bf16 compute_dtype */
+    int32_t reserved[1];
 } fl_stack_config;
 
 /* ---- process / device -------------------------------------------------------------------------- */
@@ -344,12 +346,19 @@ FL_EXPORT int fl_forward_slots(fl_model* m, fl_cache* c, const int* slots, const
 /* One step of a mixed batch (layered models): sequence i of the call lives in slot slots[i] and is fed counts[i] >= 1 new tokens
  * (a portion of a prompt, or one decoded token) at the positions that follow what the slot already holds; ids holds the tokens of
  * all sequences back to back.  want[k] indexes that flattened token list: logits_host receives f32 [n_want, vocab] in that order
- * (n_want may be 0).  The result at a position does not depend on how its sequence was cut into calls or on what else is in the
+ * (n_want may be 0; logits_host NULL: see fl_cache_logprobs).  The result at a position does not depend on how its sequence was cut into calls or on what else is in the
  * batch, beyond rounding. */
 FL_EXPORT int fl_forward_ragged(fl_model* m, fl_cache* c, const int* slots, const int* counts, int n, const uint32_t* ids,
                                 const int* want, int n_want, float* logits_host);
 FL_EXPORT int fl_cache_slot_reset(fl_cache* c, int slot);        /* the slot's sequence is finished: length := 0 */
 FL_EXPORT int fl_cache_slot_len(fl_cache* c, int slot, int* out);
+
+/* Log probabilities over the logits of the LAST forward on this cache (fl_forward, fl_forward_greedy, fl_forward_sample(_device), fl_forward_slots,
+ * fl_forward_ragged), which stay on the device until the next call: rows 0 .. rows - 1 of it, in its order.  Numbers as fl_logprobs states them;
+ * tokens [rows, given] and all results are host memory, and any result may be NULL.  With logits_host = NULL the forwards leave
+ * their logits on the device alone. */
+FL_EXPORT int fl_cache_logprobs(fl_cache* c, int rows, const int32_t* tokens, int given, double temperature, int top, float* logprob, float* logsumexp,
+                                float* entropy, int32_t* top_ids, float* top_logprobs);
 
 /* Diagnostics (no reference counterpart): the router's decisions in the LAST forward on this cache (Mixtral only) -- experts
  * [layers][rows][num_experts_per_tok] in pick order (MixtralSparseMoeBlock's sort, models/mixtral.rs via candle-transformers) and

@@ -965,7 +965,7 @@ static void ensure_ws(fl_cache& c, size_t T, size_t n_want) {
         drop_graphs(c);
         const size_t N = std::max<size_t>(n_want, 2 * y.want_cap);
         y.hf.alloc(N * m.W); y.logits.alloc(N * m.V);
-        if (m.cfg.head_bits == 8) y.head8_ws.alloc(linear8_workspace((int64_t)N, m.W));
+        if (m.cfg.head_bits == 8) y.head8_ws.alloc(N * padded8(m.W) + 256 + N * 4);        // (linear8_workspace of any number of rows up to N)
         if (!m.f32) { y.hf_hi.alloc(N * m.W); y.hf_lo.alloc(N * m.W); }
         y.want_cap = N;
     }

@@ -61,9 +61,10 @@ static L8Pair pair_plan8(int64_t rows, int64_t n, int64_t k, int clusters) {
 
 // A call's workspace: rounded rows and their scales (none for activations that are 8-bit already)
 struct L8Room { size_t scale = 0, all = 0; };
-static L8Room linear8_room(int64_t rows, int64_t k, bool given) {
+static bool small_fits(int64_t rows, int64_t n, int64_t k);
+static L8Room linear8_room(int64_t rows, int64_t n, int64_t k, bool given) {
     L8Room r;
-    if (given) return r;
+    if (given || small_fits(rows, n, k)) return r;
     r.scale = up256((size_t)rows * padded8(k));
     r.all = r.scale + (size_t)rows * 4;
     return r;
@@ -117,6 +118,9 @@ static void few_attr() {
 // One-time set-up, with fl_init: also loads the kernels, so that a caller's first call may be one inside a graph capture.
 void ops_init() {
     if (g_op_failed != nullptr) return;
+    FL_CUDA(cudaFuncSetAttribute(linear8_small_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL8SmallSmem));
+    FL_CUDA(cudaFuncSetAttribute(linear8_small_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL8SmallSmem));
+    FL_CUDA(cudaFuncSetAttribute(linear8_small_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL8SmallSmem));
     few_attr<16>(); few_attr<32>(); few_attr<64>(); few_attr<128>();
     FL_CUDA(cudaFuncSetAttribute(linear8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL8PairSmem));
     auto wide = [](auto kern) { FL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)); };
@@ -163,11 +167,29 @@ static void quantize_rows(LaunchCtx& lc, const void* x, int dtype, int64_t rows,
     else quantize_rows_t<__half>(lc, x, rows, cols, ldx, q, ldq, cols_q, scale);
 }
 
+// Blocks that share a 128-row weight tile: one per SM at most, eight k blocks each at least, and only where a block is spared 24 k blocks: the cluster's
+// barriers and the exchange take as long (8 rows, S = 1 and 2: 14336 x 4096 13.2 and 16.1 us, 5632 x 2048 7.3 and 8.5, 9472 x 14336 29.7 and 27.6; 4096 x
+// 4096, S = 1, 4 and 8: 9.9, 9.0 and 9.4).
+static int few_slices(int64_t tiles, int nk) {
+    int S = 8;
+    while (S > 1 && (S * tiles > kNumSMs || nk < 8 * S || nk - nk / S < 24)) S /= 2;
+    return S;
+}
+// whether a product's rows are rounded inside its own launch (ops.py keeps the same rule, for the workspace)
+static bool small_fits(int64_t rows, int64_t n, int64_t k) {
+    const int nk = (int)((k + kL8BK - 1) / kL8BK), S = few_slices((n + 127) / 128, nk);
+    return rows <= kL8SmallRows && rows * k <= kL8SmallValues && (nk + S - 1) / S <= kL8SmallBlocks;
+}
+template <typename T>
+static void launch_small(LaunchCtx& lc, uint64_t bytes, const void* x, int64_t ldx, const int8_t* w, int64_t ldw, const Linear8Args& g) {
+    const int tiles = (g.n + 127) / 128, S = few_slices(tiles, (g.k + kL8BK - 1) / kL8BK);
+    const CUtensorMap tw = make_tmap_i8(w, g.n, g.k, ldw, 128);
+    const bool vec = aligned(x, 16) && (g.rows == 1 || ldx * sizeof(T) % 16 == 0);
+    launch_op(lc, "linear8", bytes, linear8_small_kernel<T>, dim3((unsigned)(tiles * S)), 192, kL8SmallSmem, S, false, tw, g, S, static_cast<const T*>(x), (long long)ldx, vec);
+}
 template <int BN>
 static void launch_few(LaunchCtx& lc, uint64_t bytes, const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, const Linear8Args& g, bool pdl) {
-    const int tiles = (g.n + 127) / 128, nk = (g.k + kL8BK - 1) / kL8BK;
-    int S = 1;
-    while (S < 8 && 2 * S * tiles <= L8Few<BN>::kPerSm * kNumSMs && nk >= 8 * S) S *= 2;
+    const int tiles = (g.n + 127) / 128, S = few_slices(tiles, (g.k + kL8BK - 1) / kL8BK);
     const CUtensorMap tw = make_tmap_i8(w, g.n, g.k, ldw, 128), tx = make_tmap_i8(x, g.rows, g.k, ldx, BN);
     launch_op(lc, "linear8", bytes, linear8_few_kernel<BN>, dim3((unsigned)(tiles * S)), L8Few<BN>::kThreads, L8Few<BN>::kSmem, S, pdl, tw, tx, g, S);
 }
@@ -184,14 +206,20 @@ static void run_linear8(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
     const int8_t* q = static_cast<const int8_t*>(x);
     int64_t ldq = rows == 1 ? padded8(k) : ldx;
     Linear8Args g{(int)rows, (int)n, (int)k, x_scale, w_scale, bias, y, ldy, y_dtype, g_op_failed};
+    if (n == 1) ldw = padded8(k);
+    const uint64_t bytes = (uint64_t)n * k + (uint64_t)rows * (k + n * dtype_size(y_dtype));
+    if (!given && small_fits(rows, n, k)) {
+        if (x_dtype == FL_DTYPE_F32) launch_small<float>(lc, bytes, x, ldx, w, ldw, g);
+        else if (x_dtype == FL_DTYPE_BF16) launch_small<__nv_bfloat16>(lc, bytes, x, ldx, w, ldw, g);
+        else launch_small<__half>(lc, bytes, x, ldx, w, ldw, g);
+        return;
+    }
     if (!given) {
         int8_t* to = static_cast<int8_t*>(workspace);
-        float* s = reinterpret_cast<float*>(to + linear8_room(rows, k, false).scale);
+        float* s = reinterpret_cast<float*>(to + linear8_room(rows, n, k, false).scale);
         quantize_rows(lc, x, x_dtype, rows, k, ldx, to, padded8(k), padded8(k), s);
         q = to; ldq = padded8(k); g.xs = s;
     }
-    if (n == 1) ldw = padded8(k);
-    const uint64_t bytes = (uint64_t)n * k + (uint64_t)rows * (k + n * dtype_size(y_dtype));
     if (rows > kL8FewRows) launch_pair(lc, bytes, q, ldq, w, ldw, g, !given);
     else if (rows <= 16) launch_few<16>(lc, bytes, q, ldq, w, ldw, g, !given);
     else if (rows <= 32) launch_few<32>(lc, bytes, q, ldq, w, ldw, g, !given);
@@ -199,21 +227,23 @@ static void run_linear8(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
     else launch_few<128>(lc, bytes, q, ldq, w, ldw, g, !given);
 }
 
-// Blocks per row: as many as the chip holds (four per SM) over the rows, while every warp still has a chunk of two; the cluster of 16 is not portable
-// to every chip, but B200 has it.
+// Blocks per row: as many as the chip holds (four per SM) over the rows, while every warp has two chunks; at most eight with alternatives, whose lists
+// the first block joins (1 x 32000, five alternatives, 4, 8 and 16 blocks: 6.8, 6.2 and 6.3 us; 64 x 152064 f32, twenty: 16.6, 16.6 and 31.0; none: 10.8, 9.4
+// and 12.0).  The cluster of 16 is not portable to every chip, but B200 has it.  One block per row: small ones where there are more rows than SMs
+// hold large ones (1000 x 32003 f16, five alternatives 26.2 -> 22.0 us with 128 threads, 300 x 32000 f32 15.0 -> 19.6).
 template <typename T>
 static void run_logprobs(LaunchCtx& lc, const LogprobArgs& a) {
     const int chunks = (a.vocab + 2 * LpRow<T>::N - 1 + LpRow<T>::kChunk - 1) / LpRow<T>::kChunk;
+    const int most = a.top > 0 ? kLpMaxCluster / 2 : kLpMaxCluster;
     int C = 1;
-    while (C < kLpMaxCluster && (long long)a.rows * 2 * C <= 4 * kNumSMs && chunks >= 16 * C) C *= 2;
+    while (C < most && (long long)a.rows * 2 * C <= 4 * kNumSMs && chunks >= 16 * C) C *= 2;
     const uint64_t bytes = (uint64_t)a.rows * a.vocab * sizeof(T);
     const dim3 grid((unsigned)((long long)a.rows * C));
     const size_t smem = a.top > 0 ? (size_t)((chunks + C - 1) / C + 1) * 4 : 0;
     auto go = [&](auto kern, int threads) { launch_op(lc, "logprobs", bytes, kern, grid, threads, smem, C, false, a, C); };
-    if (C == 1) a.top > 0 ? go(logprobs_kernel<T, true, 128>, 128) : go(logprobs_kernel<T, false, 128>, 128);
+    if (a.rows > 6 * kNumSMs) a.top > 0 ? go(logprobs_kernel<T, true, 128>, 128) : go(logprobs_kernel<T, false, 128>, 128);
     else a.top > 0 ? go(logprobs_kernel<T, true, 256>, 256) : go(logprobs_kernel<T, false, 256>, 256);
 }
-
 template <typename T>
 static void run_logprobs(LaunchCtx& lc, LogprobArgs a, double temperature) {
     a.inv_t = (float)(1.0 / temperature);
@@ -225,7 +255,7 @@ static void check_temperature(double temperature) {
     FL_CHECK(temperature > 0 && std::isfinite(temperature) && std::isfinite(c) && inv_t > 0, FL_ERR_INVALID, "logprobs: the temperature is a positive number");
 }
 
-size_t linear8_workspace(int64_t rows, int64_t k) { return linear8_room(rows, k, false).all; }
+size_t linear8_workspace(int64_t rows, int64_t n, int64_t k) { return linear8_room(rows, n, k, false).all; }
 void op_quantize_rows(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale) {
     quantize_rows(lc, x, dtype, rows, cols, ldx, q, ldq, ldq, scale);
 }
@@ -262,12 +292,13 @@ FL_EXPORT int fl_quantize_rows(const void* x, int dtype, int64_t rows, int64_t c
     FL_API_END
 }
 
-FL_EXPORT int fl_linear8_workspace(int64_t rows, int64_t k, int x_dtype, size_t* bytes) {
+FL_EXPORT int fl_linear8_workspace(int64_t rows, int64_t n, int64_t k, int x_dtype, size_t* bytes) {
     FL_API_BEGIN
     FL_CHECK(bytes, FL_ERR_INVALID, "NULL argument");
     FL_CHECK(is_float(x_dtype) || x_dtype == FL_DTYPE_I8, FL_ERR_INVALID, "linear8: activations are f32, bf16, f16 or i8");
-    FL_CHECK(rows >= 0 && rows <= kMaxRows && k >= 1 && k <= kLinear8MaxK, FL_ERR_INVALID, "linear8: rows from 0 to 2^30, k from 1 to 131071");
-    *bytes = linear8_room(rows, k, x_dtype == FL_DTYPE_I8).all;
+    FL_CHECK(rows >= 0 && rows <= kMaxRows && n >= 1 && n <= kMaxRows && k >= 1 && k <= kLinear8MaxK, FL_ERR_INVALID,
+             "linear8: rows from 0 to 2^30, n from 1 to 2^30, k from 1 to 131071");
+    *bytes = linear8_room(rows, n, k, x_dtype == FL_DTYPE_I8).all;
     FL_API_END
 }
 
@@ -288,7 +319,7 @@ FL_EXPORT int fl_linear8(const void* x, int x_dtype, int64_t ldx, const float* x
     FL_CHECK(aligned(x, dtype_size(x_dtype)) && aligned(y, dtype_size(y_dtype)) && aligned(w_scale, 4) && aligned(x_scale, 4) && aligned(bias, 4), FL_ERR_INVALID,
              "linear8: a pointer is not aligned to its type");
     FL_CHECK(rows <= ((int64_t)1 << 40) / n, FL_ERR_INVALID, "linear8: more than 2^40 results");
-    const L8Room room = linear8_room(rows, k, given);
+    const L8Room room = linear8_room(rows, n, k, given);
     FL_CHECK(room.all == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= room.all), FL_ERR_INVALID,
              "linear8: the workspace is smaller than fl_linear8_workspace asks for, or not on a 256-byte border");
     DeviceScope dev;

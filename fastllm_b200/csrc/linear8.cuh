@@ -168,21 +168,7 @@ __device__ __forceinline__ void umma_i8_pair_warp(uint32_t tmem_d, uint64_t ades
 }
 // Results of one weight row n (a lane each) and 16 activation rows r, r + 1, .. with the scales xs (shared memory, 16-byte border): for a fixed row the 32
 // lanes write 32 neighbours.  (16-bit results in twos, after an exchange between neighbouring lanes, took as long or longer: 64 x 152064 20 -> 26 us.)
-__device__ __forceinline__ void l8_store16(const Linear8Args& g, int r, int n, const float* xs, float wsn, float bn, const uint32_t (&sum)[16]) {
-    float v[16];
-#pragma unroll
-    for (int j = 0; j < 16; j += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(xs + j);
-        v[j] = (float)(int)sum[j] * x.x * wsn;
-        v[j + 1] = (float)(int)sum[j + 1] * x.y * wsn;
-        v[j + 2] = (float)(int)sum[j + 2] * x.z * wsn;
-        v[j + 3] = (float)(int)sum[j + 3] * x.w * wsn;
-    }
-    if (g.bias != nullptr) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] += bn;
-    }
-    const int rows = n < g.n ? min(g.rows - r, 16) : 0;
+__device__ __forceinline__ void l8_write16(const Linear8Args& g, int r, int n, int rows, const float (&v)[16]) {
     if (g.y_dtype == 0) {
         float* o = reinterpret_cast<float*>(g.y) + (long long)r * g.ldy + n;
         if (rows == 16) {
@@ -197,19 +183,36 @@ __device__ __forceinline__ void l8_store16(const Linear8Args& g, int r, int n, c
         }
         return;
     }
-    auto half = [&](float a, float b) {
-        if (g.y_dtype == 1) return pack_bf16x2(a, b);
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&h);
-    };
     uint16_t* o = reinterpret_cast<uint16_t*>(g.y) + (long long)r * g.ldy + n;
 #pragma unroll
     for (int j = 0; j < 16; j += 2) {
-        const uint32_t w = half(v[j], v[j + 1]);
+        uint32_t w;
+        if (g.y_dtype == 1) {
+            w = pack_bf16x2(v[j], v[j + 1]);
+        } else {
+            const __half2 h = __floats2half2_rn(v[j], v[j + 1]);
+            w = *reinterpret_cast<const uint32_t*>(&h);
+        }
         if (j < rows) o[0] = (uint16_t)w;
         if (j + 1 < rows) o[g.ldy] = (uint16_t)(w >> 16);
         o += 2 * g.ldy;
     }
+}
+__device__ __forceinline__ void l8_store16(const Linear8Args& g, int r, int n, const float* xs, float wsn, float bn, const uint32_t (&sum)[16]) {
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(xs + j);
+        v[j] = (float)(int)sum[j] * x.x * wsn;
+        v[j + 1] = (float)(int)sum[j + 1] * x.y * wsn;
+        v[j + 2] = (float)(int)sum[j + 2] * x.z * wsn;
+        v[j + 3] = (float)(int)sum[j + 3] * x.w * wsn;
+    }
+    if (g.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] += bn;
+    }
+    l8_write16(g, r, n, n < g.n ? min(g.rows - r, 16) : 0, v);
 }
 // A wait ran out: report it and leave the copies in flight time to land; the block goes on to its end.
 __device__ __forceinline__ void l8_give_up(int* failed) {
@@ -230,6 +233,68 @@ template <int BN> struct L8Few {
     static constexpr uint32_t kTmem = BN < 32 ? 32 : BN;
     static_assert(kStages * kStage >= (uint32_t)BN * 512, "the parts of a tile fit the ring");
 };
+
+// The accumulators of a block's part of K (all warps call it; those from 2 on are the epilogue's): written, or added up in the cluster.  xs: the tile's row
+// scales, the calling warp's copy.
+template <int BN>
+__device__ __forceinline__ void l8_few_finish(const Linear8Args& g, const int S, int s, int r0, int n0, uint32_t tmem, uint8_t* ring, const float* xs, bool ok) {
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    const int row = (warp & 3) * 32 + lane;                                            // accumulator row = weight row of the tile
+    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const int n = n0 + row;
+    const float wsn = warp >= 2 && n < g.n ? g.ws[n] : 0.f, bn = warp >= 2 && g.bias != nullptr && n < g.n ? g.bias[n] : 0.f;
+    if (S == 1) {
+        if (warp >= 2 && ok) {
+#pragma unroll 1
+            for (int c = 0; c < BN && r0 + c < g.rows; c += 16) {
+                uint32_t v[16];
+                tmem_ld16(at + (uint32_t)c, v);
+                l8_store16(g, r0 + c, n, xs + c, wsn, bn, v);
+            }
+        }
+        return;
+    }
+    const int per = BN / S;                                                            // columns that one block of the cluster adds up and writes
+    __syncwarp();
+    cluster_sync_all();                                                                // every block's products are done: the rings are free
+    if (warp >= 2) {
+        const uint32_t base = smem_u32(ring) + (uint32_t)(s * per * 128 + row) * 4;
+#pragma unroll 1
+        for (int c = 0; c < BN && r0 + c < g.rows; c += 16) {
+            uint32_t v[16];
+            tmem_ld16(at + (uint32_t)c, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int owner = (c + j) / per;
+                asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(mapa_u32(base + (uint32_t)((c + j) - owner * per) * 512, owner)), "r"(v[j]) : "memory");
+            }
+        }
+    }
+    __syncwarp();
+    cluster_sync_all();
+    if (warp >= 2 && ok) {
+        const int* part = reinterpret_cast<const int*>(ring) + row;
+#pragma unroll 1
+        for (int c = 0; c < per && r0 + s * per + c < g.rows; c += 16) {
+            const int r = r0 + s * per + c, cnt = min(min(per - c, 16), g.rows - r);
+            int sum[16];
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sum[j] = 0;
+            for (int t = 0; t < S; ++t) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (j < cnt) sum[j] += part[(t * per + c + j) * 128];
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                v[j] = j < cnt ? (float)sum[j] * xs[s * per + c + j] * wsn : 0.f;
+                if (g.bias != nullptr) v[j] += bn;
+            }
+            l8_write16(g, r, n, n < g.n ? cnt : 0, v);
+        }
+    }
+}
 
 template <int BN>
 __global__ void __launch_bounds__(L8Few<BN>::kThreads, L8Few<BN>::kPerSm)
@@ -297,9 +362,6 @@ linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         }
         umma_commit_warp(&done);
     }
-    const int row = (warp & 3) * 32 + lane;                                            // accumulator row = weight row of the tile (epilogue warps)
-    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const int n = n0 + row;
     if (warp >= 2) {
         pdl_wait();
         for (int i = lane; i < BN; i += 32) xs[warp - 2][i] = r0 + i < g.rows ? g.xs[r0 + i] : 0.f;
@@ -307,51 +369,7 @@ linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&done, 0, kMbarTries));
         tc_fence_after();
     }
-    const float wsn = warp >= 2 && n < g.n ? g.ws[n] : 0.f, bn = warp >= 2 && g.bias != nullptr && n < g.n ? g.bias[n] : 0.f;
-    if (S == 1) {
-        if (warp >= 2 && ok) {
-#pragma unroll 1
-            for (int c = 0; c < BN && r0 + c < g.rows; c += 16) {
-                uint32_t v[16];
-                tmem_ld16(at + (uint32_t)c, v);
-                l8_store16(g, r0 + c, n, xs[warp - 2] + c, wsn, bn, v);
-            }
-        }
-    } else {
-        const int per = BN / S;                                                        // columns that one block of the cluster adds up and writes
-        __syncwarp();
-        cluster_sync_all();                                                            // every block's products are done: the rings are free
-        if (warp >= 2) {
-            const uint32_t base = smem_u32(gsm) + (uint32_t)(s * per * 128 + row) * 4;
-#pragma unroll 1
-            for (int c = 0; c < BN && r0 + c < g.rows; c += 16) {
-                uint32_t v[16];
-                tmem_ld16(at + (uint32_t)c, v);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int owner = (c + j) / per;
-                    asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(mapa_u32(base + (uint32_t)((c + j) - owner * per) * 512, owner)), "r"(v[j]) : "memory");
-                }
-            }
-        }
-        __syncwarp();
-        cluster_sync_all();
-        if (warp >= 2 && ok) {
-            const int* part = reinterpret_cast<const int*>(gsm) + row;
-            for (int c = 0; c < per && r0 + s * per + c < g.rows; ++c) {               // (few columns: BN / S)
-                int sum = 0;
-                for (int t = 0; t < S; ++t) sum += part[(t * per + c) * 128];
-                const int r = r0 + s * per + c;
-                if (n >= g.n) continue;
-                float v = (float)sum * xs[warp - 2][s * per + c] * wsn;
-                if (g.bias != nullptr) v += bn;
-                const long long at_y = (long long)r * g.ldy + n;
-                if (g.y_dtype == 0) reinterpret_cast<float*>(g.y)[at_y] = v;
-                else if (g.y_dtype == 1) reinterpret_cast<__nv_bfloat16*>(g.y)[at_y] = from_f32<__nv_bfloat16>(v);
-                else reinterpret_cast<__half*>(g.y)[at_y] = from_f32<__half>(v);
-            }
-        }
-    }
+    l8_few_finish<BN>(g, S, s, r0, n0, tmem, gsm, xs[max(warp - 2, 0)], ok);
     if (!ok) l8_give_up(g.failed);
     __syncwarp();
     tc_fence_before();
@@ -359,6 +377,141 @@ linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, L::kTmem);
+    }
+}
+
+// ---- a token or a few ---------------------------------------------------------------------------------------------------------------
+// Up to four rows of few enough values round inside the product's own launch: every block reads the rows for their maxima (from L2) and rounds its part
+// of K into the layout that the tensor cores read, while its first weights are on their way.  A launch and a workspace less: one row of
+// 4096 by 4096 takes the host 10 us instead of 14 and the device as long as before (9.8; with the rows in 8 bits already 8.9).
+constexpr int kL8SmallRows = 4, kL8SmallValues = 8192, kL8SmallBlocks = 8;              // rows; values of all of them; k blocks of one block's part
+constexpr int kL8SmallStages = 6;
+constexpr uint32_t kL8SmallX = 16 * kL8BK;                                             // 16 rows (those past the last hold anything: columns that nobody reads)
+constexpr size_t kL8SmallSmem = kL8SmallStages * kL8WBytes + kL8SmallBlocks * kL8SmallX + 1024;
+
+template <typename T>
+__global__ void __launch_bounds__(192, 2)
+linear8_small_kernel(const __grid_constant__ CUtensorMap tmW, const Linear8Args g, const int S, const T* __restrict__ x, const long long ldx, const bool vec) {
+    constexpr int kStages = kL8SmallStages, V = 16 / sizeof(T), R = kL8SmallRows;
+    extern __shared__ uint8_t gsm_raw[];
+    uint8_t* gsm = gsm_raw + ((1024u - (smem_u32(gsm_raw) & 1023u)) & 1023u);          // (the same offset in all blocks of a cluster)
+    uint8_t* sx = gsm + kStages * kL8WBytes;
+    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], done, rounded;
+    __shared__ __align__(16) float xs[4][16];
+    __shared__ uint32_t most[4][R];
+    __shared__ uint32_t tmem_base_s;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    const int s = S == 1 ? 0 : (int)cluster_rank();
+    const int n0 = blockIdx.x / S * 128;
+    const int nk = (g.k + kL8BK - 1) / kL8BK, kb0 = s * nk / S, kb1 = (s + 1) * nk / S;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        mbar_init(&done, 1);
+        mbar_init(&rounded, 128);
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc(&tmem_base_s, 32);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_s;
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int st = 0;
+            uint32_t ph = 1;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!(ok = mbar_wait_bounded(&empty[st], ph, kMbarTries))) break;
+                mbar_expect_tx(&full[st], kL8WBytes);
+                tma_load_2d(gsm + st * kL8WBytes, &tmW, kb * kL8BK, n0, &full[st]);
+                if (++st == kStages) { st = 0; ph ^= 1; }
+            }
+        }
+    } else if (warp == 1) {
+        constexpr uint32_t idesc = umma_idesc_i8(128, 16);
+        const uint64_t base = umma_smem_desc_sw128(gsm), bx = umma_smem_desc_sw128(sx);
+        int st = 0;
+        uint32_t ph = 0;
+        ok = mbar_wait_bounded(&rounded, 0, kMbarTries);
+        for (int kb = kb0; kb < kb1; ++kb) {
+            if (ok) ok = mbar_wait_bounded(&full[st], ph, kMbarTries);
+            __syncwarp();
+            tc_fence_after();
+            const uint64_t a = base + (uint64_t)(st * (kL8WBytes >> 4)), b = bx + (uint64_t)((kb - kb0) * (kL8SmallX >> 4));
+#pragma unroll
+            for (int q = 0; q < 4; ++q) umma_i8_warp(tmem, a + 2 * q, b + 2 * q, idesc, ((kb - kb0) | q) ? 1u : 0u);
+            umma_commit_warp(&empty[st]);
+            if (++st == kStages) { st = 0; ph ^= 1; }
+        }
+        umma_commit_warp(&done);
+    } else {
+        const int tid = threadIdx.x - 64;
+        uint32_t m[R] = {};
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (r >= g.rows) break;
+            const T* xr = x + r * ldx;
+            if (vec) {
+#pragma unroll 4
+                for (int i = tid * V; i < g.k; i += 128 * V) {                          // (a whole vector lies inside the row's 16-byte pieces, but not inside the row)
+                    if (i + V <= g.k) {
+                        const uint4 h = __ldg(reinterpret_cast<const uint4*>(xr + i));
+                        const T* e = reinterpret_cast<const T*>(&h);
+#pragma unroll
+                        for (int j = 0; j < V; ++j) m[r] = max(m[r], abs_bits(to_f32(e[j])));
+                    } else {
+                        for (int j = i; j < g.k; ++j) m[r] = max(m[r], abs_bits(to_f32(xr[j])));
+                    }
+                }
+            } else {
+                for (int i = tid; i < g.k; i += 128) m[r] = max(m[r], abs_bits(to_f32(xr[i])));
+            }
+            m[r] = __reduce_max_sync(0xFFFFFFFFu, m[r]);
+            if (lane == 0) most[warp - 2][r] = m[r];
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const int c1 = min(kb1 * kL8BK, g.k);
+#pragma unroll 1
+        for (int r = 0; r < g.rows; ++r) {
+            const RowScale rs(max(max(most[0][r], most[1][r]), max(most[2][r], most[3][r])));
+            if (lane == 0) xs[warp - 2][r] = rs.scale;
+            const T* xr = x + r * ldx;
+            for (int c = kb0 * kL8BK + tid * 4; c < c1; c += 512) {                     // four values a thread; past the row's end the weights are zeros
+                float v[4];
+                if (vec && c + 4 <= g.k) {
+                    if constexpr (sizeof(T) == 4) {
+                        const float4 h = __ldg(reinterpret_cast<const float4*>(xr + c));
+                        v[0] = h.x; v[1] = h.y; v[2] = h.z; v[3] = h.w;
+                    } else {
+                        const uint2 h = __ldg(reinterpret_cast<const uint2*>(xr + c));
+                        const T* e = reinterpret_cast<const T*>(&h);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] = to_f32(e[j]);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] = c + j < g.k ? to_f32(xr[c + j]) : 0.f;
+                }
+                const int kb = c / kL8BK - kb0, in = c % kL8BK;                         // 16-byte piece in / 16 of the row lies at (in / 16) ^ (row mod 8)
+                *reinterpret_cast<uint32_t*>(sx + kb * kL8SmallX + r * 128 + (((in >> 4) ^ (r & 7)) << 4) + (in & 15)) = rs.four(v[0], v[1], v[2], v[3]);
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(&rounded);
+        __syncwarp();
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&done, 0, kMbarTries));
+        tc_fence_after();
+    }
+    l8_few_finish<16>(g, S, s, 0, n0, tmem, gsm, xs[max(warp - 2, 0)], ok);
+    if (!ok) l8_give_up(g.failed);
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 32);
     }
 }
 

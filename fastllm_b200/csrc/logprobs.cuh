@@ -236,11 +236,16 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
     LpPart p{-INFINITY, 0.9f * LpVec<T>::kLow * c, 0.f, 0.f};   // (well above what -infinity is raised to, below every other value of a row that is not `far`)
     uint64_t s2 = pack2(0.f, 0.f), t2 = s2;
     const uint64_t c2 = pack2(c, c);
-    for (int ch = ch0 + warp; ch < ch1; ch += kWarps * U) {
-        uint4 v[U];
+    uint4 v[U], next[TOP ? 1 : U];                              // (with alternatives the registers are worth more as a further block per SM)
+    auto fetch = [&](int ch, uint4* to) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (ch + u * kWarps < ch1) v[u] = x.load(ch + u * kWarps, lane);
+            if (ch + u * kWarps < ch1) to[u] = x.load(ch + u * kWarps, lane);
+    };
+    if (!TOP) fetch(ch0 + warp, v);
+    for (int ch = ch0 + warp; ch < ch1; ch += kWarps * U) {
+        if constexpr (TOP) fetch(ch, v);
+        else fetch(ch + kWarps * U, next);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (ch + u * kWarps >= ch1) break;
@@ -268,6 +273,10 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
                 s2 = add2(s2, e);
                 t2 = fma2(e, d, t2);
             });
+        }
+        if constexpr (!TOP) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u] = next[u];
         }
     }
     {

@@ -11,7 +11,7 @@ P = 1 << 20             # an address that no call below gets far enough to use
 
 
 def _linear8(**change):
-    a = dict(x=P, x_dtype=1, ldx=64, x_scale=None, w=P, ldw=64, w_scale=P, bias=None, rows=4, n=32, k=64, y=P, y_dtype=1, ldy=32, workspace=P, workspace_bytes=1 << 20)
+    a = dict(x=P, x_dtype=1, ldx=64, x_scale=None, w=P, ldw=64, w_scale=P, bias=None, rows=5, n=32, k=64, y=P, y_dtype=1, ldy=32, workspace=P, workspace_bytes=1 << 20)
     a.update(change)
     return _lib.load().fl_linear8(*a.values(), None)
 
@@ -40,7 +40,7 @@ def _refused(rc, word):
     (dict(x=None), "NULL"), (dict(w=None), "NULL"), (dict(w_scale=None), "NULL"), (dict(y=None), "NULL"), (dict(x_scale=P), "x_scale"),
     (dict(x_dtype=3, ldx=64), "x_scale"), (dict(w=P + 8), "16-byte"), (dict(ldw=72), "16-byte"), (dict(x_dtype=3, x_scale=P, x=P + 4), "16-byte"),
     (dict(x_dtype=3, x_scale=P, ldx=72), "16-byte"), (dict(x=P + 1), "aligned"), (dict(y=P + 1), "aligned"), (dict(w_scale=P + 2), "aligned"), (dict(bias=P + 1), "aligned"),
-    (dict(workspace=None), "workspace"), (dict(workspace=P + 16), "workspace"), (dict(workspace_bytes=4 * 64 + 15), "workspace")])
+    (dict(workspace=None), "workspace"), (dict(workspace=P + 16), "workspace"), (dict(workspace_bytes=5 * 64 + 192 + 19), "workspace")])
 def test_linear8_refuses(change, word):
     _refused(_linear8(**change), word)
 
@@ -70,13 +70,21 @@ def test_no_rows_is_no_work():
 
 
 def test_workspace_size():
+    """ops.py keeps the rule of the C side"""
     n = C.c_size_t()
     lib = _lib.load()
-    for rows, k, dtype, want in [(1, 1, 1, 256 + 4), (16, 16, 0, 256 + 64), (3, 17, 2, 256 + 12), (9, 4096, 1, 9 * 4096 + 36), (300, 100, 1, 33792 + 1200), (9, 4096, 3, 0), (0, 5, 1, 0)]:
-        assert lib.fl_linear8_workspace(rows, k, dtype, C.byref(n)) == 0 and n.value == want
-    _refused(lib.fl_linear8_workspace(1, 0, 1, C.byref(n)), "k from")
-    _refused(lib.fl_linear8_workspace(1, 1, 9, C.byref(n)), "activations")
-    _refused(lib.fl_linear8_workspace(1, 1, 1, None), "NULL")
+    for rows in (0, 1, 2, 3, 4, 5, 9, 128, 300):
+        for cols in (1, 100, 2048, 4096, 9472, 9473, 18944, 18945, 37888, 152064):
+            for k in (1, 17, 100, 2048, 2049, 4095, 4096, 4097, 8192, 16384, 16385, 32768):
+                itself = rows <= 4 and ops._rounds_itself(rows, cols, k)
+                want = 0 if itself else (rows * ((k + 15) // 16 * 16) + 255) // 256 * 256 + 4 * rows
+                assert lib.fl_linear8_workspace(rows, cols, k, 1, C.byref(n)) == 0 and n.value == want, (rows, cols, k)
+                assert lib.fl_linear8_workspace(rows, cols, k, 3, C.byref(n)) == 0 and n.value == 0
+    assert ops._rounds_itself(1, 4096, 4096) and not ops._rounds_itself(1, 152064, 4096)
+    _refused(lib.fl_linear8_workspace(1, 1, 0, 1, C.byref(n)), "k from")
+    _refused(lib.fl_linear8_workspace(1, 0, 1, 1, C.byref(n)), "n from")
+    _refused(lib.fl_linear8_workspace(1, 1, 1, 9, C.byref(n)), "activations")
+    _refused(lib.fl_linear8_workspace(1, 1, 1, 1, None), "NULL")
 
 
 def test_tensors_off_the_gpu_are_refused():

@@ -23,9 +23,11 @@ static LaunchCtx op_ctx(void* stream) {
     LaunchCtx lc;
     lc.stream = static_cast<cudaStream_t>(stream);
     lc.pdl = false;
-    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-    FL_CUDA(cudaStreamIsCapturing(lc.stream, &st));
-    lc.capturing = st != cudaStreamCaptureStatusNone;       // (no events inside a caller's capture, and nothing launched)
+    if (g_prof.on) {                        // (no events inside a caller's capture)
+        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+        FL_CUDA(cudaStreamIsCapturing(lc.stream, &st));
+        lc.capturing = st != cudaStreamCaptureStatusNone;
+    }
     return lc;
 }
 static size_t dtype_size(int dtype) { return dtype == FL_DTYPE_F32 ? 4 : dtype == FL_DTYPE_I8 ? 1 : 2; }

@@ -67,9 +67,9 @@ template <typename T> struct LpVec;
 template <> struct LpVec<float> {
     static constexpr int N = 4;
     static constexpr float kLow = -1e30f, kFar = -1e29f;
-    static __device__ __forceinline__ float max_of(const uint4& v) {
-        return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
-    }
+    static constexpr uint32_t kNone = 0xFF800000u;              // -infinity, in every place of a word
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+    static __device__ __forceinline__ float last(uint32_t m) { return __uint_as_float(m); }
     static __device__ __forceinline__ float raise(uint32_t w) {
         float r;
         asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(w)), "f"(kLow));
@@ -89,10 +89,8 @@ template <> struct LpVec<__nv_bfloat16> {
         asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
         return r;
     }
-    static __device__ __forceinline__ float max_of(const uint4& v) {
-        const uint32_t m = max2(max2(v.x, v.y), max2(v.z, v.w));
-        return fmaxf(bf16lo(m), bf16hi(m));
-    }
+    static constexpr uint32_t kNone = 0xFF80FF80u;
+    static __device__ __forceinline__ float last(uint32_t m) { return fmaxf(bf16lo(m), bf16hi(m)); }
     template <typename F> static __device__ __forceinline__ void pairs(const uint4& v, F&& f) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -115,9 +113,10 @@ template <> struct LpVec<__half> {
         asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
         return r;
     }
-    static __device__ __forceinline__ float max_of(const uint4& v) {
-        const float2 m = two(max2(max2(v.x, v.y), max2(v.z, v.w)));
-        return fmaxf(m.x, m.y);
+    static constexpr uint32_t kNone = 0xFC00FC00u;
+    static __device__ __forceinline__ float last(uint32_t m) {
+        const float2 p = two(m);
+        return fmaxf(p.x, p.y);
     }
     template <typename F> static __device__ __forceinline__ void pairs(const uint4& v, F&& f) {
 #pragma unroll
@@ -134,6 +133,12 @@ template <> struct LpVec<__half> {
     }
 };
 
+// the maximum of a vector, of two values in a word where they are 16-bit; last(): of the word
+template <typename T> __device__ __forceinline__ uint32_t lp_max(const uint4& v) {
+    using L = LpVec<T>;
+    return L::max2(L::max2(v.x, v.y), L::max2(v.z, v.w));
+}
+
 // A row in chunks of 32 vectors of 16 bytes, from the last 16-byte border at or before its start on; chunks that reach over an end are read value by value.
 template <typename T> struct LpRow {
     static constexpr int N = LpVec<T>::N, kChunk = 32 * N;
@@ -144,13 +149,17 @@ template <typename T> struct LpRow {
         chunks = (skip + vocab + kChunk - 1) / kChunk;
     }
     __device__ __forceinline__ int first(int chunk, int lane) const { return chunk * kChunk + lane * N - skip; }        // index of the lane's first value
+    // chunks [whole(), whole_end()) lie inside the row
+    __device__ __forceinline__ int whole() const { return skip > 0; }
+    __device__ __forceinline__ int whole_end() const { return (skip + vocab) / kChunk; }
+    __device__ __forceinline__ const uint4* at(int chunk, int lane) const { return reinterpret_cast<const uint4*>(x - skip) + ((long long)chunk * 32 + lane); }
     // -infinity outside the row
     __device__ __forceinline__ uint4 load(int chunk, int lane) const {
         const int i0 = first(chunk, lane);
         if (i0 >= 0 && i0 + N <= vocab) return ldg_stream(reinterpret_cast<const uint4*>(x + i0));
         uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = sizeof(T) == 4 ? 0xFF800000u : sizeof(T) == 2 && std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
+        for (int j = 0; j < 4; ++j) w[j] = LpVec<T>::kNone;
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             if (i0 + j < 0 || i0 + j >= vocab) continue;
@@ -236,35 +245,34 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
     LpPart p{-INFINITY, 0.9f * LpVec<T>::kLow * c, 0.f, 0.f};   // (well above what -infinity is raised to, below every other value of a row that is not `far`)
     uint64_t s2 = pack2(0.f, 0.f), t2 = s2;
     const uint64_t c2 = pack2(c, c);
-    uint4 v[U], next[TOP ? 1 : U];                              // (with alternatives the registers are worth more as a further block per SM)
-    auto fetch = [&](int ch, uint4* to) {
+    // U vectors of a lane, one of each of U chunks; at(u): the u-th chunk's place in chunk_max, or -1
+    auto absorb = [&](const uint4 (&v)[U], auto&& at) {
+        uint32_t w[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) w[u] = lp_max<T>(v[u]);
+        if constexpr (TOP) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t o = __reduce_max_sync(0xFFFFFFFFu, ordered_bits(LpVec<T>::last(w[u])));
+                if (lane == 0 && at(u) >= 0) chunk_max[at(u)] = o;
+            }
+        }
+#pragma unroll
+        for (int u = 1; u < U; ++u) w[0] = LpVec<T>::max2(w[0], w[u]);
+        const float m = LpVec<T>::last(w[0]);
+        p.m = fmaxf(p.m, m);
+        if (m * c > p.r + 16.f) {
+            const float r = m * c, f = ex2(p.r - r);
+            float sa, sb, ta, tb;
+            unpack2(s2, sa, sb);
+            unpack2(t2, ta, tb);
+            s2 = pack2(sa * f, sb * f);
+            t2 = pack2((ta + sa * (p.r - r)) * f, (tb + sb * (p.r - r)) * f);
+            p.r = r;
+        }
+        const uint64_t r2 = pack2(-p.r, -p.r);
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (ch + u * kWarps < ch1) to[u] = x.load(ch + u * kWarps, lane);
-    };
-    if (!TOP) fetch(ch0 + warp, v);
-    for (int ch = ch0 + warp; ch < ch1; ch += kWarps * U) {
-        if constexpr (TOP) fetch(ch, v);
-        else fetch(ch + kWarps * U, next);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (ch + u * kWarps >= ch1) break;
-            const float m = LpVec<T>::max_of(v[u]);
-            p.m = fmaxf(p.m, m);
-            if (TOP) {
-                const uint32_t o = __reduce_max_sync(0xFFFFFFFFu, ordered_bits(m));
-                if (lane == 0) chunk_max[ch + u * kWarps - ch0] = o;
-            }
-            if (m * c > p.r + 16.f) {
-                const float r = m * c, f = ex2(p.r - r);
-                float sa, sb, ta, tb;
-                unpack2(s2, sa, sb);
-                unpack2(t2, ta, tb);
-                s2 = pack2(sa * f, sb * f);
-                t2 = pack2((ta + sa * (p.r - r)) * f, (tb + sb * (p.r - r)) * f);
-                p.r = r;
-            }
-            const uint64_t r2 = pack2(-p.r, -p.r);
             LpVec<T>::pairs(v[u], [&](float va, float vb) {
                 const uint64_t d = fma2(pack2(va, vb), c2, r2);
                 float da, db;
@@ -273,10 +281,50 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
                 s2 = add2(s2, e);
                 t2 = fma2(e, d, t2);
             });
-        }
-        if constexpr (!TOP) {
+    };
+    // batches of U chunks a warp that lie inside the row, without a look at its ends; then the chunks in front of them and behind
+    const int first = max(ch0, x.whole()), batches = max(0, min(ch1, x.whole_end()) - first) / (kWarps * U);
+    {
+        const uint4* q = x.at(first + warp, lane);
+        auto fetch = [&](uint4 (&v)[U]) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u] = next[u];
+            for (int u = 0; u < U; ++u) v[u] = ldg_stream(q + u * kWarps * 32);
+            q += U * kWarps * 32;
+        };
+        uint4 v[U];
+        int ch = first + warp - ch0;
+        auto place = [&](int u) { return ch + u * kWarps; };
+        if constexpr (TOP) {                                    // (the registers of a second set are worth more as a further block per SM)
+            for (int i = 0; i < batches; ++i, ch += U * kWarps) {
+                fetch(v);
+                absorb(v, place);
+            }
+        } else if (batches > 0) {
+            uint4 w[U];
+            fetch(v);
+            for (int i = 0; i < batches; i += 2) {
+                if (i + 1 < batches) fetch(w);
+                absorb(v, place);
+                if (i + 1 >= batches) break;
+                if (i + 2 < batches) fetch(v);
+                absorb(w, place);
+            }
+        }
+    }
+    {
+        const int head = min(first, ch1) - ch0, rest = ch1 - ch0 - batches * kWarps * U;       // chunks in front of the batches; all that are left
+        for (int j = warp; j < rest; j += U * kWarps) {
+            uint4 v[U];
+            auto place = [&](int u) {
+                const int k = j + u * kWarps;
+                return k >= rest ? -1 : k < head ? k : k + batches * kWarps * U;
+            };
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                v[u] = make_uint4(LpVec<T>::kNone, LpVec<T>::kNone, LpVec<T>::kNone, LpVec<T>::kNone);
+                if (place(u) >= 0) v[u] = x.load(ch0 + place(u), lane);
+            }
+            absorb(v, place);
         }
     }
     {
@@ -339,7 +387,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
                 for (int u = 0; u < 4; ++u) {
                     if (i + u * kWarps >= n_list) break;
                     const int i0 = x.first(list[i + u * kWarps], lane);
-                    if (ordered_bits(LpVec<T>::max_of(v[u])) < least) continue;
+                    if (ordered_bits(LpVec<T>::last(lp_max<T>(v[u]))) < least) continue;
                     for (int j = 0; j < LpVec<T>::N; ++j) {
                         const uint32_t o = ordered_bits(LpVec<T>::at(v[u], j));
                         if (o >= least && i0 + j >= 0 && i0 + j < a.vocab) {

@@ -111,7 +111,9 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, b
         _refuse(f"{what}: activations are f32, bf16, f16 or int8, got {x.dtype}")
     if weight.dtype != torch.int8 or weight.ndim != 2:
         _refuse(f"{what}: the weight is an int8 matrix [n, k], got {weight.dtype} {tuple(weight.shape)}")
-    dev = _device(x, what)
+    dev = x.get_device()
+    if dev != _bound[0]:
+        _device(x, what)
     x2 = x if x.ndim == 2 and x.stride(1) == 1 else _rows(x, what)
     rows, k = x2.shape
     n, wk = weight.shape
@@ -169,7 +171,9 @@ def logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: i
     what = "logprobs"
     if logits.dtype not in _FLOATS:
         _refuse(f"{what}: logits are f32, bf16 or f16, got {logits.dtype}")
-    dev = _device(logits, what)
+    dev = logits.get_device()
+    if dev != _bound[0]:
+        _device(logits, what)
     x = logits if logits.ndim == 2 and logits.stride(1) == 1 else _rows(logits, what)
     rows, vocab = x.shape
     lead = logits.shape[:-1]
@@ -199,10 +203,13 @@ def logprobs(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, top: i
     if rc:
         _lib.check(rc)
 
-    def part(first, cols, shape, kind=None):
-        t = mem if kind is None else mem.view(kind)
-        t = t.as_strided((rows, cols) if len(shape) == 2 else (rows * cols,), (cols, 1) if len(shape) == 2 else (1,), first * rows)
-        return t if len(shape) in (1, 2) and t.shape == shape else t.view(shape)
-
-    return LogProbs(None if tok is None else part(2, given, tokens.shape), part(0, 1, lead), part(1, 1, lead),
-                    part(2 + given, top, lead + (top,), torch.int32) if top else None, part(2 + given + top, top, lead + (top,)) if top else None)
+    if len(lead) == 1:
+        lp = None if tok is None else mem.as_strided(tokens.shape, (1,) if tokens.ndim == 1 else (given, 1), 2 * rows)
+        lse, ent, ids, tlp = mem.as_strided(lead, (1,), 0), mem.as_strided(lead, (1,), rows), None, None
+        if top:
+            ids = mem.view(torch.int32).as_strided((rows, top), (top, 1), (2 + given) * rows)
+            tlp = mem.as_strided((rows, top), (top, 1), (2 + given + top) * rows)
+        return LogProbs(lp, lse, ent, ids, tlp)
+    lse, ent, lp, ids, tlp = mem.split_with_sizes([rows, rows, given * rows, top * rows, top * rows])
+    return LogProbs(None if tok is None else lp.view(tokens.shape), lse.view(lead), ent.view(lead), ids.view(torch.int32).view(lead + (top,)) if top else None,
+                    tlp.view(lead + (top,)) if top else None)

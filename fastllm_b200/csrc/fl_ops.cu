@@ -229,21 +229,22 @@ static void run_linear8(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
     else launch_few<128>(lc, bytes, q, ldq, w, ldw, g, !given);
 }
 
-// Blocks per row: as many as the chip holds (four per SM) over the rows, while every warp has two chunks; at most eight with alternatives, whose lists
-// the first block joins (1 x 32000, five alternatives, 4, 8 and 16 blocks: 6.8, 6.2 and 6.3 us; 64 x 152064 f32, twenty: 16.6, 16.6 and 31.0; none: 10.8, 9.4
-// and 12.0).  The cluster of 16 is not portable to every chip, but B200 has it.  One block per row: small ones where there are more rows than SMs
-// hold large ones (1000 x 32003 f16, five alternatives 26.2 -> 22.0 us with 128 threads, 300 x 32000 f32 15.0 -> 19.6).
+// Blocks per row: two per SM over the rows, while every warp has two chunks; at most eight with alternatives, whose lists the first block joins (1 x 32000,
+// five alternatives, 4, 8 and 16 blocks: 6.8, 6.2 and 6.3 us; 64 x 152064 f32, none: 1, 2, 4 and 8 blocks 16.4, 11.8, 9.2 and 9.8; 128 x 32000: 6.3, 6.7, 7.1
+// and 10.3).  The cluster of 16 is not portable to every chip, but B200 has it.  Small blocks where there are more rows than SMs hold large ones (256 -> 128
+// threads, five alternatives: 1000 x 32003 f16 23.4 -> 19.6 us, 777 x 32000 f32 28.4 -> 22.1, 400 x 32000 12.7 -> 13.2), but not for 16-bit rows of 512
+// chunks and more, whose exponentials are the limit (2048 x 152064 112 -> 120).
 template <typename T>
 static void run_logprobs(LaunchCtx& lc, const LogprobArgs& a) {
     const int chunks = (a.vocab + 2 * LpRow<T>::N - 1 + LpRow<T>::kChunk - 1) / LpRow<T>::kChunk;
     const int most = a.top > 0 ? kLpMaxCluster / 2 : kLpMaxCluster;
     int C = 1;
-    while (C < most && (long long)a.rows * 2 * C <= 4 * kNumSMs && chunks >= 16 * C) C *= 2;
+    while (C < most && (long long)a.rows * 2 * C <= 2 * kNumSMs && chunks >= 16 * C) C *= 2;
     const uint64_t bytes = (uint64_t)a.rows * a.vocab * sizeof(T);
     const dim3 grid((unsigned)((long long)a.rows * C));
     const size_t smem = a.top > 0 ? (size_t)((chunks + C - 1) / C + 1) * 4 : 0;
     auto go = [&](auto kern, int threads) { launch_op(lc, "logprobs", bytes, kern, grid, threads, smem, C, false, a, C); };
-    if (a.rows > 6 * kNumSMs) a.top > 0 ? go(logprobs_kernel<T, true, 128>, 128) : go(logprobs_kernel<T, false, 128>, 128);
+    if (a.rows > 4 * kNumSMs && !(sizeof(T) == 2 && chunks >= 512)) a.top > 0 ? go(logprobs_kernel<T, true, 128>, 128) : go(logprobs_kernel<T, false, 128>, 128);
     else a.top > 0 ? go(logprobs_kernel<T, true, 256>, 256) : go(logprobs_kernel<T, false, 256>, 256);
 }
 template <typename T>

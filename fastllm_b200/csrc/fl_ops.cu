@@ -151,17 +151,18 @@ template <typename T>
 static void quantize_rows_t(LaunchCtx& lc, const void* x, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, int64_t cols_q, float* scale) {
     constexpr int V = 16 / sizeof(T);
     const uint64_t bytes = rows * cols * (sizeof(T) + 1);
-    auto go = [&](auto kern) {
-        launch_op(lc, "quantize_rows", bytes, kern, dim3((unsigned)rows), 256, 0, 1, false, static_cast<const T*>(x), (long long)ldx, (int)cols, q, (long long)ldq,
+    auto go = [&](auto kern, int threads) {
+        launch_op(lc, "quantize_rows", bytes, kern, dim3((unsigned)rows), threads, 0, 1, false, static_cast<const T*>(x), (long long)ldx, (int)cols, q, (long long)ldq,
                   (int)cols_q, scale);
     };
     const bool vec = aligned(x, 16) && aligned(q, V) && (rows == 1 || (ldx % V == 0 && ldq % V == 0));
     const int64_t vecs = (cols_q + V - 1) / V;
-    if (!vec || vecs > 8 * 256) go(quantize_rows_kernel<T, 0>);
-    else if (vecs <= 256) go(quantize_rows_kernel<T, 1>);
-    else if (vecs <= 2 * 256) go(quantize_rows_kernel<T, 2>);
-    else if (vecs <= 4 * 256) go(quantize_rows_kernel<T, 4>);
-    else go(quantize_rows_kernel<T, 8>);
+    if (!vec) go(quantize_rows_kernel<T, 0, 256>, 256);
+    else if (vecs <= 2 * 128) go(quantize_rows_kernel<T, 2, 128>, 128);
+    else if (vecs <= 2 * 256) go(quantize_rows_kernel<T, 2, 256>, 256);
+    else if (vecs <= 4 * 256) go(quantize_rows_kernel<T, 4, 256>, 256);
+    else if (vecs <= 8 * 256) go(quantize_rows_kernel<T, 8, 256>, 256);
+    else go(quantize_rows_kernel<T, -1, 256>, 256);
 }
 static void quantize_rows(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, int64_t cols_q, float* scale) {
     if (dtype == FL_DTYPE_F32) quantize_rows_t<float>(lc, x, rows, cols, ldx, q, ldq, cols_q, scale);

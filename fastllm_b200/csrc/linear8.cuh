@@ -18,7 +18,7 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 
 // One row's rounding rule: q = 127 x / a to the nearest whole number, halves to the even one, of the exact quotient (a = max |x|).
 // x * (127 / a) in f32 is off by at most 127 * 2^-23 = 1.5e-5, so only quotients that lie within 1e-4 of a half need the exact sign of
-// 254 x - (2 low + 1) a, which 64 bits hold without rounding.
+// 254 x - (2 low + 1) a.  (Rows of bf16 hold x = a / 2 once in a thousand: in 64 bits that sign took half of the kernel's time.)
 struct RowScale {
     float a, mul, up;       // max |x|; 127 / a (0: all q are 0); 1, or a power of two that keeps 127 / (a up) finite in the smallest rows
     float scale;            // a / 127; NaN for a row with a NaN or an infinity
@@ -29,11 +29,13 @@ struct RowScale {
         mul = bad || a == 0.f ? 0.f : 127.f / (a * up);
         scale = bad ? __uint_as_float(0x7FFFFFFFu) : a / 127.f;
     }
-    static __device__ __noinline__ uint32_t exact(float x, float mul, float a) {
-        const float low = floorf(x * mul);
-        const double over = fma(254.0, (double)x, -(2.0 * (double)low + 1.0) * (double)a);
+    // The sign of 254 x - (2 low + 1) a, a 512th of it so that the largest rows stay in range, without a rounding that matters: the product's own is `lo`, and
+    // next to a half the difference is exact (x is a 254th of a at least there: 18 bits are left).
+    static __device__ __forceinline__ uint32_t exact(float x, float mul, float a) {
+        const float low = floorf(x * mul), m = 2.f * low + 1.f, part = a * (1.f / 512.f), hi = m * part, lo = fmaf(m, part, -hi);
+        const float over = fmaf(254.f / 512.f, x, -hi) - lo;
         const int l = (int)low;
-        return (uint32_t)(over > 0.0 ? l + 1 : (over < 0.0 ? l : l + (l & 1)));
+        return (uint32_t)(over > 0.f ? l + 1 : (over < 0.f ? l : l + (l & 1)));
     }
     // four values, packed.  1.5 * 2^23 leaves the nearest whole number in the sum's low bits.
     __device__ __forceinline__ uint32_t four(float x0, float x1, float x2, float x3) const {
@@ -59,70 +61,86 @@ struct RowScale {
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 // A block per row; columns [cols, cols_q) of q are filled with zeros.  kVecs > 0: the row starts on 16-byte borders on both sides (8 for q) and has at
-// most 256 * kVecs vectors of 16 bytes, which stay in registers between the maximum and the rounding; 0: any row, read twice.
-template <typename T, int kVecs>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, long long ldx, int cols, int8_t* __restrict__ q, long long ldq, int cols_q,
-                                                            float* __restrict__ scale) {
-    constexpr int V = 16 / sizeof(T);
-    __shared__ uint32_t part[8];
+// most kThreads * kVecs vectors of 16 bytes, which stay in registers between the maximum and the rounding; -1: such a row of any length, read
+// again for the rounding, from L2 or nearer (1531 x 14336 15.9 us with eight vectors a thread in registers, 19.0 so; 8192 x 8192 f16 34.6, 5.8 TB/s); 0: any row.
+template <typename T, int kVecs, int kThreads>
+__global__ void __launch_bounds__(kThreads, kVecs == 8 ? 4 : 1536 / kThreads) quantize_rows_kernel(const T* __restrict__ x, long long ldx, int cols, int8_t* __restrict__ q, long long ldq,
+                                                                                  int cols_q, float* __restrict__ scale) {
+    constexpr int V = 16 / sizeof(T), kHeld = kVecs > 0 ? kVecs : 1;
+    __shared__ uint32_t part[kThreads / 32];
     const T* xr = x + (long long)blockIdx.x * ldx;
     int8_t* qr = q + (long long)blockIdx.x * ldq;
     pdl_launch_dependents();
+    auto load = [&](int at) {                                   // V values from column `at` on, zeros past the end
+        uint4 h = make_uint4(0, 0, 0, 0);
+        if (at + V <= cols) {
+            h = *reinterpret_cast<const uint4*>(xr + at);
+        } else if (at < cols) {
+            T* e = reinterpret_cast<T*>(&h);
+            for (int j = 0; j < V; ++j)
+                if (at + j < cols) e[j] = xr[at + j];
+        }
+        return h;
+    };
+    auto most = [](uint32_t m, const uint4& h) {                // the larger magnitude, of two at once where they are 16-bit: their bits are in the order of their sizes
+        if constexpr (sizeof(T) == 4)
+            return max(max(m, max(h.x & 0x7FFFFFFFu, h.y & 0x7FFFFFFFu)), max(h.z & 0x7FFFFFFFu, h.w & 0x7FFFFFFFu));
+        else
+            return __vmaxu2(m, __vmaxu2(__vmaxu2(h.x & 0x7FFF7FFFu, h.y & 0x7FFF7FFFu), __vmaxu2(h.z & 0x7FFF7FFFu, h.w & 0x7FFF7FFFu)));
+    };
     uint32_t m = 0;
-    uint4 held[kVecs > 0 ? kVecs : 1];
+    uint4 held[kHeld];
     if constexpr (kVecs > 0) {
 #pragma unroll
-        for (int u = 0; u < kVecs; ++u) {
-            const int at = (threadIdx.x + 256 * u) * V;
-            held[u] = make_uint4(0, 0, 0, 0);
-            if (at + V <= cols) {
-                held[u] = __ldg(reinterpret_cast<const uint4*>(xr + at));
-            } else if (at < cols) {
-                T* e = reinterpret_cast<T*>(&held[u]);
-                for (int j = 0; j < V; ++j)
-                    if (at + j < cols) e[j] = xr[at + j];
-            }
-        }
+        for (int u = 0; u < kVecs; ++u) held[u] = load((threadIdx.x + kThreads * u) * V);
 #pragma unroll
-        for (int u = 0; u < kVecs; ++u) {
-            if constexpr (sizeof(T) == 4) {
-                m = max(max(m, max(held[u].x & 0x7FFFFFFFu, held[u].y & 0x7FFFFFFFu)), max(held[u].z & 0x7FFFFFFFu, held[u].w & 0x7FFFFFFFu));
-            } else {                                            // two magnitudes at once: their bits are in the order of their sizes
-                const uint32_t w = __vmaxu2(__vmaxu2(held[u].x & 0x7FFF7FFFu, held[u].y & 0x7FFF7FFFu), __vmaxu2(held[u].z & 0x7FFF7FFFu, held[u].w & 0x7FFF7FFFu));
-                m = __vmaxu2(m, w);
-            }
+        for (int u = 0; u < kVecs; ++u) m = most(m, held[u]);
+    } else if constexpr (kVecs < 0) {
+        int at = threadIdx.x * V;
+        for (; at + (3 * kThreads + 1) * V <= cols; at += 4 * kThreads * V) {
+            uint4 h[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) h[u] = *reinterpret_cast<const uint4*>(xr + at + u * kThreads * V);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) m = most(m, h[u]);
         }
-        if constexpr (sizeof(T) == 2) {
-            const uint16_t h = (uint16_t)max(m & 0xFFFFu, m >> 16);
-            m = abs_bits(to_f32(*reinterpret_cast<const T*>(&h)));
-        }
+        for (; at < cols; at += kThreads * V) m = most(m, load(at));
     } else {
-        for (int i = threadIdx.x; i < cols; i += 256) m = max(m, abs_bits(to_f32(xr[i])));
+        for (int i = threadIdx.x; i < cols; i += kThreads) m = max(m, abs_bits(to_f32(xr[i])));
+    }
+    if constexpr (kVecs != 0 && sizeof(T) == 2) {
+        const uint16_t h = (uint16_t)max(m & 0xFFFFu, m >> 16);
+        m = abs_bits(to_f32(*reinterpret_cast<const T*>(&h)));
     }
     m = __reduce_max_sync(0xFFFFFFFFu, m);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, part[i]);
+    for (int i = 0; i < kThreads / 32; ++i) m = max(m, part[i]);
     const RowScale rs(m);
+    auto put = [&](int at, const uint4& h) {
+        const T* e = reinterpret_cast<const T*>(&h);
+        uint32_t w[V / 4];
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) w[i] = rs.four(to_f32(e[4 * i]), to_f32(e[4 * i + 1]), to_f32(e[4 * i + 2]), to_f32(e[4 * i + 3]));
+        if (at + V <= cols_q) {
+            if constexpr (V == 8) *reinterpret_cast<uint2*>(qr + at) = make_uint2(w[0], w[1]);
+            else *reinterpret_cast<uint32_t*>(qr + at) = w[0];
+        } else {
+            for (int j = 0; at + j < cols_q; ++j) qr[at + j] = (int8_t)(w[j / 4] >> (8 * (j % 4)));
+        }
+    };
     if constexpr (kVecs > 0) {
 #pragma unroll
         for (int u = 0; u < kVecs; ++u) {
-            const int at = (threadIdx.x + 256 * u) * V;
-            if (at >= cols_q) break;
-            const T* e = reinterpret_cast<const T*>(&held[u]);
-            uint32_t w[V / 4];
-#pragma unroll
-            for (int i = 0; i < V / 4; ++i) w[i] = rs.four(to_f32(e[4 * i]), to_f32(e[4 * i + 1]), to_f32(e[4 * i + 2]), to_f32(e[4 * i + 3]));
-            if (at + V <= cols_q) {
-                if constexpr (V == 8) *reinterpret_cast<uint2*>(qr + at) = make_uint2(w[0], w[1]);
-                else *reinterpret_cast<uint32_t*>(qr + at) = w[0];
-            } else {
-                for (int j = 0; at + j < cols_q; ++j) qr[at + j] = (int8_t)(w[j / 4] >> (8 * (j % 4)));
-            }
+            const int at = (threadIdx.x + kThreads * u) * V;
+            if (at < cols_q) put(at, held[u]);
         }
+    } else if constexpr (kVecs < 0) {
+#pragma unroll 2
+        for (int at = threadIdx.x * V; at < cols_q; at += kThreads * V) put(at, load(at));
     } else {
-        for (int i = threadIdx.x; i < cols_q; i += 256) qr[i] = i < cols ? (int8_t)rs.four(to_f32(xr[i]), 0.f, 0.f, 0.f) : (int8_t)0;
+        for (int i = threadIdx.x; i < cols_q; i += kThreads) qr[i] = i < cols ? (int8_t)rs.four(to_f32(xr[i]), 0.f, 0.f, 0.f) : (int8_t)0;
     }
     if (threadIdx.x == 0) scale[blockIdx.x] = rs.scale;
 }

@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
         uint4 v[U];
         int ch = first + warp - ch0;
         auto place = [&](int u) { return ch + u * kWarps; };
-        if constexpr (TOP) {                                    // (the registers of a second set are worth more as a further block per SM)
+        if constexpr (TOP && kThreads == 128) {                 // (many rows: the registers of a second set are worth more as a further block per SM)
             for (int i = 0; i < batches; ++i, ch += U * kWarps) {
                 fetch(v);
                 absorb(v, place);
@@ -305,9 +305,11 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
             for (int i = 0; i < batches; i += 2) {
                 if (i + 1 < batches) fetch(w);
                 absorb(v, place);
+                ch += U * kWarps;
                 if (i + 1 >= batches) break;
                 if (i + 2 < batches) fetch(v);
                 absorb(w, place);
+                ch += U * kWarps;
             }
         }
     }

@@ -1517,7 +1517,7 @@ void layered_forward(fl_cache& c, const int* slots, const int* counts, int n, co
     c.logit_rows = 0;
     ensure_ws(c, (size_t)T, (size_t)n_want);
     reserve_portions(c, slots, counts, n);
-    c.may_fail = false;
+    c.may_fail = m.cfg.head_bits == 8 && n_want > 0;
     step_pairs(c, m.f32 ? 0 : (size_t)T);
     const size_t tab_ints = (size_t)4 * T + 3 * (size_t)n + 1 + (size_t)n_want;
     if (tab_ints > y.tab_cap) {
@@ -2106,7 +2106,7 @@ static void enqueue_step(fl_cache& c, LaunchCtx& lc, const StepTab& st, const in
                eps, W, m.cfg.logit_scale != 0.f ? m.cfg.logit_scale : 1.f, y.hf.p,
                m.tc_head ? y.hf_hi.p : (uint16_t*)nullptr, y.hf_lo.p);
         if (m.cfg.head_bits == 8)
-            op_linear8(lc, y.hf.p, m.head8.p, m.head8_scale.p, n_want, m.V, W, y.logits.p, y.head8_ws.p);
+            op_linear8(lc, y.hf.p, m.head8.p, m.head8_scale.p, n_want, m.V, W, y.logits.p, y.head8_ws.p, c.step_failed.p);
         else
             gemm_tc_or_exact(c, lc, "gemm_head", y.hf.p, m.tc_head ? y.hf_hi.p : nullptr, y.hf_lo.p, m.head, m.tm_head, m.tc_head, m.V, W, y.logits.p, n_want);
         if (m.cfg.logit_softcap > 0.f) {

@@ -117,17 +117,32 @@ template <int BN>
 static void few_attr() {
     FL_CUDA(cudaFuncSetAttribute(linear8_few_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L8Few<BN>::kSmem));
 }
+// Unsafe calls for the length of a scope: set-up does not belong to a graph that the caller's thread may be capturing.
+struct RelaxedCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    RelaxedCapture() { FL_CUDA(cudaThreadExchangeStreamCaptureMode(&mode)); }
+    ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+template <typename... Kernels>
+static void load_kernels(Kernels... kernels) {
+    cudaFuncAttributes at;
+    for (cudaError_t e : {cudaFuncGetAttributes(&at, kernels)...}) FL_CUDA(e);
+}
+template <typename T>
+static void load_kernels_of() {
+    load_kernels(quantize_rows_kernel<T, 0, 256>, quantize_rows_kernel<T, 2, 128>, quantize_rows_kernel<T, 2, 256>, quantize_rows_kernel<T, 4, 256>,
+                 quantize_rows_kernel<T, 8, 256>, quantize_rows_kernel<T, -1, 256>, logprobs_kernel<T, true, 128>, logprobs_kernel<T, false, 128>);
+    FL_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, true, 256>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    FL_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, false, 256>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    FL_CUDA(cudaFuncSetAttribute(linear8_small_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL8SmallSmem));
+}
 // One-time set-up, with fl_init: also loads the kernels, so that a caller's first call may be one inside a graph capture.
 void ops_init() {
     if (g_op_failed != nullptr) return;
-    FL_CUDA(cudaFuncSetAttribute(linear8_small_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL8SmallSmem));
-    FL_CUDA(cudaFuncSetAttribute(linear8_small_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL8SmallSmem));
-    FL_CUDA(cudaFuncSetAttribute(linear8_small_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL8SmallSmem));
+    RelaxedCapture relaxed;
+    load_kernels_of<float>(); load_kernels_of<__nv_bfloat16>(); load_kernels_of<__half>();
     few_attr<16>(); few_attr<32>(); few_attr<64>(); few_attr<128>();
     FL_CUDA(cudaFuncSetAttribute(linear8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL8PairSmem));
-    auto wide = [](auto kern) { FL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)); };
-    wide(logprobs_kernel<float, false, 256>); wide(logprobs_kernel<__nv_bfloat16, false, 256>); wide(logprobs_kernel<__half, false, 256>);
-    wide(logprobs_kernel<float, true, 256>); wide(logprobs_kernel<__nv_bfloat16, true, 256>); wide(logprobs_kernel<__half, true, 256>);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(kNumSMs); cfg.blockDim = dim3(kL8PairThreads); cfg.dynamicSmemBytes = kL8PairSmem;
     cudaLaunchAttribute at[1];
@@ -204,11 +219,11 @@ static void launch_pair(LaunchCtx& lc, uint64_t bytes, const int8_t* x, int64_t 
 }
 
 static void run_linear8(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
-                        int64_t rows, int64_t n, int64_t k, void* y, int y_dtype, int64_t ldy, void* workspace) {
+                        int64_t rows, int64_t n, int64_t k, void* y, int y_dtype, int64_t ldy, void* workspace, int* failed) {
     const bool given = x_dtype == FL_DTYPE_I8;
     const int8_t* q = static_cast<const int8_t*>(x);
     int64_t ldq = rows == 1 ? padded8(k) : ldx;
-    Linear8Args g{(int)rows, (int)n, (int)k, x_scale, w_scale, bias, y, ldy, y_dtype, g_op_failed};
+    Linear8Args g{(int)rows, (int)n, (int)k, x_scale, w_scale, bias, y, ldy, y_dtype, failed};
     if (n == 1) ldw = padded8(k);
     const uint64_t bytes = (uint64_t)n * k + (uint64_t)rows * (k + n * dtype_size(y_dtype));
     if (!given && small_fits(rows, n, k)) {
@@ -263,9 +278,8 @@ size_t linear8_workspace(int64_t rows, int64_t n, int64_t k) { return linear8_ro
 void op_quantize_rows(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale) {
     quantize_rows(lc, x, dtype, rows, cols, ldx, q, ldq, ldq, scale);
 }
-void op_linear8(LaunchCtx& lc, const float* x, const int8_t* w, const float* w_scale, int64_t rows, int64_t n, int64_t k, float* y, void* workspace) {
-    check_op_failed();
-    run_linear8(lc, x, FL_DTYPE_F32, k, nullptr, w, padded8(k), w_scale, nullptr, rows, n, k, y, FL_DTYPE_F32, n, workspace);
+void op_linear8(LaunchCtx& lc, const float* x, const int8_t* w, const float* w_scale, int64_t rows, int64_t n, int64_t k, float* y, void* workspace, int* failed) {
+    run_linear8(lc, x, FL_DTYPE_F32, k, nullptr, w, padded8(k), w_scale, nullptr, rows, n, k, y, FL_DTYPE_F32, n, workspace, failed);
 }
 void op_logprobs(LaunchCtx& lc, const float* logits, int64_t rows, int64_t vocab, const int32_t* tokens, int64_t given, double temperature, int top, float* logprob,
                  float* logsumexp, float* entropy, int32_t* top_ids, float* top_logprobs) {
@@ -329,7 +343,7 @@ FL_EXPORT int fl_linear8(const void* x, int x_dtype, int64_t ldx, const float* x
     DeviceScope dev;
     LaunchCtx lc = op_ctx(stream);
     check_op_failed();
-    run_linear8(lc, x, x_dtype, ldx, x_scale, w, ldw, w_scale, bias, rows, n, k, y, y_dtype, ldy, workspace);
+    run_linear8(lc, x, x_dtype, ldx, x_scale, w, ldw, w_scale, bias, rows, n, k, y, y_dtype, ldy, workspace, g_op_failed);
     FL_API_END
 }
 

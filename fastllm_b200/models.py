@@ -251,6 +251,8 @@ class DeviceCache:
         """Log probabilities over the logits of the last forward on this cache, which are still on the device (fl_cache_logprobs): of
         `tokens` ([rows] or [rows, m]; negative ones are padding with 0), and of the `top` most likely alternatives.  rows: the first
         that many rows of that forward (default: as tokens has)."""
+        if tokens is None and rows is None:
+            raise FastllmError(-1, "log probabilities of how many rows: neither tokens nor rows are given")
         tok = None if tokens is None else np.ascontiguousarray(tokens, dtype=np.int32)
         if tok is not None and tok.ndim not in (1, 2):
             raise FastllmError(-1, f"tokens are [rows] or [rows, m], got shape {tok.shape}")
@@ -1405,13 +1407,19 @@ class Scored(NamedTuple):
 
 def score(model, texts, top: int = 0, cache: DeviceCache | None = None, portion: int = 512) -> list:
     """Log probabilities of given texts (token id lists) under a layered model -> one Scored per text.  Up to the cache's slots of texts are
-    read side by side, at most `portion` tokens a step; logits stay on the device, where they become log probabilities."""
+    read side by side, at most `portion` tokens a step; logits stay on the device, where they become log probabilities.  A given cache has no
+    sequence in any slot, and room for as many tokens as its slots can hold."""
     if cache is None:
         if not hasattr(model, "new_device_cache"):
             raise FastllmError(-5, "scoring wants the logits of every position: mixed-batch steps, offered for layered models only")
         cache = model.new_device_cache(max(1, min(len(texts), 8)), max([64] + [len(t) for t in texts]))
     if portion < cache.max_batch:
         raise FastllmError(-1, "a step brings at least one token of every text that is being read")
+    if any(cache.slot_len(s) for s in range(cache.max_batch)):
+        raise FastllmError(-3, "a slot of the cache holds a sequence")
+    for t in texts:
+        if len(t) - 1 > cache.max_seq or any(not 0 <= int(x) < cache.vocab for x in t):
+            raise FastllmError(-1, "a text is longer than the cache, or has a token outside the vocabulary")
     parts = [[] for _ in texts]
     waiting = [i for i, t in enumerate(texts) if len(t) > 1][::-1]
     free, running = list(range(cache.max_batch))[::-1], {}      # slot -> [text, tokens fed]
@@ -1427,8 +1435,13 @@ def score(model, texts, top: int = 0, cache: DeviceCache | None = None, portion:
             toks.append(part)
             want.append(range(len(part)))
             given.extend(int(x) for x in texts[t][fed + 1:fed + 1 + len(part)])
-        cache.forward_ragged(slots, toks, want, fetch=False)
-        lp, row = cache.logprobs(np.asarray(given, dtype=np.int32), top), 0
+        try:
+            cache.forward_ragged(slots, toks, want, fetch=False)
+            lp, row = cache.logprobs(np.asarray(given, dtype=np.int32), top), 0
+        except FastllmError:
+            for s in running:               # (the caller's cache as it was)
+                cache.slot_reset(s)
+            raise
         for s, part in zip(slots, toks):
             t = running[s][0]
             at = slice(row, row + len(part))

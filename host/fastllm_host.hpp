@@ -82,6 +82,20 @@ struct DeviceCache {   // paged KV cache + stream (fl_cache*)
     DeviceCache& operator=(const DeviceCache&) = delete;
 };
 
+// Log probabilities over the last forward's logits, which are still on the device: rows 0 .. rows - 1, of tokens [rows, given] (given = tokens / rows,
+// negative ones are padding) and of the `top` most likely alternatives.
+struct LogProbs {
+    std::vector<float> logprob, logsumexp, entropy, top_logprobs;
+    std::vector<int32_t> top_ids;
+};
+inline LogProbs logprobs(fl_cache* c, int rows, const std::vector<int32_t>& tokens, int top, double temperature = 1.0) {
+    LogProbs r;
+    const int given = rows > 0 ? (int)(tokens.size() / rows) : 0;
+    r.logprob.resize(tokens.size()); r.logsumexp.resize(rows); r.entropy.resize(rows);
+    r.top_ids.resize((size_t)rows * top); r.top_logprobs.resize((size_t)rows * top);
+    check(fl_cache_logprobs(c, rows, tokens.data(), given, temperature, top, r.logprob.data(), r.logsumexp.data(), r.entropy.data(), r.top_ids.data(), r.top_logprobs.data()));
+    return r;
+}
 struct LlamaCache : CommonCache {     // llama.rs:61-92: owns the KV (candle `Cache`); bound lazily on first forward
     std::unique_ptr<DeviceCache> inner;
 };

@@ -2,6 +2,9 @@
 
 Tolerances count roundings: u = 2^-24 is half a step of f32, half = finfo(type).eps / 2 that of the result's type."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -439,6 +442,33 @@ def test_other_streams():
     for x, tokens, r in got:
         for a, b in zip(r, _score(x, w, ws, tokens)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows", [1, 60, 300])
+def test_first_call_inside_a_capture(rows):
+    """a process whose first calls are captured: set-up and loading do not break the capture"""
+    code = """
+import torch
+from fastllm_b200 import ops
+rows = %d
+g = torch.Generator(device="cuda"); g.manual_seed(1)
+x = torch.randn(rows, 200, device="cuda", generator=g).bfloat16()
+w = torch.empty(900, 208, dtype=torch.int8, device="cuda").random_(-127, 128, generator=g)[:, :200]
+s = torch.rand(900, device="cuda", generator=g)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = ops.linear8(x, w, s, out_dtype=torch.float32)
+    r = ops.logprobs(y, top=5)
+graph.replay()
+torch.cuda.synchronize()
+y2 = ops.linear8(x, w, s, out_dtype=torch.float32)
+r2 = ops.logprobs(y2, top=5)
+assert torch.equal(y, y2) and torch.equal(r.logsumexp, r2.logsumexp) and torch.equal(r.top_ids, r2.top_ids)
+print("same")
+""" % rows
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=root, env=dict(os.environ, PYTHONPATH=root))
+    assert r.returncode == 0 and r.stdout.strip() == "same", r.stderr[-2000:]
 
 
 @pytest.mark.parametrize("rows", [1, 60, 300, 1100])

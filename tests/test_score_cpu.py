@@ -26,7 +26,7 @@ class _Cache:
     ragged = True
 
     def __init__(self, slots):
-        self.max_batch, self.hist, self.last, self.sizes = slots, [[] for _ in range(slots)], None, []
+        self.max_batch, self.hist, self.last, self.sizes, self.max_seq, self.vocab = slots, [[] for _ in range(slots)], None, [], 30, VOCAB
         if not self.ragged:
             self.forward_ragged = None
 
@@ -54,6 +54,9 @@ class _Cache:
         ids = np.argsort(-lp, axis=1, kind="stable")[:, :top]
         given = np.array([0.0 if t < 0 else lp[i, t] for i, t in enumerate(tokens)])
         return models.LogProbs(given, np.zeros(len(tokens)), -(np.exp(lp) * lp).sum(1), ids.astype(np.int32), np.take_along_axis(lp, ids, 1))
+
+    def slot_len(self, slot):
+        return len(self.hist[slot])
 
     def slot_reset(self, slot):
         assert self.hist[slot]
@@ -114,6 +117,25 @@ def test_score_refusals():
         models.score(_Model(), [[3, 4]])
     with pytest.raises(FastllmError, match="at least one token"):
         models.score(_Model(), [[3, 4]], cache=_Cache(4), portion=3)
+    for bad in ([3] * 32, [3, VOCAB], [3, -1]):
+        with pytest.raises(FastllmError, match="longer than the cache"):
+            models.score(_Model(), [[3, 4], bad], cache=_Cache(2))
+    assert models.score(_Model(), [[3] * 31], cache=_Cache(1))[0].logprobs.shape == (30,)
+    used = _Cache(2)
+    used.forward_slots([1], [[5, 6]], [0])
+    with pytest.raises(FastllmError, match="holds a sequence"):
+        models.score(_Model(), [[3, 4]], cache=used)
+
+
+def test_score_gives_its_slots_back_after_an_error():
+    class _Broken(_Cache):
+        def logprobs(self, *args, **kw):
+            raise FastllmError(-2, "lost")
+
+    cache = _Broken(2)
+    with pytest.raises(FastllmError, match="lost"):
+        models.score(_Model(), [[3, 4, 5], [6, 7, 8]], cache=cache)
+    assert not any(cache.hist)
 
 
 def test_head_bits_of_other_models_are_refused(tmp_path):

@@ -63,7 +63,7 @@ def test_last_forward_of_the_llama_family(name):
     _check(cache.logprobs([9, 8, 7], 5), step, [9, 8, 7], 5)
     got = cache.forward_greedy(np.asarray([[5], [6], [7]], dtype=np.uint32), 8)
     assert np.array_equal(cache.logprobs(rows=3, top=1).top_ids[:, 0], got)
-    for bad in (dict(rows=4), dict(rows=1, top=33), dict(rows=1, top=-1), dict(rows=1, temperature=0.0), dict(tokens=[1, 2], rows=1), dict(rows=-1)):
+    for bad in (dict(), dict(rows=4), dict(rows=1, top=33), dict(rows=1, top=-1), dict(rows=1, temperature=0.0), dict(tokens=[1, 2], rows=1), dict(rows=-1)):
         with pytest.raises(FastllmError):
             cache.logprobs(**bad)
     cache.decode_greedy_loop(got, 9, 3)
@@ -173,6 +173,20 @@ def test_head_in_8_bits(width, vocab):
         rms = np.sqrt((d ** 2).mean() / (y16.astype(np.float64) ** 2).mean())
         assert 1e-5 < rms < 0.03        # (steps of a 127th of the largest of a row: 1 % where that is four times the rms)
     _check(rows[1].logprobs([3], 5), y8, [3], 5)
+
+
+def test_tied_head_in_8_bits():
+    """the embedding table itself stays as it is; looped layers, every position of a prompt, then single steps"""
+    import test_latodra_gpu as latodra
+    from oracle import latodra as OL
+    cfg = latodra.deep_cfg(vocab=96)
+    w = OL.random_weights(cfg, 8)
+    make = lambda bits: models.LatodraWithConfig.initialize_model(cfg, {k: latodra.to_bits(v) for k, v in w.items()}, "bf16", head_bits=bits)[0]  # noqa: E731
+    a, b = (make(bits).new_device_cache(2, 128) for bits in (16, 8))
+    for step in [latodra.tokens(cfg, 60)] + [[t] for t in (5, 6, 7, 8)]:
+        y16, y8 = (c.forward_ragged([0], [step], [range(len(step))]).astype(np.float64) for c in (a, b))
+        assert 1e-5 < np.sqrt(((y8 - y16) ** 2).mean() / (y16 ** 2).mean()) < 0.03
+    assert a.model.streamed_bytes() - b.model.streamed_bytes() == 96 * 32
 
 
 def test_head_in_8_bits_streams_less_and_is_refused_elsewhere():

@@ -1,6 +1,9 @@
 // Matrix product in 8-bit integers with a scale per token and per channel:
 //   y[r, n] = (sum_k q[r, k] w[n, k]) s[r] t[n] + b[n],   q, w whole numbers of 8 bits, the sum exact in 32-bit integers,
-// and the rounding of activations to such rows.
+// and the rounding of activations to such rows.  Products run on tcgen05.mma.kind::i8 with the weights as the 128- or 256-row operand throughout: a lane of the
+// accumulators is a weight row, so the 32 lanes of a warp write 32 neighbours of a result row whatever its alignment, and a row count is cut
+// into tiles of any multiple of 32.  Scales are applied to the finished sum in f32: the sum rounded once (2^-24), two products, the bias, then
+// one rounding to the result's type.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -239,8 +242,10 @@ __device__ __forceinline__ void l8_give_up(int* failed) {
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------------------
-// The weights are the 128-row operand and nearly all the traffic, BN activation rows the other one; a cluster of S blocks cuts K of one tile, and
-// its blocks add up each other's parts through shared memory: whole numbers, so the order does not matter, and no workspace.
+// The weights are nearly all the traffic, BN activation rows the other operand; a cluster of S blocks cuts K of one tile, and its blocks add up each
+// other's parts through shared memory: whole numbers, so the order does not matter, and no workspace.  What bounds it: HBM behind 4 to 6 us of
+// launch, first weights and last results (64 x 4096 x 28672 25.3 us, 4.8 TB/s; 37 x 3584 x 152064 to f32 96.6, 5.9 TB/s of the measured 6.55; 64 x 4096 x 4096 10.1).
+// Two blocks per SM hold 96 KB of weights on their way each: one writes its results while the other's arrive.
 template <int BN> struct L8Few {
     static constexpr uint32_t kX = BN * kL8BK, kStage = kL8WBytes + kX;
     static constexpr int kPerSm = BN <= 128 ? 2 : 1;                                   // blocks that an SM holds
@@ -535,9 +540,10 @@ linear8_small_kernel(const __grid_constant__ CUtensorMap tmW, const Linear8Args 
 
 // ---- many rows ----------------------------------------------------------------------------------------------------------------------
 // Pairs of SMs on tiles of 256 weight rows x bn activation rows (tcgen05.mma.cta_group::2): each holds its 128 weight rows and half of the activation
-// tile, 16 KB + 64 bn bytes per k block of 128.  What bounds it: the operands' way from L2, about 90 bytes a nanosecond and SM (a k block took 268 ns at bn =
-// 128, 294 at 160, 364 at 256; the tensor cores need about 1.05 bn).  So tiles are as wide as the row count allows, up to 512: two products of bn / 2 then, in
-// the two halves of the accumulators, which tiles of up to 256 use in turn.
+// tile, 16 KB + 64 bn bytes per k block of 128.  What bounds it: below bn = 256 the operands' way from L2, about 90 bytes a nanosecond and SM (a k block took 268
+// ns at bn = 128, 294 at 160), from there on the tensor cores at the clock that the power limit leaves them (348 at 256, 705 at 512: 1.38 bn; 4096 x 3584 x
+// 37888 433 us or 2.57 Pop/s in a row, 355 and 3.1 once).  So tiles are as wide as the row count and whole waves allow, up to 512: two products of bn / 2
+// then, in the two halves of the accumulators, which tiles of up to 256 use in turn (1531 x 14336 x 4096, bn = 192 and 384: 73 and 65 us).
 constexpr int kL8PairEpi = 16, kL8PairThreads = 64 + 32 * kL8PairEpi, kL8PairMaxStages = 8;
 constexpr uint32_t kL8PairRing = 200 * 1024;
 constexpr size_t kL8PairSmem = kL8PairRing + 1024;

@@ -5,6 +5,8 @@
 // different references are brought to the largest one and joined.  The reference moves when a maximum is 2^16 above it, so the exponentials
 // stay far from overflow and the loop is nearly free of rescaling.  A row belongs to a cluster of C blocks (C = 1 when there are many rows), whose results
 // meet in the first block's shared memory: no workspace, no atomics, the same bits every time.
+// What bounds it: HBM for 32-bit rows (1000 x 152064 91 us, 6.7 TB/s), the exponentials for 16-bit ones (2048 x 152064 bf16 103 us, 6.0 TB/s: one per logit is
+// 77 % of what the special-function units do, 5.6 instructions per logit half of the issue slots), latency for few (1 x 32000: 4 us, 7 with five alternatives).
 //
 // Alternatives: the row lies in chunks of 512 bytes (one load of a warp), whose maxima are kept.  The K-th largest of a block's 256 thread maxima
 // is a lower bound for its K-th largest logit, since K threads hold one at least as large.  Only chunks that reach the bound are read again (from L2),

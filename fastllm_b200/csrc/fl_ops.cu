@@ -130,10 +130,11 @@ static void load_kernels(Kernels... kernels) {
 }
 template <typename T>
 static void load_kernels_of() {
+    if constexpr (sizeof(T) == 2) load_kernels(logprobs_kernel<T, true, 128, false>);
     load_kernels(quantize_rows_kernel<T, 0, 256>, quantize_rows_kernel<T, 2, 128>, quantize_rows_kernel<T, 2, 256>, quantize_rows_kernel<T, 4, 256>,
-                 quantize_rows_kernel<T, 8, 256>, quantize_rows_kernel<T, -1, 256>, logprobs_kernel<T, true, 128>, logprobs_kernel<T, false, 128>);
-    FL_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, true, 256>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    FL_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, false, 256>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+                 quantize_rows_kernel<T, 8, 256>, quantize_rows_kernel<T, -1, 256>, logprobs_kernel<T, true, 128, true>, logprobs_kernel<T, false, 128, true>);
+    FL_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, true, 256, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    FL_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, false, 256, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     FL_CUDA(cudaFuncSetAttribute(linear8_small_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL8SmallSmem));
 }
 // One-time set-up, with fl_init: also loads the kernels, so that a caller's first call may be one inside a graph capture.
@@ -248,8 +249,9 @@ static void run_linear8(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
 // Blocks per row: two per SM over the rows, while every warp has two chunks; at most eight with alternatives, whose lists the first block joins (1 x 32000,
 // five alternatives, 4, 8 and 16 blocks: 6.8, 6.2 and 6.3 us; 64 x 152064 f32, none: 1, 2, 4 and 8 blocks 16.4, 11.8, 9.2 and 9.8; 128 x 32000: 6.3, 6.7, 7.1
 // and 10.3).  The cluster of 16 is not portable to every chip, but B200 has it.  Small blocks where there are more rows than SMs hold large ones (256 -> 128
-// threads, five alternatives: 1000 x 32003 f16 23.4 -> 19.6 us, 777 x 32000 f32 28.4 -> 22.1, 400 x 32000 12.7 -> 13.2), but not for 16-bit rows of 512
-// chunks and more, whose exponentials are the limit (2048 x 152064 112 -> 120).
+// threads, five alternatives: 1000 x 32003 f16 25.1 -> 20.8 us, 777 x 32000 f32 28.8 -> 23.7, but 400 x 32000 12.7 -> 13.2).  With alternatives and many short
+// 16-bit rows the registers of a second batch are worth more as a further block per SM (1300 x 32000 bf16 30.7 -> 25.0 without it; 2048 x 152064 118 -> 111 with
+// it, 2048 x 32000 f32 55.0 -> 52.3).
 template <typename T>
 static void run_logprobs(LaunchCtx& lc, const LogprobArgs& a) {
     const int chunks = (a.vocab + 2 * LpRow<T>::N - 1 + LpRow<T>::kChunk - 1) / LpRow<T>::kChunk;
@@ -260,8 +262,15 @@ static void run_logprobs(LaunchCtx& lc, const LogprobArgs& a) {
     const dim3 grid((unsigned)((long long)a.rows * C));
     const size_t smem = a.top > 0 ? (size_t)((chunks + C - 1) / C + 1) * 4 : 0;
     auto go = [&](auto kern, int threads) { launch_op(lc, "logprobs", bytes, kern, grid, threads, smem, C, false, a, C); };
-    if (a.rows > 4 * kNumSMs && !(sizeof(T) == 2 && chunks >= 512)) a.top > 0 ? go(logprobs_kernel<T, true, 128>, 128) : go(logprobs_kernel<T, false, 128>, 128);
-    else a.top > 0 ? go(logprobs_kernel<T, true, 256>, 256) : go(logprobs_kernel<T, false, 256>, 256);
+    if (a.rows <= 4 * kNumSMs) {
+        a.top > 0 ? go(logprobs_kernel<T, true, 256, true>, 256) : go(logprobs_kernel<T, false, 256, true>, 256);
+    } else if (a.top == 0) {
+        go(logprobs_kernel<T, false, 128, true>, 128);
+    } else {
+        if constexpr (sizeof(T) == 2)
+            if (chunks < 512) return go(logprobs_kernel<T, true, 128, false>, 128);
+        go(logprobs_kernel<T, true, 128, true>, 128);
+    }
 }
 template <typename T>
 static void run_logprobs(LaunchCtx& lc, LogprobArgs a, double temperature) {

@@ -212,7 +212,8 @@ __device__ __forceinline__ int lp_place(const unsigned long long* keys, int n, u
     return before;
 }
 
-template <typename T, bool TOP, int kThreads>
+// TOP: with alternatives; AHEAD: the next batch is on its way while one is added up
+template <typename T, bool TOP, int kThreads, bool AHEAD>
 __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a, const int C) {
     constexpr int kWarps = kThreads / 32, U = 4;
     extern __shared__ uint32_t chunk_max[];                     // TOP: ordered maxima of this block's chunks
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
         uint4 v[U];
         int ch = first + warp - ch0;
         auto place = [&](int u) { return ch + u * kWarps; };
-        if constexpr (TOP && kThreads == 128) {                 // (many rows: the registers of a second set are worth more as a further block per SM)
+        if constexpr (!AHEAD) {
             for (int i = 0; i < batches; ++i, ch += U * kWarps) {
                 fetch(v);
                 absorb(v, place);

@@ -105,7 +105,7 @@ SYMBOLS = {
     "fl_cache_moe_routing": (_I, [_VP, _I, _VP, _VP]),
     "fl_forward_sample_device": (_I, [_VP, _VP, _VP, _I, _I, _SZ, _VP, C.POINTER(C.c_uint32)]),
     "fl_quantize_rows": (_I, [_VP, _I, _I64, _I64, _I64, _VP, _I64, _VP, _VP]),
-    "fl_linear8_workspace": (_I, [_I64, _I64, _I64, _I, C.POINTER(_SZ)]),
+    "fl_linear8_workspace": (_I, [_I64, _I64, _I, C.POINTER(_SZ)]),
     "fl_linear8": (_I, [_VP, _I, _I64, _VP, _VP, _I64, _VP, _VP, _I64, _I64, _I64, _VP, _I, _I64, _VP, _SZ, _VP]),
     "fl_logprobs": (_I, [_VP, _I, _I64, _I64, _I64, _VP, _I, _I64, C.c_double, _I, _VP, _VP, _VP, _VP, _VP, _VP]),
     "fl_embed": (_I, [_VP, _VP, _VP, _I, _I, _VP]),

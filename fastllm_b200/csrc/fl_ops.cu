@@ -63,10 +63,10 @@ static L8Pair pair_plan8(int64_t rows, int64_t n, int64_t k, int clusters) {
 
 // A call's workspace: rounded rows and their scales (none for activations that are 8-bit already)
 struct L8Room { size_t scale = 0, all = 0; };
-static bool small_fits(int64_t rows, int64_t n, int64_t k);
-static L8Room linear8_room(int64_t rows, int64_t n, int64_t k, bool given) {
+static bool token_fits(int64_t rows, int64_t k);
+static L8Room linear8_room(int64_t rows, int64_t k, bool given) {
     L8Room r;
-    if (given || small_fits(rows, n, k)) return r;
+    if (given || token_fits(rows, k)) return r;
     r.scale = up256((size_t)rows * padded8(k));
     r.all = r.scale + (size_t)rows * 4;
     return r;
@@ -135,7 +135,7 @@ static void load_kernels_of() {
                  quantize_rows_kernel<T, 8, 256>, quantize_rows_kernel<T, -1, 256>, logprobs_kernel<T, true, 128, true>, logprobs_kernel<T, false, 128, true>);
     FL_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, true, 256, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     FL_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, false, 256, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    FL_CUDA(cudaFuncSetAttribute(linear8_small_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL8SmallSmem));
+    load_kernels(linear8_token_kernel<T, 1>, linear8_token_kernel<T, 2>);
 }
 // One-time set-up, with fl_init: also loads the kernels, so that a caller's first call may be one inside a graph capture.
 void ops_init() {
@@ -195,16 +195,16 @@ static int few_slices(int64_t tiles, int nk) {
     return S;
 }
 // whether a product's rows are rounded inside its own launch (ops.py keeps the same rule, for the workspace)
-static bool small_fits(int64_t rows, int64_t n, int64_t k) {
-    const int nk = (int)((k + kL8BK - 1) / kL8BK), S = few_slices((n + 127) / 128, nk);
-    return rows <= kL8SmallRows && rows * k <= kL8SmallValues && (nk + S - 1) / S <= kL8SmallBlocks;
-}
+static bool token_fits(int64_t rows, int64_t k) { return rows <= kL8TokenRows && rows * rows * k <= kL8TokenValues; }
 template <typename T>
-static void launch_small(LaunchCtx& lc, uint64_t bytes, const void* x, int64_t ldx, const int8_t* w, int64_t ldw, const Linear8Args& g) {
-    const int tiles = (g.n + 127) / 128, S = few_slices(tiles, (g.k + kL8BK - 1) / kL8BK);
-    const CUtensorMap tw = make_tmap_i8(w, g.n, g.k, ldw, 128);
+static void launch_token(LaunchCtx& lc, uint64_t bytes, const void* x, int64_t ldx, const int8_t* w, int64_t ldw, const Linear8Args& g) {
     const bool vec = aligned(x, 16) && (g.rows == 1 || ldx * sizeof(T) % 16 == 0);
-    launch_op(lc, "linear8", bytes, linear8_small_kernel<T>, dim3((unsigned)(tiles * S)), 192, kL8SmallSmem, S, false, tw, g, S, static_cast<const T*>(x), (long long)ldx, vec);
+    const int per = kL8TokenThreads / 32;
+    const dim3 grid((unsigned)std::min<int64_t>(((int64_t)g.n + per - 1) / per, 4 * kNumSMs));
+    const size_t smem = (size_t)g.rows * padded8(g.k);
+    auto go = [&](auto kern) { launch_op(lc, "linear8", bytes, kern, grid, kL8TokenThreads, smem, 1, false, g, static_cast<const T*>(x), (long long)ldx, vec, w, (long long)ldw); };
+    if (g.rows == 1) go(linear8_token_kernel<T, 1>);
+    else go(linear8_token_kernel<T, 2>);
 }
 template <int BN>
 static void launch_few(LaunchCtx& lc, uint64_t bytes, const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, const Linear8Args& g, bool pdl) {
@@ -227,15 +227,15 @@ static void run_linear8(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
     Linear8Args g{(int)rows, (int)n, (int)k, x_scale, w_scale, bias, y, ldy, y_dtype, failed};
     if (n == 1) ldw = padded8(k);
     const uint64_t bytes = (uint64_t)n * k + (uint64_t)rows * (k + n * dtype_size(y_dtype));
-    if (!given && small_fits(rows, n, k)) {
-        if (x_dtype == FL_DTYPE_F32) launch_small<float>(lc, bytes, x, ldx, w, ldw, g);
-        else if (x_dtype == FL_DTYPE_BF16) launch_small<__nv_bfloat16>(lc, bytes, x, ldx, w, ldw, g);
-        else launch_small<__half>(lc, bytes, x, ldx, w, ldw, g);
+    if (!given && token_fits(rows, k)) {
+        if (x_dtype == FL_DTYPE_F32) launch_token<float>(lc, bytes, x, ldx, w, ldw, g);
+        else if (x_dtype == FL_DTYPE_BF16) launch_token<__nv_bfloat16>(lc, bytes, x, ldx, w, ldw, g);
+        else launch_token<__half>(lc, bytes, x, ldx, w, ldw, g);
         return;
     }
     if (!given) {
         int8_t* to = static_cast<int8_t*>(workspace);
-        float* s = reinterpret_cast<float*>(to + linear8_room(rows, n, k, false).scale);
+        float* s = reinterpret_cast<float*>(to + linear8_room(rows, k, false).scale);
         quantize_rows(lc, x, x_dtype, rows, k, ldx, to, padded8(k), padded8(k), s);
         q = to; ldq = padded8(k); g.xs = s;
     }
@@ -283,7 +283,7 @@ static void check_temperature(double temperature) {
     FL_CHECK(temperature > 0 && std::isfinite(temperature) && std::isfinite(c) && inv_t > 0, FL_ERR_INVALID, "logprobs: the temperature is a positive number");
 }
 
-size_t linear8_workspace(int64_t rows, int64_t n, int64_t k) { return linear8_room(rows, n, k, false).all; }
+size_t linear8_workspace(int64_t rows, int64_t k) { return linear8_room(rows, k, false).all; }
 void op_quantize_rows(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale) {
     quantize_rows(lc, x, dtype, rows, cols, ldx, q, ldq, ldq, scale);
 }
@@ -319,13 +319,12 @@ FL_EXPORT int fl_quantize_rows(const void* x, int dtype, int64_t rows, int64_t c
     FL_API_END
 }
 
-FL_EXPORT int fl_linear8_workspace(int64_t rows, int64_t n, int64_t k, int x_dtype, size_t* bytes) {
+FL_EXPORT int fl_linear8_workspace(int64_t rows, int64_t k, int x_dtype, size_t* bytes) {
     FL_API_BEGIN
     FL_CHECK(bytes, FL_ERR_INVALID, "NULL argument");
     FL_CHECK(is_float(x_dtype) || x_dtype == FL_DTYPE_I8, FL_ERR_INVALID, "linear8: activations are f32, bf16, f16 or i8");
-    FL_CHECK(rows >= 0 && rows <= kMaxRows && n >= 1 && n <= kMaxRows && k >= 1 && k <= kLinear8MaxK, FL_ERR_INVALID,
-             "linear8: rows from 0 to 2^30, n from 1 to 2^30, k from 1 to 131071");
-    *bytes = linear8_room(rows, n, k, x_dtype == FL_DTYPE_I8).all;
+    FL_CHECK(rows >= 0 && rows <= kMaxRows && k >= 1 && k <= kLinear8MaxK, FL_ERR_INVALID, "linear8: rows from 0 to 2^30, k from 1 to 131071");
+    *bytes = linear8_room(rows, k, x_dtype == FL_DTYPE_I8).all;
     FL_API_END
 }
 
@@ -346,7 +345,7 @@ FL_EXPORT int fl_linear8(const void* x, int x_dtype, int64_t ldx, const float* x
     FL_CHECK(aligned(x, dtype_size(x_dtype)) && aligned(y, dtype_size(y_dtype)) && aligned(w_scale, 4) && aligned(x_scale, 4) && aligned(bias, 4), FL_ERR_INVALID,
              "linear8: a pointer is not aligned to its type");
     FL_CHECK(rows <= ((int64_t)1 << 40) / n, FL_ERR_INVALID, "linear8: more than 2^40 results");
-    const L8Room room = linear8_room(rows, n, k, given);
+    const L8Room room = linear8_room(rows, k, given);
     FL_CHECK(room.all == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= room.all), FL_ERR_INVALID,
              "linear8: the workspace is smaller than fl_linear8_workspace asks for, or not on a 256-byte border");
     DeviceScope dev;

@@ -403,138 +403,145 @@ linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     }
 }
 
-// ---- a token or a few ---------------------------------------------------------------------------------------------------------------
-// Up to four rows of few enough values round inside the product's own launch: every block reads the rows for their maxima (from L2) and rounds its part
-// of K into the layout that the tensor cores read, while its first weights are on their way.  A launch and a workspace less: one row of
-// 4096 by 4096 takes the host 10 us instead of 14 and the device as long as before (9.8; with the rows in 8 bits already 8.9).
-constexpr int kL8SmallRows = 4, kL8SmallValues = 8192, kL8SmallBlocks = 8;              // rows; values of all of them; k blocks of one block's part
-constexpr int kL8SmallStages = 6;
-constexpr uint32_t kL8SmallX = 16 * kL8BK;                                             // 16 rows (those past the last hold anything: columns that nobody reads)
-constexpr size_t kL8SmallSmem = kL8SmallStages * kL8WBytes + kL8SmallBlocks * kL8SmallX + 1024;
+// ---- a token or two -----------------------------------------------------------------------------------------------------------------
+// One or two rows, rounded inside the product's own launch: a warp per weight row, 16 bytes a lane and load, four products of 8 bits per instruction.  Every
+// block rounds the rows into its shared memory (from L2) while its first weights are on their way.  What bounds it: HBM for large matrices (1 x 3584 x 152064
+// 81 us, 6.7 TB/s), launch and two trips to memory for small ones (1 x 4096 x 4096 6.2 us, with the tensor cores 9.8; 2048 x 2048 3.6 and 7.5).  The
+// products cost 7 us a row at 4096 x 28672, so from three rows on the tensor cores are faster (1, 2 and 4 rows 21.1, 22.7 and 43.9 us, there
+// 23.0, 23.5 and 24.0), and so they are for two long rows, whose rounding every block repeats (2 x 4096 x 4096 8.6 and 10.0, 2 x 8192 x 8192 18.4 and 17.7,
+// 2 x 14336 x 4096 20.2 and 16.4; 1 x 14336 x 4096 15.7 and 16.4).
+constexpr int kL8TokenRows = 2, kL8TokenValues = 16384, kL8TokenThreads = 256, kL8TokenAhead = 4;      // rows; most rows^2 k; loads on their way a lane
 
-template <typename T>
-__global__ void __launch_bounds__(192, 2)
-linear8_small_kernel(const __grid_constant__ CUtensorMap tmW, const Linear8Args g, const int S, const T* __restrict__ x, const long long ldx, const bool vec) {
-    constexpr int kStages = kL8SmallStages, V = 16 / sizeof(T), R = kL8SmallRows;
-    extern __shared__ uint8_t gsm_raw[];
-    uint8_t* gsm = gsm_raw + ((1024u - (smem_u32(gsm_raw) & 1023u)) & 1023u);          // (the same offset in all blocks of a cluster)
-    uint8_t* sx = gsm + kStages * kL8WBytes;
-    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], done, rounded;
-    __shared__ __align__(16) float xs[4][16];
-    __shared__ uint32_t most[4][R];
-    __shared__ uint32_t tmem_base_s;
-    const int warp = uniform_warp(), lane = threadIdx.x & 31;
-    const int s = S == 1 ? 0 : (int)cluster_rank();
-    const int n0 = blockIdx.x / S * 128;
-    const int nk = (g.k + kL8BK - 1) / kL8BK, kb0 = s * nk / S, kb1 = (s + 1) * nk / S;
-
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
-        mbar_init(&done, 1);
-        mbar_init(&rounded, 128);
-        mbar_fence_init();
-    }
-    if (warp == 1) tmem_alloc(&tmem_base_s, 32);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = tmem_base_s;
-    bool ok = true;
-
-    if (warp == 0) {
-        if (lane == 0) {
-            int st = 0;
-            uint32_t ph = 1;
-            for (int kb = kb0; kb < kb1; ++kb) {
-                if (!(ok = mbar_wait_bounded(&empty[st], ph, kMbarTries))) break;
-                mbar_expect_tx(&full[st], kL8WBytes);
-                tma_load_2d(gsm + st * kL8WBytes, &tmW, kb * kL8BK, n0, &full[st]);
-                if (++st == kStages) { st = 0; ph ^= 1; }
+template <typename T, int R>
+__global__ void __launch_bounds__(kL8TokenThreads) linear8_token_kernel(const Linear8Args g, const T* __restrict__ x, const long long ldx, const bool vec, const int8_t* __restrict__ w,
+                                                                        const long long ldw) {
+    constexpr int V = 16 / sizeof(T), U = kL8TokenAhead, kWarps = kL8TokenThreads / 32;
+    extern __shared__ uint4 sx[];                               // [R][pieces of 16 values], zeros past the end
+    __shared__ uint32_t most[kWarps][R];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int pieces = (g.k + 15) / 16, whole = g.k / 16, steps = (pieces + 32 * U - 1) / (32 * U), stride = gridDim.x * kWarps;
+    // a step: U pieces a lane of one weight row; pieces past the row's end are zeros, the one that holds it is read value by value
+    auto fetch = [&](int n, int step, uint4 (&to)[U]) {
+        const int8_t* row = w + (long long)n * ldw;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = (step * U + u) * 32 + lane;
+            to[u] = make_uint4(0, 0, 0, 0);
+            if (i < whole) {
+                to[u] = ldg_stream(reinterpret_cast<const uint4*>(row) + i);
+            } else if (i < pieces) {
+                uint32_t b[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (i * 16 + j < g.k) b[j / 4] |= (uint32_t)(uint8_t)row[i * 16 + j] << (8 * (j % 4));
+                to[u] = make_uint4(b[0], b[1], b[2], b[3]);
             }
         }
-    } else if (warp == 1) {
-        constexpr uint32_t idesc = umma_idesc_i8(128, 16);
-        const uint64_t base = umma_smem_desc_sw128(gsm), bx = umma_smem_desc_sw128(sx);
-        int st = 0;
-        uint32_t ph = 0;
-        ok = mbar_wait_bounded(&rounded, 0, kMbarTries);
-        for (int kb = kb0; kb < kb1; ++kb) {
-            if (ok) ok = mbar_wait_bounded(&full[st], ph, kMbarTries);
-            __syncwarp();
-            tc_fence_after();
-            const uint64_t a = base + (uint64_t)(st * (kL8WBytes >> 4)), b = bx + (uint64_t)((kb - kb0) * (kL8SmallX >> 4));
+    };
+    int n = blockIdx.x * kWarps + warp, step = 0;
+    uint4 now[U], next[U];
+    if (n < g.n) fetch(n, 0, now);
+
+    // all rows' loads of a round are on their way together
+    auto load = [&](int r, int at) {                            // V values of row r from column `at` on, zeros past the end
+        uint4 h = make_uint4(0, 0, 0, 0);
+        const T* xr = x + r * ldx;
+        if (vec && at + V <= g.k) {
+            h = __ldg(reinterpret_cast<const uint4*>(xr + at));
+        } else {
+            T* e = reinterpret_cast<T*>(&h);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) umma_i8_warp(tmem, a + 2 * q, b + 2 * q, idesc, ((kb - kb0) | q) ? 1u : 0u);
-            umma_commit_warp(&empty[st]);
-            if (++st == kStages) { st = 0; ph ^= 1; }
+            for (int j = 0; j < V; ++j)
+                if (at + j < g.k) e[j] = xr[at + j];
         }
-        umma_commit_warp(&done);
-    } else {
-        const int tid = threadIdx.x - 64;
-        uint32_t m[R] = {};
+        return h;
+    };
+    uint32_t m[R] = {};
+#pragma unroll 2
+    for (int i = threadIdx.x * V; i < g.k; i += kL8TokenThreads * V) {
+        uint4 h[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            h[r] = load(r, i);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (r >= g.rows) break;
-            const T* xr = x + r * ldx;
-            if (vec) {
-#pragma unroll 4
-                for (int i = tid * V; i < g.k; i += 128 * V) {                          // (a whole vector lies inside the row's 16-byte pieces, but not inside the row)
-                    if (i + V <= g.k) {
-                        const uint4 h = __ldg(reinterpret_cast<const uint4*>(xr + i));
-                        const T* e = reinterpret_cast<const T*>(&h);
+            const T* e = reinterpret_cast<const T*>(&h[r]);
 #pragma unroll
-                        for (int j = 0; j < V; ++j) m[r] = max(m[r], abs_bits(to_f32(e[j])));
-                    } else {
-                        for (int j = i; j < g.k; ++j) m[r] = max(m[r], abs_bits(to_f32(xr[j])));
-                    }
-                }
-            } else {
-                for (int i = tid; i < g.k; i += 128) m[r] = max(m[r], abs_bits(to_f32(xr[i])));
-            }
-            m[r] = __reduce_max_sync(0xFFFFFFFFu, m[r]);
-            if (lane == 0) most[warp - 2][r] = m[r];
+            for (int j = 0; j < V; ++j) m[r] = max(m[r], abs_bits(to_f32(e[j])));
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        const int c1 = min(kb1 * kL8BK, g.k);
-#pragma unroll 1
-        for (int r = 0; r < g.rows; ++r) {
-            const RowScale rs(max(max(most[0][r], most[1][r]), max(most[2][r], most[3][r])));
-            if (lane == 0) xs[warp - 2][r] = rs.scale;
-            const T* xr = x + r * ldx;
-            for (int c = kb0 * kL8BK + tid * 4; c < c1; c += 512) {                     // four values a thread; past the row's end the weights are zeros
-                float v[4];
-                if (vec && c + 4 <= g.k) {
-                    if constexpr (sizeof(T) == 4) {
-                        const float4 h = __ldg(reinterpret_cast<const float4*>(xr + c));
-                        v[0] = h.x; v[1] = h.y; v[2] = h.z; v[3] = h.w;
-                    } else {
-                        const uint2 h = __ldg(reinterpret_cast<const uint2*>(xr + c));
-                        const T* e = reinterpret_cast<const T*>(&h);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) v[j] = to_f32(e[j]);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) v[j] = c + j < g.k ? to_f32(xr[c + j]) : 0.f;
-                }
-                const int kb = c / kL8BK - kb0, in = c % kL8BK;                         // 16-byte piece in / 16 of the row lies at (in / 16) ^ (row mod 8)
-                *reinterpret_cast<uint32_t*>(sx + kb * kL8SmallX + r * 128 + (((in >> 4) ^ (r & 7)) << 4) + (in & 15)) = rs.four(v[0], v[1], v[2], v[3]);
-            }
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(&rounded);
-        __syncwarp();
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&done, 0, kMbarTries));
-        tc_fence_after();
     }
-    l8_few_finish<16>(g, S, s, 0, n0, tmem, gsm, xs[max(warp - 2, 0)], ok);
-    if (!ok) l8_give_up(g.failed);
-    __syncwarp();
-    tc_fence_before();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        m[r] = __reduce_max_sync(0xFFFFFFFFu, m[r]);
+        if (lane == 0) most[warp][r] = m[r];
+    }
     __syncthreads();
-    if (warp == 1) {
-        tc_fence_after();
-        tmem_dealloc(tmem, 32);
+    float scale[R];
+    {
+        float mul[R], a[R], up[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            uint32_t all = 0;
+#pragma unroll
+            for (int i = 0; i < kWarps; ++i) all = max(all, most[i][r]);
+            const RowScale rs(all);
+            scale[r] = rs.scale; mul[r] = rs.mul; a[r] = rs.a; up[r] = rs.up;
+        }
+#pragma unroll 2
+        for (int i = threadIdx.x * V; i < pieces * 16; i += kL8TokenThreads * V) {
+            uint4 h[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                h[r] = load(r, i);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                RowScale rs(0);
+                rs.mul = mul[r]; rs.a = a[r]; rs.up = up[r];
+                const T* e = reinterpret_cast<const T*>(&h[r]);
+                uint32_t* to = reinterpret_cast<uint32_t*>(sx + r * pieces) + i / 4;
+#pragma unroll
+                for (int j = 0; j < V; j += 4) to[j / 4] = rs.four(to_f32(e[j]), to_f32(e[j + 1]), to_f32(e[j + 2]), to_f32(e[j + 3]));
+            }
+        }
+    }
+    __syncthreads();
+
+    int sum[R] = {};
+    while (n < g.n) {
+        const bool last = step + 1 == steps;
+        const int n1 = last ? n + stride : n, step1 = last ? 0 : step + 1;
+        if (n1 < g.n) fetch(n1, step1, next);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = (step * U + u) * 32 + lane;
+            if (i >= pieces) break;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const uint4 q = sx[r * pieces + i];
+                sum[r] = __dp4a((int)now[u].x, (int)q.x, sum[r]);
+                sum[r] = __dp4a((int)now[u].y, (int)q.y, sum[r]);
+                sum[r] = __dp4a((int)now[u].z, (int)q.z, sum[r]);
+                sum[r] = __dp4a((int)now[u].w, (int)q.w, sum[r]);
+            }
+        }
+        if (last) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int all = __reduce_add_sync(0xFFFFFFFFu, sum[r]);
+                sum[r] = 0;
+                if (lane != r) continue;                        // (each row's result by a lane of its own)
+                float v = (float)all * scale[r] * __ldg(g.ws + n);
+                if (g.bias != nullptr) v += __ldg(g.bias + n);
+                const long long at = (long long)r * g.ldy + n;
+                if (g.y_dtype == 0) reinterpret_cast<float*>(g.y)[at] = v;
+                else if (g.y_dtype == 1) reinterpret_cast<__nv_bfloat16*>(g.y)[at] = from_f32<__nv_bfloat16>(v);
+                else reinterpret_cast<__half*>(g.y)[at] = from_f32<__half>(v);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) now[u] = next[u];
+        n = n1;
+        step = step1;
     }
 }
 

@@ -7,7 +7,7 @@ namespace fl {
 
 // 8-bit rows start on 16-byte borders
 inline int64_t padded8(int64_t k) { return (k + 15) / 16 * 16; }
-size_t linear8_workspace(int64_t rows, int64_t n, int64_t k);   // bytes (0: none is needed); the workspace starts on a 256-byte border
+size_t linear8_workspace(int64_t rows, int64_t k);              // bytes (0: none is needed); the workspace starts on a 256-byte border
 void op_quantize_rows(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale);
 // y = f32 [rows, n], x = f32 [rows, k], w = 8-bit [n, padded8(k)]; *failed is set when a wait in the kernel ran out (page-locked memory, see step_check)
 void op_linear8(LaunchCtx& lc, const float* x, const int8_t* w, const float* w_scale, int64_t rows, int64_t n, int64_t k, float* y, void* workspace, int* failed);

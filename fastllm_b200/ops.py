@@ -25,16 +25,6 @@ _TOKENS = {torch.int32: 4, torch.int64: 8}
 MAX_TOP = 32
 
 
-def _rounds_itself(rows: int, n: int, k: int) -> bool:
-    """whether a product of up to four rows needs no workspace"""
-    if rows * k > 8192:
-        return False
-    tiles, blocks, slices = (n + 127) // 128, (k + 127) // 128, 8
-    while slices > 1 and (slices * tiles > 148 or blocks < 8 * slices or blocks - blocks // slices < 24):
-        slices //= 2
-    return blocks <= 8 * slices
-
-
 def _refuse(msg: str):
     raise FastllmError(-1, msg)
 
@@ -143,7 +133,7 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, b
         ldy = y2.stride(0)
     lib = _lib.load()
     # (fl_linear8_workspace's rule)
-    room = 0 if x_type == _lib.FL_DTYPE_I8 or rows <= 4 and _rounds_itself(rows, n, k) else (rows * ((k + 15) // 16 * 16) + 255) // 256 * 256 + 4 * rows
+    room = 0 if x_type == _lib.FL_DTYPE_I8 or rows <= 2 and rows * rows * k <= 16384 else (rows * ((k + 15) // 16 * 16) + 255) // 256 * 256 + 4 * rows
     work = work_ptr = None
     if room:
         work = x.new_empty(room, dtype=torch.uint8)

@@ -407,7 +407,7 @@ FL_EXPORT int fl_quantize_rows(const void* x, int dtype, int64_t rows, int64_t c
  * already (FL_DTYPE_I8) with their x_scale [rows].  w [n, k] with w_scale [n]: an 8-bit checkpoint's, or fl_quantize_rows of a weight.
  * 8-bit rows start on 16-byte borders (pointer and row stride); what lies between a row's end and the next row is not read.
  * workspace: fl_linear8_workspace bytes on a 256-byte border (the answer may be 0: none), free again when the call's work on the stream is done. */
-FL_EXPORT int fl_linear8_workspace(int64_t rows, int64_t n, int64_t k, int x_dtype, size_t* bytes);
+FL_EXPORT int fl_linear8_workspace(int64_t rows, int64_t k, int x_dtype, size_t* bytes);
 FL_EXPORT int fl_linear8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
                          int64_t rows, int64_t n, int64_t k, void* y, int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
 /* Log probabilities over logits [rows, vocab] (f32, bf16, f16), z = logits / temperature:

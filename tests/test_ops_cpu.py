@@ -70,21 +70,17 @@ def test_no_rows_is_no_work():
 
 
 def test_workspace_size():
-    """ops.py keeps the rule of the C side"""
+    """the rule that ops.py keeps too"""
     n = C.c_size_t()
     lib = _lib.load()
     for rows in (0, 1, 2, 3, 4, 5, 9, 128, 300):
-        for cols in (1, 100, 2048, 4096, 9472, 9473, 18944, 18945, 37888, 152064):
-            for k in (1, 17, 100, 2048, 2049, 4095, 4096, 4097, 8192, 16384, 16385, 32768):
-                itself = rows <= 4 and ops._rounds_itself(rows, cols, k)
-                want = 0 if itself else (rows * ((k + 15) // 16 * 16) + 255) // 256 * 256 + 4 * rows
-                assert lib.fl_linear8_workspace(rows, cols, k, 1, C.byref(n)) == 0 and n.value == want, (rows, cols, k)
-                assert lib.fl_linear8_workspace(rows, cols, k, 3, C.byref(n)) == 0 and n.value == 0
-    assert ops._rounds_itself(1, 4096, 4096) and not ops._rounds_itself(1, 152064, 4096)
-    _refused(lib.fl_linear8_workspace(1, 1, 0, 1, C.byref(n)), "k from")
-    _refused(lib.fl_linear8_workspace(1, 0, 1, 1, C.byref(n)), "n from")
-    _refused(lib.fl_linear8_workspace(1, 1, 1, 9, C.byref(n)), "activations")
-    _refused(lib.fl_linear8_workspace(1, 1, 1, 1, None), "NULL")
+        for k in (1, 17, 100, 2048, 4096, 4097, 8192, 8193, 10922, 10923, 16384, 16385, 32768, 32769):
+            want = 0 if rows <= 2 and rows * rows * k <= 16384 else (rows * ((k + 15) // 16 * 16) + 255) // 256 * 256 + 4 * rows
+            assert lib.fl_linear8_workspace(rows, k, 1, C.byref(n)) == 0 and n.value == want, (rows, k)
+            assert lib.fl_linear8_workspace(rows, k, 3, C.byref(n)) == 0 and n.value == 0
+    _refused(lib.fl_linear8_workspace(1, 0, 1, C.byref(n)), "k from")
+    _refused(lib.fl_linear8_workspace(1, 1, 9, C.byref(n)), "activations")
+    _refused(lib.fl_linear8_workspace(1, 1, 1, None), "NULL")
 
 
 def test_tensors_off_the_gpu_are_refused():

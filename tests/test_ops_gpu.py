@@ -137,6 +137,21 @@ def test_linear8(rows, n, k, dtype):
     _check_product(y, q, most / 127.0, w, ws, bias)
 
 
+@pytest.mark.parametrize("rows, n, k", [(1, 5000, 4096), (1, 9, 16384), (1, 20000, 100), (1, 1, 16385), (2, 100, 4096), (2, 4097, 2050), (2, 333, 4001), (2, 40, 4097), (4, 700, 8192),
+                                        (4, 130, 8193), (4, 6000, 513), (5, 700, 2048)])
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("shift", [0, 1])
+def test_linear8_tokens(rows, n, k, dtype, shift):
+    """a token or a few, on both sides of the line to products that round their rows beforehand; rows that start on odd elements"""
+    store = (torch.randn(rows, k + 8, device="cuda", generator=_gen(rows + k)) * 2).to(dtype)
+    x = store[:, shift:k + shift]
+    w, ws = _weight(n, k, n)
+    bias = torch.randn(n, device="cuda", generator=_gen(k)) if rows % 2 else None
+    q, most = _exact_rows(x)
+    for out in (dtype, torch.float32):
+        _check_product(ops.linear8(x, w, ws, bias, out_dtype=out), q, most / 127.0, w, ws, bias)
+
+
 @pytest.mark.parametrize("rows", [1, 40, 300, 1200])
 @pytest.mark.parametrize("out_dtype", FLOATS)
 def test_linear8_types_of_the_result(rows, out_dtype):

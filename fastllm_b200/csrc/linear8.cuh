@@ -246,10 +246,12 @@ __device__ __forceinline__ void l8_give_up(int* failed) {
 // other's parts through shared memory: whole numbers, so the order does not matter, and no workspace.  What bounds it: HBM behind 4 to 6 us of
 // launch, first weights and last results (64 x 4096 x 28672 25.3 us, 4.8 TB/s; 37 x 3584 x 152064 to f32 96.6, 5.9 TB/s of the measured 6.55; 64 x 4096 x 4096 10.1).
 // Two blocks per SM hold 96 KB of weights on their way each: one writes its results while the other's arrive.
+// Tiles of 64 weight rows instead, to even out the last wave, were slower nearly everywhere (64 x 4096 x 28672 23.9 -> 27.5 us, 37 x 3584 x 152064 95.8 -> 106.6,
+// 16 x 4096 x 28672 23.3 -> 22.1): each needs its copy of the activations.
 template <int BN> struct L8Few {
     static constexpr uint32_t kX = BN * kL8BK, kStage = kL8WBytes + kX;
-    static constexpr int kPerSm = BN <= 128 ? 2 : 1;                                   // blocks that an SM holds
-    static constexpr uint32_t kRing = kPerSm == 2 ? 108 * 1024 : 208 * 1024;
+    static constexpr int kPerSm = 2;                                                   // blocks that an SM holds
+    static constexpr uint32_t kRing = 108 * 1024;
     static constexpr int kStages = kRing / kStage < 8 ? kRing / kStage : 8;
     static constexpr size_t kSmem = (size_t)kStages * kStage + 1024;
     static constexpr int kThreads = 192;
@@ -260,7 +262,7 @@ template <int BN> struct L8Few {
 // The accumulators of a block's part of K (all warps call it; those from 2 on are the epilogue's): written, or added up in the cluster.  xs: the tile's row
 // scales, the calling warp's copy.
 template <int BN>
-__device__ __forceinline__ void l8_few_finish(const Linear8Args& g, const int S, int s, int r0, int n0, uint32_t tmem, uint8_t* ring, const float* xs, bool ok) {
+__device__ __forceinline__ void l8_few_finish(const Linear8Args& g, const int S, int s, int n0, uint32_t tmem, uint8_t* ring, const float* xs, bool ok) {
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const int row = (warp & 3) * 32 + lane;                                            // accumulator row = weight row of the tile
     const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -269,10 +271,10 @@ __device__ __forceinline__ void l8_few_finish(const Linear8Args& g, const int S,
     if (S == 1) {
         if (warp >= 2 && ok) {
 #pragma unroll 1
-            for (int c = 0; c < BN && r0 + c < g.rows; c += 16) {
+            for (int c = 0; c < BN && c < g.rows; c += 16) {
                 uint32_t v[16];
                 tmem_ld16(at + (uint32_t)c, v);
-                l8_store16(g, r0 + c, n, xs + c, wsn, bn, v);
+                l8_store16(g, c, n, xs + c, wsn, bn, v);
             }
         }
         return;
@@ -283,7 +285,7 @@ __device__ __forceinline__ void l8_few_finish(const Linear8Args& g, const int S,
     if (warp >= 2) {
         const uint32_t base = smem_u32(ring) + (uint32_t)(s * per * 128 + row) * 4;
 #pragma unroll 1
-        for (int c = 0; c < BN && r0 + c < g.rows; c += 16) {
+        for (int c = 0; c < BN && c < g.rows; c += 16) {
             uint32_t v[16];
             tmem_ld16(at + (uint32_t)c, v);
 #pragma unroll
@@ -298,8 +300,8 @@ __device__ __forceinline__ void l8_few_finish(const Linear8Args& g, const int S,
     if (warp >= 2 && ok) {
         const int* part = reinterpret_cast<const int*>(ring) + row;
 #pragma unroll 1
-        for (int c = 0; c < per && r0 + s * per + c < g.rows; c += 16) {
-            const int r = r0 + s * per + c, cnt = min(min(per - c, 16), g.rows - r);
+        for (int c = 0; c < per && s * per + c < g.rows; c += 16) {
+            const int r = s * per + c, cnt = min(min(per - c, 16), g.rows - r);
             int sum[16];
             float v[16];
 #pragma unroll
@@ -331,7 +333,7 @@ linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     __shared__ uint32_t tmem_base_s;
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const int s = S == 1 ? 0 : (int)cluster_rank();
-    const int n0 = blockIdx.x / S * 128, r0 = blockIdx.y * BN;
+    const int n0 = blockIdx.x / S * 128;
     const int nk = (g.k + kL8BK - 1) / kL8BK, kb0 = (int)((long long)s * nk / S), kb1 = (int)((long long)(s + 1) * nk / S);
 
     if (threadIdx.x == 0) {
@@ -352,7 +354,7 @@ linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
                 mbar_expect_tx(&full[st], L::kStage);
                 tma_load_2d(gsm + st * L::kStage, &tmW, kb * kL8BK, n0, &full[st]);
             };
-            auto rows = [&](int kb, int st) { tma_load_2d(gsm + st * L::kStage + kL8WBytes, &tmX, kb * kL8BK, r0, &full[st]); };
+            auto rows = [&](int kb, int st) { tma_load_2d(gsm + st * L::kStage + kL8WBytes, &tmX, kb * kL8BK, 0, &full[st]); };
             // the weights do not depend on the kernel that rounds the rows: a ring-full of them is requested ahead of the wait
             const int pre = min(kb1, kb0 + kStages);
             for (int kb = kb0; kb < pre; ++kb) weights(kb, kb - kb0);
@@ -387,12 +389,12 @@ linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     }
     if (warp >= 2) {
         pdl_wait();
-        for (int i = lane; i < BN; i += 32) xs[warp - 2][i] = r0 + i < g.rows ? g.xs[r0 + i] : 0.f;
+        for (int i = lane; i < BN; i += 32) xs[warp - 2][i] = i < g.rows ? g.xs[i] : 0.f;
         __syncwarp();
         ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&done, 0, kMbarTries));
         tc_fence_after();
     }
-    l8_few_finish<BN>(g, S, s, r0, n0, tmem, gsm, xs[max(warp - 2, 0)], ok);
+    l8_few_finish<BN>(g, S, s, n0, tmem, gsm, xs[max(warp - 2, 0)], ok);
     if (!ok) l8_give_up(g.failed);
     __syncwarp();
     tc_fence_before();

@@ -246,22 +246,23 @@ static void run_linear8(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
     else launch_few<128>(lc, bytes, q, ldq, w, ldw, g, !given);
 }
 
-// Blocks per row: two per SM over the rows, while every warp has two chunks; at most eight with alternatives, whose lists the first block joins (1 x 32000,
-// five alternatives, 4, 8 and 16 blocks: 6.8, 6.2 and 6.3 us; 64 x 152064 f32, none: 1, 2, 4 and 8 blocks 16.4, 11.8, 9.2 and 9.8; 128 x 32000: 6.3, 6.7, 7.1
-// and 10.3).  The cluster of 16 is not portable to every chip, but B200 has it.  Small blocks where there are more rows than SMs hold large ones (256 -> 128
+// Blocks per row: three per SM over the rows, as many as run at once, with 16 chunks each at least (200 x 152064 f32, 1, 2 and 3 blocks a row: 30.2, 23.3 and 30.5
+// us; 100 x 152064, 2, 4 and 6: 17.9, 14.0 and 18.5; 64 x 152064 and five alternatives, 4, 6 and 7: 13.1, 12.2 and 17.8).  At most six, since larger clusters find a
+// place on fewer SMs (37 x 128256 bf16, 6 and 8: 5.9 and 6.4, with five alternatives 8.5 and 9.4), except where all have an SM each: 16 then, or eight
+// with alternatives, whose lists the first block joins (3 x 152064 f32, 6, 8 and 16: 4.7, 4.2 and 3.6, with twenty 8.1, 8.0 and 9.9).  A cluster of 16 is not
+// portable to every chip, but B200 has it.  Small blocks where there are more rows than SMs hold large ones (256 -> 128
 // threads, five alternatives: 1000 x 32003 f16 25.1 -> 20.8 us, 777 x 32000 f32 28.8 -> 23.7, but 400 x 32000 12.7 -> 13.2).  With alternatives and many short
 // 16-bit rows the registers of a second batch are worth more as a further block per SM (1300 x 32000 bf16 30.7 -> 25.0 without it; 2048 x 152064 118 -> 111 with
 // it, 2048 x 32000 f32 55.0 -> 52.3).
 template <typename T>
 static void run_logprobs(LaunchCtx& lc, const LogprobArgs& a) {
     const int chunks = (a.vocab + 2 * LpRow<T>::N - 1 + LpRow<T>::kChunk - 1) / LpRow<T>::kChunk;
-    const int most = a.top > 0 ? kLpMaxCluster / 2 : kLpMaxCluster;
-    int C = 1;
-    while (C < most && (long long)a.rows * 2 * C <= 2 * kNumSMs && chunks >= 16 * C) C *= 2;
+    const int most = a.rows > kNumSMs / kLpMaxCluster ? 6 : a.top > 0 ? kLpMaxCluster / 2 : kLpMaxCluster;
+    const int C = std::max(1, std::min({most, 3 * kNumSMs / a.rows, chunks / 16})), per = (chunks + C - 1) / C;
     const uint64_t bytes = (uint64_t)a.rows * a.vocab * sizeof(T);
     const dim3 grid((unsigned)((long long)a.rows * C));
-    const size_t smem = a.top > 0 ? (size_t)((chunks + C - 1) / C + 1) * 4 : 0;
-    auto go = [&](auto kern, int threads) { launch_op(lc, "logprobs", bytes, kern, grid, threads, smem, C, false, a, C); };
+    const size_t smem = a.top > 0 ? (size_t)per * 4 : 0;
+    auto go = [&](auto kern, int threads) { launch_op(lc, "logprobs", bytes, kern, grid, threads, smem, C, false, a, C, per); };
     if (a.rows <= 4 * kNumSMs) {
         a.top > 0 ? go(logprobs_kernel<T, true, 256, true>, 256) : go(logprobs_kernel<T, false, 256, true>, 256);
     } else if (a.top == 0) {

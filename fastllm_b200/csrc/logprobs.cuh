@@ -5,13 +5,17 @@
 // different references are brought to the largest one and joined.  The reference moves when a maximum is 2^16 above it, so the exponentials
 // stay far from overflow and the loop is nearly free of rescaling.  A row belongs to a cluster of C blocks (C = 1 when there are many rows), whose results
 // meet in the first block's shared memory: no workspace, no atomics, the same bits every time.
-// What bounds it: HBM for 32-bit rows (1000 x 152064 91 us, 6.7 TB/s), the exponentials for 16-bit ones (2048 x 152064 bf16 103 us, 6.0 TB/s: one per logit is
-// 77 % of what the special-function units do, 5.6 instructions per logit half of the issue slots), latency for few (1 x 32000: 4 us, 7 with five alternatives).
+// What bounds it: HBM for 32-bit rows (1000 x 152064 91 us, 6.7 TB/s), the exponentials for 16-bit ones (2048 x 152064 bf16 99 us, 6.3 TB/s: one per logit is
+// 77 % of what the special-function units do, 5.6 instructions per logit half of the issue slots), latency for few (1 x 32000: 2.8 us, 5.3 with five
+// alternatives): trips to memory one after the other.  So the given token is looked up while the row is read (1000 cycles when waited for), and chunks at the
+// row's ends are asked for before the batches between them, not behind them.
 //
-// Alternatives: the row lies in chunks of 512 bytes (one load of a warp), whose maxima are kept.  The K-th largest of a block's 256 thread maxima
-// is a lower bound for its K-th largest logit, since K threads hold one at least as large.  Only chunks that reach the bound are read again (from L2),
-// only logits that reach it are ranked: about K + K^2 / 512 of them where the order is random.  Where equal logits leave more than the tables hold, the K
-// best chunks by (maximum, lower index) are taken instead: a logit outside them is behind K others, one per chunk; then K rounds pick one each.
+// Alternatives: the row lies in chunks of 512 bytes (one load of a warp), whose maxima are kept.  A block's threads form 64 groups; the K-th largest of the groups'
+// maxima is a lower bound for the block's K-th largest logit, since K groups hold one at least as large.  Only chunks that reach the bound are read again (from
+// L2), only logits that reach it are ranked: 5 of 5, 24 of 20 or 44 of 32 where the order is random.  (Groups of one thread bring those to 21 and 34, but the
+// bound is found in K steps over what a warp holds, 31 cycles each with two values a lane, 80 with eight.)  Where fewer than K logits are above -infinity, all of them
+// are ranked and the lowest indices fill up.  Where equal logits leave more than the tables hold, the K best chunks by (maximum, lower index) are
+// taken instead: a logit outside them is behind K others, one per chunk; then K rounds pick one each.
 #pragma once
 #include "linear8.cuh"
 
@@ -20,6 +24,8 @@ namespace fl {
 constexpr int kLpMaxTop = 32;
 constexpr int kLpMaxVocab = 1 << 20;
 constexpr int kLpMaxCluster = 16;
+constexpr int kLpGroups = 64;                       // of a block's threads
+constexpr uint32_t kLpFinite = 0x00800000u;         // ordered_bits of the lowest finite value: the next above -infinity's
 constexpr int kLpList = 96, kLpCand = 256;          // chunks that are read again, logits that are ranked
 
 struct LogprobArgs {
@@ -177,27 +183,32 @@ template <typename T> struct LpRow {
 };
 
 struct __align__(16) LpPart { float m, r, s, t; };     // largest x; reference; sum of e; sum of e (c x - r)
-// n of them as one, about the largest reference
-__device__ __forceinline__ LpPart lp_join(const LpPart* part, int n) {
-    LpPart p = part[0];
-    for (int i = 1; i < n; ++i) { p.m = fmaxf(p.m, part[i].m); p.r = fmaxf(p.r, part[i].r); }
-    p.s = p.t = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-        const LpPart q = part[i];
-        const float f = ex2(q.r - p.r);
-        p.s += q.s * f;
-        p.t += (q.t + q.s * (q.r - p.r)) * f;
+// the warp's largest value; NaN is passed over
+__device__ __forceinline__ float lp_warp_max(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xFFFFFFFF;" : "=f"(r) : "f"(v));
+    return r;
+}
+// those of the lanes (of each 2 WIDTH of them) as one, about the largest reference
+template <int WIDTH>
+__device__ __forceinline__ LpPart lp_join_warp(LpPart p) {
+    const float r = lp_warp_max(p.r), f = ex2(p.r - r);
+    p.m = lp_warp_max(p.m);
+    p.t = (p.t + p.s * (p.r - r)) * f;
+    p.s *= f;
+#pragma unroll
+    for (int o = WIDTH; o > 0; o >>= 1) {
+        p.s += __shfl_xor_sync(0xFFFFFFFFu, p.s, o);
+        p.t += __shfl_xor_sync(0xFFFFFFFFu, p.t, o);
     }
+    p.r = r;
     return p;
 }
-__device__ __forceinline__ LpPart lp_join_warp(LpPart p) {
-    const float r = warp_max(p.r), f = ex2(p.r - r);
-    p.t = warp_sum((p.t + p.s * (p.r - r)) * f);
-    p.s = warp_sum(p.s * f);
-    p.r = r;
-    p.m = warp_max(p.m);
-    return p;
+// n of them, 16 at most, in shared memory (whole warps)
+__device__ __forceinline__ LpPart lp_join(const LpPart* part, int n, int lane) {
+    LpPart p = part[min(lane & 15, n - 1)];
+    if ((lane & 15) >= n) p.s = p.t = 0.f;
+    return lp_join_warp<8>(p);
 }
 // how many of the keys lie before `key`; n a multiple of 8 (zeros fill it up)
 __device__ __forceinline__ int lp_place(const unsigned long long* keys, int n, unsigned long long key) {
@@ -212,38 +223,48 @@ __device__ __forceinline__ int lp_place(const unsigned long long* keys, int n, u
     return before;
 }
 
-// TOP: with alternatives; AHEAD: the next batch is on its way while one is added up
+__device__ __forceinline__ int cluster_id() {
+    int r;
+    asm("mov.u32 %0, %clusterid.x;" : "=r"(r));
+    return r;
+}
+
+// TOP: with alternatives; AHEAD: the next batch is on its way while one is added up.  A cluster of C blocks per row, `per` chunks each.
 template <typename T, bool TOP, int kThreads, bool AHEAD>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a, const int C) {
+__global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a, const int C, const int per) {
     constexpr int kWarps = kThreads / 32, U = 4;
-    extern __shared__ uint32_t chunk_max[];                     // TOP: ordered maxima of this block's chunks
+    extern __shared__ float chunk_max[];                        // TOP: maxima of this block's chunks
     __shared__ LpPart part[kWarps], parts[kLpMaxCluster];
-    __shared__ uint32_t sup[TOP ? kThreads : 1];
+    __shared__ float sup[TOP ? kThreads : 1];
     __shared__ __align__(16) unsigned long long cand[TOP ? kLpCand : 1], best[TOP ? kLpMaxCluster * kLpMaxTop : 1];
     __shared__ unsigned long long round_best[TOP ? kWarps : 1];
     __shared__ int list[TOP ? kLpList : 1];
     __shared__ int n_list, n_cand;
-    __shared__ uint32_t bound;
+    __shared__ float bound;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int rank = C == 1 ? 0 : (int)cluster_rank(), row = blockIdx.x / C;
+    const int rank = C == 1 ? 0 : (int)cluster_rank(), row = C == 1 ? (int)blockIdx.x : cluster_id();
     const LpRow<T> x(a, row);
-    const int ch0 = (int)((long long)rank * x.chunks / C), ch1 = (int)((long long)(rank + 1) * x.chunks / C);
+    const int ch0 = min(rank * per, x.chunks), ch1 = min(ch0 + per, x.chunks);
     const float c = a.c, nan = __uint_as_float(0x7FFFFFFFu);
     if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // (that the first block has started, before anyone writes to it)
     if (tid == 0) { n_list = 0; n_cand = 0; }
-
-    // the given tokens' logits, on their way while the row is read
-    long long token = -1;
-    float token_x = 0.f;
-    const bool mine = rank == 0 && tid < a.given;
-    auto token_at = [&](int j) {
-        const long long at = (long long)row * a.given + j;
-        return a.wide ? reinterpret_cast<const long long*>(a.tokens)[at] : (long long)reinterpret_cast<const int*>(a.tokens)[at];
-    };
-    if (mine) {
-        token = token_at(tid);
-        if (token >= 0 && token < a.vocab) token_x = to_f32(x.x[token]);
+    const int K = a.top;
+    unsigned long long* mine_best = best + rank * K;            // (in the first block's table, this block's place)
+    if (TOP) {
+        for (int i = tid; i < kLpCand; i += kThreads) cand[i] = 0;
+        if (tid < K) mine_best[tid] = 0;
     }
+
+    // the given tokens, on their way while the row is read (as they lie: a conversion here would wait for them)
+    const int turn = kThreads - 1 - tid;                        // (the last warp's, so that they do not wait for the alternatives, nor these for them)
+    const bool mine = rank == 0 && turn < a.given;
+    int2 token_bits{-1, -1};
+    if (mine) {
+        const long long at = (long long)row * a.given + turn;
+        if (a.wide) token_bits = reinterpret_cast<const int2*>(a.tokens)[at];
+        else token_bits.x = reinterpret_cast<const int*>(a.tokens)[at];
+    }
+    auto token_of = [&](int2 bits) { return a.wide ? (long long)bits.y << 32 | (uint32_t)bits.x : (long long)bits.x; };
 
     LpPart p{-INFINITY, 0.9f * LpVec<T>::kLow * c, 0.f, 0.f};   // (well above what -infinity is raised to, below every other value of a row that is not `far`)
     uint64_t s2 = pack2(0.f, 0.f), t2 = s2;
@@ -256,8 +277,8 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
         if constexpr (TOP) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const uint32_t o = __reduce_max_sync(0xFFFFFFFFu, ordered_bits(LpVec<T>::last(w[u])));
-                if (lane == 0 && at(u) >= 0) chunk_max[at(u)] = o;
+                const float m = lp_warp_max(LpVec<T>::last(w[u]));
+                if (lane == 0 && at(u) >= 0) chunk_max[at(u)] = m;
             }
         }
 #pragma unroll
@@ -285,8 +306,21 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
                 t2 = fma2(e, d, t2);
             });
     };
-    // batches of U chunks a warp that lie inside the row, without a look at its ends; then the chunks in front of them and behind
+    // batches of U chunks a warp that lie inside the row, without a look at its ends, and the chunks in front of them and behind
     const int first = max(ch0, x.whole()), batches = max(0, min(ch1, x.whole_end()) - first) / (kWarps * U);
+    const int head = min(first, ch1) - ch0, rest = ch1 - ch0 - batches * kWarps * U;       // chunks in front of the batches; all that are in none
+    auto rest_place = [&](int j, int u) {
+        const int k = j + u * kWarps;
+        return k >= rest ? -1 : k < head ? k : k + batches * kWarps * U;
+    };
+    auto fetch_rest = [&](uint4 (&v)[U], int j) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            v[u] = make_uint4(LpVec<T>::kNone, LpVec<T>::kNone, LpVec<T>::kNone, LpVec<T>::kNone);
+            if (rest_place(j, u) >= 0) v[u] = x.load(ch0 + rest_place(j, u), lane);
+        }
+    };
+    int j_rest = warp;
     {
         const uint4* q = x.at(first + warp, lane);
         auto fetch = [&](uint4 (&v)[U]) {
@@ -294,7 +328,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
             for (int u = 0; u < U; ++u) v[u] = ldg_stream(q + u * kWarps * 32);
             q += U * kWarps * 32;
         };
-        uint4 v[U];
+        uint4 v[U], w[U];
         int ch = first + warp - ch0;
         auto place = [&](int u) { return ch + u * kWarps; };
         if constexpr (!AHEAD) {
@@ -302,9 +336,11 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
                 fetch(v);
                 absorb(v, place);
             }
-        } else if (batches > 0) {
-            uint4 w[U];
-            fetch(v);
+        } else {
+            if (j_rest < rest) fetch_rest(w, j_rest);
+            if (batches > 0) fetch(v);
+            if (j_rest < rest) absorb(w, [&](int u) { return rest_place(warp, u); });
+            j_rest += U * kWarps;
             for (int i = 0; i < batches; i += 2) {
                 if (i + 1 < batches) fetch(w);
                 absorb(v, place);
@@ -316,21 +352,16 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
             }
         }
     }
-    {
-        const int head = min(first, ch1) - ch0, rest = ch1 - ch0 - batches * kWarps * U;       // chunks in front of the batches; all that are left
-        for (int j = warp; j < rest; j += U * kWarps) {
-            uint4 v[U];
-            auto place = [&](int u) {
-                const int k = j + u * kWarps;
-                return k >= rest ? -1 : k < head ? k : k + batches * kWarps * U;
-            };
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                v[u] = make_uint4(LpVec<T>::kNone, LpVec<T>::kNone, LpVec<T>::kNone, LpVec<T>::kNone);
-                if (place(u) >= 0) v[u] = x.load(ch0 + place(u), lane);
-            }
-            absorb(v, place);
-        }
+    for (; j_rest < rest; j_rest += U * kWarps) {
+        uint4 v[U];
+        fetch_rest(v, j_rest);
+        absorb(v, [&](int u) { return rest_place(j_rest, u); });
+    }
+    // the given tokens' logits (again not converted yet)
+    T token_x{};
+    if (mine) {
+        const long long t = token_of(token_bits);
+        if (t >= 0 && t < a.vocab) token_x = x.x[t];
     }
     {
         float sa, sb, ta, tb;
@@ -339,42 +370,30 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
         p.s = sa + sb;
         p.t = ta + tb;
     }
-    if (TOP) sup[tid] = p.m == -INFINITY ? 0u : ordered_bits(p.m);
-    p = lp_join_warp(p);
+    if (TOP) sup[tid] = p.m;
+    p = lp_join_warp<16>(p);
     if (lane == 0) part[warp] = p;
     __syncthreads();
 
     // ---- this block's K best logits, largest first ----
-    const int K = a.top;
-    unsigned long long* mine_best = best + rank * K;            // (in the first block's table, this block's place)
     if (TOP) {
         const int n = ch1 - ch0;
-        for (int i = tid; i < K; i += kThreads) mine_best[i] = 0;
-        if (warp == 0) {                                        // the K-th largest thread maximum: the lanes' sorted shares, K times the largest head
-            uint32_t v[kWarps];
+        if (warp == 0) {                                        // the K-th largest group maximum: K times the largest, which its lane drops; a lane's number in
+            float f0 = -INFINITY, f1 = -INFINITY;               // the lowest bits keeps them apart
 #pragma unroll
-            for (int i = 0; i < kWarps; ++i) v[i] = sup[lane + 32 * i];
-#pragma unroll
-            for (int i = 0; i < kWarps - 1; ++i)
-#pragma unroll
-                for (int j = 0; j < kWarps - 1 - i; ++j) {
-                    const uint32_t x0 = max(v[j], v[j + 1]), x1 = min(v[j], v[j + 1]);
-                    v[j] = x0; v[j + 1] = x1;
-                }
-            uint32_t least = 0;
-            for (int k = 0; k < K; ++k) {
-                least = __reduce_max_sync(0xFFFFFFFFu, v[0]);
-                const uint32_t who = __ballot_sync(0xFFFFFFFFu, v[0] == least);
-                if (lane == __ffs(who) - 1) {
-#pragma unroll
-                    for (int i = 0; i < kWarps - 1; ++i) v[i] = v[i + 1];
-                    v[kWarps - 1] = 0;
-                }
+            for (int i = 0; i < kThreads; i += kLpGroups) {
+                f0 = fmaxf(f0, sup[i + lane]);
+                f1 = fmaxf(f1, sup[i + 32 + lane]);
             }
-            if (lane == 0) bound = least;
+            uint32_t v = ordered_bits(fmaxf(f0, f1)) & ~31u | lane, next = ordered_bits(fminf(f0, f1)) & ~31u | lane, least = 0;
+            for (int k = 0; k < K; ++k) {
+                least = __reduce_max_sync(0xFFFFFFFFu, v);
+                if (v == least) { v = next; next = 0; }
+            }
+            if (lane == 0) bound = from_ordered(max(least & ~31u, kLpFinite));
         }
         __syncthreads();
-        const uint32_t least = bound;
+        const float least = bound;
         for (int i = tid; i < n; i += kThreads)
             if (chunk_max[i] >= least) {
                 const int at = atomicAdd(&n_list, 1);
@@ -385,33 +404,38 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
         if (fits) {
             for (int i = warp; i < n_list; i += 4 * kWarps) {
                 uint4 v[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (i + u * kWarps < n_list) v[u] = x.load(list[i + u * kWarps], lane);
+                uint32_t hits = 0;                              // (N values of a vector, 4 vectors: 32 bits at most; -infinity, outside the row too, is none)
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    if (i + u * kWarps >= n_list) break;
-                    const int i0 = x.first(list[i + u * kWarps], lane);
-                    if (ordered_bits(LpVec<T>::last(lp_max<T>(v[u]))) < least) continue;
-                    for (int j = 0; j < LpVec<T>::N; ++j) {
-                        const uint32_t o = ordered_bits(LpVec<T>::at(v[u], j));
-                        if (o >= least && i0 + j >= 0 && i0 + j < a.vocab) {
-                            const int at = atomicAdd(&n_cand, 1);
-                            if (at < kLpCand) cand[at] = order_key(o, i0 + j);
-                        }
-                    }
+                    v[u] = make_uint4(LpVec<T>::kNone, LpVec<T>::kNone, LpVec<T>::kNone, LpVec<T>::kNone);
+                    if (i + u * kWarps < n_list) v[u] = x.load(list[i + u * kWarps], lane);
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int j = 0; j < LpVec<T>::N; ++j) hits |= (uint32_t)(LpVec<T>::at(v[u], j) >= least) << (u * LpVec<T>::N + j);
+                int at = hits != 0 ? atomicAdd(&n_cand, __popc(hits)) : 0;
+                for (; hits != 0; hits &= hits - 1, ++at) {
+                    const int b = __ffs(hits) - 1, u = b / LpVec<T>::N, j = b % LpVec<T>::N;
+                    const uint4 low = (u & 1) ? v[1] : v[0], high = (u & 1) ? v[3] : v[2];
+                    if (at < kLpCand) cand[at] = order_key(ordered_bits(LpVec<T>::at((u & 2) ? high : low, j)), x.first(list[i + u * kWarps], lane) + j);
                 }
             }
             __syncthreads();
             fits = n_cand <= kLpCand;
         }
         if (fits) {
-            const int held = n_cand, even = (held + 7) / 8 * 8;
-            if (tid < even - held) cand[held + tid] = 0;
-            __syncthreads();
+            const int held = n_cand, even = (held + 7) / 8 * 8;         // (zeros behind them)
             for (int i = tid; i < held; i += kThreads) {
                 const int at = lp_place(cand, even, cand[i]);
                 if (at < K) mine_best[at] = cand[i];
+            }
+            // fewer than K logits above -infinity: its lowest indices, all of which lie in the block's first K values
+            if (held < K && warp == 0) {
+                const int i = max(x.first(ch0, 0), 0) + lane;
+                const bool out = lane < K && i < min(x.first(ch1, 0), a.vocab) && to_f32(x.x[i]) == -INFINITY;
+                const int at = held + __popc(__ballot_sync(0xFFFFFFFFu, out) & ((1u << lane) - 1));
+                if (out && at < K) mine_best[at] = order_key(kLpFinite - 1, i);
             }
         } else {
             // the K-th best chunk by (maximum, lower index), then K rounds over the chunks up to it
@@ -422,7 +446,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
                 while (hi - lo > 1) {
                     const unsigned long long mid = lo + (hi - lo) / 2;
                     int k = 0;
-                    for (int i = lane; i < n; i += 32) k += order_key(chunk_max[i], i) >= mid;
+                    for (int i = lane; i < n; i += 32) k += order_key(ordered_bits(chunk_max[i]), i) >= mid;
                     k = __reduce_add_sync(0xFFFFFFFFu, k);
                     if (k >= K) lo = mid; else hi = mid;
                     if (k == K) break;
@@ -431,13 +455,13 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
             }
             __syncthreads();
             for (int i = tid; i < n; i += kThreads)
-                if (order_key(chunk_max[i], i) >= chunk_bound) list[atomicAdd(&n_list, 1)] = ch0 + i;       // (K of them at most: keys are distinct)
+                if (order_key(ordered_bits(chunk_max[i]), i) >= chunk_bound) list[atomicAdd(&n_list, 1)] = ch0 + i;       // (K of them at most: keys are distinct)
             __syncthreads();
-            const int held = n_list;
+            const int chunks = n_list;
             unsigned long long last = ~0ull;
             for (int k = 0; k < K; ++k) {
                 unsigned long long b = 0;
-                for (int i = warp; i < held; i += kWarps) {
+                for (int i = warp; i < chunks; i += kWarps) {
                     const uint4 v = x.load(list[i], lane);
                     const int i0 = x.first(list[i], lane);
 #pragma unroll
@@ -468,7 +492,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
     if (C > 1) {
         asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (rank != 0) {
-            p = lp_join(part, kWarps);
+            p = lp_join(part, kWarps, lane);
             if (TOP && tid < K)
                 asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(mapa_u32(smem_u32(mine_best + tid), 0)), "l"(mine_best[tid]) : "memory");
             if (tid == 0) {
@@ -480,14 +504,14 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
             return;
         }
         if (warp == 0) {
-            p = lp_join(part, kWarps);
+            p = lp_join(part, kWarps, lane);
             if (lane == 0) parts[0] = p;
         }
         __syncwarp();
         cluster_sync_all();
-        p = lp_join(parts, C);
+        p = lp_join(parts, C, lane);
     } else {
-        p = lp_join(part, kWarps);
+        p = lp_join(part, kWarps, lane);
     }
 
     // ---- the row's numbers, the same in all threads ----
@@ -522,16 +546,19 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a,
     }
     const float log_z = fmaf(p.m, a.inv_t, log_s);
     auto lp = [&](float v) { return bad ? nan : (none || v == -INFINITY ? -INFINITY : fmaf(v - p.m, a.inv_t, -log_s)); };
-    if (tid == 0) {
+    if (tid == kThreads / 2) {
         if (a.logsumexp) a.logsumexp[row] = bad ? nan : (none ? -INFINITY : log_z);
         if (a.entropy) a.entropy[row] = bad ? nan : (none ? 0.f : entropy);
     }
-    for (int j = tid; j < a.given; j += kThreads) {
+    for (int j = turn; j < a.given; j += kThreads) {
+        const long long at = (long long)row * a.given + j;
         if (j >= kThreads) {
-            token = token_at(j);
-            token_x = token >= 0 && token < a.vocab ? to_f32(x.x[token]) : 0.f;
+            if (a.wide) token_bits = reinterpret_cast<const int2*>(a.tokens)[at];
+            else token_bits.x = reinterpret_cast<const int*>(a.tokens)[at];
         }
-        a.logprob[(long long)row * a.given + j] = token < 0 ? 0.f : (token >= a.vocab ? nan : lp(token_x));
+        const long long t = token_of(token_bits);
+        if (j >= kThreads && t >= 0 && t < a.vocab) token_x = x.x[t];
+        a.logprob[at] = t < 0 ? 0.f : (t >= a.vocab ? nan : lp(to_f32(token_x)));
     }
     if (TOP) {
         const int all = C * K, even = (all + 7) / 8 * 8;

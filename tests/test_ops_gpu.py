@@ -360,6 +360,24 @@ def test_logprobs_tokens_outside():
     _check_logprobs(ops.logprobs(x, tokens, 3), x, tokens, 3, 1.0)
 
 
+@pytest.mark.parametrize("rows, vocab", [(2, 40), (4, 1000), (4, 32003), (30, 32003), (4, 152064), (700, 5001)])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_logprobs_few_allowed(rows, vocab, dtype):
+    """fewer logits above -infinity than alternatives are wanted, as many, and more than the tables hold: the lowest indices fill up"""
+    g = _gen(27)
+    values = (torch.randn(rows, vocab, device="cuda", generator=g) * 3).to(dtype)
+    tokens = torch.randint(0, vocab, (rows,), device="cuda", generator=g)
+    at = torch.rand(rows, vocab, device="cuda", generator=g).argsort(-1)
+    for allowed in (0, 1, 3, 19, 20, 21, 33, 64, 250, 257, 300):
+        x = torch.where(at < allowed, values, -math.inf)                 # anywhere
+        x[1::4] = torch.where(torch.arange(vocab, device="cuda") < allowed, values[1::4], -math.inf)
+        x[2::4] = torch.where(torch.arange(vocab, device="cuda") >= vocab - allowed, values[2::4], -math.inf)
+        if rows > 3:
+            x[3, vocab // 2] = math.nan
+        for top in (1, 20, 32):
+            _check_logprobs(ops.logprobs(x, tokens, top), x, tokens, top, 1.0)
+
+
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("vocab", [300, 5001, 152064])
 def test_logprobs_many_equal(vocab, dtype):

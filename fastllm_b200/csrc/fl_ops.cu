@@ -130,11 +130,10 @@ static void load_kernels(Kernels... kernels) {
 }
 template <typename T>
 static void load_kernels_of() {
-    if constexpr (sizeof(T) == 2) load_kernels(logprobs_kernel<T, true, 128, false>);
     load_kernels(quantize_rows_kernel<T, 0, 256>, quantize_rows_kernel<T, 2, 128>, quantize_rows_kernel<T, 2, 256>, quantize_rows_kernel<T, 4, 256>,
-                 quantize_rows_kernel<T, 8, 256>, quantize_rows_kernel<T, -1, 256>, logprobs_kernel<T, true, 128, true>, logprobs_kernel<T, false, 128, true>);
-    FL_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, true, 256, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    FL_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, false, 256, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+                 quantize_rows_kernel<T, 8, 256>, quantize_rows_kernel<T, -1, 256>, logprobs_kernel<T, true, 128>, logprobs_kernel<T, false, 128>);
+    FL_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, true, 256>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    FL_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, false, 256>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     load_kernels(linear8_token_kernel<T, 1>, linear8_token_kernel<T, 2>);
 }
 // One-time set-up, with fl_init: also loads the kernels, so that a caller's first call may be one inside a graph capture.
@@ -250,10 +249,8 @@ static void run_linear8(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
 // us; 100 x 152064, 2, 4 and 6: 17.9, 14.0 and 18.5; 64 x 152064 and five alternatives, 4, 6 and 7: 13.1, 12.2 and 17.8).  At most six, since larger clusters find a
 // place on fewer SMs (37 x 128256 bf16, 6 and 8: 5.9 and 6.4, with five alternatives 8.5 and 9.4), except where all have an SM each: 16 then, or eight
 // with alternatives, whose lists the first block joins (3 x 152064 f32, 6, 8 and 16: 4.7, 4.2 and 3.6, with twenty 8.1, 8.0 and 9.9).  A cluster of 16 is not
-// portable to every chip, but B200 has it.  Small blocks where there are more rows than SMs hold large ones (256 -> 128
-// threads, five alternatives: 1000 x 32003 f16 25.1 -> 20.8 us, 777 x 32000 f32 28.8 -> 23.7, but 400 x 32000 12.7 -> 13.2).  With alternatives and many short
-// 16-bit rows the registers of a second batch are worth more as a further block per SM (1300 x 32000 bf16 30.7 -> 25.0 without it; 2048 x 152064 118 -> 111 with
-// it, 2048 x 32000 f32 55.0 -> 52.3).
+// portable to every chip, but B200 has it.  Small blocks where there are more rows than SMs hold large ones (256 and 128
+// threads, five alternatives: 1000 x 32003 f16 20.8 and 18.2 us, 777 x 32000 f32 23.8 and 22.3, 4000 x 5000 f32 46 and 26, but 400 x 32000 f32 13.5 and 16.3).
 template <typename T>
 static void run_logprobs(LaunchCtx& lc, const LogprobArgs& a) {
     const int chunks = (a.vocab + 2 * LpRow<T>::N - 1 + LpRow<T>::kChunk - 1) / LpRow<T>::kChunk;
@@ -264,13 +261,9 @@ static void run_logprobs(LaunchCtx& lc, const LogprobArgs& a) {
     const size_t smem = a.top > 0 ? (size_t)per * 4 : 0;
     auto go = [&](auto kern, int threads) { launch_op(lc, "logprobs", bytes, kern, grid, threads, smem, C, false, a, C, per); };
     if (a.rows <= 4 * kNumSMs) {
-        a.top > 0 ? go(logprobs_kernel<T, true, 256, true>, 256) : go(logprobs_kernel<T, false, 256, true>, 256);
-    } else if (a.top == 0) {
-        go(logprobs_kernel<T, false, 128, true>, 128);
+        a.top > 0 ? go(logprobs_kernel<T, true, 256>, 256) : go(logprobs_kernel<T, false, 256>, 256);
     } else {
-        if constexpr (sizeof(T) == 2)
-            if (chunks < 512) return go(logprobs_kernel<T, true, 128, false>, 128);
-        go(logprobs_kernel<T, true, 128, true>, 128);
+        a.top > 0 ? go(logprobs_kernel<T, true, 128>, 128) : go(logprobs_kernel<T, false, 128>, 128);
     }
 }
 template <typename T>

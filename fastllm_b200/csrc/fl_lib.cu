@@ -2037,10 +2037,10 @@ FL_EXPORT int fl_cache_logprobs(fl_cache* c, int rows, const int32_t* tokens, in
     use_device();
     try {
         const size_t n = (size_t)rows * 4, tok = n * given, res = n * (given + 2 + 2 * (size_t)top);
-        if (c->lp_dev.n < tok + res) {
+        if (c->lp_dev.n < tok + res || c->lp_host.n < tok + res) {      // (the second: after an allocation that failed)
             FL_CUDA(cudaStreamSynchronize(c->stream));
-            c->lp_dev.alloc(tok + res);
             c->lp_host.alloc(tok + res);
+            c->lp_dev.alloc(tok + res);
         }
         if (tok > 0) {
             std::memcpy(c->lp_host.p, tokens, tok);

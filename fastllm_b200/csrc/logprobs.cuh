@@ -12,8 +12,8 @@
 //
 // Alternatives: the row lies in chunks of 512 bytes (one load of a warp), whose maxima are kept.  A block's threads form 64 groups; the K-th largest of the groups'
 // maxima is a lower bound for the block's K-th largest logit, since K groups hold one at least as large.  Only chunks that reach the bound are read again (from
-// L2), only logits that reach it are ranked: 5 of 5, 24 of 20 or 44 of 32 where the order is random.  (Groups of one thread bring those to 21 and 34, but the
-// bound is found in K steps over what a warp holds, 31 cycles each with two values a lane, 80 with eight.)  Where fewer than K logits are above -infinity, all of them
+// L2), only logits that reach it are ranked: 5 of 5, 24 of 20 or 44 of 32 where the order is random.  (Groups of one thread bring those to 21 and 34,
+// but the bound is found in K steps over what a warp holds, 31 cycles each with two values a lane.)  Where fewer than K logits are above -infinity, all of them
 // are ranked and the lowest indices fill up.  Where equal logits leave more than the tables hold, the K best chunks by (maximum, lower index) are
 // taken instead: a logit outside them is behind K others, one per chunk; then K rounds pick one each.
 #pragma once

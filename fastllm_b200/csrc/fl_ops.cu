@@ -245,8 +245,8 @@ static void run_linear8(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
     else launch_few<128>(lc, bytes, q, ldq, w, ldw, g, !given);
 }
 
-// Blocks per row: three per SM over the rows, as many as run at once, with 16 chunks each at least (200 x 152064 f32, 1, 2 and 3 blocks a row: 30.2, 23.3 and 30.5
-// us; 100 x 152064, 2, 4 and 6: 17.9, 14.0 and 18.5; 64 x 152064 and five alternatives, 4, 6 and 7: 13.1, 12.2 and 17.8).  At most six, since larger clusters find a
+// Blocks per row: three per SM over the rows, of the four that run at once, with 16 chunks each at least (200 x 152064 f32, 1, 2 and 3 blocks a row: 30, 21.5 and
+// 27.9 us; 100 x 152064, 2, 4 and 6: 16.2, 13.2 and 16.9; 64 x 152064 and twenty alternatives, 4, 6 and 7: 14.1, 13.8 and 14.7).  At most six, since larger clusters find a
 // place on fewer SMs (37 x 128256 bf16, 6 and 8: 5.9 and 6.4, with five alternatives 8.5 and 9.4), except where all have an SM each: 16 then, or eight
 // with alternatives, whose lists the first block joins (3 x 152064 f32, 6, 8 and 16: 4.7, 4.2 and 3.6, with twenty 8.1, 8.0 and 9.9).  A cluster of 16 is not
 // portable to every chip, but B200 has it.  Small blocks where there are more rows than SMs hold large ones (256 and 128

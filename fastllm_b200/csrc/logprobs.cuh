@@ -231,8 +231,9 @@ __device__ __forceinline__ int cluster_id() {
 
 // TOP: with alternatives.  A cluster of C blocks per row, `per` chunks each.  A batch is on its way while the one before is added up (16-bit rows with alternatives
 // of one batch at a time, whose registers let two more blocks onto an SM: 1000 x 32003 f16 18.2 -> 19.2 us, 2048 x 32000 bf16 32.4 -> 34.4, 1300 x 32000 24.5 -> 21.9).
+// Four large blocks to an SM (64 registers a thread instead of 66: 500 x 128256 f32 with five alternatives 59 -> 44 us); for small ones the compiler keeps to 64 by itself.
 template <typename T, bool TOP, int kThreads>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobArgs a, const int C, const int per) {
+__global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 0) logprobs_kernel(const LogprobArgs a, const int C, const int per) {
     constexpr int kWarps = kThreads / 32, U = 4;
     extern __shared__ float chunk_max[];                        // TOP: maxima of this block's chunks
     __shared__ LpPart part[kWarps], parts[kLpMaxCluster];

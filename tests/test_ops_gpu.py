@@ -360,6 +360,18 @@ def test_logprobs_tokens_outside():
     _check_logprobs(ops.logprobs(x, tokens, 3), x, tokens, 3, 1.0)
 
 
+@pytest.mark.parametrize("rows", [2, 9, 10, 60, 75, 89, 100, 120, 148, 149, 222, 223, 445, 592, 593])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_logprobs_row_counts(rows, dtype):
+    """every number of blocks that a row is shared by, rows that start on no 16-byte border, a value alone behind the last chunk"""
+    g = _gen(28)
+    for vocab in (32001, 33025, 9000):
+        x = (torch.randn(rows, vocab + 2, device="cuda", generator=g) * 3).to(dtype)[:, 1:vocab + 1]
+        tokens = torch.randint(0, vocab, (rows, 2), device="cuda", generator=g)
+        for top in (0, 7, 32):
+            _check_logprobs(ops.logprobs(x, tokens, top), x, tokens, top, 1.0)
+
+
 @pytest.mark.parametrize("rows, vocab", [(2, 40), (4, 1000), (4, 32003), (30, 32003), (4, 152064), (700, 5001)])
 @pytest.mark.parametrize("dtype", FLOATS)
 def test_logprobs_few_allowed(rows, vocab, dtype):

@@ -516,6 +516,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 0) logprobs_ke
     float log_s, entropy;                                       // log of the sum about the maximum
     bool bad;
     if (far) {
+        __syncthreads();                                        // (part is written again below: with one block per row a warp may still read it)
         float s = 0.f, t = 0.f;
         for (int i = tid; i < a.vocab; i += kThreads) {
             const float d = (to_f32(x.x[i]) - p.m) * a.inv_t, e = expf(d);

@@ -25,6 +25,11 @@ constexpr int kLpMaxTop = 32;
 constexpr int kLpMaxVocab = 1 << 20;
 constexpr int kLpMaxCluster = 16;
 constexpr int kLpGroups = 64;                       // of a block's threads
+// Where the loop over a row holds.  A distance c x - r is off by half a step of r, 4 up to 2^27: up to there sums stay far from overflow and lose a few bits at
+// most.  So references begin at -2^27, and what lies below (masks: -infinity or any large negative number) does not move them; they begin kLpNothing above
+// what -infinity is raised to (kLow) where that is higher, so that it counts 2^-256, which is 0.  Rows whose maximum is not that far above kLow or lies more than
+// 2^27 from 0, and temperatures at which c kLow would overflow, are summed once more.
+constexpr float kLpFarAt = 0x1p27f, kLpNothing = 256.f;
 constexpr uint32_t kLpFinite = 0x00800000u;         // ordered_bits of the lowest finite value: the next above -infinity's
 constexpr int kLpList = 96, kLpCand = 256;          // chunks that are read again, logits that are ranked
 
@@ -69,12 +74,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return r;
 }
 
-// 16 bytes of logits.  low: what -infinity is raised to before the sums, so that e (c x - r) is 0 and not 0 times infinity (NaN stays NaN); a row whose
-// maximum lies below `far` is summed by another loop.
+// 16 bytes of logits.  kLow: what lies below is raised to it before the sums, so that e (c x - r) is 0 and not 0 times infinity (NaN stays NaN)
 template <typename T> struct LpVec;
 template <> struct LpVec<float> {
     static constexpr int N = 4;
-    static constexpr float kLow = -1e30f, kFar = -1e29f;
+    static constexpr float kLow = -1e30f;
     static constexpr uint32_t kNone = 0xFF800000u;              // -infinity, in every place of a word
     static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
     static __device__ __forceinline__ float last(uint32_t m) { return __uint_as_float(m); }
@@ -91,7 +95,7 @@ template <> struct LpVec<float> {
 };
 template <> struct LpVec<__nv_bfloat16> {
     static constexpr int N = 8;
-    static constexpr float kLow = -1e30f, kFar = -1e29f;
+    static constexpr float kLow = -1e30f;
     static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
         uint32_t r;
         asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -114,7 +118,7 @@ template <> struct LpVec<__nv_bfloat16> {
 };
 template <> struct LpVec<__half> {
     static constexpr int N = 8;
-    static constexpr float kLow = -65504.f, kFar = -30000.f;
+    static constexpr float kLow = -65504.f;
     static __device__ __forceinline__ float2 two(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
     static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
         uint32_t r;
@@ -268,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 0) logprobs_ke
     }
     auto token_of = [&](int2 bits) { return a.wide ? (long long)bits.y << 32 | (uint32_t)bits.x : (long long)bits.x; };
 
-    LpPart p{-INFINITY, 0.9f * LpVec<T>::kLow * c, 0.f, 0.f};   // (well above what -infinity is raised to, below every other value of a row that is not `far`)
+    LpPart p{-INFINITY, fmaxf(-kLpFarAt, fmaf(LpVec<T>::kLow, c, kLpNothing)), 0.f, 0.f};
     uint64_t s2 = pack2(0.f, 0.f), t2 = s2;
     const uint64_t c2 = pack2(c, c);
     // U vectors of a lane, one of each of U chunks; at(u): the u-th chunk's place in chunk_max, or -1
@@ -509,9 +513,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 256 ? 4 : 0) logprobs_ke
     }
 
     // ---- the row's numbers, the same in all threads ----
-    // Rows far from 0 (c x near the end of the range, or a maximum near what -infinity was raised to): summed once more, about the maximum itself.
-    // So are temperatures at which the raised -infinity would not vanish, or overflows.
-    const bool far = p.m > -INFINITY && p.m < INFINITY && (fabsf(p.m) * c > 1e37f || p.m < LpVec<T>::kFar || c > 1e6f || c * (LpVec<T>::kFar - LpVec<T>::kLow) < 1000.f);
+    // a row that the loop's references do not hold for (see kLpFarAt): summed once more, about the maximum itself
+    const bool far = p.m > -INFINITY && p.m < INFINITY && (fabsf(p.m) * c > kLpFarAt || (p.m - LpVec<T>::kLow) * c < kLpNothing || LpVec<T>::kLow * c < -1e38f);
     const bool none = p.m == -INFINITY && p.s == p.s;
     float log_s, entropy;                                       // log of the sum about the maximum
     bool bad;

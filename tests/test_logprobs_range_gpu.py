@@ -94,3 +94,17 @@ def test_masks_at_any_temperature(vocab, temperature, dtype):
     tokens = torch.randint(0, vocab, (10, 2), device="cuda", generator=_gen(7))
     for top in (0, 7):
         _check_logprobs(ops.logprobs(x, tokens, top, temperature), x, tokens, top, temperature)
+
+
+@pytest.mark.parametrize("temperature", [1e36, 1e37, 1e38])
+@pytest.mark.parametrize("vocab", [40, 32003])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_differences_past_the_largest_number(vocab, temperature, dtype):
+    """numbers of both signs whose difference is none of 32 bits, over temperatures that bring it back"""
+    x = ((torch.rand(6, vocab, device="cuda", generator=_gen(8)) * 2 - 1) * 3.3e38).to(dtype)
+    x[3, vocab // 2] = -torch.inf
+    x[4] = x[4].abs()
+    x[5] = -x[5].abs()
+    tokens = torch.randint(0, vocab, (6, 4), device="cuda", generator=_gen(9))
+    for top in (0, 7):
+        _check_logprobs(ops.logprobs(x, tokens, top, temperature), x, tokens, top, temperature)

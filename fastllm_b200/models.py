@@ -1244,6 +1244,23 @@ class Model:
         return outs
 
 
+MAX_TOP = 32            # alternatives of a row (fl_cache_logprobs)
+
+
+def _check_top(top: int, vocab: int):
+    if not 0 <= top <= min(MAX_TOP, vocab):
+        raise FastllmError(-1, f"from 0 to {min(MAX_TOP, vocab)} alternatives, got {top}")
+
+
+def _give_back(cache, slots):
+    """after a step that failed; a cache that cannot be used any more has nothing to give back"""
+    for s in slots:
+        try:
+            cache.slot_reset(s)
+        except FastllmError:
+            pass
+
+
 class ContinuousBatcher:
     """Continuous batching above fl_forward_slots.  The reference serialises chat requests at batch 1
     under one mutex (api/chat.rs:206-208); here up to `max_batch` requests of ANY lengths share the decode steps: a request is
@@ -1273,8 +1290,15 @@ class ContinuousBatcher:
     def generate(self, prompts, max_tokens: int, temperature: float = 0.0, logprobs: int | None = None):
         """-> one id list per prompt, in request order.  logprobs = K (0 to 32): -> (id lists, per prompt and token a dict with the token's
         "logprob" and "top", the K most likely (id, logprob) pairs), from the distribution at temperature 1 on the device."""
+        if logprobs is not None:
+            _check_top(logprobs, getattr(self.cache, "vocab", MAX_TOP))
         self._told = None if logprobs is None else [[] for _ in prompts]
-        out = self._generate(prompts, max_tokens, temperature, logprobs)
+        free = list(range(self.max_batch))[::-1]
+        try:
+            out = self._generate(prompts, max_tokens, temperature, logprobs, free)
+        except BaseException:
+            _give_back(self.cache, set(range(self.max_batch)) - set(free))      # (what the next call would go on from)
+            raise
         told, self._told = self._told, None
         return out if logprobs is None else (out, told)
 
@@ -1289,12 +1313,11 @@ class ContinuousBatcher:
         for row, req, _ in picked:
             self._told[req].append({"logprob": float(lp.logprob[row]), "top": [(int(i), float(v)) for i, v in zip(lp.top_ids[row], lp.top_logprobs[row])]})
 
-    def _generate(self, prompts, max_tokens: int, temperature: float, logprobs):
+    def _generate(self, prompts, max_tokens: int, temperature: float, logprobs, free):
         if self.prefill_chunk and hasattr(self.cache, "forward_ragged"):
-            return self._generate_mixed(prompts, max_tokens, temperature, logprobs)
+            return self._generate_mixed(prompts, max_tokens, temperature, logprobs, free)
         out = [[] for _ in prompts]
         waiting = list(range(len(prompts)))[::-1]
-        free = list(range(self.max_batch))[::-1]
         running = {}            # slot -> [request, next RoPE position, LogitsProcessor, token to feed]
         if max_tokens <= 0:
             return out
@@ -1342,7 +1365,7 @@ class ContinuousBatcher:
         return out
 
 
-    def _generate_mixed(self, prompts, max_tokens: int, temperature: float, logprobs=None):
+    def _generate_mixed(self, prompts, max_tokens: int, temperature: float, logprobs, free):
         """Mixed steps: a request takes a free slot as soon as there is one; each step carries, per running request, either the next
         portion of its prompt (at most prefill_chunk tokens) or its one new token.  Sampling, EOS and the token budget are those of
         generate(); a finished request gives its slot (pages and state) back."""
@@ -1350,7 +1373,6 @@ class ContinuousBatcher:
         if max_tokens <= 0:
             return out
         waiting = list(range(len(prompts)))[::-1]
-        free = list(range(self.max_batch))[::-1]
         running = {}            # slot -> [request, prompt tokens fed, LogitsProcessor, token to feed]
         while waiting or running:
             while waiting and free:

@@ -1437,6 +1437,7 @@ def score(model, texts, top: int = 0, cache: DeviceCache | None = None, portion:
         cache = model.new_device_cache(max(1, min(len(texts), 8)), max([64] + [len(t) for t in texts]))
     if portion < cache.max_batch:
         raise FastllmError(-1, "a step brings at least one token of every text that is being read")
+    _check_top(top, cache.vocab)
     if any(cache.slot_len(s) for s in range(cache.max_batch)):
         raise FastllmError(-3, "a slot of the cache holds a sequence")
     for t in texts:
@@ -1460,9 +1461,8 @@ def score(model, texts, top: int = 0, cache: DeviceCache | None = None, portion:
         try:
             cache.forward_ragged(slots, toks, want, fetch=False)
             lp, row = cache.logprobs(np.asarray(given, dtype=np.int32), top), 0
-        except FastllmError:
-            for s in running:               # (the caller's cache as it was)
-                cache.slot_reset(s)
+        except BaseException:
+            _give_back(cache, running)      # (the caller's cache as it was)
             raise
         for s, part in zip(slots, toks):
             t = running[s][0]

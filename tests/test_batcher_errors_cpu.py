@@ -73,3 +73,24 @@ def test_a_cache_that_gives_nothing_back_shows_its_first_error():
 
     with pytest.raises(FastllmError, match="lost"):
         _batcher(_Lost(3, "forward", 2, True, FastllmError(-2, "lost")), 4).generate(_prompts([5, 9]), 6)
+
+
+@pytest.mark.parametrize("top", [-1, 24, 33])
+def test_scoring_refuses_a_number_of_alternatives_before_any_step(top):
+    cache = _Cache(2)
+    with pytest.raises(FastllmError, match="alternatives"):
+        models.score(_Model(), [[3, 4]], top=top, cache=cache)
+    assert cache.last is None
+
+
+@pytest.mark.parametrize("what", ["forward", "logprobs"])
+@pytest.mark.parametrize("good", [0, 2])
+@pytest.mark.parametrize("error", [FastllmError(-2, "lost"), MemoryError(), KeyboardInterrupt()])
+def test_a_scoring_after_one_that_failed(what, good, error):
+    texts = _prompts([5, 9, 1, 7, 3])
+    want = [s.total for s in models.score(_Model(), texts, cache=_Cache(2), portion=4)]
+    cache = _Failing(2, what, good, True, error)
+    with pytest.raises(type(error)):
+        models.score(_Model(), texts, cache=cache, portion=4)
+    assert not any(cache.hist)
+    assert [s.total for s in models.score(_Model(), texts, cache=cache, portion=4)] == want

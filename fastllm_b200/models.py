@@ -253,9 +253,16 @@ class DeviceCache:
         that many rows of that forward (default: as tokens has)."""
         if tokens is None and rows is None:
             raise FastllmError(-1, "log probabilities of how many rows: neither tokens nor rows are given")
-        tok = None if tokens is None else np.ascontiguousarray(tokens, dtype=np.int32)
-        if tok is not None and tok.ndim not in (1, 2):
-            raise FastllmError(-1, f"tokens are [rows] or [rows, m], got shape {tok.shape}")
+        tok = None
+        if tokens is not None:
+            tok = np.asarray(tokens)
+            if tok.size and tok.dtype.kind not in "iu":
+                raise FastllmError(-1, f"tokens are whole numbers, got {tok.dtype}")
+            if tok.dtype != np.int32:               # (what 32 bits do not hold stays padding, or past the vocabulary)
+                tok = np.clip(tok, -1, 2 ** 31 - 1) if tok.dtype.kind == "i" else np.minimum(tok, 2 ** 31 - 1)
+            tok = np.ascontiguousarray(tok, dtype=np.int32)
+            if tok.ndim not in (1, 2):
+                raise FastllmError(-1, f"tokens are [rows] or [rows, m], got shape {tok.shape}")
         n = rows if rows is not None else (0 if tok is None else tok.shape[0])
         if tok is not None and tok.shape[0] != n:
             raise FastllmError(-1, f"{tok.shape[0]} rows of tokens for {n} rows of logits")

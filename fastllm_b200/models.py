@@ -258,7 +258,7 @@ class DeviceCache:
             tok = np.asarray(tokens)
             if tok.size and tok.dtype.kind not in "iu":
                 raise FastllmError(-1, f"tokens are whole numbers, got {tok.dtype}")
-            if tok.dtype != np.int32:               # (what 32 bits do not hold stays padding, or past the vocabulary)
+            if tok.dtype == np.uint32 or tok.dtype.itemsize > 4:        # (what 32 bits do not hold stays padding, or past the vocabulary)
                 tok = np.clip(tok, -1, 2 ** 31 - 1) if tok.dtype.kind == "i" else np.minimum(tok, 2 ** 31 - 1)
             tok = np.ascontiguousarray(tok, dtype=np.int32)
             if tok.ndim not in (1, 2):

@@ -89,6 +89,8 @@ struct LogProbs {
     std::vector<int32_t> top_ids;
 };
 inline LogProbs logprobs(fl_cache* c, int rows, const std::vector<int32_t>& tokens, int top, double temperature = 1.0) {
+    if (rows < 0 || (rows == 0 ? !tokens.empty() : tokens.size() % rows != 0)) throw Error(FL_ERR_INVALID, "log probabilities: every row has the same number of tokens");
+    if (top < 0 || top > 32) throw Error(FL_ERR_INVALID, "log probabilities: from 0 to 32 alternatives");
     LogProbs r;
     const int given = rows > 0 ? (int)(tokens.size() / rows) : 0;
     r.logprob.resize(tokens.size()); r.logsumexp.resize(rows); r.entropy.resize(rows);

@@ -1737,7 +1737,6 @@ FL_EXPORT int fl_init(int device) {
     const int cur = g_device.load();
     FL_CHECK(cur < 0 || cur == device, FL_ERR_STATE, "fl_init: this process is already bound to device " + std::to_string(cur));
     FL_CUDA(cudaSetDevice(device));
-    ops_init();
     g_device.store(device);
     FL_API_END
 }

@@ -1,5 +1,7 @@
 // Operators on device memory: argument checks and launches behind the C ABI (include/fastllm_b200.h, "operators on device memory").
+#include <atomic>
 #include <cmath>
+#include <mutex>
 
 #include "../../include/fastllm_b200.h"
 #include "bert_model.cuh"
@@ -136,9 +138,13 @@ static void load_kernels_of() {
     FL_CUDA(cudaFuncSetAttribute(logprobs_kernel<T, false, 256>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     load_kernels(linear8_token_kernel<T, 1>, linear8_token_kernel<T, 2>);
 }
-// One-time set-up, with fl_init: also loads the kernels, so that a caller's first call may be one inside a graph capture.
-void ops_init() {
-    if (g_op_failed != nullptr) return;
+// One-time set-up on the bound device, by the first call that launches an operator.  It also loads the kernels, so that this call may be one inside a graph capture.
+static void set_up() {
+    static std::atomic<bool> done{false};
+    static std::mutex one;
+    if (done.load(std::memory_order_acquire)) return;
+    std::lock_guard<std::mutex> lock(one);
+    if (done.load(std::memory_order_relaxed)) return;
     RelaxedCapture relaxed;
     load_kernels_of<float>(); load_kernels_of<__nv_bfloat16>(); load_kernels_of<__half>();
     few_attr<16>(); few_attr<32>(); few_attr<64>(); few_attr<128>();
@@ -151,12 +157,12 @@ void ops_init() {
     cfg.attrs = at; cfg.numAttrs = 1;
     int k = 0;
     FL_CUDA(cudaOccupancyMaxActiveClusters(&k, linear8_pair_kernel, &cfg));
-    FL_CHECK(k >= 1, FL_ERR_UNSUPPORTED, "no two SMs of this device form a pair");
     g_pair_clusters = std::min(k, kNumSMs / 2);
     int* p = nullptr;
     FL_CUDA(cudaMallocHost(&p, sizeof(int)));
     *p = 0;
     g_op_failed = p;
+    done.store(true, std::memory_order_release);
 }
 static void check_op_failed() {
     FL_CHECK(*reinterpret_cast<volatile int*>(g_op_failed) == 0, FL_ERR_CUDA, "a wait inside an operator's kernel ran out in an earlier call: its results are not valid");
@@ -212,6 +218,7 @@ static void launch_few(LaunchCtx& lc, uint64_t bytes, const int8_t* x, int64_t l
     launch_op(lc, "linear8", bytes, linear8_few_kernel<BN>, dim3((unsigned)(tiles * S)), L8Few<BN>::kThreads, L8Few<BN>::kSmem, S, pdl, tw, tx, g, S);
 }
 static void launch_pair(LaunchCtx& lc, uint64_t bytes, const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, const Linear8Args& g, bool pdl) {
+    FL_CHECK(g_pair_clusters >= 1, FL_ERR_UNSUPPORTED, "linear8: no two SMs of this device form a pair");
     const L8Pair p = pair_plan8(g.rows, g.n, g.k, g_pair_clusters);
     const CUtensorMap tx = make_tmap_i8(x, g.rows, g.k, ldx, p.bn / (p.bn > 256 ? 4 : 2)), tw = make_tmap_i8(w, g.n, g.k, ldw, 128);
     const long long clusters = std::min<long long>(g_pair_clusters, (long long)p.mt * p.nt);
@@ -279,9 +286,11 @@ static void check_temperature(double temperature) {
 
 size_t linear8_workspace(int64_t rows, int64_t k) { return linear8_room(rows, k, false).all; }
 void op_quantize_rows(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* q, int64_t ldq, float* scale) {
+    set_up();
     quantize_rows(lc, x, dtype, rows, cols, ldx, q, ldq, ldq, scale);
 }
 void op_linear8(LaunchCtx& lc, const float* x, const int8_t* w, const float* w_scale, int64_t rows, int64_t n, int64_t k, float* y, void* workspace, int* failed) {
+    set_up();
     run_linear8(lc, x, FL_DTYPE_F32, k, nullptr, w, padded8(k), w_scale, nullptr, rows, n, k, y, FL_DTYPE_F32, n, workspace, failed);
 }
 void op_logprobs(LaunchCtx& lc, const float* logits, int64_t rows, int64_t vocab, const int32_t* tokens, int64_t given, double temperature, int top, float* logprob,
@@ -289,6 +298,7 @@ void op_logprobs(LaunchCtx& lc, const float* logits, int64_t rows, int64_t vocab
     FL_CHECK(vocab <= kLpMaxVocab, FL_ERR_UNSUPPORTED, "logprobs: a vocabulary of at most 2^20");
     FL_CHECK(top >= 0 && top <= kLpMaxTop && top <= vocab, FL_ERR_INVALID, "logprobs: from 0 to 32 alternatives, and no more than the vocabulary has");
     check_temperature(temperature);
+    set_up();
     run_logprobs<float>(lc, LogprobArgs{logits, vocab, (int)rows, (int)vocab, 1.f, 1.f, tokens, (int)given, 0, top, given ? logprob : nullptr, logsumexp, entropy, top_ids,
                                         top_logprobs}, temperature);
 }
@@ -308,6 +318,7 @@ FL_EXPORT int fl_quantize_rows(const void* x, int dtype, int64_t rows, int64_t c
     FL_CHECK(x && q && scale, FL_ERR_INVALID, "NULL argument");
     FL_CHECK(aligned(x, dtype_size(dtype)) && aligned(scale, 4), FL_ERR_INVALID, "quantize_rows: a pointer is not aligned to its type");
     DeviceScope dev;
+    set_up();
     LaunchCtx lc = op_ctx(stream);
     quantize_rows(lc, x, dtype, rows, cols, ldx, q, ldq, cols, scale);
     FL_API_END
@@ -343,6 +354,7 @@ FL_EXPORT int fl_linear8(const void* x, int x_dtype, int64_t ldx, const float* x
     FL_CHECK(room.all == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= room.all), FL_ERR_INVALID,
              "linear8: the workspace is smaller than fl_linear8_workspace asks for, or not on a 256-byte border");
     DeviceScope dev;
+    set_up();
     LaunchCtx lc = op_ctx(stream);
     check_op_failed();
     run_linear8(lc, x, x_dtype, ldx, x_scale, w, ldw, w_scale, bias, rows, n, k, y, y_dtype, ldy, workspace, g_op_failed);
@@ -363,6 +375,7 @@ FL_EXPORT int fl_logprobs(const void* logits, int dtype, int64_t rows, int64_t v
     FL_CHECK(aligned(logits, dtype_size(dtype)) && (given == 0 || aligned(tokens, token_bytes)) && aligned(logprob, 4) && aligned(logsumexp, 4) && aligned(entropy, 4) &&
                  aligned(top_ids, 4) && aligned(top_logprobs, 4), FL_ERR_INVALID, "logprobs: a pointer is not aligned to its type");
     DeviceScope dev;
+    set_up();
     LaunchCtx lc = op_ctx(stream);
     const LogprobArgs a{logits, ld, (int)rows, (int)vocab, 1.f, 1.f, tokens, (int)given, token_bytes == 8, top, given ? logprob : nullptr, logsumexp, entropy, top_ids, top_logprobs};
     if (dtype == FL_DTYPE_F32) run_logprobs<float>(lc, a, temperature);

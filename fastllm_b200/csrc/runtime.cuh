@@ -32,7 +32,6 @@ struct Profiler {
 };
 extern Profiler g_prof;
 int bound_device();             // the device of fl_init; throws before it
-void ops_init();                // fl_ops.cu: what the operators set up once, part of fl_init
 
 // what stands around the body of every entry point
 #define FL_API_BEGIN try {

@@ -107,6 +107,7 @@ SYMBOLS = {
     "fl_quantize_rows": (_I, [_VP, _I, _I64, _I64, _I64, _VP, _I64, _VP, _VP]),
     "fl_linear8_workspace": (_I, [_I64, _I64, _I, C.POINTER(_SZ)]),
     "fl_linear8": (_I, [_VP, _I, _I64, _VP, _VP, _I64, _VP, _VP, _I64, _I64, _I64, _VP, _I, _I64, _VP, _SZ, _VP]),
+    "fl_operators_check": (_I, []),
     "fl_logprobs": (_I, [_VP, _I, _I64, _I64, _I64, _VP, _I, _I64, C.c_double, _I, _VP, _VP, _VP, _VP, _VP, _VP]),
     "fl_embed": (_I, [_VP, _VP, _VP, _I, _I, _VP]),
     "fl_embed_timed": (_I, [_VP, _VP, _VP, _I, _I, _VP, _I, C.POINTER(C.c_float)]),

@@ -5,6 +5,7 @@
 
 #include "../../include/fastllm_b200.h"
 #include "bert_model.cuh"
+#include "failed_word.hpp"
 #include "linear8.cuh"
 #include "logprobs.cuh"
 #include "ops.hpp"
@@ -111,8 +112,9 @@ static void launch_op(LaunchCtx& lc, const char* tag, uint64_t bytes, void (*ker
     else g_launches.fetch_add(1, std::memory_order_relaxed);
 }
 
-// What the operators keep for the process: one page-locked word that a kernel sets when a wait inside it ran out; the next call reports it.
-static int* g_op_failed = nullptr;
+// What the operators keep for the process: one page-locked word that a kernel sets when a wait inside it ran out; the next product or fl_operators_check
+// tells of it, once.
+static FailedWord g_op_failed;
 static int g_pair_clusters = 0;                 // pairs of SMs that can be resident at once
 
 template <int BN>
@@ -161,11 +163,11 @@ static void set_up() {
     int* p = nullptr;
     FL_CUDA(cudaMallocHost(&p, sizeof(int)));
     *p = 0;
-    g_op_failed = p;
+    g_op_failed.word = p;
     done.store(true, std::memory_order_release);
 }
 static void check_op_failed() {
-    FL_CHECK(*reinterpret_cast<volatile int*>(g_op_failed) == 0, FL_ERR_CUDA, "a wait inside an operator's kernel ran out in an earlier call: its results are not valid");
+    FL_CHECK(!g_op_failed.take(), FL_ERR_CUDA, "a wait inside an operator's kernel ran out: a product since the last check is not valid");
 }
 
 template <typename T>
@@ -357,7 +359,7 @@ FL_EXPORT int fl_linear8(const void* x, int x_dtype, int64_t ldx, const float* x
     set_up();
     LaunchCtx lc = op_ctx(stream);
     check_op_failed();
-    run_linear8(lc, x, x_dtype, ldx, x_scale, w, ldw, w_scale, bias, rows, n, k, y, y_dtype, ldy, workspace, g_op_failed);
+    run_linear8(lc, x, x_dtype, ldx, x_scale, w, ldw, w_scale, bias, rows, n, k, y, y_dtype, ldy, workspace, g_op_failed.word);
     FL_API_END
 }
 
@@ -381,6 +383,12 @@ FL_EXPORT int fl_logprobs(const void* logits, int dtype, int64_t rows, int64_t v
     if (dtype == FL_DTYPE_F32) run_logprobs<float>(lc, a, temperature);
     else if (dtype == FL_DTYPE_BF16) run_logprobs<__nv_bfloat16>(lc, a, temperature);
     else run_logprobs<__half>(lc, a, temperature);
+    FL_API_END
+}
+
+FL_EXPORT int fl_operators_check(void) {
+    FL_API_BEGIN
+    check_op_failed();
     FL_API_END
 }
 

@@ -3,6 +3,7 @@
     quantize_rows(x)                          rows as 8-bit whole numbers with a scale each
     linear8(x, weight, weight_scale, bias)    matrix product in 8-bit integers with a scale per token and per channel
     logprobs(logits, tokens, top=K)           log probabilities of given tokens, log-sum-exp, entropy, the K most likely alternatives
+    check()                                   raises when a product that has run is not valid
 
 Thin over the C ABI (include/fastllm_b200.h, "operators on device memory", which states the formulas and what NaN, infinities, padding and
 rows without probabilities give).  Calls are asynchronous, allocate their results (and linear8 its workspace) with torch, and can be captured into a CUDA graph.
@@ -143,6 +144,12 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, b
     if rc:
         _lib.check(rc)
     return out
+
+
+def check():
+    """Raises FastllmError when a product since the last check gave up on a wait inside its kernel, once (fl_operators_check; the next linear8 would raise it too).
+    To be asked after a synchronize, or after the replay of a graph has been waited for."""
+    _lib.check(_lib.load().fl_operators_check())
 
 
 class LogProbs(NamedTuple):

@@ -410,6 +410,10 @@ FL_EXPORT int fl_quantize_rows(const void* x, int dtype, int64_t rows, int64_t c
 FL_EXPORT int fl_linear8_workspace(int64_t rows, int64_t k, int x_dtype, size_t* bytes);
 FL_EXPORT int fl_linear8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
                          int64_t rows, int64_t n, int64_t k, void* y, int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
+/* Whether all products that have run are valid.  Waits inside their kernels have a limit; a product that gave up on one has returned FL_OK long before, and its
+ * result is not valid.  FL_ERR_CUDA: one of those since the last check was such; told once, by this call or by the next fl_linear8, which then does nothing else,
+ * to whichever thread asks first.  To be asked after waiting for the work in question, a replayed graph's too. */
+FL_EXPORT int fl_operators_check(void);
 /* Log probabilities over logits [rows, vocab] (f32, bf16, f16), z = logits / temperature:
  *     logsumexp = log sum exp z,   logprob[r, j] = z[tokens[r, j]] - logsumexp,   entropy = -sum p log p,
  * and the `top` (0 to 32) largest logits of a row in falling order, the lowest index first among equals: top_ids, top_logprobs [rows, top].

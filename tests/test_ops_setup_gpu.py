@@ -57,3 +57,18 @@ threads = [threading.Thread(target=work, args=(i, n)) for i in range(2) for n in
 assert len(got) == 10 and all(same(y, calls[n]()) for (_, n), y in got.items())
 print("same")
 """)
+
+
+def test_products_that_ran_are_valid():
+    """by calls and by a replayed graph"""
+    _run("""
+got = [calls[n]() for n in ("token", "few", "pair")]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    again = [calls[n]() for n in ("token", "few", "pair")]
+graph.replay()
+torch.cuda.synchronize()
+ops.check()
+assert all(same(a, b) for a, b in zip(got, again))
+print("same")
+""")

@@ -965,7 +965,7 @@ static void ensure_ws(fl_cache& c, size_t T, size_t n_want) {
         drop_graphs(c);
         const size_t N = std::max<size_t>(n_want, 2 * y.want_cap);
         y.hf.alloc(N * m.W); y.logits.alloc(N * m.V);
-        if (m.cfg.head_bits == 8) y.head8_ws.alloc(N * padded8(m.W) + 256 + N * 4);        // (linear8_workspace of any number of rows up to N)
+        if (m.cfg.head_bits == 8) y.head8_ws.alloc(linear8_workspace(N, m.W));       // (no less than of fewer rows)
         if (!m.f32) { y.hf_hi.alloc(N * m.W); y.hf_lo.alloc(N * m.W); }
         y.want_cap = N;
     }
@@ -2106,7 +2106,7 @@ static void enqueue_step(fl_cache& c, LaunchCtx& lc, const StepTab& st, const in
                eps, W, m.cfg.logit_scale != 0.f ? m.cfg.logit_scale : 1.f, y.hf.p,
                m.tc_head ? y.hf_hi.p : (uint16_t*)nullptr, y.hf_lo.p);
         if (m.cfg.head_bits == 8)
-            op_linear8(lc, y.hf.p, m.head8.p, m.head8_scale.p, n_want, m.V, W, y.logits.p, y.head8_ws.p, c.step_failed.p);
+            op_linear8(lc, y.hf.p, m.head8.p, m.head8_scale.p, n_want, m.V, W, y.logits.p, y.head8_ws.p, y.head8_ws.n, c.step_failed.p);
         else
             gemm_tc_or_exact(c, lc, "gemm_head", y.hf.p, m.tc_head ? y.hf_hi.p : nullptr, y.hf_lo.p, m.head, m.tm_head, m.tc_head, m.V, W, y.logits.p, n_want);
         if (m.cfg.logit_softcap > 0.f) {

@@ -291,7 +291,8 @@ void op_quantize_rows(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int
     set_up();
     quantize_rows(lc, x, dtype, rows, cols, ldx, q, ldq, ldq, scale);
 }
-void op_linear8(LaunchCtx& lc, const float* x, const int8_t* w, const float* w_scale, int64_t rows, int64_t n, int64_t k, float* y, void* workspace, int* failed) {
+void op_linear8(LaunchCtx& lc, const float* x, const int8_t* w, const float* w_scale, int64_t rows, int64_t n, int64_t k, float* y, void* workspace, size_t workspace_bytes, int* failed) {
+    FL_CHECK(workspace_bytes >= linear8_workspace(rows, k), FL_ERR_INVALID, "linear8: the workspace is smaller than the product needs");
     set_up();
     run_linear8(lc, x, FL_DTYPE_F32, k, nullptr, w, padded8(k), w_scale, nullptr, rows, n, k, y, FL_DTYPE_F32, n, workspace, failed);
 }

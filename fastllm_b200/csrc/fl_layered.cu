@@ -197,7 +197,8 @@ void layered_build(LayeredModel& m, const fl_layer_desc* descs) {
     auto reg = [&](auto** pp, size_t bytes) { regs.push_back({(void**)pp, bytes}); };
     const size_t W = m.W;
     reg(&m.embed, (size_t)m.V * W * 2); reg(&m.final_norm, W * 4);
-    if (!c.tied_head) reg(&m.head, (size_t)m.V * W * 2);
+    const bool head_goes = !c.tied_head && c.head_bits == 8;        // the 16-bit matrix is given back once it has been rounded
+    if (!c.tied_head && !head_goes) reg(&m.head, (size_t)m.V * W * 2);
     if (c.embed_norm) reg(&m.embed_norm, W * 4);
     if (c.norm_tanh) { reg(&m.final_bias, W * 4); reg(&m.final_alpha, 4); }
     if (c.bigram_buckets > 0) reg(&m.bigram, ((size_t)c.bigram_buckets + 1) * W * 2);
@@ -399,7 +400,11 @@ void layered_build(LayeredModel& m, const fl_layer_desc* descs) {
     size_t off = 0;
     for (const Reg& r : regs) { *r.pp = m.slab.p + off; off += up256(r.bytes); }
     if (c.tied_head) m.head = m.embed;
-    m.weight_bytes = total - (c.tied_head ? 0 : up256((size_t)m.V * W * 2)) - (c.max_positions > 0 ? up256((size_t)c.max_positions * W * 2) : 0) -
+    if (head_goes) {
+        m.head16.alloc((size_t)m.V * W, /*zero=*/true);
+        m.head = m.head16.p;
+    }
+    m.weight_bytes = total + (head_goes ? up256((size_t)m.V * W * 2) : 0) - (c.tied_head ? 0 : up256((size_t)m.V * W * 2)) - (c.max_positions > 0 ? up256((size_t)c.max_positions * W * 2) : 0) -
                      (m.bigram ? up256(((size_t)c.bigram_buckets + 1) * W * 2) : 0) - (m.side_embed ? up256((size_t)m.V * m.L * c.token_side * 2) : 0);
 
     // names -> destinations
@@ -723,6 +728,10 @@ void layered_finalize(LayeredModel& m) {
         LaunchCtx lc;
         op_quantize_rows(lc, m.head, FL_DTYPE_BF16, m.V, m.W, m.W, m.head8.p, ld, m.head8_scale.p);
         FL_CUDA(cudaStreamSynchronize(lc.stream));
+        if (!m.cfg.tied_head) {
+            m.head16.release();
+            m.head = nullptr;
+        }
         m.weight_bytes -= (uint64_t)m.V * m.W;          // (a byte a weight instead of two)
     }
     m.finalized = true;

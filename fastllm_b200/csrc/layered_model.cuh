@@ -126,6 +126,7 @@ struct LayeredModel {
     bool tc_head = false;
     DevBuf<int8_t> head8;               // head_bits = 8: [V, padded8(W)] and a scale per row
     DevBuf<float> head8_scale;
+    DevBuf<uint16_t> head16;            // head_bits = 8 and no tied embedding: the matrix as it came, until the model is finalized
     std::set<std::string> have;
     std::vector<std::string> expected;
     int ignored = 0;

@@ -8,13 +8,25 @@
 `generate` loads the model the registry picks for DIR/config.json and continues every prompt (token ids in, token ids out: the
 tokenizer stays with the server above this library) through the continuous batcher; one JSON line per prompt, with --logprobs also every
 token's log probability and its K most likely alternatives.  `score` prints, per text, the log probability of every token but the first given
-those before it (layered models).  --head-bits 8: output projection in 8-bit integers (layered models, bf16).
+those before it (layered models); a number that is none, as that of a token of probability 0, is null.  --head-bits 8: output projection in 8-bit integers (layered models, bf16).
 """
 from __future__ import annotations
 
 import argparse
 import json
+import math
 import sys
+
+
+def _json(value) -> str:
+    """JSON has no infinities and no NaN (a token of probability 0, a row without probabilities): null"""
+    def plain(v):
+        if isinstance(v, float):
+            return v if math.isfinite(v) else None
+        if isinstance(v, dict):
+            return {k: plain(x) for k, x in v.items()}
+        return [plain(x) for x in v] if isinstance(v, (list, tuple)) else v
+    return json.dumps(plain(value), allow_nan=False)
 
 
 def _generate(argv) -> int:
@@ -43,7 +55,7 @@ def _generate(argv) -> int:
         got, told = got
     for p, ids, about in zip(prompts, got, told):
         line = {"prompt": p, "generated": [int(t) for t in ids]}
-        print(json.dumps(line if about is None else {**line, "logprobs": about}))
+        print(_json(line if about is None else {**line, "logprobs": about}))
     return 0
 
 
@@ -65,7 +77,7 @@ def _score(argv) -> int:
         line = {"ids": t, "logprobs": [float(v) for v in s.logprobs], "total": s.total}
         if a.top:
             line["top"] = [[(int(i), float(v)) for i, v in zip(*row)] for row in zip(s.top_ids, s.top_logprobs)]
-        print(json.dumps(line))
+        print(_json(line))
     return 0
 
 

@@ -2034,13 +2034,19 @@ FL_EXPORT int fl_cache_logprobs(fl_cache* c, int rows, const int32_t* tokens, in
     FL_CHECK(given <= (1 << 20) && top <= 32 && (size_t)top <= V, FL_ERR_INVALID, "from 0 to 32 alternatives, no more than the vocabulary has, and at most 2^20 given tokens a row");
     if (rows == 0) return FL_OK;
     use_device();
+    const size_t n = (size_t)rows * 4, tok = n * given, res = n * (given + 2 + 2 * (size_t)top);
+    const bool grows = c->lp_dev.n < tok + res || c->lp_host.n < tok + res;      // (the second: after an allocation that failed)
     try {
-        const size_t n = (size_t)rows * 4, tok = n * given, res = n * (given + 2 + 2 * (size_t)top);
-        if (c->lp_dev.n < tok + res || c->lp_host.n < tok + res) {      // (the second: after an allocation that failed)
-            FL_CUDA(cudaStreamSynchronize(c->stream));
-            c->lp_host.alloc(tok + res);
-            c->lp_dev.alloc(tok + res);
-        }
+        if (grows) FL_CUDA(cudaStreamSynchronize(c->stream));
+    } catch (const fl::Error&) {
+        c->poisoned = true;
+        throw;
+    }
+    if (grows) {            // (memory that cannot be had does not cost the cache)
+        c->lp_host.alloc(tok + res);
+        c->lp_dev.alloc(tok + res);
+    }
+    try {
         if (tok > 0) {
             std::memcpy(c->lp_host.p, tokens, tok);
             FL_CUDA(cudaMemcpyAsync(c->lp_dev.p, c->lp_host.p, tok, cudaMemcpyHostToDevice, c->stream));

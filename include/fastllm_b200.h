@@ -393,7 +393,7 @@ FL_EXPORT int fl_forward_sample_device(fl_model* m, fl_cache* c, const uint32_t*
 /* ---- operators on device memory (no reference counterpart) ---------------------------------------
  * Pointers are memory of the device that fl_init bound, strides are counted in elements between rows, the last dimension is dense.
  * `stream` is a cudaStream_t (NULL: the default stream).  A call checks its arguments on the host, launches on that stream and returns:
- * it neither allocates nor waits, keeps nothing of its arguments, may be captured into a CUDA graph, and runs beside other calls on
+ * it neither allocates nor waits (but the process's first one, which loads the operators' kernels, also inside a capture), keeps nothing of its arguments, may be captured into a CUDA graph, and runs beside other calls on
  * other streams as long as they do not share a workspace or an output.  Calls of zero rows do nothing.
  *
  * fl_quantize_rows: rows of f32, bf16 or f16 [rows, cols] as whole numbers of 8 bits and a scale: with a = max |x| of the row,

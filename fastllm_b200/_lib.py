@@ -18,7 +18,7 @@ FL_ACT = {"swish_clamp": 0, "gelu_tanh": 1, "relu2": 2, "relu": 3, "silu": 4}
 FL_ROT_SCALE = {"yarn": 0, "bands": 1}
 FL_ROUTER = {"softmax": 0, "sigmoid_groups": 1, "softmax_groups": 2}
 FL_FFN = {"none": 0, "dense": 1, "moe": 2}
-FL_DTYPE_F32, FL_DTYPE_BF16, FL_DTYPE_F16, FL_DTYPE_I8 = 0, 1, 2, 3
+FL_DTYPE_F32, FL_DTYPE_BF16, FL_DTYPE_F16, FL_DTYPE_I8, FL_DTYPE_MX4 = 0, 1, 2, 3, 4
 
 
 class FlConfig(C.Structure):
@@ -107,6 +107,13 @@ SYMBOLS = {
     "fl_quantize_rows": (_I, [_VP, _I, _I64, _I64, _I64, _VP, _I64, _VP, _VP]),
     "fl_linear8_workspace": (_I, [_I64, _I64, _I, C.POINTER(_SZ)]),
     "fl_linear8": (_I, [_VP, _I, _I64, _VP, _VP, _I64, _VP, _VP, _I64, _I64, _I64, _VP, _I, _I64, _VP, _SZ, _VP]),
+    "fl_quantize4": (_I, [_VP, _I, _I64, _I64, _I64, _VP, _I64, _VP, _I64, _VP]),
+    "fl_dequantize4": (_I, [_VP, _I64, _VP, _I64, _I64, _I64, _VP, _I, _I64, _VP]),
+    "fl_glu4": (_I, [_VP, _I, _I64, _I64, _I64, _I, C.c_float, _VP, _I64, _VP, _I64, _VP]),
+    "fl_weight4_bytes": (_I, [_I64, _I64, C.POINTER(_SZ)]),
+    "fl_weight4": (_I, [_VP, _I64, _I64, _I64, _VP, _VP]),
+    "fl_linear4_workspace": (_I, [_I64, _I64, _I, C.POINTER(_SZ)]),
+    "fl_linear4": (_I, [_VP, _I, _I64, _VP, _I64, _VP, _I64, _VP, _VP, _I64, _I64, _I64, _VP, _I, _I64, _VP, _SZ, _VP]),
     "fl_operators_check": (_I, []),
     "fl_logprobs": (_I, [_VP, _I, _I64, _I64, _I64, _VP, _I, _I64, C.c_double, _I, _VP, _VP, _VP, _VP, _VP, _VP]),
     "fl_embed": (_I, [_VP, _VP, _VP, _I, _I, _VP]),

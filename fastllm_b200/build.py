@@ -8,7 +8,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libfastllm_b200.so")
-SOURCES = ["fl_lib.cu", "fl_bert.cu", "fl_layered.cu", "fl_ops.cu"]
+SOURCES = ["fl_lib.cu", "fl_bert.cu", "fl_layered.cu", "fl_ops.cu", "fl_ops4.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--expt-relaxed-constexpr",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden", "-Xptxas", "-v"]
 

@@ -1,0 +1,224 @@
+// Operators on rows of 4-bit numbers (include/fastllm_b200.h, "operators on device memory"): argument checks and launches behind the C ABI.
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <mutex>
+
+#include "../../include/fastllm_b200.h"
+#include "linear4.cuh"
+#include "op_launch.cuh"
+#include "ops.hpp"
+
+namespace fl {
+
+constexpr int64_t kMaxCols4 = (int64_t)1 << 20;
+
+static int64_t blocks4(int64_t cols) { return (cols + kR4Block - 1) / kR4Block; }
+static int64_t groups4(int64_t cols) { return 2 * ((blocks4(cols) + 7) / 8); }              // k blocks of 256 values are whole
+static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+// rows that scales in tiles of `tile` rows have room for, in whole 128 rows a tile
+static int64_t slots4(int64_t rows, int tile) { return (rows + tile - 1) / tile * ((tile + 127) / 128 * 128); }
+
+struct Span { dim3 grid; int threads; };
+static Span spans4(int64_t rows, int64_t cols) {
+    const int64_t spans = (cols + kR4Span - 1) / kR4Span;
+    const int warps = (int)std::min<int64_t>(spans, 8);
+    return {dim3((unsigned)rows, (unsigned)((spans + warps - 1) / warps)), 32 * warps};
+}
+template <typename T>
+static bool starts_vec(const void* x, int64_t rows, int64_t ldx) { return aligned(x, 16) && (rows == 1 || ldx * sizeof(T) % 16 == 0); }
+
+// f(T{}) with the element type of a float dtype
+template <typename F>
+static void by_type(int dtype, F f) {
+    if (dtype == FL_DTYPE_F32) f(float{});
+    else if (dtype == FL_DTYPE_BF16) f(__nv_bfloat16{});
+    else f(__half{});
+}
+
+static void quantize4(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, const Rows4Out& o) {
+    const Span s = spans4(rows, o.tile > 0 ? (int64_t)o.groups * 128 : cols);
+    by_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        launch_op(lc, "quantize4", (uint64_t)rows * (cols * sizeof(T) + o.blocks * 17), quantize4_kernel<T>, s.grid, s.threads, 0, 1, false, static_cast<const T*>(x), (long long)ldx, (int)cols,
+                  starts_vec<T>(x, rows, ldx), o);
+    });
+}
+
+size_t weight4_bytes(int64_t n, int64_t k) { return (size_t)(slots4(n, 128) * groups4(k) * 4); }
+static void arrange4(LaunchCtx& lc, const uint8_t* scale, int64_t lds, int64_t rows, int64_t k, int tile, uint8_t* tiles, bool pdl) {
+    const int64_t slots = slots4(rows, tile), groups = groups4(k);
+    launch_op(lc, "arrange4", (uint64_t)(2 * slots * groups * 4), arrange4_kernel, dim3((unsigned)((slots + 127) / 128), (unsigned)groups), 128, 0, 1, pdl, scale, (long long)lds,
+              (long long)rows, (int)blocks4(k), tiles, tile, (int)groups, (long long)slots);
+}
+
+struct Linear4Room { size_t scale = 0, all = 0; };
+static Linear4Room linear4_room(int64_t rows, int64_t k, bool given) {
+    Linear4Room r;
+    r.scale = given ? 0 : up256((size_t)rows * blocks4(k) * 16);
+    r.all = r.scale + (size_t)slots4(rows, 128) * groups4(k) * 4;
+    return r;
+}
+size_t linear4_workspace(int64_t rows, int64_t k) { return linear4_room(rows, k, false).all; }
+
+// x in 4 bits: lds its scales' row stride; else their type's
+static void run_linear4(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, const uint8_t* x_scale, int64_t lds, const uint8_t* w, int64_t ldw, const uint8_t* w_tiles, const float* bias,
+                        int64_t rows, int64_t n, int64_t k, void* y, int y_dtype, int64_t ldy, void* workspace) {
+    const bool given = x_dtype == FL_DTYPE_MX4;
+    const Linear4Room room = linear4_room(rows, k, given);
+    uint8_t *q = static_cast<uint8_t*>(workspace), *xs = q + room.scale;
+    const int blocks = (int)blocks4(k), groups = (int)groups4(k);
+    if (given) {
+        arrange4(lc, x_scale, lds, rows, k, 128, xs, false);
+    } else {
+        quantize4(lc, x, x_dtype, rows, k, ldx, Rows4Out{q, blocks * 16, xs, 0, blocks, 128, groups});
+    }
+    const Linear4Args a{(int)rows, (int)n, blocks, given ? static_cast<const uint8_t*>(x) : q, given ? ldx : blocks * 16, xs, 128, w, ldw, w_tiles, groups, bias, y, ldy, y_dtype};
+    launch_op(lc, "linear4", (uint64_t)(n + rows) * blocks * 17 + rows * n * dtype_size(y_dtype), linear4_plain_kernel, dim3((unsigned)((n + 31) / 32), (unsigned)((rows + 31) / 32)), 256, 0, 1,
+              false, a);
+}
+
+// One-time set-up on the bound device, by the first call that launches an operator.  It also loads the kernels, so that this call may be one inside a graph capture.
+static void set_up() {
+    static std::atomic<bool> done{false};
+    static std::mutex one;
+    if (done.load(std::memory_order_acquire)) return;
+    std::lock_guard<std::mutex> lock(one);
+    if (done.load(std::memory_order_relaxed)) return;
+    RelaxedCapture relaxed;
+    for (int dtype : {FL_DTYPE_F32, FL_DTYPE_BF16, FL_DTYPE_F16})
+        by_type(dtype, [](auto t) { load_kernels(quantize4_kernel<decltype(t)>); load_kernels(dequantize4_kernel<decltype(t)>); load_kernels(glu4_kernel<decltype(t)>); });
+    load_kernels(arrange4_kernel);
+    load_kernels(linear4_plain_kernel);
+    done.store(true, std::memory_order_release);
+}
+
+static void check_rows4(const char* what, const void* q, int64_t ldq, const void* scale, int64_t lds, int64_t rows, int64_t cols) {
+    FL_CHECK(rows <= 1 || (ldq >= 16 * blocks4(cols) && lds >= blocks4(cols)), FL_ERR_INVALID, std::string(what) + ": a row stride of the 4-bit rows or their scales is smaller than the row");
+    FL_CHECK(aligned(q, 16) && (rows <= 1 || ldq % 16 == 0), FL_ERR_INVALID, std::string(what) + ": 4-bit rows start on 16-byte borders (pointer and row stride)");
+}
+
+}  // namespace fl
+
+using namespace fl;
+
+extern "C" {
+
+FL_EXPORT int fl_quantize4(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, void* stream) {
+    FL_API_BEGIN
+    FL_CHECK(is_float(dtype), FL_ERR_INVALID, "quantize4: rows of f32, bf16 or f16");
+    FL_CHECK(rows >= 0 && rows <= kMaxRows && cols >= 1 && cols <= kMaxCols4, FL_ERR_INVALID, "quantize4: rows from 0 to 2^30, columns from 1 to 2^20");
+    FL_CHECK(rows <= 1 || ldx >= cols, FL_ERR_INVALID, "quantize4: the row stride is smaller than the row");
+    if (rows == 0) return FL_OK;
+    FL_CHECK(x && q && scale, FL_ERR_INVALID, "NULL argument");
+    FL_CHECK(aligned(x, dtype_size(dtype)), FL_ERR_INVALID, "quantize4: a pointer is not aligned to its type");
+    check_rows4("quantize4", q, ldq, scale, lds, rows, cols);
+    DeviceScope dev;
+    set_up();
+    LaunchCtx lc = op_ctx(stream);
+    quantize4(lc, x, dtype, rows, cols, ldx, Rows4Out{q, ldq, scale, lds, (int)blocks4(cols), 0, 0});
+    FL_API_END
+}
+
+FL_EXPORT int fl_dequantize4(const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds, int64_t rows, int64_t cols, void* y, int dtype, int64_t ldy, void* stream) {
+    FL_API_BEGIN
+    FL_CHECK(is_float(dtype), FL_ERR_INVALID, "dequantize4: results are f32, bf16 or f16");
+    FL_CHECK(rows >= 0 && rows <= kMaxRows && cols >= 1 && cols <= kMaxCols4, FL_ERR_INVALID, "dequantize4: rows from 0 to 2^30, columns from 1 to 2^20");
+    FL_CHECK(rows <= 1 || ldy >= cols, FL_ERR_INVALID, "dequantize4: the row stride is smaller than the row");
+    if (rows == 0) return FL_OK;
+    FL_CHECK(q && scale && y, FL_ERR_INVALID, "NULL argument");
+    FL_CHECK(aligned(y, dtype_size(dtype)), FL_ERR_INVALID, "dequantize4: a pointer is not aligned to its type");
+    check_rows4("dequantize4", q, ldq, scale, lds, rows, cols);
+    DeviceScope dev;
+    set_up();
+    LaunchCtx lc = op_ctx(stream);
+    const Span s = spans4(rows, cols);
+    by_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        launch_op(lc, "dequantize4", (uint64_t)rows * (cols * sizeof(T) + blocks4(cols) * 17), dequantize4_kernel<T>, s.grid, s.threads, 0, 1, false, q, (long long)ldq, scale, (long long)lds,
+                  (int)cols, static_cast<T*>(y), (long long)ldy, starts_vec<T>(y, rows, ldy));
+    });
+    FL_API_END
+}
+
+FL_EXPORT int fl_glu4(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int act, float limit, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, void* stream) {
+    FL_API_BEGIN
+    FL_CHECK(is_float(dtype), FL_ERR_INVALID, "glu4: rows of f32, bf16 or f16");
+    FL_CHECK(act == FL_ACT_SILU || act == FL_ACT_GELU_TANH || act == FL_ACT_RELU || act == FL_ACT_SWISH_CLAMP, FL_ERR_INVALID, "glu4: the activation is silu, gelu_tanh, relu or swish_clamp");
+    FL_CHECK(act != FL_ACT_SWISH_CLAMP || (limit > 0 && std::isfinite(limit)), FL_ERR_INVALID, "glu4: the limit is a positive number");
+    FL_CHECK(rows >= 0 && rows <= kMaxRows && cols >= 1 && cols <= kMaxCols4, FL_ERR_INVALID, "glu4: rows from 0 to 2^30, columns from 1 to 2^20");
+    FL_CHECK(rows <= 1 || ldx >= 2 * cols, FL_ERR_INVALID, "glu4: the row stride is smaller than the row");
+    if (rows == 0) return FL_OK;
+    FL_CHECK(x && q && scale, FL_ERR_INVALID, "NULL argument");
+    FL_CHECK(aligned(x, dtype_size(dtype)), FL_ERR_INVALID, "glu4: a pointer is not aligned to its type");
+    check_rows4("glu4", q, ldq, scale, lds, rows, cols);
+    DeviceScope dev;
+    set_up();
+    LaunchCtx lc = op_ctx(stream);
+    const Span s = spans4(rows, cols);
+    by_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        const bool vec = starts_vec<T>(x, rows, ldx);
+        launch_op(lc, "glu4", (uint64_t)rows * (2 * cols * sizeof(T) + blocks4(cols) * 17), glu4_kernel<T>, s.grid, s.threads, 0, 1, false, static_cast<const T*>(x), (long long)ldx, (int)cols, vec,
+                  vec && cols * sizeof(T) % 16 == 0, act, limit, Rows4Out{q, ldq, scale, lds, (int)blocks4(cols), 0, 0});
+    });
+    FL_API_END
+}
+
+FL_EXPORT int fl_weight4_bytes(int64_t n, int64_t k, size_t* bytes) {
+    FL_API_BEGIN
+    FL_CHECK(bytes, FL_ERR_INVALID, "NULL argument");
+    FL_CHECK(n >= 1 && n <= kMaxRows && k >= 1 && k <= kMaxCols4, FL_ERR_INVALID, "weight4: n from 1 to 2^30, k from 1 to 2^20");
+    *bytes = weight4_bytes(n, k);
+    FL_API_END
+}
+
+FL_EXPORT int fl_weight4(const uint8_t* scale, int64_t lds, int64_t n, int64_t k, void* tiles, void* stream) {
+    FL_API_BEGIN
+    FL_CHECK(n >= 1 && n <= kMaxRows && k >= 1 && k <= kMaxCols4, FL_ERR_INVALID, "weight4: n from 1 to 2^30, k from 1 to 2^20");
+    FL_CHECK(n == 1 || lds >= blocks4(k), FL_ERR_INVALID, "weight4: the row stride is smaller than the row");
+    FL_CHECK(scale && tiles, FL_ERR_INVALID, "NULL argument");
+    FL_CHECK(aligned(tiles, 16), FL_ERR_INVALID, "weight4: the result starts on a 16-byte border");
+    DeviceScope dev;
+    set_up();
+    LaunchCtx lc = op_ctx(stream);
+    arrange4(lc, scale, lds, n, k, 128, static_cast<uint8_t*>(tiles), false);
+    FL_API_END
+}
+
+FL_EXPORT int fl_linear4_workspace(int64_t rows, int64_t k, int x_dtype, size_t* bytes) {
+    FL_API_BEGIN
+    FL_CHECK(bytes, FL_ERR_INVALID, "NULL argument");
+    FL_CHECK(is_float(x_dtype) || x_dtype == FL_DTYPE_MX4, FL_ERR_INVALID, "linear4: activations are f32, bf16, f16 or 4-bit rows");
+    FL_CHECK(rows >= 0 && rows <= kMaxRows && k >= 1 && k <= kMaxCols4, FL_ERR_INVALID, "linear4: rows from 0 to 2^30, k from 1 to 2^20");
+    *bytes = linear4_room(rows, k, x_dtype == FL_DTYPE_MX4).all;
+    FL_API_END
+}
+
+FL_EXPORT int fl_linear4(const void* x, int x_dtype, int64_t ldx, const uint8_t* x_scale, int64_t lds, const uint8_t* w, int64_t ldw, const void* w_tiles, const float* bias, int64_t rows,
+                         int64_t n, int64_t k, void* y, int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
+    FL_API_BEGIN
+    const bool given = x_dtype == FL_DTYPE_MX4;
+    FL_CHECK(is_float(x_dtype) || given, FL_ERR_INVALID, "linear4: activations are f32, bf16, f16 or 4-bit rows");
+    FL_CHECK(is_float(y_dtype), FL_ERR_INVALID, "linear4: results are f32, bf16 or f16");
+    FL_CHECK(rows >= 0 && rows <= kMaxRows && n >= 1 && n <= kMaxRows && k >= 1 && k <= kMaxCols4, FL_ERR_INVALID, "linear4: rows from 0 to 2^30, n from 1 to 2^30, k from 1 to 2^20");
+    FL_CHECK((rows <= 1 || (ldx >= (given ? 16 * blocks4(k) : k) && ldy >= n)) && (n == 1 || ldw >= 16 * blocks4(k)), FL_ERR_INVALID, "linear4: a row stride is smaller than the row");
+    if (rows == 0) return FL_OK;
+    FL_CHECK(x && w && w_tiles && y, FL_ERR_INVALID, "NULL argument");
+    FL_CHECK(given == (x_scale != nullptr), FL_ERR_INVALID, "linear4: x_scale comes with activations of 4 bits, and only with them");
+    FL_CHECK(aligned(w, 16) && (n == 1 || ldw % 16 == 0), FL_ERR_INVALID, "linear4: the weight's rows start on 16-byte borders (pointer and row stride)");
+    FL_CHECK(aligned(w_tiles, 16), FL_ERR_INVALID, "linear4: the weight's scales start on a 16-byte border");
+    if (given) check_rows4("linear4", x, ldx, x_scale, lds, rows, k);
+    FL_CHECK((given || aligned(x, dtype_size(x_dtype))) && aligned(y, dtype_size(y_dtype)) && aligned(bias, 4), FL_ERR_INVALID, "linear4: a pointer is not aligned to its type");
+    FL_CHECK(rows <= ((int64_t)1 << 40) / n, FL_ERR_INVALID, "linear4: more than 2^40 results");
+    const Linear4Room room = linear4_room(rows, k, given);
+    FL_CHECK(workspace && aligned(workspace, 256) && workspace_bytes >= room.all, FL_ERR_INVALID,
+             "linear4: the workspace is smaller than fl_linear4_workspace asks for, or not on a 256-byte border");
+    DeviceScope dev;
+    set_up();
+    LaunchCtx lc = op_ctx(stream);
+    run_linear4(lc, x, x_dtype, ldx, x_scale, lds, w, ldw, static_cast<const uint8_t*>(w_tiles), bias, rows, n, k, y, y_dtype, ldy, workspace);
+    FL_API_END
+}
+
+}  // extern "C"

@@ -5,19 +5,10 @@
 // into tiles of any multiple of 32.  Scales are applied to the finished sum in f32: the sum rounded once (2^-24), two products, the bias, then
 // one rounding to the result's type.
 #pragma once
-#include <cuda_fp16.h>
-
 #include "gemm_pair.cuh"
+#include "op_values.cuh"
 
 namespace fl {
-
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T from_f32(float v);
-template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
 // One row's rounding rule: q = 127 x / a to the nearest whole number, halves to the even one, of the exact quotient (a = max |x|).
 // x * (127 / a) in f32 is off by at most 127 * 2^-23 = 1.5e-5, so only quotients that lie within 1e-4 of a half need the exact sign of
@@ -60,9 +51,6 @@ struct RowScale {
         return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     }
 };
-// larger for every NaN than for an infinity, and for that than for any number
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-
 // A block per row; columns [cols, cols_q) of q are filled with zeros.  kVecs > 0: the row starts on 16-byte borders on both sides (8 for q) and has at
 // most kThreads * kVecs vectors of 16 bytes, which stay in registers between the maximum and the rounding; -1: such a row of any length, read
 // again for the rounding, from L2 or nearer (1531 x 14336 15.9 us with eight vectors a thread in registers, 19.0 so; 8192 x 8192 f16 34.6, 5.8 TB/s); 0: any row.

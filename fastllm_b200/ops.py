@@ -2,11 +2,14 @@
 
     quantize_rows(x)                          rows as 8-bit whole numbers with a scale each
     linear8(x, weight, weight_scale, bias)    matrix product in 8-bit integers with a scale per token and per channel
+    quantize4(x), dequantize4(q, scale)       rows as 4-bit numbers with a scale per 32 neighbours (MXFP4), and back
+    glu4(x, act)                              a feed-forward's gated activation, ending in 4-bit rows
+    weight4(q, scale), linear4(x, weight)     matrix product of 4-bit rows
     logprobs(logits, tokens, top=K)           log probabilities of given tokens, log-sum-exp, entropy, the K most likely alternatives
     check()                                   raises when a product that has run is not valid
 
 Thin over the C ABI (include/fastllm_b200.h, "operators on device memory", which states the formulas and what NaN, infinities, padding and
-rows without probabilities give).  Calls are asynchronous, allocate their results (and linear8 its workspace) with torch, and can be captured into a CUDA graph.
+rows without probabilities give).  Calls are asynchronous, allocate their results (and linear8 and linear4 their workspace) with torch, and can be captured into a CUDA graph.
 No autograd: results do not require gradients.
 """
 from __future__ import annotations
@@ -141,6 +144,169 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, b
         work_ptr = work.data_ptr()
     rc = lib.fl_linear8(x2.data_ptr(), x_type, x2.stride(0), xs_ptr, weight.data_ptr(), ldw, ws_ptr, bias_ptr, rows, n, k, y2.data_ptr(), y_type, ldy, work_ptr, room,
                         _stream(dev))
+    if rc:
+        _lib.check(rc)
+    return out
+
+
+def _rows4(q: torch.Tensor, scale: torch.Tensor, dev: int, what: str, name: str):
+    """4-bit rows [..., 16 blocks] and their scales [..., blocks] as matrices"""
+    if q.dtype != torch.uint8 or scale.dtype != torch.uint8 or q.ndim == 0 or scale.ndim == 0 or q.shape[:-1] != scale.shape[:-1] or q.shape[-1] != 16 * scale.shape[-1]:
+        _refuse(f"{what}: {name} are uint8 rows of 16 bytes per block with a uint8 scale per block, got {q.dtype} {tuple(q.shape)} and {scale.dtype} {tuple(scale.shape)}")
+    if scale.shape[-1] == 0:
+        _refuse(f"{what}: {name} have no columns")
+    _same(dev, q, what, name)
+    _same(dev, scale, what, f"the scales of {name}")
+    return _rows(q, what), _rows(scale, what)
+
+
+def _new_rows4(x: torch.Tensor, rows: int, cols: int, lead):
+    """room for 4-bit rows and their scales, in one piece of memory: (q, scale)"""
+    blocks = (cols + 31) // 32
+    mem = x.new_empty(rows * blocks * 17, dtype=torch.uint8)
+    q, scale = mem.as_strided((rows, 16 * blocks), (16 * blocks, 1), 0), mem.as_strided((rows, blocks), (blocks, 1), 16 * rows * blocks)
+    return (q, scale) if len(lead) == 1 else (q.view(lead + (16 * blocks,)), scale.view(lead + (blocks,)))
+
+
+def quantize4(x: torch.Tensor):
+    """[..., cols] f32 / bf16 / f16 -> (q uint8 [..., 16 blocks], scale uint8 [..., blocks]), blocks = cols / 32 rounded up: two e2m1 numbers a byte, the even column in
+    the low half, and a power of two 2^(scale - 127) per block of 32 neighbours (OCP Microscaling, MXFP4).  What the last block has behind the row is zero."""
+    what = "quantize4"
+    if x.dtype not in _FLOATS:
+        _refuse(f"{what}: f32, bf16 or f16 rows are wanted, got {x.dtype}")
+    dev = _device(x, what)
+    x2 = _rows(x, what)
+    rows, cols = x2.shape
+    q, scale = _new_rows4(x, rows, cols, x.shape[:-1])
+    rc = _lib.load().fl_quantize4(x2.data_ptr(), _FLOATS[x.dtype], rows, cols, x2.stride(0), q.data_ptr(), 16 * scale.shape[-1], scale.data_ptr(), scale.shape[-1], _stream(dev))
+    if rc:
+        _lib.check(rc)
+    return q, scale
+
+
+def dequantize4(q: torch.Tensor, scale: torch.Tensor, cols: Optional[int] = None, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The numbers that 4-bit rows stand for, [..., cols], rounded once to f32, bf16 or f16.  cols: how many of a row's columns (default: those of all its blocks)."""
+    what = "dequantize4"
+    if dtype not in _FLOATS:
+        _refuse(f"{what}: results are f32, bf16 or f16, got {dtype}")
+    dev = _device(q, what)
+    q2, s2 = _rows4(q, scale, dev, what, "the rows")
+    most = 32 * scale.shape[-1]
+    cols = most if cols is None else cols
+    if not most - 32 < cols <= most:
+        _refuse(f"{what}: rows of {scale.shape[-1]} blocks have from {most - 31} to {most} columns, not {cols}")
+    y = q.new_empty(q.shape[:-1] + (cols,), dtype=dtype)
+    rc = _lib.load().fl_dequantize4(q2.data_ptr(), q2.stride(0), s2.data_ptr(), s2.stride(0), len(q2), cols, y.data_ptr(), _FLOATS[dtype], cols, _stream(dev))
+    if rc:
+        _lib.check(rc)
+    return y
+
+
+_GATED = {"silu": _lib.FL_ACT["silu"], "gelu_tanh": _lib.FL_ACT["gelu_tanh"], "relu": _lib.FL_ACT["relu"], "swish_clamp": _lib.FL_ACT["swish_clamp"]}
+
+
+def glu4(x: torch.Tensor, act: str = "silu", *, limit: float = 7.0):
+    """x [..., 2 cols] f32 / bf16 / f16, a row the gates and behind them the ups: h = act(gate) * up as 4-bit rows, (q, scale) as quantize4 gives them; each h is rounded
+    once.  act: "silu", "gelu_tanh", "relu", or "swish_clamp" with c = min(gate, limit): c / (1 + exp(-1.702 c)) * (clamp(up, -limit, limit) + 1)."""
+    what = "glu4"
+    if x.dtype not in _FLOATS:
+        _refuse(f"{what}: f32, bf16 or f16 rows are wanted, got {x.dtype}")
+    if act not in _GATED:
+        _refuse(f"{what}: the activation is one of {', '.join(_GATED)}, got {act!r}")
+    dev = _device(x, what)
+    x2 = _rows(x, what)
+    rows, both = x2.shape
+    if both % 2:
+        _refuse(f"{what}: a row holds as many gates as ups, got {both} numbers")
+    q, scale = _new_rows4(x, rows, both // 2, x.shape[:-1])
+    rc = _lib.load().fl_glu4(x2.data_ptr(), _FLOATS[x.dtype], rows, both // 2, x2.stride(0), _GATED[act], limit, q.data_ptr(), 16 * scale.shape[-1], scale.data_ptr(), scale.shape[-1],
+                             _stream(dev))
+    if rc:
+        _lib.check(rc)
+    return q, scale
+
+
+class Weight4(NamedTuple):
+    q: torch.Tensor             # uint8 [n, 16 blocks], as given
+    tiles: torch.Tensor         # the scales in the order that linear4 takes them
+    scale: torch.Tensor         # uint8 [n, blocks], as given
+
+
+def weight4(q: torch.Tensor, scale: torch.Tensor) -> Weight4:
+    """A weight of linear4 from 4-bit rows [n, 16 blocks] and their scales [n, blocks] (a checkpoint's, or quantize4's): the scales laid out once.  The rows are not copied."""
+    what = "weight4"
+    if q.ndim != 2:
+        _refuse(f"{what}: the weight is a matrix of 4-bit rows, got {tuple(q.shape)}")
+    dev = _device(q, what)
+    q2, s2 = _rows4(q, scale, dev, what, "the weight's rows")
+    n, blocks = s2.shape
+    if n == 0:
+        _refuse(f"{what}: the weight has no rows")
+    tiles = q.new_empty((n + 127) // 128 * ((blocks + 7) // 8) * 1024)
+    _lib.check(_lib.load().fl_weight4(s2.data_ptr(), s2.stride(0), n, 32 * blocks, tiles.data_ptr(), _stream(dev)))
+    return Weight4(q, tiles, scale)
+
+
+def _room4(rows: int, blocks: int, given: bool) -> int:
+    """fl_linear4_workspace's rule"""
+    return (0 if given else (rows * blocks * 16 + 255) // 256 * 256) + (rows + 127) // 128 * ((blocks + 7) // 8) * 1024
+
+
+def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = None, *, x_scale: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+            out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y[..., i] = sum_j x[..., j] w[i, j] (+ bias[i]) over the numbers that 4-bit rows stand for, the sum in f32, rounded once.
+
+    x [..., k]: f32 / bf16 / f16, rounded to 4-bit rows as quantize4 does; or such rows (uint8 [..., 16 blocks]) with x_scale [..., blocks].  weight: weight4(q, scale) with
+    k / 32 blocks, rounded up.  bias f32 [n] or None.  out_dtype: f32 / bf16 / f16 (default: x's type, f32 for 4-bit rows); out: where the result goes, [..., n] with a
+    dense last dimension, not overlapping an input."""
+    what = "linear4"
+    given = x.dtype == torch.uint8
+    if not given and x.dtype not in _FLOATS:
+        _refuse(f"{what}: activations are f32, bf16, f16 or 4-bit rows (uint8), got {x.dtype}")
+    if not isinstance(weight, Weight4):
+        _refuse(f"{what}: the weight is what weight4 gives, got {type(weight).__name__}")
+    dev = x.get_device()
+    if dev != _bound[0]:
+        _device(x, what)
+    n, blocks = weight.scale.shape
+    if weight.q.get_device() != dev:
+        _same(dev, weight.q, what, "the weight")
+    xs_ptr, lds = None, 0
+    if given:
+        if x_scale is None:
+            _refuse(f"{what}: 4-bit rows come with their x_scale")
+        x2, s2 = _rows4(x, x_scale, dev, what, "the activations")
+        xs_ptr, lds, k, x_type = s2.data_ptr(), s2.stride(0), 32 * s2.shape[1], _lib.FL_DTYPE_MX4
+    else:
+        if x_scale is not None:
+            _refuse(f"{what}: x_scale comes with activations of 4 bits, and only with them")
+        x2, x_type = (x if x.ndim == 2 and x.stride(1) == 1 else _rows(x, what)), _FLOATS[x.dtype]
+        k = x2.shape[1]
+    rows = x2.shape[0]
+    if (k + 31) // 32 != blocks:
+        _refuse(f"{what}: the weight has {blocks} blocks of 32 columns, the activations have {k} columns")
+    bias_ptr = None if bias is None else _vector(bias, n, dev, what, "bias")
+    lead = x.shape[:-1]
+    if out is not None:
+        if out.shape != lead + (n,) or (out_dtype is not None and out.dtype != out_dtype):
+            _refuse(f"{what}: out is {tuple(lead + (n,))}, got {tuple(out.shape)} {out.dtype}")
+        _same(dev, out, what, "out")
+        out_dtype = out.dtype
+    elif out_dtype is None:
+        out_dtype = torch.float32 if given else x.dtype
+    y_type = _FLOATS.get(out_dtype)
+    if y_type is None:
+        _refuse(f"{what}: results are f32, bf16 or f16, got {out_dtype}")
+    if out is None:
+        y2 = x.new_empty((rows, n), dtype=out_dtype)
+        out, ldy = (y2 if x.ndim == 2 else y2.view(lead + (n,))), n
+    else:
+        y2 = _rows(out, what)
+        ldy = y2.stride(0)
+    room = _room4(rows, blocks, given)
+    work = x.new_empty(room, dtype=torch.uint8)
+    rc = _lib.load().fl_linear4(x2.data_ptr(), x_type, x2.stride(0), xs_ptr, lds, weight.q.data_ptr(), weight.q.stride(0), weight.tiles.data_ptr(), bias_ptr, rows, n, k, y2.data_ptr(),
+                                y_type, ldy, work.data_ptr(), room, _stream(dev))
     if rc:
         _lib.check(rc)
     return out

@@ -90,7 +90,7 @@ typedef enum fl_arch {
                               beside a shared expert; hashed bigram rows in the embedding, per-layer token vectors, looped layers */
 } fl_arch;
 
-typedef enum fl_dtype { FL_DTYPE_F32 = 0, FL_DTYPE_BF16 = 1, FL_DTYPE_F16 = 2, FL_DTYPE_I8 = 3 /* operators only */ } fl_dtype;
+typedef enum fl_dtype { FL_DTYPE_F32 = 0, FL_DTYPE_BF16 = 1, FL_DTYPE_F16 = 2, FL_DTYPE_I8 = 3, FL_DTYPE_MX4 = 4 /* the last two: operators only */ } fl_dtype;
 
 /* Mirrors the fields the reference adapters read from config.json
  * (llama.rs:17-29, mistral.rs:78-91, models/config.rs:5-18, models/embeddings.rs:46-54). */
@@ -410,6 +410,31 @@ FL_EXPORT int fl_quantize_rows(const void* x, int dtype, int64_t rows, int64_t c
 FL_EXPORT int fl_linear8_workspace(int64_t rows, int64_t k, int x_dtype, size_t* bytes);
 FL_EXPORT int fl_linear8(const void* x, int x_dtype, int64_t ldx, const float* x_scale, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias,
                          int64_t rows, int64_t n, int64_t k, void* y, int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
+/* Rows of 4-bit numbers with a scale per block of 32 neighbours (OCP Microscaling, MXFP4): a value is e2m1 * 2^(s - 127), e2m1 one of 0, 0.5, 1, 1.5, 2, 3, 4, 6
+ * and their negatives, s the block's byte in `scale` [rows, lds] (lds in bytes).  Two values a byte, the even column in the low half; a row takes 16 bytes per
+ * block, the last block's too, and starts on a 16-byte border (pointer and ldq, in bytes).  s = 255: the block's values are NaN.
+ *
+ * fl_quantize4: rows of f32, bf16 or f16 [rows, cols] as such rows: with a = max |x| of the block, s - 127 = max(floor(log2 a) - 2, -127) and e2m1 = x / 2^(s - 127) to
+ * the nearest one, halves to the even mantissa, beyond 6 to 6.  A block of zeros has s = 0; one with a NaN or an infinity s = 255 and zeros.  What a row's last block
+ * has behind the row is zero.  cols <= 2^20. */
+FL_EXPORT int fl_quantize4(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, void* stream);
+/* The values that such rows stand for, rounded once to y's type (f32, bf16, f16), [rows, cols]. */
+FL_EXPORT int fl_dequantize4(const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds, int64_t rows, int64_t cols, void* y, int dtype, int64_t ldy, void* stream);
+/* A feed-forward's gated activation that ends in such rows: x holds rows [gate | up] of 2 cols numbers, h = act(gate) * up, rounded once as fl_quantize4 does (of the exact h:
+ * next to a border between two numbers it is taken in 64 bits).  act (fl_ffn_act): FL_ACT_SILU g / (1 + e^-g) u; FL_ACT_GELU_TANH g / (1 + e^(-2 sqrt(2/pi) (g + 0.044715
+ * g^3))) u, which is gelu's tanh form; FL_ACT_RELU max(g, 0) u; FL_ACT_SWISH_CLAMP with c = min(g, limit): c / (1 + e^(-1.702 c)) (clamp(u, -limit, limit) + 1).  A block with a
+ * NaN or an infinity among its gates, its ups or (in f32) its products has s = 255. */
+FL_EXPORT int fl_glu4(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int act, float limit, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, void* stream);
+/* The scales of a weight [n, k] of such rows in the order in which fl_linear4 takes them, once per weight: fl_weight4_bytes bytes on a 16-byte border. */
+FL_EXPORT int fl_weight4_bytes(int64_t n, int64_t k, size_t* bytes);
+FL_EXPORT int fl_weight4(const uint8_t* scale, int64_t lds, int64_t n, int64_t k, void* tiles, void* stream);
+/* Matrix product of such rows:  y[r, i] = sum over j of x[r, j] * w[i, j] (+ bias[i]),  r < rows, i < n, j < k, the sum in f32, rounded once to y's type (f32, bf16, f16).
+ * x: f32, bf16 or f16 rows, which the call rounds as fl_quantize4 does (x_scale NULL), or 4-bit rows (FL_DTYPE_MX4, ldx in bytes) with their x_scale [rows, lds].  w [n, k]
+ * 4-bit rows (ldw in bytes), w_tiles fl_weight4 of its scales.  A row of x with a NaN or an infinity gives NaN.  Where one of x and w holds zeros, what the other's last
+ * block has behind the row does not matter.  workspace: fl_linear4_workspace bytes on a 256-byte border, free again when the call's work on the stream is done. */
+FL_EXPORT int fl_linear4_workspace(int64_t rows, int64_t k, int x_dtype, size_t* bytes);
+FL_EXPORT int fl_linear4(const void* x, int x_dtype, int64_t ldx, const uint8_t* x_scale, int64_t lds, const uint8_t* w, int64_t ldw, const void* w_tiles, const float* bias, int64_t rows,
+                         int64_t n, int64_t k, void* y, int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
 /* Whether all products that have run are valid.  Waits inside their kernels have a limit; a product that gave up on one has returned FL_OK long before, and its
  * result is not valid.  FL_ERR_CUDA: one of those since the last check was such; told once, by this call or by the next fl_linear8, which then does nothing else,
  * to whichever thread asks first.  To be asked after waiting for the work in question, a replayed graph's too. */

@@ -1,0 +1,492 @@
+"""GPU tests of the operators on 4-bit rows against their definitions in 64 bits.
+
+Roundings to 4 bits are compared bit for bit; other tolerances count roundings: half = finfo(type).eps / 2 is half a step of the result's type."""
+import math
+
+import pytest
+import torch
+
+from fastllm_b200 import ops
+from fastllm_b200._lib import FastllmError
+
+pytestmark = pytest.mark.gpu
+FLOATS = [torch.bfloat16, torch.float16, torch.float32]
+E2M1 = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+ACTS = ["silu", "gelu_tanh", "relu", "swish_clamp"]
+
+
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def _codes4(h, bad):
+    """numbers in 64 bits [rows, k] -> (codes [rows, 32 blocks], scales [rows, blocks]): the nearest e2m1 by the borders between neighbours, a border itself to
+    the even mantissa.  bad: blocks [rows, blocks] without a scale"""
+    rows, k = h.shape
+    b = torch.nn.functional.pad(h, (0, -k % 32)).view(rows, -1, 32)
+    a = b.abs().amax(-1)
+    e = torch.where(a > 0, torch.frexp(a).exponent - 3, -127).clamp(min=-127)
+    t = torch.ldexp(b.abs(), -e[..., None])
+    code = torch.zeros_like(t)
+    for border, above in ((0.25, False), (0.75, True), (1.25, False), (1.75, True), (2.5, False), (3.5, True), (5.0, False)):
+        code += (t >= border) if above else (t > border)
+    code += 8 * (torch.signbit(b))
+    scale = torch.where(bad, 255, e + 127)
+    return torch.where(bad[..., None], 0, code).view(rows, -1).to(torch.uint8), scale.to(torch.uint8)
+
+
+def _bad(x):
+    rows, k = x.shape
+    return ~torch.nn.functional.pad(x.float(), (0, -k % 32)).view(rows, -1, 32).isfinite().all(-1)
+
+
+def _unpack(q):
+    return torch.stack([q & 15, q >> 4], -1).flatten(-2)
+
+
+def _same_codes(got, want):
+    """equal but for the sign of a zero"""
+    return torch.equal(torch.where(got == 8, 0, got), torch.where(want == 8, 0, want))
+
+
+def _check_rows(x, q, scale):
+    assert q.dtype == scale.dtype == torch.uint8 and q.shape[:-1] == scale.shape[:-1] == x.shape[:-1] and q.shape[-1] == 16 * scale.shape[-1] == 16 * ((x.shape[-1] + 31) // 32)
+    x2, q2, s2 = x.reshape(-1, x.shape[-1]), q.reshape(-1, q.shape[-1]), scale.reshape(-1, scale.shape[-1])
+    bad = _bad(x2)
+    want, s = _codes4(torch.nan_to_num(x2.double(), 0.0, 0.0, 0.0), bad)
+    assert torch.equal(s2, s)
+    assert _same_codes(_unpack(q2), want)
+
+
+def _values(q, scale):
+    """in 64 bits"""
+    table = torch.tensor(E2M1, device="cuda", dtype=torch.float64)
+    v = torch.cat([table, -table])[_unpack(q).long()].unflatten(-1, (-1, 32))
+    s = torch.where(scale == 255, math.nan, torch.ldexp(torch.ones_like(scale, dtype=torch.float64), scale.int() - 127))
+    return (v * s[..., None]).flatten(-2)
+
+
+# ---- rounding and back --------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows, cols", [(1, 1), (3, 2), (5, 31), (2, 32), (4, 33), (7, 255), (3, 256), (2, 257), (2, 1000), (2, 1999), (5, 4096), (3, 5001), (2, 14336), (1, 131073), (400, 96), (1, 1 << 20)])
+def test_quantize4(dtype, rows, cols):
+    x = (torch.randn(rows, cols, device="cuda", generator=_gen(cols)) * 3).to(dtype)
+    _check_rows(x, *ops.quantize4(x))
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_quantize4_at_the_borders(dtype):
+    """every border between neighbours and the numbers next to it, at several scales; block maxima next to powers of two"""
+    borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0], device="cuda")
+    rows = []
+    for size in (1.0, 2.0 ** -9, 2.0 ** 7):
+        r = (borders * size).to(dtype)
+        up, down = torch.nextafter(r, torch.full_like(r, math.inf)), torch.nextafter(r, torch.full_like(r, -math.inf))
+        for most in (4.0, 7.99):
+            rows.append(torch.cat([r.clamp(max=most * size), up.clamp(max=most * size), down, -r[:4], torch.tensor([most * size], device="cuda").to(dtype)]))
+        for top in (4.0, 8.0):
+            t = torch.tensor([top * size], device="cuda").to(dtype)
+            for m in (t, torch.nextafter(t, torch.zeros_like(t)), torch.nextafter(t, 2 * t)):
+                rows.append(torch.cat([r / 4, -r / 2, m, torch.zeros(13, device="cuda", dtype=dtype)]).clamp(-m.item(), m.item())[:32])
+    for r in rows:
+        _check_rows(r[None], *ops.quantize4(r[None]))
+        _check_rows(-r[None], *ops.quantize4(-r[None]))
+
+
+def test_quantize4_of_any_size():
+    tiny = torch.finfo(torch.float32).smallest_normal
+    base = torch.randn(10, 300, device="cuda", generator=_gen(1))
+    base = base / base.abs().amax(-1, keepdim=True)
+    x = base * torch.tensor([1e-45, 1e-44, 1e-41, tiny, 4 * tiny, 1e-30, 1e-20, 1e20, 1e38, 3.4e38], device="cuda")[:, None]
+    _check_rows(x, *ops.quantize4(x))
+    h = torch.tensor([[2.0 ** -24, 2.0 ** -23, 0, -2.0 ** -24], [65504, -65504, 1, 0]], device="cuda").half()
+    _check_rows(h, *ops.quantize4(h))
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("shift", [0, 1])
+def test_quantize4_without_a_scale(dtype, shift):
+    x = torch.randn(6, 340, device="cuda", generator=_gen(2)).to(dtype)[:, shift:333 + shift]
+    x[0] = 0
+    x[1] = -0.0
+    x[2, 100] = math.nan
+    x[3, 332] = -math.inf
+    x[4, 64:96] = 0
+    q, scale = ops.quantize4(x)
+    _check_rows(x, q, scale)
+    assert (scale[:2] == 0).all() and scale[2, 3] == 255 and scale[3, 10] == 255 and (scale == 255).sum() == 2 and scale[4, 2] == 0
+
+
+def test_quantize4_strides_and_shapes():
+    base = torch.randn(2, 6, 7, 100, device="cuda", generator=_gen(3)).bfloat16()
+    x = base[:, :, 3, 1:98]                     # rows that start on odd elements, one row stride
+    with pytest.raises(FastllmError, match="leading dimensions"):
+        ops.quantize4(base[:, :4, 3, :])
+    _check_rows(x, *ops.quantize4(x))
+    q, scale = ops.quantize4(x[0, 0])
+    assert q.shape == (64,) and scale.shape == (4,)
+    _check_rows(x[0, 0], q, scale)
+    with pytest.raises(FastllmError, match="not dense"):
+        ops.quantize4(base[0, 0, :, ::2])
+    q, scale = ops.quantize4(base[:, :0, 3, 1:98])
+    assert q.shape == (2, 0, 64) and scale.shape == (2, 0, 4)
+    assert ops.dequantize4(q, scale, 97).shape == (2, 0, 97)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_dequantize4_of_every_code(dtype):
+    """16 numbers at 256 scales: rounded once"""
+    scale = torch.arange(256, device="cuda").to(torch.uint8)[:, None]
+    q = torch.arange(16, device="cuda").to(torch.uint8) * 17
+    q = q.repeat(256, 1)
+    y = ops.dequantize4(q, scale, dtype=dtype)
+    want = _values(q, scale)
+    f32 = want.float()                          # exact but for what passes its largest number
+    assert ((f32.double() == want) | f32.isinf() | f32.isnan()).all()
+    assert y.shape == (256, 32) and y[255].isnan().all() and torch.equal(y[:255], f32[:255].to(dtype))
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows, cols", [(1, 1), (3, 31), (2, 32), (5, 33), (7, 1999), (3, 4096), (300, 250)])
+def test_dequantize4(dtype, rows, cols):
+    blocks = (cols + 31) // 32
+    store = torch.randint(0, 256, (rows, blocks * 16 + 32), device="cuda", generator=_gen(cols), dtype=torch.uint8)
+    q, scale = store[:, 16:16 + blocks * 16], torch.randint(100, 130, (rows, blocks + 3), device="cuda", generator=_gen(rows), dtype=torch.uint8)[:, 1:blocks + 1]
+    y = ops.dequantize4(q, scale, cols, dtype)
+    assert torch.equal(y, _values(q, scale)[:, :cols].to(dtype))
+    if cols % 32 == 0:
+        assert torch.equal(ops.dequantize4(q, scale, dtype=dtype), y)
+    for bad in (cols + 32, cols - 32, 0):
+        if not 32 * blocks - 32 < bad <= 32 * blocks:
+            with pytest.raises(FastllmError, match="columns"):
+                ops.dequantize4(q, scale, bad)
+
+
+# ---- the gated activation -----------------------------------------------------------------------------------------------------------
+def _activation(x, act, limit):
+    g, u = x.double().chunk(2, -1)
+    if act == "silu":
+        return g / (1.0 + torch.exp(-g)) * u
+    if act == "gelu_tanh":
+        return g / (1.0 + torch.exp(-2.0 * math.sqrt(2.0 / math.pi) * (g + 0.044715 * g ** 3))) * u
+    if act == "relu":
+        return g.clamp(min=0) * u
+    g = g.clamp(max=limit)
+    return g / (1.0 + torch.exp(-1.702 * g)) * (u.clamp(-limit, limit) + 1.0)
+
+
+def _check_glu(x, act, q, scale, limit=7.0):
+    f = x.shape[-1] // 2
+    x2 = x.reshape(-1, 2 * f)
+    h = _activation(x2, act, limit)
+    bad = _bad(x2[:, :f]) | _bad(x2[:, f:]) | _bad(torch.where(h.abs() >= 2.0 ** 128, math.inf, 0.0))
+    want, s = _codes4(torch.where(h.isfinite(), h, 0.0), bad)
+    assert torch.equal(scale.reshape(s.shape), s)
+    assert _same_codes(_unpack(q.reshape(len(s), -1)), want)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows, f", [(1, 1), (2, 7), (3, 32), (5, 33), (2, 1000), (7, 2048), (37, 5001), (64, 4096), (2, 14336)])
+def test_glu4(act, dtype, rows, f):
+    x = (torch.randn(rows, 2 * f, device="cuda", generator=_gen(f)) * 3).to(dtype)
+    _check_glu(x, act, *ops.glu4(x, act))
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_glu4_of_many(act):
+    """so many numbers that some lie next to a border: 64 million, of which f32's exponential would put hundreds on the wrong side"""
+    for seed in range(4):
+        x = torch.randn(1024, 32768, device="cuda", generator=_gen(seed)) * 2
+        _check_glu(x, act, *ops.glu4(x, act))
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_glu4_extremes(act, dtype):
+    """gates from far below to far above, blocks whose results are all tiny, products that pass f32's range, numbers that are none"""
+    big = min(torch.finfo(dtype).max, 1e30)
+    x = torch.randn(16, 2 * 320, device="cuda", generator=_gen(4)).to(dtype)
+    g, u = x[:, :320], x[:, 320:]
+    g[0] = torch.linspace(-200, 200, 320, device="cuda").to(dtype)
+    g[1] = torch.linspace(-120, -20, 320, device="cuda").to(dtype)
+    g[2] = -30.0
+    g[3] = 0.0
+    g[4] = torch.linspace(0, 60, 320, device="cuda").to(dtype)
+    u[4] = 1.25
+    g[5] *= 1e-3
+    u[5] *= 1e-3
+    g[6], u[6] = big, big
+    g[7, 5], u[7, 40] = math.nan, math.nan
+    g[8, 5], u[8, 40], g[8, 100] = math.inf, -math.inf, -math.inf
+    u[9] = -1.0
+    u[10] = torch.linspace(-1.01, -0.99, 320, device="cuda").to(dtype)
+    g[11] = -big
+    u[12] = 0.0
+    g[13] *= torch.finfo(dtype).smallest_normal
+    g[14], u[14] = 40.0, 1.0
+    g[15], u[15] = 1.0, 5.0 / torch.arange(1, 321, device="cuda").to(dtype)
+    _check_glu(x, act, *ops.glu4(x, act))
+
+
+def test_glu4_limits_strides_and_shapes():
+    base = (torch.randn(2, 6, 7, 100, device="cuda", generator=_gen(5)) * 4).bfloat16()
+    x = base[:, :, 3, 1:99]
+    for limit in (0.5, 7.0, 100.0):
+        _check_glu(x, "swish_clamp", *ops.glu4(x, "swish_clamp", limit=limit), limit)
+    for act in ACTS:
+        _check_glu(x, act, *ops.glu4(x, act))
+    q, scale = ops.glu4(x[0, 0])
+    assert q.shape == (32,) and scale.shape == (2,)
+    assert ops.glu4(x[:, :0])[0].shape == (2, 0, 32)
+    for bad in (lambda: ops.glu4(x[..., 1:]), lambda: ops.glu4(x, "gelu"), lambda: ops.glu4(x, "swish_clamp", limit=-1.0), lambda: ops.glu4(x[..., ::2])):
+        with pytest.raises(FastllmError):
+            bad()
+
+
+# ---- the product --------------------------------------------------------------------------------------------------------------------
+def _rows4(n, k, middle, seed):
+    """4-bit rows with garbage behind their last column and between the rows"""
+    g, blocks = _gen(seed), (k + 31) // 32
+    q = torch.randint(0, 256, (n, blocks * 16 + 16), dtype=torch.uint8, device="cuda", generator=g)
+    scale = torch.randint(middle - 3, middle + 4, (n, blocks + 1), dtype=torch.uint8, device="cuda", generator=g)
+    return q[:, :blocks * 16], scale[:, 1:]
+
+
+def _check_product(y, x, w, bias):
+    """x, w in 64 bits.  Products of two e2m1 and two powers of two are exact.  A step of 64 products is summed with at most a step of f32 (2^-23) lost at each addition, and
+    so is its sum's way into the accumulator, k / 64 times: (64 + k / 64) 2^-23 of the sum of magnitudes.  Then the bias (2^-24) and one rounding to y's type."""
+    k = x.shape[1]
+    want, size = x @ w.T, x.abs() @ w.abs().T
+    tol = (64 + k / 64) * 2.0 ** -23 * size
+    if bias is not None:
+        want = want + bias.double()
+    half = torch.finfo(y.dtype).eps / 2
+    least = torch.finfo(y.dtype).smallest_normal * half
+    tol = 1.001 * (tol + (half + (2.0 ** -24 if bias is not None else 0.0)) * (want.abs() + tol)) + least
+    far = (y.double() - want).abs()
+    assert y.shape == want.shape and bool((far <= tol).all()), float((far / tol).max())
+
+
+SIZES = [(1, 1, 1), (1, 128, 128), (2, 5, 17), (3, 129, 15), (7, 64, 32), (8, 1000, 127), (9, 127, 129), (16, 256, 1000), (17, 130, 640), (31, 4096, 256), (33, 96, 2050),
+         (64, 257, 513), (65, 5001, 96), (100, 640, 4096), (127, 384, 300), (128, 128, 1280), (129, 333, 128), (203, 1001, 1999), (255, 512, 160), (256, 256, 512),
+         (257, 300, 400), (511, 2049, 144), (700, 200, 4097), (1025, 1030, 272), (1500, 777, 130), (2100, 2500, 64)]
+
+
+def _exact_x(x):
+    code, scale = _codes4(x.double(), _bad(x))
+    q = code.view(len(x), -1, 2)
+    return _values((q[..., 0] | q[..., 1] << 4), scale)
+
+
+@pytest.mark.parametrize("rows, n, k", SIZES)
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_linear4(rows, n, k, dtype):
+    x = (torch.randn(rows, k, device="cuda", generator=_gen(rows)) * 2).to(dtype)
+    q, scale = _rows4(n, k, 122, n)
+    bias = torch.randn(n, device="cuda", generator=_gen(k)) if (rows + n) % 2 else None
+    y = ops.linear4(x, ops.weight4(q, scale), bias)
+    assert y.dtype == dtype
+    _check_product(y, _exact_x(x), _values(q, scale), bias)
+
+
+@pytest.mark.parametrize("rows, n, k", SIZES)
+def test_linear4_of_4_bit_rows(rows, n, k):
+    x, xs = _rows4(rows, k, 127, rows)
+    q, scale = _rows4(n, k, 122, n)
+    y = ops.linear4(x, ops.weight4(q, scale), x_scale=xs)
+    assert y.dtype == torch.float32
+    _check_product(y, _values(x, xs), _values(q, scale), None)
+
+
+@pytest.mark.parametrize("rows", [1, 20, 100, 300, 1200])
+@pytest.mark.parametrize("k", [64, 480, 4096])
+def test_linear4_of_whole_numbers_is_exact(rows, k):
+    """sums of quarters up to 36 k < 2^22: nothing is lost in 24 bits, in whatever order"""
+    n = 300
+    x = torch.randint(0, 256, (rows, k // 2), dtype=torch.uint8, device="cuda", generator=_gen(rows))
+    q = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda", generator=_gen(k))
+    one = torch.full((max(rows, n), k // 32), 127, dtype=torch.uint8, device="cuda")
+    y = ops.linear4(x, ops.weight4(q, one[:n]), x_scale=one[:rows])
+    assert torch.equal(y.double(), _values(x, one[:rows]) @ _values(q, one[:n]).T)
+
+
+@pytest.mark.parametrize("rows", [1, 9, 40, 70, 128, 200, 600])
+def test_linear4_takes_every_block_at_its_scale(rows):
+    """one column alone is not zero, and every block has a scale of its own: a scale read from the wrong place shows at once"""
+    n, blocks = 140, 19
+    k = 32 * blocks
+    code = torch.randint(1, 8, (rows, blocks), device="cuda", generator=_gen(rows)).to(torch.uint8)
+    xs = torch.randint(110, 140, (rows, blocks), device="cuda", generator=_gen(rows + 1)).to(torch.uint8)
+    q = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda", generator=_gen(rows + 2))
+    scale = torch.randint(110, 140, (n, blocks), device="cuda", generator=_gen(rows + 3)).to(torch.uint8)
+    w = ops.weight4(q, scale)
+    wv = _values(q, scale)
+    for b in range(blocks):
+        x = torch.zeros(rows, k // 2, dtype=torch.uint8, device="cuda")
+        x[:, 16 * b + 5] = code[:, b] << 4
+        y = ops.linear4(x, w, x_scale=xs)
+        assert torch.equal(y.double(), _values(x, xs) @ wv.T), b
+
+
+@pytest.mark.parametrize("rows", [1, 40, 300, 1200])
+@pytest.mark.parametrize("out_dtype", FLOATS)
+def test_linear4_types_of_the_result(rows, out_dtype):
+    x = torch.randn(rows, 272, device="cuda", generator=_gen(rows)).half()
+    q, scale = _rows4(390, 272, 122, 5)
+    y = ops.linear4(x, ops.weight4(q, scale), out_dtype=out_dtype)
+    assert y.dtype == out_dtype
+    _check_product(y, _exact_x(x), _values(q, scale), None)
+
+
+@pytest.mark.parametrize("rows", [3, 100, 300, 1111])
+def test_linear4_rows_without_a_scale(rows):
+    """a row with a NaN or an infinity is NaN, a row of zeros the bias, the other rows are their own; likewise a weight row"""
+    x = torch.randn(rows, 200, device="cuda", generator=_gen(9)).bfloat16()
+    x[0] = 0
+    x[1, 7] = math.nan
+    x[2, 199] = math.inf
+    q, scale = _rows4(150, 200, 122, 10)
+    q, scale = q.clone(), scale.clone()
+    bias = torch.randn(150, device="cuda", generator=_gen(11))
+    y = ops.linear4(x, ops.weight4(q, scale), bias, out_dtype=torch.float32)
+    assert torch.equal(y[0], bias) and y[1:3].isnan().all()
+    if rows > 3:
+        _check_product(y[3:], _exact_x(x[3:]), _values(q, scale), bias)
+    scale[77, 4] = 255
+    y2 = ops.linear4(x, ops.weight4(q, scale), bias, out_dtype=torch.float32)
+    assert y2[:, 77].isnan().all()
+    keep = torch.arange(150, device="cuda") != 77
+    assert torch.equal(y2[3:, keep], y[3:, keep]) and torch.equal(y2[0, keep], y[0, keep])
+
+
+@pytest.mark.parametrize("rows", [1, 6, 90, 200, 280, 1040])
+def test_linear4_writes_its_rows_and_nothing_else(rows):
+    """strided input and result: rows behind the last one and columns behind the row stay as they were"""
+    k, n = 160, 190
+    x = torch.randn(rows + 2, 3, k + 5, device="cuda", generator=_gen(12)).bfloat16()[:, 1, 3:k + 3]
+    q, scale = _rows4(n, k, 122, 13)
+    store = torch.full((rows + 2, n + 9), 7.0, device="cuda", dtype=torch.bfloat16)
+    out = ops.linear4(x[:rows], ops.weight4(q, scale), out=store[:rows, 1:n + 1])
+    assert out.data_ptr() == store[:, 1:].data_ptr()
+    _check_product(out, _exact_x(x[:rows]), _values(q, scale), None)
+    assert (store[rows:] == 7).all() and (store[:, 0] == 7).all() and (store[:, n + 1:] == 7).all()
+
+
+def test_linear4_shapes_and_refusals():
+    q, scale = ops.quantize4(torch.randn(40, 64, device="cuda", generator=_gen(14)))
+    w = ops.weight4(q, scale)
+    x = torch.randn(2, 3, 64, device="cuda", generator=_gen(15)).bfloat16()
+    assert torch.equal(ops.linear4(x, w).view(6, 40), ops.linear4(x.view(6, 64), w))
+    assert torch.equal(ops.linear4(x[0, 0], w), ops.linear4(x[0], w)[0])
+    assert ops.linear4(x[:, :0], w).shape == (2, 0, 40)
+    xq, xs = ops.quantize4(x)
+    assert torch.equal(ops.linear4(xq, w, x_scale=xs, out_dtype=torch.bfloat16), ops.linear4(x, w))
+    assert torch.equal(ops.linear4(x[..., :50], w), ops.linear4(torch.nn.functional.pad(x[..., :50], (0, 14)), w))      # (a last block that is not whole)
+    bias = torch.zeros(40, device="cuda")
+    for bad in (lambda: ops.linear4(x[..., :32], w), lambda: ops.linear4(x, q), lambda: ops.linear4(x, w, bias[:39]), lambda: ops.linear4(x, w, bias.half()), lambda: ops.linear4(xq, w),
+                lambda: ops.linear4(x, w, x_scale=xs), lambda: ops.linear4(xq, w, x_scale=xs[..., :1]), lambda: ops.linear4(xq, w, x_scale=xs.int()), lambda: ops.linear4(x[..., ::2], w),
+                lambda: ops.linear4(x, w, out=torch.empty(2, 3, 41, device="cuda")), lambda: ops.linear4(x, w, out_dtype=torch.float64), lambda: ops.linear4(x, w, bias.cpu()),
+                lambda: ops.weight4(q[:, :16], scale), lambda: ops.weight4(q, scale.cpu()), lambda: ops.weight4(q[:0], scale[:0]), lambda: ops.weight4(q[:, ::2], scale[:, :1])):
+        with pytest.raises(FastllmError):
+            bad()
+    odd = torch.zeros(40, 40, dtype=torch.uint8, device="cuda")
+    with pytest.raises(FastllmError, match="16-byte"):
+        ops.linear4(x, ops.weight4(odd[:, :32], scale))
+
+
+def test_linear4_far_offsets():
+    """weights and results whose offsets pass 2^31 bytes"""
+    n, k = 9, 64
+    stride = (1 << 31) // 8 + 16
+    store = torch.zeros(8 * stride + k, dtype=torch.uint8, device="cuda")
+    q = store.as_strided((n, k // 2), (stride, 1))
+    q.random_(0, 256, generator=_gen(16))
+    scale = torch.randint(120, 125, (n, 2), device="cuda", generator=_gen(17)).to(torch.uint8)
+    x = torch.randn(200, k, device="cuda", generator=_gen(18)).bfloat16()
+    for rows in (1, 20, 200):
+        _check_product(ops.linear4(x[:rows], ops.weight4(q, scale)), _exact_x(x[:rows]), _values(q, scale), None)
+    far = store.view(torch.bfloat16)[: 8 * (stride // 2) + n].as_strided((9, n), (stride // 2, 1))
+    del store
+    dense = q.clone().contiguous()
+    y = ops.linear4(x[:9], ops.weight4(dense, scale), out=far)
+    _check_product(y, _exact_x(x[:9]), _values(dense, scale), None)
+
+
+# ---- together, on streams, in graphs ------------------------------------------------------------------------------------------------
+def _feed_forward(x, w_in, w_out, act="silu"):
+    """a feed-forward with 4-bit weights: two products with the activation between them"""
+    h, hs = ops.glu4(ops.linear4(x, w_in, out_dtype=torch.float32), act)
+    return ops.linear4(h, w_out, x_scale=hs, out_dtype=torch.bfloat16)
+
+
+def _weights(width, hidden, seed):
+    g = _gen(seed)
+    first, second = torch.randn(2 * hidden, width, device="cuda", generator=g) * width ** -0.5, torch.randn(width, hidden, device="cuda", generator=g) * hidden ** -0.5
+    return [(ops.quantize4(w), ops.weight4(*ops.quantize4(w))) for w in (first, second)]
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("rows", [1, 19, 150, 700])
+def test_feed_forward(rows, act):
+    """each operator on what the one before it left, as it is used"""
+    (w1, w_in), (w2, w_out) = _weights(512, 1000, 20)
+    x = torch.randn(rows, 512, device="cuda", generator=_gen(21)).bfloat16()
+    y = ops.linear4(x, w_in, out_dtype=torch.float32)
+    _check_product(y, _exact_x(x), _values(*w1), None)
+    h, hs = ops.glu4(y, act)
+    _check_glu(y, act, h, hs)
+    out = ops.linear4(h, w_out, x_scale=hs, out_dtype=torch.bfloat16)
+    _check_product(out, _values(h, hs), _values(*w2), None)
+    assert torch.equal(out, _feed_forward(x, w_in, w_out, act))
+
+
+def test_same_bits_every_time():
+    (_, w_in), (_, w_out) = _weights(640, 3000, 22)
+    for rows in (1, 70, 400):
+        x = torch.randn(rows, 640, device="cuda", generator=_gen(23)).bfloat16()
+        first = _feed_forward(x, w_in, w_out)
+        for _ in range(5):
+            assert torch.equal(first, _feed_forward(x, w_in, w_out))
+
+
+def test_other_streams():
+    """calls on several streams at once, each behind its own input"""
+    (_, w_in), (_, w_out) = _weights(600, 2000, 24)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for i in range(9):
+        with torch.cuda.stream(streams[i % 3]):
+            x = torch.randn((1, 50, 400)[i % 3], 600, device="cuda", generator=_gen(34 + i)).bfloat16()
+            got.append((x, _feed_forward(x, w_in, w_out)))
+    torch.cuda.synchronize()
+    for x, y in got:
+        assert torch.equal(y, _feed_forward(x, w_in, w_out))
+    ops.check()
+
+
+@pytest.mark.parametrize("rows", [1, 60, 300, 1100])
+def test_graphs(rows):
+    """two captured graphs, replayed on new inputs and side by side"""
+    (_, w_in), (_, w_out) = _weights(256, 700, 25)
+    graphs = []
+    for i in range(2):
+        x = torch.zeros(rows, 256, device="cuda", dtype=torch.bfloat16)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = _feed_forward(x, w_in, w_out)
+        graphs.append((g, x, y, torch.cuda.Stream()))
+    for step in range(3):
+        for i, (g, x, y, s) in enumerate(graphs):
+            x.copy_(torch.randn(rows, 256, device="cuda", generator=_gen(60 + 2 * step + i)))
+        torch.cuda.synchronize()
+        for g, x, y, s in graphs:
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for g, x, y, s in graphs:
+            assert torch.equal(y, _feed_forward(x, w_in, w_out))
+    ops.check()

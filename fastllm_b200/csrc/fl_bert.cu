@@ -65,6 +65,19 @@ CUtensorMap make_tmap_i8(const void* ptr, uint64_t rows, uint64_t cols, uint64_t
     return m;
 }
 
+// Scales of 4-bit rows in the tensor cores' order, [atoms][512 bytes] (linear4.cuh), as 4-byte words: boxes of `box` whole atoms.
+CUtensorMap make_tmap_scales(const void* ptr, uint64_t atoms, uint32_t box) {
+    CUtensorMap m;
+    const cuuint64_t dims[2] = {128, atoms};
+    const cuuint64_t strides[1] = {512};
+    const cuuint32_t boxes[2] = {128, box};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = encode_tiled_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(ptr), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                         CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    FL_CHECK(r == CUDA_SUCCESS, -2, "cuTensorMapEncodeTiled (scales) failed (" + std::to_string((int)r) + ")");
+    return m;
+}
+
 // Weight matrix [N, K] bf16 (K % 64 == 0) as the persistent decode kernel streams it: a 3-D view {64 columns, N rows, K/64
 // column blocks} whose box {64, 16, 16} is ONE 32 KB request = 16 rows x 1024 columns, landing in shared memory as
 // [column block][row][128 bytes] with the 128-byte swizzle keyed by the row: conflict-free ldmatrix of 16 x 16 tiles.

@@ -316,7 +316,9 @@ FL_EXPORT int fl_logprobs(const void* logits, int dtype, int64_t rows, int64_t v
 
 FL_EXPORT int fl_operators_check(void) {
     FL_API_BEGIN
+    const bool of4 = products4_failed();            // (both words are taken)
     check_op_failed();
+    FL_CHECK(!of4, FL_ERR_CUDA, "a wait inside an operator's kernel ran out: a product since the last check is not valid");
     FL_API_END
 }
 

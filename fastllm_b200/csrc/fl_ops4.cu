@@ -5,6 +5,7 @@
 #include <mutex>
 
 #include "../../include/fastllm_b200.h"
+#include "failed_word.hpp"
 #include "linear4.cuh"
 #include "op_launch.cuh"
 #include "ops.hpp"
@@ -56,28 +57,92 @@ struct Linear4Room { size_t scale = 0, all = 0; };
 static Linear4Room linear4_room(int64_t rows, int64_t k, bool given) {
     Linear4Room r;
     r.scale = given ? 0 : up256((size_t)rows * blocks4(k) * 16);
-    r.all = r.scale + (size_t)slots4(rows, 128) * groups4(k) * 4;
+    // the scales lie in tiles of as many rows as a product takes: 64 at least beyond 128 rows, padded to 128
+    r.all = r.scale + (size_t)slots4(rows, rows > 128 ? 64 : 128) * groups4(k) * 4;
     return r;
 }
 size_t linear4_workspace(int64_t rows, int64_t k) { return linear4_room(rows, k, false).all; }
 
-// x in 4 bits: lds its scales' row stride; else their type's
-static void run_linear4(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, const uint8_t* x_scale, int64_t lds, const uint8_t* w, int64_t ldw, const uint8_t* w_tiles, const float* bias,
-                        int64_t rows, int64_t n, int64_t k, void* y, int y_dtype, int64_t ldy, void* workspace) {
-    const bool given = x_dtype == FL_DTYPE_MX4;
-    const Linear4Room room = linear4_room(rows, k, given);
-    uint8_t *q = static_cast<uint8_t*>(workspace), *xs = q + room.scale;
-    const int blocks = (int)blocks4(k), groups = (int)groups4(k);
-    if (given) {
-        arrange4(lc, x_scale, lds, rows, k, 128, xs, false);
-    } else {
-        quantize4(lc, x, x_dtype, rows, k, ldx, Rows4Out{q, blocks * 16, xs, 0, blocks, 128, groups});
+// How a product of more than kL4FewRows rows goes over the pairs of SMs: the tile width whose waves cost least, by what a k block takes.
+constexpr int kL4FewRows = 128;
+static L4Pair pair_plan4(int64_t rows, int64_t n, int64_t k, int clusters) {
+    static constexpr struct { int bn, parts; } kForms[] = {{416, 2}, {384, 2}, {320, 2}, {256, 2}, {224, 1}, {192, 1}, {160, 1}, {128, 1}, {96, 1}, {64, 1}};
+    L4Pair best{};
+    double cost = -1;
+    for (const auto& f : kForms) {
+        L4Pair p{};
+        p.bn = f.bn;
+        p.parts = f.parts;
+        p.nk = (int)(groups4(k) / 2);
+        p.mt = (int)((n + 255) / 256);
+        p.nt = (int)((rows + f.bn - 1) / f.bn);
+        p.stages = (int)std::min<uint32_t>(kL4PairMaxStages, kL4PairRing / l4_pair_stage(f.bn, f.parts));
+        const double block = std::max(1.38 * f.bn, l4_pair_stage(f.bn, f.parts) / 90.0), tail = f.parts == 2 ? 13.0 * f.bn : 0.0;      // ns; results that no product hides
+        const double waves = (double)(((long long)p.mt * p.nt + clusters - 1) / clusters);
+        const double c = waves * (p.nk * block + tail);
+        if (cost < 0 || c < cost) { cost = c; best = p; }
     }
-    const Linear4Args a{(int)rows, (int)n, blocks, given ? static_cast<const uint8_t*>(x) : q, given ? ldx : blocks * 16, xs, 128, w, ldw, w_tiles, groups, bias, y, ldy, y_dtype};
-    launch_op(lc, "linear4", (uint64_t)(n + rows) * blocks * 17 + rows * n * dtype_size(y_dtype), linear4_plain_kernel, dim3((unsigned)((n + 31) / 32), (unsigned)((rows + 31) / 32)), 256, 0, 1,
-              false, a);
+    return best;
 }
 
+// What the operators keep for the process: a page-locked word that a kernel sets when a wait inside it ran out, told of once.
+static FailedWord g_op4_failed;
+static int g_pair_clusters = 0;                 // pairs of SMs that can be resident at once
+bool products4_failed() { return g_op4_failed.take(); }
+
+// Blocks that share a 128-row weight tile (see few_slices of the 8-bit product).
+static int few_slices4(int64_t tiles, int nk) {
+    int S = 8;
+    while (S > 1 && (S * tiles > kNumSMs || nk < 8 * S || nk - nk / S < 24)) S /= 2;
+    return S;
+}
+template <int BN>
+static void launch_few4(LaunchCtx& lc, uint64_t bytes, const uint8_t* x, int64_t ldx, const uint8_t* w, int64_t ldw, const Linear4Args& g) {
+    const int tiles = (g.n + 127) / 128, S = few_slices4(tiles, g.groups / 2);
+    const CUtensorMap tw = make_tmap_i8(w, g.n, g.blocks * 16, ldw, 128), tx = make_tmap_i8(x, g.rows, g.blocks * 16, ldx, BN);
+    launch_op(lc, "linear4", bytes, linear4_few_kernel<BN>, dim3((unsigned)(tiles * S)), L4Few<BN>::kThreads, L4Few<BN>::kSmem, S, true, tw, tx, g, S);
+}
+static void launch_pair4(LaunchCtx& lc, uint64_t bytes, const uint8_t* x, int64_t ldx, const uint8_t* w, int64_t ldw, const Linear4Args& g, const L4Pair& p) {
+    const int pn = p.bn / p.parts, atoms = l4_pair_atoms(pn);
+    const CUtensorMap tx = make_tmap_i8(x, g.rows, g.blocks * 16, ldx, pn / 2), tw = make_tmap_i8(w, g.n, g.blocks * 16, ldw, 128);
+    const CUtensorMap tws = make_tmap_scales(g.ws, (int64_t)((g.n + 127) / 128) * g.groups, 2), txs = make_tmap_scales(g.xs, (int64_t)((g.rows + pn - 1) / pn) * g.groups * atoms, 2 * atoms);
+    const long long clusters = std::min<long long>(g_pair_clusters, (long long)p.mt * p.nt);
+    launch_op(lc, "linear4", bytes, linear4_pair_kernel, dim3((unsigned)(2 * clusters)), kL4PairThreads, kL4PairSmem, 1, true, tw, tx, tws, txs, g, p);
+}
+
+// x in 4 bits: lds its scales' row stride
+static void run_linear4(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, const uint8_t* x_scale, int64_t lds, const uint8_t* w, int64_t ldw, const uint8_t* w_tiles, const float* bias,
+                        int64_t rows, int64_t n, int64_t k, void* y, int y_dtype, int64_t ldy, void* workspace, int* failed) {
+    const bool given = x_dtype == FL_DTYPE_MX4, many = rows > kL4FewRows;
+    FL_CHECK(!many || g_pair_clusters >= 1, FL_ERR_UNSUPPORTED, "linear4: no two SMs of this device form a pair");
+    const Linear4Room room = linear4_room(rows, k, given);
+    uint8_t *to = static_cast<uint8_t*>(workspace), *xs = to + room.scale;
+    const int blocks = (int)blocks4(k), groups = (int)groups4(k);
+    const L4Pair p = many ? pair_plan4(rows, n, k, g_pair_clusters) : L4Pair{};
+    const int tile = many ? p.bn / p.parts : 128;
+    const uint8_t* q = to;
+    int64_t ldq = 16 * blocks;
+    if (given) {
+        arrange4(lc, x_scale, lds, rows, k, tile, xs, false);
+        q = static_cast<const uint8_t*>(x);
+        if (rows > 1) ldq = ldx;
+    } else {
+        quantize4(lc, x, x_dtype, rows, k, ldx, Rows4Out{to, ldq, xs, 0, blocks, tile, groups});
+    }
+    if (n == 1) ldw = 16 * blocks;
+    const Linear4Args a{(int)rows, (int)n, blocks, xs, w_tiles, groups, bias, y, ldy, y_dtype, failed};
+    const uint64_t bytes = (uint64_t)(n + rows) * blocks * 17 + rows * n * dtype_size(y_dtype);
+    if (many) launch_pair4(lc, bytes, q, ldq, w, ldw, a, p);
+    else if (rows <= 16) launch_few4<16>(lc, bytes, q, ldq, w, ldw, a);
+    else if (rows <= 32) launch_few4<32>(lc, bytes, q, ldq, w, ldw, a);
+    else if (rows <= 64) launch_few4<64>(lc, bytes, q, ldq, w, ldw, a);
+    else launch_few4<128>(lc, bytes, q, ldq, w, ldw, a);
+}
+
+template <int BN>
+static void few_attr4() {
+    FL_CUDA(cudaFuncSetAttribute(linear4_few_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L4Few<BN>::kSmem));
+}
 // One-time set-up on the bound device, by the first call that launches an operator.  It also loads the kernels, so that this call may be one inside a graph capture.
 static void set_up() {
     static std::atomic<bool> done{false};
@@ -89,7 +154,21 @@ static void set_up() {
     for (int dtype : {FL_DTYPE_F32, FL_DTYPE_BF16, FL_DTYPE_F16})
         by_type(dtype, [](auto t) { load_kernels(quantize4_kernel<decltype(t)>); load_kernels(dequantize4_kernel<decltype(t)>); load_kernels(glu4_kernel<decltype(t)>); });
     load_kernels(arrange4_kernel);
-    load_kernels(linear4_plain_kernel);
+    few_attr4<16>(); few_attr4<32>(); few_attr4<64>(); few_attr4<128>();
+    FL_CUDA(cudaFuncSetAttribute(linear4_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL4PairSmem));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(kNumSMs); cfg.blockDim = dim3(kL4PairThreads); cfg.dynamicSmemBytes = kL4PairSmem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    int pairs = 0;
+    FL_CUDA(cudaOccupancyMaxActiveClusters(&pairs, linear4_pair_kernel, &cfg));
+    g_pair_clusters = std::min(pairs, kNumSMs / 2);
+    int* p = nullptr;
+    FL_CUDA(cudaMallocHost(&p, sizeof(int)));
+    *p = 0;
+    g_op4_failed.word = p;
     done.store(true, std::memory_order_release);
 }
 
@@ -210,14 +289,15 @@ FL_EXPORT int fl_linear4(const void* x, int x_dtype, int64_t ldx, const uint8_t*
     FL_CHECK(aligned(w_tiles, 16), FL_ERR_INVALID, "linear4: the weight's scales start on a 16-byte border");
     if (given) check_rows4("linear4", x, ldx, x_scale, lds, rows, k);
     FL_CHECK((given || aligned(x, dtype_size(x_dtype))) && aligned(y, dtype_size(y_dtype)) && aligned(bias, 4), FL_ERR_INVALID, "linear4: a pointer is not aligned to its type");
-    FL_CHECK(rows <= ((int64_t)1 << 40) / n, FL_ERR_INVALID, "linear4: more than 2^40 results");
+    FL_CHECK(rows <= ((int64_t)1 << 40) / n && n <= ((int64_t)1 << 43) / k && rows <= ((int64_t)1 << 43) / k, FL_ERR_INVALID, "linear4: more than 2^40 results, or an operand of more than 2^43 numbers");
     const Linear4Room room = linear4_room(rows, k, given);
     FL_CHECK(workspace && aligned(workspace, 256) && workspace_bytes >= room.all, FL_ERR_INVALID,
              "linear4: the workspace is smaller than fl_linear4_workspace asks for, or not on a 256-byte border");
     DeviceScope dev;
     set_up();
     LaunchCtx lc = op_ctx(stream);
-    run_linear4(lc, x, x_dtype, ldx, x_scale, lds, w, ldw, static_cast<const uint8_t*>(w_tiles), bias, rows, n, k, y, y_dtype, ldy, workspace);
+    FL_CHECK(!products4_failed(), FL_ERR_CUDA, "a wait inside an operator's kernel ran out: a product since the last check is not valid");
+    run_linear4(lc, x, x_dtype, ldx, x_scale, lds, w, ldw, static_cast<const uint8_t*>(w_tiles), bias, rows, n, k, y, y_dtype, ldy, workspace, g_op4_failed.word);
     FL_API_END
 }
 

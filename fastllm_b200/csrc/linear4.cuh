@@ -1,61 +1,420 @@
 // Matrix product of 4-bit rows with a scale per 32 values (rows4.cuh):
 //   y[r, n] = sum_k x[r, k] w[n, k] (+ b[n]),   x, w the values that the rows stand for, sums in f32, one rounding to the result's type.
+// tcgen05.mma.kind::mxf4: 64 values of K per instruction, products of two e2m1 and two powers of two, accumulators in f32.  As in linear8.cuh the weights are the 128- or
+// 256-row operand: a lane of the accumulators is a weight row.  A k block is 256 values, 128 bytes of a row, and eight scales of it.
+//
+// Scales reach the products through tensor memory.  Of 128 rows and a group of four blocks (128 values) they are 512 bytes, [32 lanes][4 runs of 32 rows][4 blocks], which
+// tcgen05.cp puts into four columns, the same in all four lane quarters; a product names the columns and which half of their words it takes.  scale4_at is that order in
+// memory, so a k block's scales of a tile are one run of 1024 bytes per 128 rows.
 #pragma once
+#include "op_tiles.cuh"
 #include "rows4.cuh"
 
 namespace fl {
 
 struct Linear4Args {
-    int rows, n, blocks;                                        // blocks of 32 values of a row
-    const uint8_t* x; long long ldx;                            // bytes
-    const uint8_t* xs; int x_tile;                              // scales as the tensor cores take them, in tiles of so many rows
-    const uint8_t* w; long long ldw;
-    const uint8_t* ws;                                          // in tiles of 128 rows
-    int groups;                                                 // of four blocks, as the scales' layout counts them
-    const float* bias;                                          // [n] or null
-    void* y; long long ldy; int y_dtype;                        // fl_dtype
+    int rows, n, blocks;                                    // blocks of 32 values of a row
+    const uint8_t *xs, *ws;                                 // scales in the order of scale4_at, xs in tiles of the product's rows, ws of 128
+    int groups;                                             // of four blocks in them (even)
+    const float* bias;                                      // [n] or null
+    void* y; long long ldy; int y_dtype;                    // fl_dtype
+    int* failed;                                            // set when a wait ran out
 };
 
-// 32 x 32 results of a block, a block of 32 values at a time through shared memory
-__global__ void __launch_bounds__(256) linear4_plain_kernel(const Linear4Args a) {
-    __shared__ float xv[32][33], wv[32][33];
-    const int r0 = blockIdx.y * 32, n0 = blockIdx.x * 32, col = threadIdx.x & 31, row = threadIdx.x >> 5;
-    float sum[4] = {};
-    for (int b = 0; b < a.blocks; ++b) {
-        const int i = threadIdx.x / 8, part = threadIdx.x & 7;         // a row's four columns
-        auto fill = [&](const uint8_t* q, long long ld, const uint8_t* scales, int tile, int at, int rows, float (&to)[32][33]) {
-            float s = 0.f;
-            uint32_t w = 0;
-            if (at < rows) {
-                s = down4(scales[scale4_at(at, b / 4, tile, a.groups) + b % 4]);
-                w = reinterpret_cast<const uint16_t*>(q + at * ld + b * 16)[part];
+constexpr int kL4Row = 128;                                 // bytes of a row in a k block: one swizzle row
+constexpr uint32_t kL4WBytes = 128 * kL4Row;                // a box of 128 weight rows
+constexpr uint32_t kL4Scales = 1024;                        // scales of 128 rows in a k block
+
+// Instruction descriptor, kind::mxf4: scale ids of B and A at 4 and 29, both e2m1 (bits 7-9 = 1, 10-11 = 1), K-major, N>>3 at 17, scales are powers of two (bit 23), M>>7 at 27.
+__host__ __device__ constexpr uint32_t umma_idesc_mx4(int M, int N, int half) {
+    return ((uint32_t)(2 * half) << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 7) << 27) | ((uint32_t)(2 * half) << 29);
+}
+// [32 lanes][16 bytes] without a swizzle: 8 x 16 bytes in a row, 128 bytes to the next
+__device__ __forceinline__ uint64_t umma_smem_desc_scales(const void* p) {
+    return (uint64_t)((smem_u32(p) & 0x3FFFF) >> 4) | ((uint64_t)8 << 32) | ((uint64_t)1 << 46);
+}
+// whole warps, one elected lane issues (see uniform_warp); a copy is ordered before the products behind it
+template <int kCtas>
+__device__ __forceinline__ void umma_mx4_warp(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t tmem_sa, uint32_t tmem_sb, uint32_t accumulate) {
+    if constexpr (kCtas == 1)
+        asm volatile(
+            "{\n"
+            ".reg .pred p, e;\n"
+            "setp.ne.b32 p, %6, 0;\n"
+            "elect.sync _|e, 0xFFFFFFFF;\n"
+            "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
+            "}\n" ::"r"(tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n"
+            ".reg .pred p, e;\n"
+            "setp.ne.b32 p, %6, 0;\n"
+            "elect.sync _|e, 0xFFFFFFFF;\n"
+            "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
+            "}\n" ::"r"(tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+            : "memory");
+}
+template <int kCtas>
+__device__ __forceinline__ void tmem_scales_warp(uint32_t tmem, uint64_t desc) {
+    if constexpr (kCtas == 1)
+        asm volatile(
+            "{\n"
+            ".reg .pred e;\n"
+            "elect.sync _|e, 0xFFFFFFFF;\n"
+            "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n"
+            "}\n" ::"r"(tmem),
+            "l"(desc)
+            : "memory");
+    else
+        asm volatile(
+            "{\n"
+            ".reg .pred e;\n"
+            "elect.sync _|e, 0xFFFFFFFF;\n"
+            "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n"
+            "}\n" ::"r"(tmem),
+            "l"(desc)
+            : "memory");
+}
+// Results of one weight row n (a lane each) and 16 activation rows from r on
+__device__ __forceinline__ void l4_store16(const Linear4Args& g, int r, int n, int rows, float bn, const uint32_t (&sum)[16]) {
+    float v[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] = g.bias != nullptr ? __uint_as_float(sum[j]) + bn : __uint_as_float(sum[j]);
+    write16(g.y, g.ldy, g.y_dtype, r, n, n < g.n ? rows : 0, v);
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------------------------------
+// As linear8_few_kernel: the weights are nearly all the traffic, BN activation rows the other operand; a cluster of S blocks cuts K of one tile, and its blocks add up
+// each other's parts in order through shared memory.
+template <int BN> struct L4Few {
+    static constexpr uint32_t kX = BN * kL4Row, kSW = kL4WBytes + kX, kStage = kSW + 2 * kL4Scales;     // weights | activations | their scales
+    static constexpr int kPerSm = 2;                                                   // blocks that an SM holds
+    static constexpr uint32_t kRing = 108 * 1024;
+    static constexpr int kStages = kRing / kStage < 8 ? kRing / kStage : 8;
+    static constexpr size_t kSmem = (size_t)kStages * kStage + 1024;
+    static constexpr int kThreads = 192;
+    static constexpr uint32_t kCols = BN + 16 * kStages, kTmem = kCols <= 64 ? 64 : (kCols <= 128 ? 128 : 256);      // every stage has its own columns for scales
+    static_assert(kStages * kStage >= (uint32_t)BN * 512, "the parts of a tile fit the ring");
+    static_assert(kCols <= 256, "two blocks share an SM's tensor memory");
+};
+
+// The accumulators of a block's part of K (all warps call it; those from 2 on are the epilogue's): written, or added up in the cluster.
+template <int BN>
+__device__ __forceinline__ void l4_few_finish(const Linear4Args& g, const int S, int s, int n0, uint32_t tmem, uint8_t* ring, bool ok) {
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    const int row = (warp & 3) * 32 + lane;                                            // accumulator row = weight row of the tile
+    const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const int n = n0 + row;
+    const float bn = warp >= 2 && g.bias != nullptr && n < g.n ? g.bias[n] : 0.f;
+    if (S == 1) {
+        if (warp >= 2 && ok) {
+#pragma unroll 1
+            for (int c = 0; c < BN && c < g.rows; c += 16) {
+                uint32_t v[16];
+                tmem_ld16(at + (uint32_t)c, v);
+                l4_store16(g, c, n, min(g.rows - c, 16), bn, v);
             }
-            float v[8];
-            from_e2m1x8(w, v);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) to[i][part * 4 + j] = v[j] * s;
-        };
-        fill(a.x, a.ldx, a.xs, a.x_tile, r0 + i, a.rows, xv);
-        fill(a.w, a.ldw, a.ws, 128, n0 + i, a.n, wv);
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            const float w = wv[col][j];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) sum[c] = fmaf(xv[row + 8 * c][j], w, sum[c]);
         }
-        __syncthreads();
+        return;
     }
-    const int n = n0 + col;
+    const int per = BN / S;                                                            // columns that one block of the cluster adds up and writes
+    __syncwarp();
+    cluster_sync_all();                                                                // every block's products are done: the rings are free
+    if (warp >= 2) {
+        const uint32_t base = smem_u32(ring) + (uint32_t)(s * per * 128 + row) * 4;
+#pragma unroll 1
+        for (int c = 0; c < BN && c < g.rows; c += 16) {
+            uint32_t v[16];
+            tmem_ld16(at + (uint32_t)c, v);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        const int r = r0 + row + 8 * c;
-        if (r >= a.rows || n >= a.n) continue;
-        const float v = a.bias != nullptr ? sum[c] + a.bias[n] : sum[c];
-        const long long at = (long long)r * a.ldy + n;
-        if (a.y_dtype == 0) reinterpret_cast<float*>(a.y)[at] = v;
-        else if (a.y_dtype == 1) reinterpret_cast<__nv_bfloat16*>(a.y)[at] = from_f32<__nv_bfloat16>(v);
-        else reinterpret_cast<__half*>(a.y)[at] = from_f32<__half>(v);
+            for (int j = 0; j < 16; ++j) {
+                const int owner = (c + j) / per;
+                asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(mapa_u32(base + (uint32_t)((c + j) - owner * per) * 512, owner)), "r"(v[j]) : "memory");
+            }
+        }
+    }
+    __syncwarp();
+    cluster_sync_all();
+    if (warp >= 2 && ok) {
+        const float* part = reinterpret_cast<const float*>(ring) + row;
+#pragma unroll 1
+        for (int c = 0; c < per && s * per + c < g.rows; c += 16) {
+            const int r = s * per + c, cnt = min(min(per - c, 16), g.rows - r);
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = 0.f;
+            for (int t = 0; t < S; ++t) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (j < cnt) v[j] += part[(t * per + c + j) * 128];
+            }
+            if (g.bias != nullptr) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] += bn;
+            }
+            write16(g.y, g.ldy, g.y_dtype, r, n, n < g.n ? cnt : 0, v);
+        }
+    }
+}
+
+template <int BN>
+__global__ void __launch_bounds__(L4Few<BN>::kThreads, L4Few<BN>::kPerSm)
+linear4_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Linear4Args g, const int S) {
+    using L = L4Few<BN>;
+    constexpr int kStages = L::kStages;
+    extern __shared__ uint8_t gsm_raw[];
+    uint8_t* gsm = gsm_raw + ((1024u - (smem_u32(gsm_raw) & 1023u)) & 1023u);          // (the same offset in all blocks of a cluster)
+    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], done;
+    __shared__ uint32_t tmem_base_s;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    const int s = S == 1 ? 0 : (int)cluster_rank();
+    const int tile = blockIdx.x / S, n0 = tile * 128;
+    const int nk = g.groups / 2, kb0 = (int)((long long)s * nk / S), kb1 = (int)((long long)(s + 1) * nk / S);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        mbar_init(&done, 1);
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc(&tmem_base_s, L::kTmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_s;
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            auto weights = [&](int kb, int st) {
+                mbar_expect_tx(&full[st], L::kStage);
+                tma_load_2d(gsm + st * L::kStage, &tmW, kb * kL4Row, n0, &full[st]);
+                bulk_g2s(gsm + st * L::kStage + L::kSW, g.ws + ((long long)tile * nk + kb) * kL4Scales, kL4Scales, &full[st]);
+            };
+            auto rows = [&](int kb, int st) {
+                tma_load_2d(gsm + st * L::kStage + kL4WBytes, &tmX, kb * kL4Row, 0, &full[st]);
+                bulk_g2s(gsm + st * L::kStage + L::kSW + kL4Scales, g.xs + (long long)kb * kL4Scales, kL4Scales, &full[st]);
+            };
+            // the weights do not depend on the kernel that rounds the rows: a ring-full of them is requested ahead of the wait
+            const int pre = min(kb1, kb0 + kStages);
+            for (int kb = kb0; kb < pre; ++kb) weights(kb, kb - kb0);
+            pdl_wait();
+            asm volatile("fence.proxy.async;" ::: "memory");                           // the rows were written through the generic proxy
+            for (int kb = kb0; kb < pre; ++kb) rows(kb, kb - kb0);
+            int st = 0;
+            uint32_t ph = 0;
+            for (int kb = pre; kb < kb1; ++kb) {
+                if (!(ok = mbar_wait_bounded(&empty[st], ph, kMbarTries))) break;
+                weights(kb, st);
+                rows(kb, st);
+                if (++st == kStages) { st = 0; ph ^= 1; }
+            }
+        }
+    } else if (warp == 1) {
+        const uint64_t base = umma_smem_desc_sw128(gsm), scales = umma_smem_desc_scales(gsm + L::kSW);
+        int st = 0;
+        uint32_t ph = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            if (ok) ok = mbar_wait_bounded(&full[st], ph, kMbarTries);
+            __syncwarp();
+            tc_fence_after();
+            const uint64_t at = (uint64_t)(st * (L::kStage >> 4)), a = base + at, b = a + (kL4WBytes >> 4);
+            const uint32_t sa = tmem + BN + 16 * st, sb = sa + 8;                      // (free: what was filled from this stage before has been used up)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                tmem_scales_warp<1>(sa + 4 * i, scales + at + i * (512 >> 4));
+                tmem_scales_warp<1>(sb + 4 * i, scales + at + (kL4Scales >> 4) + i * (512 >> 4));
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                umma_mx4_warp<1>(tmem, a + 2 * q, b + 2 * q, umma_idesc_mx4(128, BN, q & 1), sa + 4 * (q >> 1), sb + 4 * (q >> 1), ((kb - kb0) | q) ? 1u : 0u);
+            umma_commit_warp(&empty[st]);
+            if (++st == kStages) { st = 0; ph ^= 1; }
+        }
+        umma_commit_warp(&done);
+    }
+    if (warp >= 2) {
+        pdl_wait();                                                                    // (no block ends before the kernel that rounds the rows has)
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&done, 0, kMbarTries));
+        tc_fence_after();
+    }
+    l4_few_finish<BN>(g, S, s, n0, tmem, gsm, ok);
+    if (!ok) op_give_up(g.failed);
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, L::kTmem);
+    }
+}
+
+// ---- many rows ----------------------------------------------------------------------------------------------------------------------
+// As linear8_pair_kernel: pairs of SMs on tiles of 256 weight rows x bn activation rows, each with its 128 weight rows and half of the activation tile, and the scales
+// of its weight rows and of all the tile's activation rows.
+constexpr int kL4PairEpi = 16, kL4PairThreads = 64 + 32 * kL4PairEpi, kL4PairMaxStages = 8;
+constexpr uint32_t kL4PairRing = 200 * 1024;
+constexpr size_t kL4PairSmem = kL4PairRing + 1024;
+
+struct L4Pair {
+    int bn;                     // activation rows of a tile
+    int parts;                  // products of a tile, bn / parts rows each: 1, with two accumulators in turn, or 2
+    int nk, mt, nt;             // k blocks; weight and activation tiles
+    int stages;
+};
+inline int l4_pair_atoms(int pn) { return (pn + 127) / 128; }
+// bytes of a stage: weights | half of the activations | scales of the weights | of the activations
+inline uint32_t l4_pair_stage(int bn, int parts) { return kL4WBytes + (uint32_t)bn * (kL4Row / 2) + kL4Scales * (uint32_t)(1 + parts * l4_pair_atoms(bn / parts)); }
+// columns of tensor memory: two accumulators, and twice a k block's scales
+inline int l4_pair_cols(int bn, int parts) { return 2 * (bn / parts) + 2 * (8 + 8 * parts * l4_pair_atoms(bn / parts)); }
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kL4PairThreads, 1)
+linear4_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmWS, const __grid_constant__ CUtensorMap tmXS,
+                    const Linear4Args g, const L4Pair p) {
+    extern __shared__ uint8_t gsm_raw[];
+    uint8_t* gsm = gsm_raw + ((1024u - (smem_u32(gsm_raw) & 1023u)) & 1023u);          // (the same offset in both CTAs)
+    __shared__ __align__(8) uint64_t full[kL4PairMaxStages], empty[kL4PairMaxStages], acc_full[2], acc_empty[2];
+    __shared__ uint32_t tmem_base_s;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const int cl = blockIdx.x >> 1, G = gridDim.x >> 1, nk = p.nk, T = p.mt * p.nt, bn = p.bn, parts = p.parts;
+    const int pn = parts == 2 ? bn / 2 : bn, atoms = (pn + 127) / 128;
+    const uint32_t x_bytes = (uint32_t)bn * (kL4Row / 2), stage = kL4WBytes + x_bytes + kL4Scales * (uint32_t)(1 + parts * atoms);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < p.stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 2 * kL4PairEpi); }
+        mbar_fence_init();
+        tma_prefetch_desc(&tmX);
+        tma_prefetch_desc(&tmW);
+        tma_prefetch_desc(&tmXS);
+        tma_prefetch_desc(&tmWS);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_base_s)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_base_s;
+    // 8 activation tiles share a weight tile before the walk moves on (see kGemmRasterRows)
+    auto place = [&](int tile, int& n, int& rt) {
+        constexpr int RM = kGemmRasterRows / 2;
+        const int per = RM * p.mt, first = tile / per * RM, local = tile % per, cnt = min(RM, p.nt - first);
+        rt = first + local % cnt;
+        n = local / cnt * 256 + (int)rank * 128;
+    };
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            pdl_wait();
+            asm volatile("fence.proxy.async;" ::: "memory");
+            int st = 0;
+            uint32_t ph = 1;
+            const int w_last = (g.n + 127) / 128 - 1, x_last = (g.rows + pn - 1) / pn - 1;     // scales exist for tiles that hold a row
+            for (int tile = cl; ok && tile < T; tile += G) {
+                int n0, rt;
+                place(tile, n0, rt);
+                const int r0 = rt * bn + (int)rank * (pn >> 1);
+                const int ws0 = min(n0 / 128, w_last) * nk * 2, xs0 = min(rt * parts, x_last) * nk * 2 * atoms, xs1 = min(rt * parts + 1, x_last) * nk * 2 * atoms;
+                for (int kb = 0; kb < nk; ++kb) {
+                    if (!(ok = pair_wait(&empty[st], ph))) break;
+                    if (rank == 0) mbar_expect_tx(&full[st], 2 * stage);               // both CTAs' loads complete on the first one's barrier
+                    const uint32_t bar = mapa_u32(smem_u32(&full[st]), 0), sa = smem_u32(gsm) + st * stage, ss = sa + kL4WBytes + x_bytes;
+                    tma_load_2d_pair(sa, &tmW, kb * kL4Row, n0, bar);
+                    tma_load_2d_pair(sa + kL4WBytes, &tmX, kb * kL4Row, r0, bar);
+                    if (parts == 2) tma_load_2d_pair(sa + kL4WBytes + (uint32_t)pn * (kL4Row / 2), &tmX, kb * kL4Row, r0 + pn, bar);
+                    tma_load_2d_pair(ss, &tmWS, 0, ws0 + 2 * kb, bar);
+                    tma_load_2d_pair(ss + kL4Scales, &tmXS, 0, xs0 + 2 * atoms * kb, bar);
+                    if (parts == 2) tma_load_2d_pair(ss + kL4Scales * (1 + atoms), &tmXS, 0, xs1 + 2 * atoms * kb, bar);
+                    if (++st == p.stages) { st = 0; ph ^= 1; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {
+            const uint32_t second = ((uint32_t)pn * (kL4Row / 2)) >> 4, id0 = umma_idesc_mx4(256, pn, 0), id1 = umma_idesc_mx4(256, pn, 1);
+            const uint32_t scale_cols = 8 + 8 * parts * atoms, scale0 = tmem_base + 2 * pn;
+            const uint64_t base = umma_smem_desc_sw128(gsm), scales = umma_smem_desc_scales(gsm + kL4WBytes + x_bytes);
+            int st = 0, back = 0;                                                      // back: the stage of two k blocks ago
+            uint32_t ph = 0, back_ph = 0, seg = 0;
+            int count = 0;
+            auto wait = [&](uint64_t* bar, uint32_t parity) {
+                if (ok) ok = pair_wait(bar, parity);
+                __syncwarp();
+                tc_fence_after();
+            };
+            for (int tile = cl; tile < T; tile += G, ++seg) {
+                const uint32_t as = parts == 2 ? 0 : seg & 1, uses = parts == 2 ? seg : seg >> 1, tacc = tmem_base + as * pn;
+                wait(&acc_empty[as], (uses & 1) ^ 1);
+                if (parts == 2) wait(&acc_empty[1], (uses & 1) ^ 1);
+                for (int kb = 0; kb < nk; ++kb, ++count) {
+                    wait(&full[st], ph);
+                    if (count >= 2) {                                                  // the columns for scales are free when the products of two k blocks ago are done
+                        wait(&empty[back], back_ph);
+                        if (++back == p.stages) { back = 0; back_ph ^= 1; }
+                    }
+                    const uint64_t at = (uint64_t)(st * (stage >> 4)), a = base + at, b = a + (kL4WBytes >> 4);
+                    const uint32_t sa = scale0 + (count & 1) * scale_cols, sb = sa + 8;
+                    // columns: weights' groups 0 and 1, then for each product and group the atoms of its rows
+                    tmem_scales_warp<2>(sa, scales + at);
+                    tmem_scales_warp<2>(sa + 4, scales + at + (512 >> 4));
+                    for (int i = 0; i < 2 * parts * atoms; ++i) tmem_scales_warp<2>(sb + 4 * i, scales + at + (kL4Scales >> 4) + i * (512 >> 4));
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        umma_mx4_warp<2>(tacc, a + 2 * q, b + 2 * q, (q & 1) ? id1 : id0, sa + 4 * (q >> 1), sb + 4 * atoms * (q >> 1), (kb | q) ? 1u : 0u);
+                    if (parts == 2) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            umma_mx4_warp<2>(tacc + pn, a + 2 * q, b + second + 2 * q, (q & 1) ? id1 : id0, sa + 4 * (q >> 1), sb + 8 * atoms + 4 * atoms * (q >> 1), (kb | q) ? 1u : 0u);
+                    }
+                    umma_commit_pair_warp(&empty[st]);
+                    if (++st == p.stages) { st = 0; ph ^= 1; }
+                }
+                umma_commit_pair_warp(&acc_full[as]);
+                if (parts == 2) umma_commit_pair_warp(&acc_full[1]);
+            }
+        }
+    } else {
+        const int q = warp & 3, cs = (warp - 2) >> 2;                                  // TMEM lane quarter (hardware rule); every fourth run of 16 columns
+        uint32_t seg = 0;
+        pdl_wait();                                                                    // (no block ends before the kernel that rounds the rows has)
+        for (int tile = cl; tile < T; tile += G, ++seg) {
+            int n0, rt;
+            place(tile, n0, rt);
+            const int n = n0 + q * 32 + lane;
+            const float bias = g.bias != nullptr && n < g.n ? __ldg(g.bias + n) : 0.f;
+            for (int h = 0; h < parts; ++h) {
+                const uint32_t as = parts == 2 ? (uint32_t)h : seg & 1, uses = parts == 2 ? seg : seg >> 1;
+                const int r0 = rt * bn + h * pn, last_col = min(pn, g.rows - r0);
+                if (ok) ok = __all_sync(0xFFFFFFFFu, pair_wait(&acc_full[as], uses & 1));
+                tc_fence_after();
+                const uint32_t at = tmem_base + as * pn + ((uint32_t)(q * 32) << 16);
+#pragma unroll 1
+                for (int c = cs * 16; ok && c < last_col; c += 64) {
+                    uint32_t v[16];
+                    tmem_ld16(at + (uint32_t)c, v);
+                    l4_store16(g, r0 + c, n, min(last_col - c, 16), bias, v);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[as]), 0));
+            }
+        }
+    }
+    if (!ok) op_give_up(g.failed);
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();          // the other CTA's products read this one's shared memory, its epilogue arrives on this one's barriers
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u) : "memory");
     }
 }
 

@@ -6,7 +6,7 @@
 // one rounding to the result's type.
 #pragma once
 #include "gemm_pair.cuh"
-#include "op_values.cuh"
+#include "op_tiles.cuh"
 
 namespace fl {
 
@@ -175,38 +175,6 @@ __device__ __forceinline__ void umma_i8_pair_warp(uint32_t tmem_d, uint64_t ades
         "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// Results of one weight row n (a lane each) and 16 activation rows r, r + 1, .. with the scales xs (shared memory, 16-byte border): for a fixed row the 32
-// lanes write 32 neighbours.  (16-bit results in twos, after an exchange between neighbouring lanes, took as long or longer: 64 x 152064 20 -> 26 us.)
-__device__ __forceinline__ void l8_write16(const Linear8Args& g, int r, int n, int rows, const float (&v)[16]) {
-    if (g.y_dtype == 0) {
-        float* o = reinterpret_cast<float*>(g.y) + (long long)r * g.ldy + n;
-        if (rows == 16) {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) { *o = v[j]; o += g.ldy; }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                if (j < rows) *o = v[j];
-                o += g.ldy;
-            }
-        }
-        return;
-    }
-    uint16_t* o = reinterpret_cast<uint16_t*>(g.y) + (long long)r * g.ldy + n;
-#pragma unroll
-    for (int j = 0; j < 16; j += 2) {
-        uint32_t w;
-        if (g.y_dtype == 1) {
-            w = pack_bf16x2(v[j], v[j + 1]);
-        } else {
-            const __half2 h = __floats2half2_rn(v[j], v[j + 1]);
-            w = *reinterpret_cast<const uint32_t*>(&h);
-        }
-        if (j < rows) o[0] = (uint16_t)w;
-        if (j + 1 < rows) o[g.ldy] = (uint16_t)(w >> 16);
-        o += 2 * g.ldy;
-    }
-}
 __device__ __forceinline__ void l8_store16(const Linear8Args& g, int r, int n, const float* xs, float wsn, float bn, const uint32_t (&sum)[16]) {
     float v[16];
 #pragma unroll
@@ -221,14 +189,8 @@ __device__ __forceinline__ void l8_store16(const Linear8Args& g, int r, int n, c
 #pragma unroll
         for (int j = 0; j < 16; ++j) v[j] += bn;
     }
-    l8_write16(g, r, n, n < g.n ? min(g.rows - r, 16) : 0, v);
+    write16(g.y, g.ldy, g.y_dtype, r, n, n < g.n ? min(g.rows - r, 16) : 0, v);
 }
-// A wait ran out: report it and leave the copies in flight time to land; the block goes on to its end.
-__device__ __forceinline__ void l8_give_up(int* failed) {
-    if ((threadIdx.x & 31) == 0) *failed = 1;
-    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-}
-
 // ---- few rows -----------------------------------------------------------------------------------------------------------------------
 // The weights are nearly all the traffic, BN activation rows the other operand; a cluster of S blocks cuts K of one tile, and its blocks add up each
 // other's parts through shared memory: whole numbers, so the order does not matter, and no workspace.  What bounds it: HBM behind 4 to 6 us of
@@ -304,7 +266,7 @@ __device__ __forceinline__ void l8_few_finish(const Linear8Args& g, const int S,
                 v[j] = j < cnt ? (float)sum[j] * xs[s * per + c + j] * wsn : 0.f;
                 if (g.bias != nullptr) v[j] += bn;
             }
-            l8_write16(g, r, n, n < g.n ? cnt : 0, v);
+            write16(g.y, g.ldy, g.y_dtype, r, n, n < g.n ? cnt : 0, v);
         }
     }
 }
@@ -383,7 +345,7 @@ linear8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         tc_fence_after();
     }
     l8_few_finish<BN>(g, S, s, n0, tmem, gsm, xs[max(warp - 2, 0)], ok);
-    if (!ok) l8_give_up(g.failed);
+    if (!ok) op_give_up(g.failed);
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -675,7 +637,7 @@ linear8_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             }
         }
     }
-    if (!ok) l8_give_up(g.failed);
+    if (!ok) op_give_up(g.failed);
     __syncwarp();
     tc_fence_before();
     __syncthreads();

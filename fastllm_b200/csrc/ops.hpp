@@ -15,4 +15,7 @@ void op_linear8(LaunchCtx& lc, const float* x, const int8_t* w, const float* w_s
 void op_logprobs(LaunchCtx& lc, const float* logits, int64_t rows, int64_t vocab, const int32_t* tokens, int64_t given, double temperature, int top, float* logprob,
                  float* logsumexp, float* entropy, int32_t* top_ids, float* top_logprobs);
 
+// whether a wait in a 4-bit product's kernel ran out since this was last asked
+bool products4_failed();
+
 }  // namespace fl

@@ -66,7 +66,7 @@ size_t linear4_workspace(int64_t rows, int64_t k) { return linear4_room(rows, k,
 // How a product of more than kL4FewRows rows goes over the pairs of SMs: the tile width whose waves cost least, by what a k block takes.
 constexpr int kL4FewRows = 128;
 static L4Pair pair_plan4(int64_t rows, int64_t n, int64_t k, int clusters) {
-    static constexpr struct { int bn, parts; } kForms[] = {{416, 2}, {384, 2}, {320, 2}, {256, 2}, {224, 1}, {192, 1}, {160, 1}, {128, 1}, {96, 1}, {64, 1}};
+    static constexpr struct { int bn, parts; } kForms[] = {{416, 2}, {384, 2}, {320, 2}, {256, 2}, {224, 1}, {208, 1}, {192, 1}, {160, 1}, {128, 1}, {96, 1}, {64, 1}};
     L4Pair best{};
     double cost = -1;
     for (const auto& f : kForms) {
@@ -77,6 +77,7 @@ static L4Pair pair_plan4(int64_t rows, int64_t n, int64_t k, int clusters) {
         p.mt = (int)((n + 255) / 256);
         p.nt = (int)((rows + f.bn - 1) / f.bn);
         p.stages = (int)std::min<uint32_t>(kL4PairMaxStages, kL4PairRing / l4_pair_stage(f.bn, f.parts));
+        p.slots = std::min(l4_pair_slots(f.bn, f.parts), p.stages);
         const double block = std::max(1.38 * f.bn, l4_pair_stage(f.bn, f.parts) / 90.0), tail = f.parts == 2 ? 13.0 * f.bn : 0.0;      // ns; results that no product hides
         const double waves = (double)(((long long)p.mt * p.nt + clusters - 1) / clusters);
         const double c = waves * (p.nk * block + tail);
@@ -107,7 +108,9 @@ static void launch_pair4(LaunchCtx& lc, uint64_t bytes, const uint8_t* x, int64_
     const CUtensorMap tx = make_tmap_i8(x, g.rows, g.blocks * 16, ldx, pn / 2), tw = make_tmap_i8(w, g.n, g.blocks * 16, ldw, 128);
     const CUtensorMap tws = make_tmap_scales(g.ws, (int64_t)((g.n + 127) / 128) * g.groups, 2), txs = make_tmap_scales(g.xs, (int64_t)((g.rows + pn - 1) / pn) * g.groups * atoms, 2 * atoms);
     const long long clusters = std::min<long long>(g_pair_clusters, (long long)p.mt * p.nt);
-    launch_op(lc, "linear4", bytes, linear4_pair_kernel, dim3((unsigned)(2 * clusters)), kL4PairThreads, kL4PairSmem, 1, true, tw, tx, tws, txs, g, p);
+    auto go = [&](auto kern) { launch_op(lc, "linear4", bytes, kern, dim3((unsigned)(2 * clusters)), kL4PairThreads, kL4PairSmem, 1, true, tw, tx, tws, txs, g, p); };
+    if (p.parts == 1) atoms == 1 ? go(linear4_pair_kernel<1, 1>) : go(linear4_pair_kernel<1, 2>);
+    else atoms == 1 ? go(linear4_pair_kernel<2, 1>) : go(linear4_pair_kernel<2, 2>);
 }
 
 // x in 4 bits: lds its scales' row stride
@@ -155,7 +158,8 @@ static void set_up() {
         by_type(dtype, [](auto t) { load_kernels(quantize4_kernel<decltype(t)>); load_kernels(dequantize4_kernel<decltype(t)>); load_kernels(glu4_kernel<decltype(t)>); });
     load_kernels(arrange4_kernel);
     few_attr4<16>(); few_attr4<32>(); few_attr4<64>(); few_attr4<128>();
-    FL_CUDA(cudaFuncSetAttribute(linear4_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL4PairSmem));
+    for (auto kern : {linear4_pair_kernel<1, 1>, linear4_pair_kernel<1, 2>, linear4_pair_kernel<2, 1>, linear4_pair_kernel<2, 2>})
+        FL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL4PairSmem));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(kNumSMs); cfg.blockDim = dim3(kL4PairThreads); cfg.dynamicSmemBytes = kL4PairSmem;
     cudaLaunchAttribute at[1];
@@ -163,7 +167,7 @@ static void set_up() {
     at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = 1;
     int pairs = 0;
-    FL_CUDA(cudaOccupancyMaxActiveClusters(&pairs, linear4_pair_kernel, &cfg));
+    FL_CUDA(cudaOccupancyMaxActiveClusters(&pairs, linear4_pair_kernel<2, 2>, &cfg));
     g_pair_clusters = std::min(pairs, kNumSMs / 2);
     int* p = nullptr;
     FL_CUDA(cudaMallocHost(&p, sizeof(int)));

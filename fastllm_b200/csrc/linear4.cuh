@@ -33,50 +33,75 @@ __host__ __device__ constexpr uint32_t umma_idesc_mx4(int M, int N, int half) {
 __device__ __forceinline__ uint64_t umma_smem_desc_scales(const void* p) {
     return (uint64_t)((smem_u32(p) & 0x3FFFF) >> 4) | ((uint64_t)8 << 32) | ((uint64_t)1 << 46);
 }
-// whole warps, one elected lane issues (see uniform_warp); a copy is ordered before the products behind it
-template <int kCtas>
-__device__ __forceinline__ void umma_mx4_warp(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t tmem_sa, uint32_t tmem_sb, uint32_t accumulate) {
-    if constexpr (kCtas == 1)
-        asm volatile(
-            "{\n"
-            ".reg .pred p, e;\n"
-            "setp.ne.b32 p, %6, 0;\n"
-            "elect.sync _|e, 0xFFFFFFFF;\n"
-            "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
-            "}\n" ::"r"(tmem_d),
-            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
-            : "memory");
-    else
-        asm volatile(
-            "{\n"
-            ".reg .pred p, e;\n"
-            "setp.ne.b32 p, %6, 0;\n"
-            "elect.sync _|e, 0xFFFFFFFF;\n"
-            "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
-            "}\n" ::"r"(tmem_d),
-            "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
-            : "memory");
+// Issued by the lane that `lead` marks, in whole warps (see uniform_warp).  One election for all of a k block's instructions: an election each made the issuing warp's
+// way through a k block, 690 clocks with all its waits, longer than the products.
+__device__ __forceinline__ uint32_t elect_lead() {
+    uint32_t e;
+    asm volatile(
+        "{\n"
+        ".reg .pred e;\n"
+        "elect.sync _|e, 0xFFFFFFFF;\n"
+        "selp.u32 %0, 1, 0, e;\n"
+        "}\n"
+        : "=r"(e));
+    return e;
 }
+// The four products of a k block: 32 bytes of every operand row each, groups of four scales in columns sa (weights) and sb, sa + 4 and sb + step, two scales of a group at
+// a time (id0, id1)
 template <int kCtas>
-__device__ __forceinline__ void tmem_scales_warp(uint32_t tmem, uint64_t desc) {
-    if constexpr (kCtas == 1)
-        asm volatile(
-            "{\n"
-            ".reg .pred e;\n"
-            "elect.sync _|e, 0xFFFFFFFF;\n"
-            "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n"
-            "}\n" ::"r"(tmem),
-            "l"(desc)
-            : "memory");
-    else
-        asm volatile(
-            "{\n"
-            ".reg .pred e;\n"
-            "elect.sync _|e, 0xFFFFFFFF;\n"
-            "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n"
-            "}\n" ::"r"(tmem),
-            "l"(desc)
-            : "memory");
+__device__ __forceinline__ void umma_mx4_block(uint32_t lead, uint32_t acc, uint64_t a, uint64_t b, uint32_t id0, uint32_t id1, uint32_t sa, uint32_t sb, uint32_t step, uint32_t accumulate) {
+#define FL_MX4_BLOCK(ctas)                                                                                                    \
+    asm volatile(                                                                                                             \
+        "{\n"                                                                                                                 \
+        ".reg .pred p, e, t;\n"                                                                                               \
+        ".reg .b64 x, y;\n"                                                                                                   \
+        ".reg .b32 u, v;\n"                                                                                                   \
+        "setp.ne.b32 e, %8, 0;\n"                                                                                             \
+        "setp.ne.b32 p, %7, 0;\n"                                                                                             \
+        "setp.eq.b32 t, 0, 0;\n"                                                                                              \
+        "@e tcgen05.mma.cta_group::" ctas ".kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n"          \
+        "add.s64 x, %1, 2; add.s64 y, %2, 2;\n"                                                                               \
+        "@e tcgen05.mma.cta_group::" ctas ".kind::mxf4.block_scale.scale_vec::2X [%0], x, y, %4, [%5], [%6], t;\n"            \
+        "add.s64 x, %1, 4; add.s64 y, %2, 4; add.u32 u, %5, 4; add.u32 v, %6, %9;\n"                                          \
+        "@e tcgen05.mma.cta_group::" ctas ".kind::mxf4.block_scale.scale_vec::2X [%0], x, y, %3, [u], [v], t;\n"              \
+        "add.s64 x, %1, 6; add.s64 y, %2, 6;\n"                                                                               \
+        "@e tcgen05.mma.cta_group::" ctas ".kind::mxf4.block_scale.scale_vec::2X [%0], x, y, %4, [u], [v], t;\n"              \
+        "}\n" ::"r"(acc),                                                                                                     \
+        "l"(a), "l"(b), "r"(id0), "r"(id1), "r"(sa), "r"(sb), "r"(accumulate), "r"(lead), "r"(step)                           \
+        : "memory")
+    if constexpr (kCtas == 1) FL_MX4_BLOCK("1");
+    else FL_MX4_BLOCK("2");
+#undef FL_MX4_BLOCK
+}
+// two groups' scales of 128 rows, 512 bytes each, into columns tmem and tmem + step; copies are ordered before the products behind them
+template <int kCtas>
+__device__ __forceinline__ void tmem_scales(uint32_t lead, uint32_t tmem, uint32_t step, uint64_t desc, uint32_t desc_step) {
+#define FL_SCALES(ctas)                                                                   \
+    asm volatile(                                                                         \
+        "{\n"                                                                             \
+        ".reg .pred e;\n"                                                                 \
+        ".reg .b64 d;\n"                                                                  \
+        ".reg .b32 c;\n"                                                                  \
+        "setp.ne.b32 e, %2, 0;\n"                                                         \
+        "@e tcgen05.cp.cta_group::" ctas ".32x128b.warpx4 [%0], %1;\n"                    \
+        "add.s64 d, %1, %4; add.u32 c, %0, %3;\n"                                         \
+        "@e tcgen05.cp.cta_group::" ctas ".32x128b.warpx4 [c], d;\n"                      \
+        "}\n" ::"r"(tmem),                                                                \
+        "l"(desc), "r"(lead), "r"(step), "l"((uint64_t)desc_step)                         \
+        : "memory")
+    if constexpr (kCtas == 1) FL_SCALES("1");
+    else FL_SCALES("2");
+#undef FL_SCALES
+}
+__device__ __forceinline__ void umma_commit_lead(uint32_t lead, uint64_t* bar) {
+    asm volatile("{\n.reg .pred e;\nsetp.ne.b32 e, %1, 0;\n@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)), "r"(lead) : "memory");
+}
+// arrives on the barrier of both CTAs
+__device__ __forceinline__ void umma_commit_pair_lead(uint32_t lead, uint64_t* bar) {
+    asm volatile(
+        "{\n.reg .pred e;\nsetp.ne.b32 e, %1, 0;\n@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n}\n" ::"r"(smem_u32(bar)),
+        "r"(lead), "h"((uint16_t)3)
+        : "memory");
 }
 // Results of one weight row n (a lane each) and 16 activation rows from r on
 __device__ __forceinline__ void l4_store16(const Linear4Args& g, int r, int n, int rows, float bn, const uint32_t (&sum)[16]) {
@@ -214,26 +239,21 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
         }
     } else if (warp == 1) {
         const uint64_t base = umma_smem_desc_sw128(gsm), scales = umma_smem_desc_scales(gsm + L::kSW);
+        const uint32_t lead = elect_lead();
         int st = 0;
         uint32_t ph = 0;
         for (int kb = kb0; kb < kb1; ++kb) {
             if (ok) ok = mbar_wait_bounded(&full[st], ph, kMbarTries);
             __syncwarp();
-            tc_fence_after();
             const uint64_t at = (uint64_t)(st * (L::kStage >> 4)), a = base + at, b = a + (kL4WBytes >> 4);
             const uint32_t sa = tmem + BN + 16 * st, sb = sa + 8;                      // (free: what was filled from this stage before has been used up)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                tmem_scales_warp<1>(sa + 4 * i, scales + at + i * (512 >> 4));
-                tmem_scales_warp<1>(sb + 4 * i, scales + at + (kL4Scales >> 4) + i * (512 >> 4));
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                umma_mx4_warp<1>(tmem, a + 2 * q, b + 2 * q, umma_idesc_mx4(128, BN, q & 1), sa + 4 * (q >> 1), sb + 4 * (q >> 1), ((kb - kb0) | q) ? 1u : 0u);
-            umma_commit_warp(&empty[st]);
+            tmem_scales<1>(lead, sa, 4, scales + at, 512 >> 4);
+            tmem_scales<1>(lead, sb, 4, scales + at + (kL4Scales >> 4), 512 >> 4);
+            umma_mx4_block<1>(lead, tmem, a, b, umma_idesc_mx4(128, BN, 0), umma_idesc_mx4(128, BN, 1), sa, sb, 4, kb > kb0 ? 1u : 0u);
+            umma_commit_lead(lead, &empty[st]);
             if (++st == kStages) { st = 0; ph ^= 1; }
         }
-        umma_commit_warp(&done);
+        umma_commit_lead(lead, &done);
     }
     if (warp >= 2) {
         pdl_wait();                                                                    // (no block ends before the kernel that rounds the rows has)
@@ -262,14 +282,28 @@ struct L4Pair {
     int bn;                     // activation rows of a tile
     int parts;                  // products of a tile, bn / parts rows each: 1, with two accumulators in turn, or 2
     int nk, mt, nt;             // k blocks; weight and activation tiles
-    int stages;
+    int stages, slots;          // of the ring; k blocks whose scales tensor memory holds
 };
 inline int l4_pair_atoms(int pn) { return (pn + 127) / 128; }
 // bytes of a stage: weights | half of the activations | scales of the weights | of the activations
 inline uint32_t l4_pair_stage(int bn, int parts) { return kL4WBytes + (uint32_t)bn * (kL4Row / 2) + kL4Scales * (uint32_t)(1 + parts * l4_pair_atoms(bn / parts)); }
-// columns of tensor memory: two accumulators, and twice a k block's scales
-inline int l4_pair_cols(int bn, int parts) { return 2 * (bn / parts) + 2 * (8 + 8 * parts * l4_pair_atoms(bn / parts)); }
+// k blocks whose scales find a place in tensor memory beside two accumulators
+inline int l4_pair_slots(int bn, int parts) { return (512 - 2 * (bn / parts)) / (8 + 8 * parts * l4_pair_atoms(bn / parts)); }
 
+__device__ __forceinline__ void expect_tx_lead(uint32_t lead, uint32_t bar, uint32_t bytes) {
+    asm volatile("{\n.reg .pred e;\nsetp.ne.b32 e, %2, 0;\n@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}\n" ::"r"(bar), "r"(bytes), "r"(lead) : "memory");
+}
+// completes on a barrier of the pair's first CTA (mbar: its shared::cluster address)
+__device__ __forceinline__ void tma_load_2d_pair_lead(uint32_t lead, uint32_t dst, const CUtensorMap* tmap, int c0, int c1, uint32_t mbar) {
+    asm volatile(
+        "{\n.reg .pred e;\nsetp.ne.b32 e, %5, 0;\n"
+        "@e cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n}\n" ::"r"(dst),
+        "l"(tmap), "r"(c0), "r"(c1), "r"(mbar), "r"(lead)
+        : "memory");
+}
+
+// kParts, kAtoms: L4Pair's parts and l4_pair_atoms of a part's rows
+template <int kParts, int kAtoms>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kL4PairThreads, 1)
 linear4_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmWS, const __grid_constant__ CUtensorMap tmXS,
                     const Linear4Args g, const L4Pair p) {
@@ -279,9 +313,8 @@ linear4_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     __shared__ uint32_t tmem_base_s;
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
-    const int cl = blockIdx.x >> 1, G = gridDim.x >> 1, nk = p.nk, T = p.mt * p.nt, bn = p.bn, parts = p.parts;
-    const int pn = parts == 2 ? bn / 2 : bn, atoms = (pn + 127) / 128;
-    const uint32_t x_bytes = (uint32_t)bn * (kL4Row / 2), stage = kL4WBytes + x_bytes + kL4Scales * (uint32_t)(1 + parts * atoms);
+    const int cl = blockIdx.x >> 1, G = gridDim.x >> 1, nk = p.nk, T = p.mt * p.nt, bn = p.bn, pn = bn / kParts;
+    const uint32_t x_bytes = (uint32_t)bn * (kL4Row / 2), stage = kL4WBytes + x_bytes + kL4Scales * (uint32_t)(1 + kParts * kAtoms);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
@@ -311,73 +344,77 @@ linear4_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     bool ok = true;
 
     if (warp == 0) {
-        if (lane == 0) {
-            pdl_wait();
-            asm volatile("fence.proxy.async;" ::: "memory");
-            int st = 0;
-            uint32_t ph = 1;
-            const int w_last = (g.n + 127) / 128 - 1, x_last = (g.rows + pn - 1) / pn - 1;     // scales exist for tiles that hold a row
-            for (int tile = cl; ok && tile < T; tile += G) {
-                int n0, rt;
-                place(tile, n0, rt);
-                const int r0 = rt * bn + (int)rank * (pn >> 1);
-                const int ws0 = min(n0 / 128, w_last) * nk * 2, xs0 = min(rt * parts, x_last) * nk * 2 * atoms, xs1 = min(rt * parts + 1, x_last) * nk * 2 * atoms;
-                for (int kb = 0; kb < nk; ++kb) {
-                    if (!(ok = pair_wait(&empty[st], ph))) break;
-                    if (rank == 0) mbar_expect_tx(&full[st], 2 * stage);               // both CTAs' loads complete on the first one's barrier
-                    const uint32_t bar = mapa_u32(smem_u32(&full[st]), 0), sa = smem_u32(gsm) + st * stage, ss = sa + kL4WBytes + x_bytes;
-                    tma_load_2d_pair(sa, &tmW, kb * kL4Row, n0, bar);
-                    tma_load_2d_pair(sa + kL4WBytes, &tmX, kb * kL4Row, r0, bar);
-                    if (parts == 2) tma_load_2d_pair(sa + kL4WBytes + (uint32_t)pn * (kL4Row / 2), &tmX, kb * kL4Row, r0 + pn, bar);
-                    tma_load_2d_pair(ss, &tmWS, 0, ws0 + 2 * kb, bar);
-                    tma_load_2d_pair(ss + kL4Scales, &tmXS, 0, xs0 + 2 * atoms * kb, bar);
-                    if (parts == 2) tma_load_2d_pair(ss + kL4Scales * (1 + atoms), &tmXS, 0, xs1 + 2 * atoms * kb, bar);
-                    if (++st == p.stages) { st = 0; ph ^= 1; }
-                }
+        const uint32_t lead = elect_lead();
+        pdl_wait();
+        asm volatile("fence.proxy.async;" ::: "memory");
+        int st = 0;
+        uint32_t ph = 1;
+        const int w_last = (g.n + 127) / 128 - 1, x_last = (g.rows + pn - 1) / pn - 1;         // scales exist for tiles that hold a row
+        for (int tile = cl; ok && tile < T; tile += G) {
+            int n0, rt;
+            place(tile, n0, rt);
+            const int r0 = rt * bn + (int)rank * (pn >> 1);
+            const int ws0 = min(n0 / 128, w_last) * nk * 2, xs0 = min(rt * kParts, x_last) * nk * 2 * kAtoms, xs1 = min(rt * kParts + 1, x_last) * nk * 2 * kAtoms;
+            for (int kb = 0; kb < nk; ++kb) {
+                if (!(ok = mbar_wait_bounded(&empty[st], ph, kMbarTries))) break;
+                const uint32_t bar = mapa_u32(smem_u32(&full[st]), 0), sa = smem_u32(gsm) + st * stage, ss = sa + kL4WBytes + x_bytes;
+                if (rank == 0) expect_tx_lead(lead, smem_u32(&full[st]), 2 * stage);                           // both CTAs' loads complete on the first one's barrier
+                tma_load_2d_pair_lead(lead, sa, &tmW, kb * kL4Row, n0, bar);
+                tma_load_2d_pair_lead(lead, sa + kL4WBytes, &tmX, kb * kL4Row, r0, bar);
+                if (kParts == 2) tma_load_2d_pair_lead(lead, sa + kL4WBytes + (uint32_t)pn * (kL4Row / 2), &tmX, kb * kL4Row, r0 + pn, bar);
+                tma_load_2d_pair_lead(lead, ss, &tmWS, 0, ws0 + 2 * kb, bar);
+                tma_load_2d_pair_lead(lead, ss + kL4Scales, &tmXS, 0, xs0 + 2 * kAtoms * kb, bar);
+                if (kParts == 2) tma_load_2d_pair_lead(lead, ss + kL4Scales * (1 + kAtoms), &tmXS, 0, xs1 + 2 * kAtoms * kb, bar);
+                if (++st == p.stages) { st = 0; ph ^= 1; }
             }
         }
     } else if (warp == 1) {
         if (rank == 0) {
             const uint32_t second = ((uint32_t)pn * (kL4Row / 2)) >> 4, id0 = umma_idesc_mx4(256, pn, 0), id1 = umma_idesc_mx4(256, pn, 1);
-            const uint32_t scale_cols = 8 + 8 * parts * atoms, scale0 = tmem_base + 2 * pn;
+            constexpr uint32_t kCols = 8 + 8 * kParts * kAtoms;
+            const uint32_t scale0 = tmem_base + 2 * pn, lead = elect_lead();
             const uint64_t base = umma_smem_desc_sw128(gsm), scales = umma_smem_desc_scales(gsm + kL4WBytes + x_bytes);
-            int st = 0, back = 0;                                                      // back: the stage of two k blocks ago
+            const bool look_back = p.slots < p.stages;
+            int st = 0, back = 0, slot = 0, free = p.slots;                            // back: the stage of p.slots k blocks ago
             uint32_t ph = 0, back_ph = 0, seg = 0;
-            int count = 0;
+            // Both waits of a k block are looked at while the products before it are issued: a look takes 160 clocks even where there is nothing to wait for.
+            bool here = false, unused = false;
             auto wait = [&](uint64_t* bar, uint32_t parity) {
                 if (ok) ok = pair_wait(bar, parity);
                 __syncwarp();
                 tc_fence_after();
             };
             for (int tile = cl; tile < T; tile += G, ++seg) {
-                const uint32_t as = parts == 2 ? 0 : seg & 1, uses = parts == 2 ? seg : seg >> 1, tacc = tmem_base + as * pn;
+                const uint32_t as = kParts == 2 ? 0 : seg & 1, uses = kParts == 2 ? seg : seg >> 1, tacc = tmem_base + as * pn;
                 wait(&acc_empty[as], (uses & 1) ^ 1);
-                if (parts == 2) wait(&acc_empty[1], (uses & 1) ^ 1);
-                for (int kb = 0; kb < nk; ++kb, ++count) {
-                    wait(&full[st], ph);
-                    if (count >= 2) {                                                  // the columns for scales are free when the products of two k blocks ago are done
-                        wait(&empty[back], back_ph);
-                        if (++back == p.stages) { back = 0; back_ph ^= 1; }
-                    }
-                    const uint64_t at = (uint64_t)(st * (stage >> 4)), a = base + at, b = a + (kL4WBytes >> 4);
-                    const uint32_t sa = scale0 + (count & 1) * scale_cols, sb = sa + 8;
-                    // columns: weights' groups 0 and 1, then for each product and group the atoms of its rows
-                    tmem_scales_warp<2>(sa, scales + at);
-                    tmem_scales_warp<2>(sa + 4, scales + at + (512 >> 4));
-                    for (int i = 0; i < 2 * parts * atoms; ++i) tmem_scales_warp<2>(sb + 4 * i, scales + at + (kL4Scales >> 4) + i * (512 >> 4));
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        umma_mx4_warp<2>(tacc, a + 2 * q, b + 2 * q, (q & 1) ? id1 : id0, sa + 4 * (q >> 1), sb + 4 * atoms * (q >> 1), (kb | q) ? 1u : 0u);
-                    if (parts == 2) {
-#pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            umma_mx4_warp<2>(tacc + pn, a + 2 * q, b + second + 2 * q, (q & 1) ? id1 : id0, sa + 4 * (q >> 1), sb + 8 * atoms + 4 * atoms * (q >> 1), (kb | q) ? 1u : 0u);
-                    }
-                    umma_commit_pair_warp(&empty[st]);
+                if (kParts == 2) wait(&acc_empty[1], (uses & 1) ^ 1);
+                for (int kb = 0; kb < nk; ++kb) {
+                    // (no fence behind these two: what they wait for are copies into shared memory and this thread's own products)
+                    if (!here && ok) ok = mbar_wait_bounded(&full[st], ph, kMbarTries);
+                    const int st0 = st;
                     if (++st == p.stages) { st = 0; ph ^= 1; }
+                    if (look_back && free == 0) {                                      // the columns for scales are free when the products that took them last are done
+                        if (!unused && ok) ok = mbar_wait_bounded(&empty[back], back_ph, kMbarTries);
+                        if (++back == p.stages) { back = 0; back_ph ^= 1; }
+                        unused = mbar_test(&empty[back], back_ph);
+                    } else {
+                        --free;
+                    }
+                    here = mbar_test(&full[st], ph);
+                    __syncwarp();
+                    const uint64_t at = (uint64_t)(st0 * (stage >> 4)), a = base + at, b = a + (kL4WBytes >> 4), sd = scales + at;
+                    const uint32_t sa = scale0 + slot * kCols, sb = sa + 8, more = kb > 0 ? 1u : 0u;
+                    if (++slot == p.slots) slot = 0;
+                    // columns: weights' groups 0 and 1, then for each product and group the atoms of its rows
+                    tmem_scales<2>(lead, sa, 4, sd, 512 >> 4);
+#pragma unroll
+                    for (int i = 0; i < kParts * kAtoms; ++i) tmem_scales<2>(lead, sb + 8 * i, 4, sd + (kL4Scales >> 4) * (1 + i), 512 >> 4);
+                    umma_mx4_block<2>(lead, tacc, a, b, id0, id1, sa, sb, 4 * kAtoms, more);
+                    if (kParts == 2) umma_mx4_block<2>(lead, tacc + pn, a, b + second, id0, id1, sa, sb + 8 * kAtoms, 4 * kAtoms, more);
+                    umma_commit_pair_lead(lead, &empty[st0]);
                 }
-                umma_commit_pair_warp(&acc_full[as]);
-                if (parts == 2) umma_commit_pair_warp(&acc_full[1]);
+                umma_commit_pair_lead(lead, &acc_full[as]);
+                if (kParts == 2) umma_commit_pair_lead(lead, &acc_full[1]);
             }
         }
     } else {
@@ -389,8 +426,8 @@ linear4_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             place(tile, n0, rt);
             const int n = n0 + q * 32 + lane;
             const float bias = g.bias != nullptr && n < g.n ? __ldg(g.bias + n) : 0.f;
-            for (int h = 0; h < parts; ++h) {
-                const uint32_t as = parts == 2 ? (uint32_t)h : seg & 1, uses = parts == 2 ? seg : seg >> 1;
+            for (int h = 0; h < kParts; ++h) {
+                const uint32_t as = kParts == 2 ? (uint32_t)h : seg & 1, uses = kParts == 2 ? seg : seg >> 1;
                 const int r0 = rt * bn + h * pn, last_col = min(pn, g.rows - r0);
                 if (ok) ok = __all_sync(0xFFFFFFFFu, pair_wait(&acc_full[as], uses & 1));
                 tc_fence_after();

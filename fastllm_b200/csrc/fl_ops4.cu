@@ -12,7 +12,7 @@
 
 namespace fl {
 
-constexpr int64_t kMaxCols4 = (int64_t)1 << 20;
+constexpr int64_t kMaxCols4 = (int64_t)1 << 20, kMaxNumbers4 = (int64_t)1 << 39;         // (grids of threads of four numbers each, 2^31 - 1 blocks)
 
 static int64_t blocks4(int64_t cols) { return (cols + kR4Block - 1) / kR4Block; }
 static int64_t groups4(int64_t cols) { return 2 * ((blocks4(cols) + 7) / 8); }              // k blocks of 256 values are whole
@@ -20,14 +20,9 @@ static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 // rows that scales in tiles of `tile` rows have room for, in whole 128 rows a tile
 static int64_t slots4(int64_t rows, int tile) { return (rows + tile - 1) / tile * ((tile + 127) / 128 * 128); }
 
-struct Span { dim3 grid; int threads; };
-static Span spans4(int64_t rows, int64_t cols) {
-    const int64_t spans = (cols + kR4Span - 1) / kR4Span;
-    const int warps = (int)std::min<int64_t>(spans, 8);
-    return {dim3((unsigned)rows, (unsigned)((spans + warps - 1) / warps)), 32 * warps};
-}
-template <typename T>
-static bool starts_vec(const void* x, int64_t rows, int64_t ldx) { return aligned(x, 16) && (rows == 1 || ldx * sizeof(T) % 16 == 0); }
+// threads of `per` pieces a row
+static dim3 pieces_grid(int64_t rows, int64_t per) { return dim3((unsigned)((rows * per + kR4Threads - 1) / kR4Threads)); }
+static bool rows_on_16(const void* x, int64_t rows, int64_t ld, size_t size) { return aligned(x, 16) && (rows == 1 || ld * size % 16 == 0); }
 
 // f(T{}) with the element type of a float dtype
 template <typename F>
@@ -38,11 +33,27 @@ static void by_type(int dtype, F f) {
 }
 
 static void quantize4(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, const Rows4Out& o) {
-    const Span s = spans4(rows, o.tile > 0 ? (int64_t)o.groups * 128 : cols);
+    const int64_t per = o.tile > 0 ? o.groups * 4 : o.blocks;                  // (tiles hold scales of whole k blocks)
     by_type(dtype, [&](auto t) {
         using T = decltype(t);
-        launch_op(lc, "quantize4", (uint64_t)rows * (cols * sizeof(T) + o.blocks * 17), quantize4_kernel<T>, s.grid, s.threads, 0, 1, false, static_cast<const T*>(x), (long long)ldx, (int)cols,
-                  starts_vec<T>(x, rows, ldx), o);
+        launch_op(lc, "quantize4", (uint64_t)rows * (cols * sizeof(T) + o.blocks * 17), rows_on_16(x, rows, ldx, sizeof(T)) ? quantize4_kernel<T, true> : quantize4_kernel<T, false>,
+                  pieces_grid(rows, per), kR4Threads, 0, 1, false, static_cast<const T*>(x), (long long)ldx, (long long)rows, (int)cols, (int)per, o);
+    });
+}
+
+template <typename T, bool kVec>
+static void (*glu4_form(int act))(const T*, long long, long long, int, int, float, Rows4Out) {
+    if (act == FL_ACT_SILU) return glu4_kernel<T, kGlu4Silu, kVec>;
+    if (act == FL_ACT_GELU_TANH) return glu4_kernel<T, kGlu4GeluTanh, kVec>;
+    if (act == FL_ACT_RELU) return glu4_kernel<T, kGlu4Relu, kVec>;
+    return glu4_kernel<T, kGlu4SwishClamp, kVec>;
+}
+static void glu4(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int act, float limit, const Rows4Out& o) {
+    by_type(dtype, [&](auto t) {
+        using T = decltype(t);
+        const bool vec = rows_on_16(x, rows, ldx, sizeof(T)) && cols * sizeof(T) % 16 == 0;
+        launch_op(lc, "glu4", (uint64_t)rows * (2 * cols * sizeof(T) + o.blocks * 17), vec ? glu4_form<T, true>(act) : glu4_form<T, false>(act), pieces_grid(rows, o.blocks), kR4Threads, 0, 1, false,
+                  static_cast<const T*>(x), (long long)ldx, (long long)rows, (int)cols, o.blocks, limit, o);
     });
 }
 
@@ -155,7 +166,12 @@ static void set_up() {
     if (done.load(std::memory_order_relaxed)) return;
     RelaxedCapture relaxed;
     for (int dtype : {FL_DTYPE_F32, FL_DTYPE_BF16, FL_DTYPE_F16})
-        by_type(dtype, [](auto t) { load_kernels(quantize4_kernel<decltype(t)>); load_kernels(dequantize4_kernel<decltype(t)>); load_kernels(glu4_kernel<decltype(t)>); });
+        by_type(dtype, [](auto t) {
+            using T = decltype(t);
+            load_kernels(quantize4_kernel<T, false>, quantize4_kernel<T, true>);
+            load_kernels(dequantize4_kernel<T, false>, dequantize4_kernel<T, true>);
+            for (int act : {FL_ACT_SILU, FL_ACT_GELU_TANH, FL_ACT_RELU, FL_ACT_SWISH_CLAMP}) load_kernels(glu4_form<T, false>(act), glu4_form<T, true>(act));
+        });
     load_kernels(arrange4_kernel);
     few_attr4<16>(); few_attr4<32>(); few_attr4<64>(); few_attr4<128>();
     for (auto kern : {linear4_pair_kernel<1, 1>, linear4_pair_kernel<1, 2>, linear4_pair_kernel<2, 1>, linear4_pair_kernel<2, 2>})
@@ -191,6 +207,7 @@ FL_EXPORT int fl_quantize4(const void* x, int dtype, int64_t rows, int64_t cols,
     FL_API_BEGIN
     FL_CHECK(is_float(dtype), FL_ERR_INVALID, "quantize4: rows of f32, bf16 or f16");
     FL_CHECK(rows >= 0 && rows <= kMaxRows && cols >= 1 && cols <= kMaxCols4, FL_ERR_INVALID, "quantize4: rows from 0 to 2^30, columns from 1 to 2^20");
+    FL_CHECK(rows <= kMaxNumbers4 / cols, FL_ERR_INVALID, "quantize4: more than 2^39 numbers");
     FL_CHECK(rows <= 1 || ldx >= cols, FL_ERR_INVALID, "quantize4: the row stride is smaller than the row");
     if (rows == 0) return FL_OK;
     FL_CHECK(x && q && scale, FL_ERR_INVALID, "NULL argument");
@@ -207,6 +224,7 @@ FL_EXPORT int fl_dequantize4(const uint8_t* q, int64_t ldq, const uint8_t* scale
     FL_API_BEGIN
     FL_CHECK(is_float(dtype), FL_ERR_INVALID, "dequantize4: results are f32, bf16 or f16");
     FL_CHECK(rows >= 0 && rows <= kMaxRows && cols >= 1 && cols <= kMaxCols4, FL_ERR_INVALID, "dequantize4: rows from 0 to 2^30, columns from 1 to 2^20");
+    FL_CHECK(rows <= kMaxNumbers4 / cols, FL_ERR_INVALID, "dequantize4: more than 2^39 numbers");
     FL_CHECK(rows <= 1 || ldy >= cols, FL_ERR_INVALID, "dequantize4: the row stride is smaller than the row");
     if (rows == 0) return FL_OK;
     FL_CHECK(q && scale && y, FL_ERR_INVALID, "NULL argument");
@@ -215,11 +233,13 @@ FL_EXPORT int fl_dequantize4(const uint8_t* q, int64_t ldq, const uint8_t* scale
     DeviceScope dev;
     set_up();
     LaunchCtx lc = op_ctx(stream);
-    const Span s = spans4(rows, cols);
     by_type(dtype, [&](auto t) {
         using T = decltype(t);
-        launch_op(lc, "dequantize4", (uint64_t)rows * (cols * sizeof(T) + blocks4(cols) * 17), dequantize4_kernel<T>, s.grid, s.threads, 0, 1, false, q, (long long)ldq, scale, (long long)lds,
-                  (int)cols, static_cast<T*>(y), (long long)ldy, starts_vec<T>(y, rows, ldy));
+        constexpr int V = 16 / sizeof(T);
+        const bool shift = !rows_on_16(y, rows, ldy, sizeof(T));
+        const int64_t per = (cols + (shift ? V - 1 : 0) + V - 1) / V;                          // (from the last border before the row on)
+        launch_op(lc, "dequantize4", (uint64_t)rows * (cols * sizeof(T) + blocks4(cols) * 17), shift ? dequantize4_kernel<T, true> : dequantize4_kernel<T, false>, pieces_grid(rows, per), kR4Threads,
+                  0, 1, false, q, (long long)ldq, scale, (long long)lds, (long long)rows, (int)cols, (int)(4 * blocks4(cols)), (int)per, static_cast<T*>(y), (long long)ldy);
     });
     FL_API_END
 }
@@ -230,6 +250,7 @@ FL_EXPORT int fl_glu4(const void* x, int dtype, int64_t rows, int64_t cols, int6
     FL_CHECK(act == FL_ACT_SILU || act == FL_ACT_GELU_TANH || act == FL_ACT_RELU || act == FL_ACT_SWISH_CLAMP, FL_ERR_INVALID, "glu4: the activation is silu, gelu_tanh, relu or swish_clamp");
     FL_CHECK(act != FL_ACT_SWISH_CLAMP || (limit > 0 && std::isfinite(limit)), FL_ERR_INVALID, "glu4: the limit is a positive number");
     FL_CHECK(rows >= 0 && rows <= kMaxRows && cols >= 1 && cols <= kMaxCols4, FL_ERR_INVALID, "glu4: rows from 0 to 2^30, columns from 1 to 2^20");
+    FL_CHECK(rows <= kMaxNumbers4 / cols, FL_ERR_INVALID, "glu4: more than 2^39 numbers");
     FL_CHECK(rows <= 1 || ldx >= 2 * cols, FL_ERR_INVALID, "glu4: the row stride is smaller than the row");
     if (rows == 0) return FL_OK;
     FL_CHECK(x && q && scale, FL_ERR_INVALID, "NULL argument");
@@ -238,13 +259,7 @@ FL_EXPORT int fl_glu4(const void* x, int dtype, int64_t rows, int64_t cols, int6
     DeviceScope dev;
     set_up();
     LaunchCtx lc = op_ctx(stream);
-    const Span s = spans4(rows, cols);
-    by_type(dtype, [&](auto t) {
-        using T = decltype(t);
-        const bool vec = starts_vec<T>(x, rows, ldx);
-        launch_op(lc, "glu4", (uint64_t)rows * (2 * cols * sizeof(T) + blocks4(cols) * 17), glu4_kernel<T>, s.grid, s.threads, 0, 1, false, static_cast<const T*>(x), (long long)ldx, (int)cols, vec,
-                  vec && cols * sizeof(T) % 16 == 0, act, limit, Rows4Out{q, ldq, scale, lds, (int)blocks4(cols), 0, 0});
-    });
+    glu4(lc, x, dtype, rows, cols, ldx, act, limit, Rows4Out{q, ldq, scale, lds, (int)blocks4(cols), 0, 0});
     FL_API_END
 }
 
@@ -293,7 +308,7 @@ FL_EXPORT int fl_linear4(const void* x, int x_dtype, int64_t ldx, const uint8_t*
     FL_CHECK(aligned(w_tiles, 16), FL_ERR_INVALID, "linear4: the weight's scales start on a 16-byte border");
     if (given) check_rows4("linear4", x, ldx, x_scale, lds, rows, k);
     FL_CHECK((given || aligned(x, dtype_size(x_dtype))) && aligned(y, dtype_size(y_dtype)) && aligned(bias, 4), FL_ERR_INVALID, "linear4: a pointer is not aligned to its type");
-    FL_CHECK(rows <= ((int64_t)1 << 40) / n && n <= ((int64_t)1 << 43) / k && rows <= ((int64_t)1 << 43) / k, FL_ERR_INVALID, "linear4: more than 2^40 results, or an operand of more than 2^43 numbers");
+    FL_CHECK(rows <= ((int64_t)1 << 40) / n && n <= kMaxNumbers4 / k && rows <= kMaxNumbers4 / k, FL_ERR_INVALID, "linear4: more than 2^40 results, or an operand of more than 2^39 numbers");
     const Linear4Room room = linear4_room(rows, k, given);
     FL_CHECK(workspace && aligned(workspace, 256) && workspace_bytes >= room.all, FL_ERR_INVALID,
              "linear4: the workspace is smaller than fl_linear4_workspace asks for, or not on a 256-byte border");

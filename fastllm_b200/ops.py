@@ -25,6 +25,7 @@ _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: t
 _bound = [None]             # the device of the last call
 _FLOATS = {torch.float32: _lib.FL_DTYPE_F32, torch.bfloat16: _lib.FL_DTYPE_BF16, torch.float16: _lib.FL_DTYPE_F16}
 _TYPES = {**_FLOATS, torch.int8: _lib.FL_DTYPE_I8}
+_FLOATS4 = {**_FLOATS, torch.uint8: _lib.FL_DTYPE_MX4}
 _TOKENS = {torch.int32: 4, torch.int64: 8}
 MAX_TOP = 32
 
@@ -151,55 +152,58 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, b
 
 def _rows4(q: torch.Tensor, scale: torch.Tensor, dev: int, what: str, name: str):
     """4-bit rows [..., 16 blocks] and their scales [..., blocks] as matrices"""
-    if q.dtype != torch.uint8 or scale.dtype != torch.uint8 or q.ndim == 0 or scale.ndim == 0 or q.shape[:-1] != scale.shape[:-1] or q.shape[-1] != 16 * scale.shape[-1]:
+    u8 = torch.uint8
+    if q.dtype is not u8 or scale.dtype is not u8 or q.ndim == 0 or scale.ndim == 0 or q.shape[:-1] != scale.shape[:-1] or q.shape[-1] != 16 * scale.shape[-1]:
         _refuse(f"{what}: {name} are uint8 rows of 16 bytes per block with a uint8 scale per block, got {q.dtype} {tuple(q.shape)} and {scale.dtype} {tuple(scale.shape)}")
     if scale.shape[-1] == 0:
         _refuse(f"{what}: {name} have no columns")
-    _same(dev, q, what, name)
-    _same(dev, scale, what, f"the scales of {name}")
-    return _rows(q, what), _rows(scale, what)
-
-
-def _new_rows4(x: torch.Tensor, rows: int, cols: int, lead):
-    """room for 4-bit rows and their scales, in one piece of memory: (q, scale)"""
-    blocks = (cols + 31) // 32
-    mem = x.new_empty(rows * blocks * 17, dtype=torch.uint8)
-    q, scale = mem.as_strided((rows, 16 * blocks), (16 * blocks, 1), 0), mem.as_strided((rows, blocks), (blocks, 1), 16 * rows * blocks)
-    return (q, scale) if len(lead) == 1 else (q.view(lead + (16 * blocks,)), scale.view(lead + (blocks,)))
+    if q.get_device() != dev:
+        _same(dev, q, what, name)
+    if scale.get_device() != dev:
+        _same(dev, scale, what, f"the scales of {name}")
+    return (q if q.ndim == 2 and q.stride(1) == 1 else _rows(q, what)), (scale if scale.ndim == 2 and scale.stride(1) == 1 else _rows(scale, what))
 
 
 def quantize4(x: torch.Tensor):
     """[..., cols] f32 / bf16 / f16 -> (q uint8 [..., 16 blocks], scale uint8 [..., blocks]), blocks = cols / 32 rounded up: two e2m1 numbers a byte, the even column in
     the low half, and a power of two 2^(scale - 127) per block of 32 neighbours (OCP Microscaling, MXFP4).  What the last block has behind the row is zero."""
     what = "quantize4"
-    if x.dtype not in _FLOATS:
+    kind = _FLOATS.get(x.dtype)
+    if kind is None:
         _refuse(f"{what}: f32, bf16 or f16 rows are wanted, got {x.dtype}")
-    dev = _device(x, what)
-    x2 = _rows(x, what)
+    dev = x.get_device()
+    if dev != _bound[0]:
+        _device(x, what)
+    x2 = x if x.ndim == 2 and x.stride(1) == 1 else _rows(x, what)
     rows, cols = x2.shape
-    q, scale = _new_rows4(x, rows, cols, x.shape[:-1])
-    rc = _lib.load().fl_quantize4(x2.data_ptr(), _FLOATS[x.dtype], rows, cols, x2.stride(0), q.data_ptr(), 16 * scale.shape[-1], scale.data_ptr(), scale.shape[-1], _stream(dev))
+    blocks = (cols + 31) // 32
+    q, scale = x.new_empty((rows, 16 * blocks), dtype=torch.uint8), x.new_empty((rows, blocks), dtype=torch.uint8)
+    rc = _lib.load().fl_quantize4(x2.data_ptr(), kind, rows, cols, x2.stride(0), q.data_ptr(), 16 * blocks, scale.data_ptr(), blocks, _stream(dev))
     if rc:
         _lib.check(rc)
-    return q, scale
+    return (q, scale) if x.ndim == 2 else (q.view(x.shape[:-1] + (16 * blocks,)), scale.view(x.shape[:-1] + (blocks,)))
 
 
 def dequantize4(q: torch.Tensor, scale: torch.Tensor, cols: Optional[int] = None, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The numbers that 4-bit rows stand for, [..., cols], rounded once to f32, bf16 or f16.  cols: how many of a row's columns (default: those of all its blocks)."""
     what = "dequantize4"
-    if dtype not in _FLOATS:
+    kind = _FLOATS.get(dtype)
+    if kind is None:
         _refuse(f"{what}: results are f32, bf16 or f16, got {dtype}")
-    dev = _device(q, what)
+    dev = q.get_device()
+    if dev != _bound[0]:
+        _device(q, what)
     q2, s2 = _rows4(q, scale, dev, what, "the rows")
-    most = 32 * scale.shape[-1]
-    cols = most if cols is None else cols
-    if not most - 32 < cols <= most:
-        _refuse(f"{what}: rows of {scale.shape[-1]} blocks have from {most - 31} to {most} columns, not {cols}")
-    y = q.new_empty(q.shape[:-1] + (cols,), dtype=dtype)
-    rc = _lib.load().fl_dequantize4(q2.data_ptr(), q2.stride(0), s2.data_ptr(), s2.stride(0), len(q2), cols, y.data_ptr(), _FLOATS[dtype], cols, _stream(dev))
+    rows, blocks = s2.shape
+    if cols is None:
+        cols = 32 * blocks
+    elif not 32 * blocks - 32 < cols <= 32 * blocks:
+        _refuse(f"{what}: rows of {blocks} blocks have from {32 * blocks - 31} to {32 * blocks} columns, not {cols}")
+    y = q.new_empty((rows, cols), dtype=dtype)
+    rc = _lib.load().fl_dequantize4(q2.data_ptr(), q2.stride(0), s2.data_ptr(), s2.stride(0), rows, cols, y.data_ptr(), kind, cols, _stream(dev))
     if rc:
         _lib.check(rc)
-    return y
+    return y if q.ndim == 2 else y.view(q.shape[:-1] + (cols,))
 
 
 _GATED = {"silu": _lib.FL_ACT["silu"], "gelu_tanh": _lib.FL_ACT["gelu_tanh"], "relu": _lib.FL_ACT["relu"], "swish_clamp": _lib.FL_ACT["swish_clamp"]}
@@ -209,21 +213,25 @@ def glu4(x: torch.Tensor, act: str = "silu", *, limit: float = 7.0):
     """x [..., 2 cols] f32 / bf16 / f16, a row the gates and behind them the ups: h = act(gate) * up as 4-bit rows, (q, scale) as quantize4 gives them; each h is rounded
     once.  act: "silu", "gelu_tanh", "relu", or "swish_clamp" with c = min(gate, limit): c / (1 + exp(-1.702 c)) * (clamp(up, -limit, limit) + 1)."""
     what = "glu4"
-    if x.dtype not in _FLOATS:
+    kind, way = _FLOATS.get(x.dtype), _GATED.get(act)
+    if kind is None:
         _refuse(f"{what}: f32, bf16 or f16 rows are wanted, got {x.dtype}")
-    if act not in _GATED:
+    if way is None:
         _refuse(f"{what}: the activation is one of {', '.join(_GATED)}, got {act!r}")
-    dev = _device(x, what)
-    x2 = _rows(x, what)
+    dev = x.get_device()
+    if dev != _bound[0]:
+        _device(x, what)
+    x2 = x if x.ndim == 2 and x.stride(1) == 1 else _rows(x, what)
     rows, both = x2.shape
     if both % 2:
         _refuse(f"{what}: a row holds as many gates as ups, got {both} numbers")
-    q, scale = _new_rows4(x, rows, both // 2, x.shape[:-1])
-    rc = _lib.load().fl_glu4(x2.data_ptr(), _FLOATS[x.dtype], rows, both // 2, x2.stride(0), _GATED[act], limit, q.data_ptr(), 16 * scale.shape[-1], scale.data_ptr(), scale.shape[-1],
-                             _stream(dev))
+    cols = both // 2
+    blocks = (cols + 31) // 32
+    q, scale = x.new_empty((rows, 16 * blocks), dtype=torch.uint8), x.new_empty((rows, blocks), dtype=torch.uint8)
+    rc = _lib.load().fl_glu4(x2.data_ptr(), kind, rows, cols, x2.stride(0), way, limit, q.data_ptr(), 16 * blocks, scale.data_ptr(), blocks, _stream(dev))
     if rc:
         _lib.check(rc)
-    return q, scale
+    return (q, scale) if x.ndim == 2 else (q.view(x.shape[:-1] + (16 * blocks,)), scale.view(x.shape[:-1] + (blocks,)))
 
 
 class Weight4(NamedTuple):
@@ -260,34 +268,36 @@ def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = Non
     k / 32 blocks, rounded up.  bias f32 [n] or None.  out_dtype: f32 / bf16 / f16 (default: x's type, f32 for 4-bit rows); out: where the result goes, [..., n] with a
     dense last dimension, not overlapping an input."""
     what = "linear4"
-    given = x.dtype == torch.uint8
-    if not given and x.dtype not in _FLOATS:
+    x_type = _FLOATS4.get(x.dtype)
+    if x_type is None:
         _refuse(f"{what}: activations are f32, bf16, f16 or 4-bit rows (uint8), got {x.dtype}")
     if not isinstance(weight, Weight4):
         _refuse(f"{what}: the weight is what weight4 gives, got {type(weight).__name__}")
     dev = x.get_device()
     if dev != _bound[0]:
         _device(x, what)
-    n, blocks = weight.scale.shape
-    if weight.q.get_device() != dev:
-        _same(dev, weight.q, what, "the weight")
+    w, tiles, scale = weight
+    n, blocks = scale.shape
+    if w.get_device() != dev:
+        _same(dev, w, what, "the weight")
+    given = x_type == _lib.FL_DTYPE_MX4
     xs_ptr, lds = None, 0
     if given:
         if x_scale is None:
             _refuse(f"{what}: 4-bit rows come with their x_scale")
         x2, s2 = _rows4(x, x_scale, dev, what, "the activations")
-        xs_ptr, lds, k, x_type = s2.data_ptr(), s2.stride(0), 32 * s2.shape[1], _lib.FL_DTYPE_MX4
+        rows, k = s2.shape
+        xs_ptr, lds, k = s2.data_ptr(), s2.stride(0), 32 * k
     else:
         if x_scale is not None:
             _refuse(f"{what}: x_scale comes with activations of 4 bits, and only with them")
-        x2, x_type = (x if x.ndim == 2 and x.stride(1) == 1 else _rows(x, what)), _FLOATS[x.dtype]
-        k = x2.shape[1]
-    rows = x2.shape[0]
+        x2 = x if x.ndim == 2 and x.stride(1) == 1 else _rows(x, what)
+        rows, k = x2.shape
     if (k + 31) // 32 != blocks:
         _refuse(f"{what}: the weight has {blocks} blocks of 32 columns, the activations have {k} columns")
     bias_ptr = None if bias is None else _vector(bias, n, dev, what, "bias")
-    lead = x.shape[:-1]
     if out is not None:
+        lead = x.shape[:-1]
         if out.shape != lead + (n,) or (out_dtype is not None and out.dtype != out_dtype):
             _refuse(f"{what}: out is {tuple(lead + (n,))}, got {tuple(out.shape)} {out.dtype}")
         _same(dev, out, what, "out")
@@ -299,14 +309,17 @@ def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = Non
         _refuse(f"{what}: results are f32, bf16 or f16, got {out_dtype}")
     if out is None:
         y2 = x.new_empty((rows, n), dtype=out_dtype)
-        out, ldy = (y2 if x.ndim == 2 else y2.view(lead + (n,))), n
+        out, ldy = (y2 if x.ndim == 2 else y2.view(x.shape[:-1] + (n,))), n
     else:
         y2 = _rows(out, what)
         ldy = y2.stride(0)
     room = _room4(rows, blocks, given)
-    work = x.new_empty(room, dtype=torch.uint8)
-    rc = _lib.load().fl_linear4(x2.data_ptr(), x_type, x2.stride(0), xs_ptr, lds, weight.q.data_ptr(), weight.q.stride(0), weight.tiles.data_ptr(), bias_ptr, rows, n, k, y2.data_ptr(),
-                                y_type, ldy, work.data_ptr(), room, _stream(dev))
+    work = work_ptr = None
+    if room:
+        work = x.new_empty(room, dtype=torch.uint8)
+        work_ptr = work.data_ptr()
+    rc = _lib.load().fl_linear4(x2.data_ptr(), x_type, x2.stride(0), xs_ptr, lds, w.data_ptr(), w.stride(0), tiles.data_ptr(), bias_ptr, rows, n, k, y2.data_ptr(), y_type, ldy, work_ptr, room,
+                                _stream(dev))
     if rc:
         _lib.check(rc)
     return out

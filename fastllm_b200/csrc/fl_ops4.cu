@@ -33,9 +33,9 @@ static void by_type(int dtype, F f) {
 }
 
 static void quantize4(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, const Rows4Out& o) {
-    const int64_t per = o.tile > 0 ? o.groups * 4 : o.blocks;                  // (tiles hold scales of whole k blocks)
     by_type(dtype, [&](auto t) {
         using T = decltype(t);
+        const int64_t per = (o.tile > 0 ? o.groups * 4 : o.blocks) * kR4Lanes<T>;              // (tiles hold scales of whole k blocks)
         launch_op(lc, "quantize4", (uint64_t)rows * (cols * sizeof(T) + o.blocks * 17), rows_on_16(x, rows, ldx, sizeof(T)) ? quantize4_kernel<T, true> : quantize4_kernel<T, false>,
                   pieces_grid(rows, per), kR4Threads, 0, 1, false, static_cast<const T*>(x), (long long)ldx, (long long)rows, (int)cols, (int)per, o);
     });
@@ -52,8 +52,9 @@ static void glu4(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t 
     by_type(dtype, [&](auto t) {
         using T = decltype(t);
         const bool vec = rows_on_16(x, rows, ldx, sizeof(T)) && cols * sizeof(T) % 16 == 0;
-        launch_op(lc, "glu4", (uint64_t)rows * (2 * cols * sizeof(T) + o.blocks * 17), vec ? glu4_form<T, true>(act) : glu4_form<T, false>(act), pieces_grid(rows, o.blocks), kR4Threads, 0, 1, false,
-                  static_cast<const T*>(x), (long long)ldx, (long long)rows, (int)cols, o.blocks, limit, o);
+        const int64_t per = o.blocks * kR4Lanes<T>;
+        launch_op(lc, "glu4", (uint64_t)rows * (2 * cols * sizeof(T) + o.blocks * 17), vec ? glu4_form<T, true>(act) : glu4_form<T, false>(act), pieces_grid(rows, per), kR4Threads, 0, 1, false,
+                  static_cast<const T*>(x), (long long)ldx, (long long)rows, (int)cols, (int)per, limit, o);
     });
 }
 
@@ -238,8 +239,10 @@ FL_EXPORT int fl_dequantize4(const uint8_t* q, int64_t ldq, const uint8_t* scale
         constexpr int V = 16 / sizeof(T);
         const bool shift = !rows_on_16(y, rows, ldy, sizeof(T));
         const int64_t per = (cols + (shift ? V - 1 : 0) + V - 1) / V;                          // (from the last border before the row on)
-        launch_op(lc, "dequantize4", (uint64_t)rows * (cols * sizeof(T) + blocks4(cols) * 17), shift ? dequantize4_kernel<T, true> : dequantize4_kernel<T, false>, pieces_grid(rows, per), kR4Threads,
-                  0, 1, false, q, (long long)ldq, scale, (long long)lds, (long long)rows, (int)cols, (int)(4 * blocks4(cols)), (int)per, static_cast<T*>(y), (long long)ldy);
+        const int threads = (int)std::min<int64_t>(256, (per + 63) / 64 * 32);                 // two pieces each
+        launch_op(lc, "dequantize4", (uint64_t)rows * (cols * sizeof(T) + blocks4(cols) * 17), shift ? dequantize4_kernel<T, true> : dequantize4_kernel<T, false>,
+                  dim3((unsigned)rows, (unsigned)((per + 2 * threads - 1) / (2 * threads))), threads, 0, 1, false, q, (long long)ldq, scale, (long long)lds, (int)cols, (int)(4 * blocks4(cols)),
+                  static_cast<T*>(y), (long long)ldy);
     });
     FL_API_END
 }

@@ -30,7 +30,13 @@ __device__ __forceinline__ uint32_t scale4(uint32_t max_bits) { return max_bits 
 __device__ __forceinline__ float up4(uint32_t s) { return s == 255u ? 0.f : __uint_as_float((254u - s) << 23); }
 __device__ __forceinline__ float down4(uint32_t s) { return __uint_as_float(s == 0u ? 0x00400000u : (s == 255u ? 0x7FFFFFFFu : s << 23)); }
 
-// number j of words of T, the bits of one, and words of V numbers
+__device__ __forceinline__ uint32_t down4_bf16(uint32_t s) { return s == 0u ? 0x0040u : (s == 255u ? 0x7FFFu : s << 7); }
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// number j of words of T, and the bits of one
 template <typename T> __device__ __forceinline__ float number_of(const uint32_t* w, int j);
 template <> __device__ __forceinline__ float number_of<float>(const uint32_t* w, int j) { return __uint_as_float(w[j]); }
 template <> __device__ __forceinline__ float number_of<__nv_bfloat16>(const uint32_t* w, int j) { return j & 1 ? bf16hi(w[j / 2]) : bf16lo(w[j / 2]); }
@@ -39,53 +45,28 @@ __device__ __forceinline__ uint32_t bits_of(float v) { return __float_as_uint(v)
 __device__ __forceinline__ uint32_t bits_of(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 __device__ __forceinline__ uint32_t bits_of(__half v) { return __half_as_ushort(v); }
 
-// To the nearest e2m1, halves to the even mantissa, beyond 6 to 6, of a c >= 0 (c = 1 or folded into the sums): numbers up to 2 lie half a step apart, up to 4 a whole, then two, so the
-// code is the least of 2 a, a + 2 and a / 2 + 4, each rounded to a whole number, and 7; 2^23 leaves a whole number in a sum's low bits.  (cvt.e2m1x2 did 5 numbers a
-// clock and SM: 28672 x 4096 bf16 took 75 us.)
-constexpr float kE2m1Big = 8388608.f;
-__device__ __forceinline__ float e2m1_sum(float a, float c) {
-    return fminf(fminf(fmaf(a, 2.f * c, kE2m1Big), fmaf(a, c, kE2m1Big + 2.f)), fminf(fmaf(a, 0.5f * c, kE2m1Big + 4.f), kE2m1Big + 7.f));
-}
-// Codes of eight columns, the first in the low bits, from such sums and what has the numbers' signs in its top bits
-__device__ __forceinline__ uint32_t e2m1x8(const float (&sum)[8], const uint32_t (&sign)[8]) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int j = 7; j >= 0; --j) w = __funnelshift_l(sign[j], w, 1) * 8u + __float_as_uint(sum[j]);
-    constexpr uint32_t kBits = 0x4B000000u;                     // of 2^23
-    return w - kBits * 0x11111111u;
-}
-// the same of eight bf16 numbers times a power of two, two at a time: bf16's sums with 128 round to whole numbers
-__device__ __forceinline__ uint32_t e2m1x8_bf16(const uint32_t* in, uint32_t up2) {
-    auto bf = [](uint32_t v) { return __halves2bfloat162(__ushort_as_bfloat16((unsigned short)v), __ushort_as_bfloat16((unsigned short)(v >> 16))); };
-    auto sum = [&](uint32_t v) {                                // 128 + code in both halves
-        const __nv_bfloat162 a = __hmul2(bf(v & 0x7FFF7FFFu), bf(up2));
-        const __nv_bfloat162 t = __hmin2(__hmin2(__hfma2(a, bf(0x40004000u), bf(0x43004300u)), __hadd2(a, bf(0x43024302u))),
-                                         __hmin2(__hfma2(a, bf(0x3F003F00u), bf(0x43044304u)), bf(0x43074307u)));
-        return (uint32_t)__bfloat16_as_ushort(__low2bfloat16(t)) | (uint32_t)__bfloat16_as_ushort(__high2bfloat16(t)) << 16;
-    };
-    auto four = [&](uint32_t v0, uint32_t v1) {                 // four codes in the low half
-        const uint32_t sign = ((v0 >> 12) & 0x00080008u) | ((v1 >> 4) & 0x08000800u);
-        const uint32_t c = sum(v1) * 256u + (sum(v0) + sign - 0x43004300u * 257u);     // codes of columns 0, 2, 1, 3 in the low halves of the bytes
-        return c | (c >> 12);
-    };
-    return __byte_perm(four(in[0], in[1]), four(in[2], in[3]), 0x5410);
-}
-__device__ __forceinline__ void from_e2m1x8(uint32_t w, float (&v)[8]) {
-    uint32_t h[4];
+// to the nearest e2m1, halves to the even mantissa, beyond 6 to 6; eight columns, the first in the low bits
+__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
+    uint32_t w;
     asm("{\n"
         ".reg .b8 a, b, c, d;\n"
-        "mov.b32 {a, b, c, d}, %4;\n"
-        "cvt.rn.f16x2.e2m1x2 %0, a;\n"
-        "cvt.rn.f16x2.e2m1x2 %1, b;\n"
-        "cvt.rn.f16x2.e2m1x2 %2, c;\n"
-        "cvt.rn.f16x2.e2m1x2 %3, d;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
+        "mov.b32 %0, {a, b, c, d};\n"
         "}\n"
-        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-        : "r"(w));
+        : "=r"(w)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return w;
+}
+// eight codes, the first in the low bits, as bf16 numbers: both bytes of a number by a look-up among eight, then the sign
+__device__ __forceinline__ void from_e2m1x8(uint32_t w, uint32_t (&bf16)[4]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = number_of<__half>(h, 2 * i);
-        v[2 * i + 1] = number_of<__half>(h, 2 * i + 1);
+    for (int i = 0; i < 2; ++i, w >>= 16) {
+        const uint32_t at = w & 0x7777u, low = __byte_perm(0xC0800000u, 0xC0804000u, at), high = __byte_perm(0x3F3F3F00u, 0x40404040u, at);
+        bf16[2 * i] = __byte_perm(low, high, 0x5140) | ((w << 12) & 0x8000u) | ((w << 24) & 0x80000000u);
+        bf16[2 * i + 1] = __byte_perm(low, high, 0x7362) | ((w << 4) & 0x8000u) | ((w << 16) & 0x80000000u);
     }
 }
 
@@ -130,10 +111,10 @@ __device__ __forceinline__ void load_row(const T* row, int at, int cols, uint32_
             if (at + j < cols) w[j * kWords / V] |= bits_of(p[j]) << (32 / (V / kWords) * (j % (V / kWords)));
     }
 }
-// A thread takes a block: which one, of all rows' blocks (`per` a row) in order
+// A thread takes 64 bytes of a row: a block of 16-bit numbers, half a block of 32-bit ones.  Which one, of all rows' pieces (`per` a row) in order
 struct At4 {
     long long r;
-    int block;
+    int piece;
     bool here;
     __device__ At4(long long rows, int per) {
         const unsigned long long id = (unsigned long long)blockIdx.x * kR4Threads + threadIdx.x, all = (unsigned long long)rows * per;
@@ -141,126 +122,143 @@ struct At4 {
         if (all <= 0xFFFFFFFFull) {
             const uint32_t q = (uint32_t)id / (uint32_t)per;
             r = q;
-            block = (int)((uint32_t)id - q * (uint32_t)per);
+            piece = (int)((uint32_t)id - q * (uint32_t)per);
         } else {
             r = (long long)(id / per);
-            block = (int)(id - (unsigned long long)r * per);
+            piece = (int)(id - (unsigned long long)r * per);
         }
     }
 };
-__device__ __forceinline__ void put4(const Rows4Out& o, long long r, int block, const uint32_t (&codes)[4], uint32_t s) {
-    if (block < o.blocks) *reinterpret_cast<uint4*>(o.q + r * o.ldq + block * 16) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+template <typename T> constexpr int kR4Lanes = sizeof(T) == 4 ? 2 : 1;                 // threads of a block of 32
+template <typename T> constexpr int kR4Own = kR4Block / kR4Lanes<T>;                   // numbers of a thread
+template <typename T>
+__device__ __forceinline__ void put4(const Rows4Out& o, long long r, int piece, const uint32_t (&codes)[kR4Own<T> / 8], uint32_t s) {
+    const int block = piece / kR4Lanes<T>;
+    uint8_t* q = o.q + r * o.ldq + piece * (kR4Own<T> / 2);
+    if (block < o.blocks) {
+        if constexpr (kR4Lanes<T> == 1) *reinterpret_cast<uint4*>(q) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+        else *reinterpret_cast<uint2*>(q) = make_uint2(codes[0], codes[1]);
+    }
     uint8_t* to = o.tile == 0 ? o.scale + r * o.lds + block : o.scale + scale4_at(r, block / 4, o.tile, o.groups) + block % 4;
-    *to = (uint8_t)s;
+    if (piece % kR4Lanes<T> == 0) *to = (uint8_t)s;
 }
-// 32 values from column `at` on, zeros past the row's end.  kVec: rows start on 16-byte borders.
+// 64 bytes from column `at` on, zeros past the row's end.  kVec: rows start on 16-byte borders.
 template <typename T, bool kVec>
-__device__ __forceinline__ void load32(const T* row, int at, int cols, uint32_t (&w)[8 * sizeof(T)]) {
-    if (kVec && at + kR4Block <= cols) {
+__device__ __forceinline__ void load64(const T* row, int at, int cols, uint32_t (&w)[16]) {
+    if (kVec && at + kR4Own<T> <= cols) {
 #pragma unroll
-        for (int i = 0; i < (int)(2 * sizeof(T)); ++i) {
+        for (int i = 0; i < 4; ++i) {
             const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + at) + i);
             w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            uint32_t part[2 * sizeof(T)];
-            load_row(row, at + 8 * i, cols, part);
+            uint32_t part[4];
+            load_row(row, at + kR4Own<T> / 4 * i, cols, part);
 #pragma unroll
-            for (int j = 0; j < (int)(2 * sizeof(T)); ++j) w[2 * sizeof(T) * i + j] = part[j];
+            for (int j = 0; j < 4; ++j) w[4 * i + j] = part[j];
         }
     }
 }
 // bits, as of f32, of the largest magnitude among the words' numbers; those of 16 bits are in the order of their bits too
-template <typename T, int kWords>
-__device__ __forceinline__ uint32_t most_of(const uint32_t (&w)[kWords]) {
+template <typename T>
+__device__ __forceinline__ uint32_t most_of(const uint32_t (&w)[16]) {
     uint32_t m = 0;
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int j = 0; j < kWords; ++j) m = max(m, w[j] & 0x7FFFFFFFu);
+        for (int j = 0; j < 16; j += 2) m = __vimax3_u32(m, w[j] & 0x7FFFFFFFu, w[j + 1] & 0x7FFFFFFFu);
         return m;
     } else {
 #pragma unroll
-        for (int j = 0; j < kWords; ++j) m = __vmaxu2(m, w[j] & 0x7FFF7FFFu);
+        for (int j = 0; j < 16; j += 2) m = __vimax3_u16x2(m, w[j] & 0x7FFF7FFFu, w[j + 1] & 0x7FFF7FFFu);
         m = max(m & 0xFFFFu, m >> 16);
         return abs_bits(number_of<T>(&m, 0));
     }
 }
+// the largest of a block's threads
+template <typename T>
+__device__ __forceinline__ uint32_t block_max(uint32_t m) { return kR4Lanes<T> == 1 ? m : max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1)); }
 
-// A thread per block: nothing passes between threads, and what a block costs once (its place, its scale) counts little beside its 32 numbers: with eight numbers a
-// thread the instructions were the bound, 19 a number.
+// What a block costs once, its place and its scale, counts little beside the 32 numbers of a thread: with eight a thread the instructions were the bound, 19 a number.  What
+// bounds it: HBM.
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kR4Threads) quantize4_kernel(const T* __restrict__ x, long long ldx, long long rows, int cols, int per, const Rows4Out o) {
     pdl_launch_dependents();
     const At4 at(rows, per);
+    uint32_t w[16] = {}, codes[kR4Own<T> / 8] = {};
+    if (at.here) load64<T, kVec>(x + at.r * ldx, at.piece * kR4Own<T>, cols, w);
+    const uint32_t s = scale4(block_max<T>(most_of<T>(w)));
     if (!at.here) return;
-    uint32_t w[8 * sizeof(T)], codes[4] = {};
-    load32<T, kVec>(x + at.r * ldx, at.block * kR4Block, cols, w);
-    const uint32_t s = scale4(most_of<T>(w));
     if (s != 255u) {
-        if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        const float up = up4(s);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) codes[i] = e2m1x8_bf16(w + 4 * i, (254u - s) * 0x00800080u);
-        } else {
-            const float up = up4(s);
+        for (int i = 0; i < kR4Own<T> / 8; ++i) {
+            float v[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float sum[8];
-                uint32_t sign[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float v = number_of<T>(w, 8 * i + j);
-                    sign[j] = __float_as_uint(v);
-                    sum[j] = e2m1_sum(fabsf(v) * up, 1.f);      // (the product is exact, or far below the smallest border)
-                }
-                codes[i] = e2m1x8(sum, sign);
-            }
+            for (int j = 0; j < 8; ++j) v[j] = number_of<T>(w, 8 * i + j) * up;        // exact, or far below the smallest border
+            codes[i] = e2m1x8(v);
         }
     }
-    put4(o, at.r, at.block, codes, s);
+    put4<T>(o, at.r, at.piece, codes, s);
 }
 
 // Eight numbers a thread (of 32 bits: four), which it writes at once.  kShift: rows of results may start anywhere, some numbers behind a 16-byte border; a thread then takes the
-// columns between two borders, and its codes out of two words.
+// columns between two borders, and its codes out of two words.  grid (rows, threads' pieces of a row): a division for eight numbers cost a fifth of the time.
 template <typename T, bool kShift>
-__global__ void __launch_bounds__(kR4Threads) dequantize4_kernel(const uint8_t* __restrict__ q, long long ldq, const uint8_t* __restrict__ scale, long long lds, long long rows, int cols, int words,
-                                                                 int per, T* __restrict__ y, long long ldy) {
-    constexpr int V = 16 / sizeof(T);
-    const At4 place(rows, per);
-    if (!place.here) return;
-    const uint32_t* qr = reinterpret_cast<const uint32_t*>(q + place.r * ldq);         // `words` of eight codes
-    const uint8_t* sr = scale + place.r * lds;
-    T* yr = y + place.r * ldy;
-    int at = place.block * V;
-    uint32_t w, s0, s1;
-    if constexpr (kShift) {
-        at -= (int)((reinterpret_cast<uintptr_t>(yr) & 15u) / sizeof(T));
-        if (at >= cols) return;
-        const int lo = at >> 3, hi = (at + V - 1) >> 3;
-        const uint32_t w0 = lo >= 0 ? __ldg(qr + lo) : 0u, w1 = hi != lo && hi < words ? __ldg(qr + hi) : 0u;
-        s0 = lo >= 0 ? __ldg(sr + (lo >> 2)) : 0u;
-        s1 = hi >> 2 != lo >> 2 && hi < words ? __ldg(sr + (hi >> 2)) : s0;
-        w = __funnelshift_r(w0, w1, 4 * (at & 7));
-    } else {
-        w = __ldg(qr + (at >> 3)) >> (4 * (at & 7));
-        s0 = s1 = __ldg(sr + (at >> 5));
+__global__ void __launch_bounds__(256) dequantize4_kernel(const uint8_t* __restrict__ q, long long ldq, const uint8_t* __restrict__ scale, long long lds, int cols, int words,
+                                                                 T* __restrict__ y, long long ldy) {
+    constexpr int V = 16 / sizeof(T), U = 2;                    // pieces of a thread
+    const long long r = blockIdx.x;
+    const uint32_t* qr = reinterpret_cast<const uint32_t*>(q + r * ldq);               // `words` of eight codes
+    const uint8_t* sr = scale + r * lds;
+    T* yr = y + r * ldy;
+    const int at0 = (blockIdx.y * U * blockDim.x + threadIdx.x) * V - (kShift ? (int)((reinterpret_cast<uintptr_t>(yr) & 15u) / sizeof(T)) : 0), step = blockDim.x * V;
+    uint32_t w[U], s0[U], s1[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int at = at0 + i * step;
+        w[i] = s0[i] = s1[i] = 0u;
+        if (at >= cols) break;
+        if constexpr (kShift) {
+            const int lo = at >> 3, hi = (at + V - 1) >> 3;
+            const uint32_t w0 = lo >= 0 ? __ldg(qr + lo) : 0u, w1 = hi != lo && hi < words ? __ldg(qr + hi) : 0u;
+            s0[i] = lo >= 0 ? __ldg(sr + (lo >> 2)) : 0u;
+            s1[i] = hi >> 2 != lo >> 2 && hi < words ? __ldg(sr + (hi >> 2)) : s0[i];
+            w[i] = __funnelshift_r(w0, w1, 4 * (at & 7));
+        } else {
+            w[i] = __ldg(qr + (at >> 3)) >> (4 * (at & 7));
+            s0[i] = __ldg(sr + (at >> 5));
+        }
     }
-    float v[8];
-    from_e2m1x8(w, v);
-    const float d0 = down4(s0), d1 = kShift ? down4(s1) : d0;
-    const int own = 32 - (at & 31);                             // columns left in the first word's block
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] *= kShift && j >= own ? d1 : d0;
-    if ((!kShift || at >= 0) && at + V <= cols) {
+    for (int i = 0; i < U; ++i) {
+        const int at = at0 + i * step;
+        if (at >= cols) break;
+        uint32_t e2m1[4];
+        from_e2m1x8(w[i], e2m1);
+        const int own = 32 - (at & 31);                         // columns left in the first word's block
         uint32_t t[4] = {};
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) {       // powers of two and e2m1 are bf16 numbers, and so is every product in range
+            const uint32_t d0 = down4_bf16(s0[i]), d1 = kShift ? down4_bf16(s1[i]) : d0;
 #pragma unroll
-        for (int j = 0; j < V; ++j) t[j * 4 / V] |= bits_of(from_f32<T>(v[j])) << (V == 8 ? 16 * (j & 1) : 0);
-        *reinterpret_cast<uint4*>(yr + at) = make_uint4(t[0], t[1], t[2], t[3]);
-    } else {
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t d = (kShift && 2 * j >= own ? d1 : d0) | (kShift && 2 * j + 1 >= own ? d1 : d0) << 16;
+                t[j] = mul_bf16x2(e2m1[j], d);
+            }
+        } else {
+            const float d0 = down4(s0[i]), d1 = kShift ? down4(s1[i]) : d0;
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (at + j >= 0 && at + j < cols) yr[at + j] = from_f32<T>(v[j]);
+            for (int j = 0; j < V; ++j)
+                t[j * 4 / V] |= bits_of(from_f32<T>(number_of<__nv_bfloat16>(e2m1, j) * (kShift && j >= own ? d1 : d0))) << (V == 8 ? 16 * (j & 1) : 0);
+        }
+        if ((!kShift || at >= 0) && at + V <= cols) {
+            *reinterpret_cast<uint4*>(yr + at) = make_uint4(t[0], t[1], t[2], t[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (at + j >= 0 && at + j < cols) yr[at + j] = from_f32<T>(number_of<T>(t, j));
+        }
     }
 }
 
@@ -275,12 +273,13 @@ __device__ __forceinline__ double glu4_exact(float limit, float gf, float uf) {
     const double c = fmin(g, (double)limit);
     return c / (1.0 + exp(-1.702 * c)) * (fmin(fmax(u, -(double)limit), (double)limit) + 1.0);
 }
-// |h| in f32, with e = 2^t = e^-z, t held to 100.  t is off by |t| 2^-22 at most (a cubic's sum: four roundings), which moves h as far as e counts beside 1; ex2 and the
-// reciprocal are off by 2^-22 and 2^-23, the sum and the products by 2^-24 each: h (2^-20 + max(t, 0) 2^-21) is more than all of it.  Where t is held h is too large.
+// h in f32, with e = 2^t = e^-z.  t is off by |t| 2^-22 at most (a cubic's sum: four roundings), which moves h as far as e counts beside 1; ex2 and the reciprocal are
+// off by 2^-22 and 2^-23, the sum and the products by 2^-24 each: h (2^-20 + max(t, 0) 2^-21) is more than all of it.  From t = 126 on h is 0, and has fewer bits from
+// t = 100 on: there it is below |g u| 2^-99.
 template <int kAct>
 __device__ __forceinline__ float glu4_near(float limit, float g, float u) {
     constexpr float kLog2e = 1.4426950408889634f;
-    if constexpr (kAct == kGlu4Relu) return fabsf(fmaxf(g, 0.f)) * fabsf(u);
+    if constexpr (kAct == kGlu4Relu) return fmaxf(g, 0.f) * u;
     float t, gate = g, up = u;
     if constexpr (kAct == kGlu4Silu) {
         t = -kLog2e * g;
@@ -293,11 +292,11 @@ __device__ __forceinline__ float glu4_near(float limit, float g, float u) {
         t = -1.702f * kLog2e * gate;
     }
     float e, r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(fminf(t, 100.f)));
-    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-    return fabsf(gate * r) * fabsf(up);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return gate * r * up;
 }
-// no less than max(t, 0) of gates up to `in`
+// no less than max(t, 0) of gates up to `in`, where that is below 100
 template <int kAct>
 __device__ __forceinline__ float glu4_far(float in) {
     if constexpr (kAct == kGlu4Relu) return 0.f;
@@ -322,69 +321,71 @@ __device__ __forceinline__ uint32_t glu4_block_exact(float limit, float g, float
 // block is taken in 64 bits by its warp.  All in 64 bits took 287 us at 4096 x 14336.
 template <typename T, int kAct, bool kVec>
 __global__ void __launch_bounds__(kR4Threads) glu4_kernel(const T* __restrict__ x, long long ldx, long long rows, int cols, int per, float limit, const Rows4Out o) {
-    __shared__ float2 unsure[kR4Threads / 32][kR4Block];
+    constexpr int kOwn = kR4Own<T>;
     pdl_launch_dependents();
     const At4 at(rows, per);
-    uint32_t gw[8 * sizeof(T)] = {}, uw[8 * sizeof(T)] = {}, codes[4] = {};
-    if (at.here) {
-        load32<T, kVec>(x + at.r * ldx, at.block * kR4Block, cols, gw);
-        load32<T, kVec>(x + at.r * ldx + cols, at.block * kR4Block, cols, uw);
-    }
-    const uint32_t in_bits = max(most_of<T>(gw), most_of<T>(uw));
-    uint32_t s = 255u;
-    bool sure = true;
-    if (in_bits < 0x7F800000u) {
-        const float in = __uint_as_float(in_bits), off = kAct == kGlu4Relu ? 0x1p-22f : fmaf(glu4_far<kAct>(in), 0x1p-21f, 0x1p-20f);
-        float h[kR4Block], most = 0.f;
+    uint32_t codes[kOwn / 8] = {}, s, in_bits = 0;
+    float h[kOwn], most = 0.f;
+    {
+        uint32_t gw[16] = {}, uw[16] = {};
+        if (at.here) {
+            load64<T, kVec>(x + at.r * ldx, at.piece * kOwn, cols, gw);
+            load64<T, kVec>(x + at.r * ldx + cols, at.piece * kOwn, cols, uw);
+        }
+        in_bits = block_max<T>(max(most_of<T>(gw), most_of<T>(uw)));
 #pragma unroll
-        for (int j = 0; j < kR4Block; ++j) {
+        for (int j = 0; j < kOwn; ++j) {
             h[j] = glu4_near<kAct>(limit, number_of<T>(gw, j), number_of<T>(uw, j));
-            most = fmaxf(most, h[j]);
+            most = fmaxf(most, fabsf(h[j]));
         }
-        const float most_hi = most * (1.f + off), most_lo = most * (1.f - off);
-        s = scale4(__float_as_uint(most_hi));
-        // 64 bits too where f32 has fewer, and where a number whose exponent was held (below |g u| 2^-98) might count
-        const float least = fmaxf(0x1p-100f, in * 0x1p-45f * (in * 0x1p-45f));
-        sure = most == 0.f || (most_hi < INFINITY && most_hi >= least && s == scale4(__float_as_uint(most_lo)));
-        if (sure && most != 0.f) {
-            const float up = up4(s), hi = up * (1.f + off), lo = up * (1.f - off);
-            uint32_t other = 0;
+    }
+    most = __uint_as_float(block_max<T>(__float_as_uint(most)));
+    const float in = __uint_as_float(in_bits), off = kAct == kGlu4Relu ? 0x1p-22f : fmaf(glu4_far<kAct>(in), 0x1p-21f, 0x1p-20f);
+    const float most_hi = most * (1.f + off), most_lo = most * (1.f - off);
+    s = scale4(__float_as_uint(most_hi));
+    // not where f32 has fewer bits, nor where a number from t = 100 on might count
+    const float least = fmaxf(0x1p-100f, in * 0x1p-45f * (in * 0x1p-45f));
+    bool sure = most == 0.f ? kAct == kGlu4Relu || in == 0.f : most_hi < INFINITY && most_hi >= least && s == scale4(__float_as_uint(most_lo));
+    if (sure && most != 0.f) {
+        const float up = up4(s), hi = up * (1.f + off), lo = up * (1.f - off);
+        uint32_t other = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float sum[8];
-                uint32_t sign[8];
+        for (int i = 0; i < kOwn / 8; ++i) {
+            float a[8], b[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float v = number_of<T>(uw, 8 * i + j);
-                    sign[j] = __float_as_uint(number_of<T>(gw, 8 * i + j)) ^ __float_as_uint(kAct == kGlu4SwishClamp ? fminf(fmaxf(v, -limit), limit) + 1.f : v);
-                    sum[j] = e2m1_sum(h[8 * i + j], hi);
-                    other |= __float_as_uint(sum[j]) ^ __float_as_uint(e2m1_sum(h[8 * i + j], lo));
-                }
-                codes[i] = e2m1x8(sum, sign);
+            for (int j = 0; j < 8; ++j) {
+                a[j] = h[8 * i + j] * hi;
+                b[j] = h[8 * i + j] * lo;
             }
-            sure = other == 0u;
+            codes[i] = e2m1x8(a);
+            other |= codes[i] ^ e2m1x8(b);
         }
+        sure = other == 0u;
+    }
+    if (in_bits >= 0x7F800000u) {
+        sure = true;
+        s = 255u;
+#pragma unroll
+        for (int i = 0; i < kOwn / 8; ++i) codes[i] = 0u;
     }
     const int lane = threadIdx.x & 31;
-    for (uint32_t left = __ballot_sync(0xFFFFFFFFu, !sure); left != 0u; left &= left - 1u) {
+    uint32_t left = __ballot_sync(0xFFFFFFFFu, !sure && at.here);
+    if constexpr (kR4Lanes<T> == 2) left = (left | left >> 1) & 0x55555555u;           // a block by its first thread
+    for (; left != 0u; left &= left - 1u) {
         const int who = __ffs((int)left) - 1;
-        float2* mine = unsure[threadIdx.x / 32];
-        if (lane == who) {
+        const long long r = __shfl_sync(0xFFFFFFFFu, at.r, who);
+        const int col = __shfl_sync(0xFFFFFFFFu, at.piece, who) * kOwn + lane;
+        const bool here = col < cols;
+        const T* row = x + r * ldx + col;
+        uint32_t exact[4];
+        const uint32_t es = glu4_block_exact<kAct>(limit, here ? to_f32(row[0]) : 0.f, here ? to_f32(row[cols]) : 0.f, here, exact);
+        if (lane / kR4Lanes<T> == who / kR4Lanes<T>) {
+            s = es;
 #pragma unroll
-            for (int j = 0; j < kR4Block; ++j) mine[j] = make_float2(number_of<T>(gw, j), number_of<T>(uw, j));
+            for (int i = 0; i < kOwn / 8; ++i) codes[i] = kR4Lanes<T> == 2 && (lane & 1) ? exact[2 + i] : exact[i];
         }
-        __syncwarp();
-        const int count = __shfl_sync(0xFFFFFFFFu, cols - at.block * kR4Block, who);
-        uint32_t other[4];
-        const uint32_t exact = glu4_block_exact<kAct>(limit, mine[lane].x, mine[lane].y, lane < count, other);
-        if (lane == who) {
-            s = exact;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) codes[i] = other[i];
-        }
-        __syncwarp();
     }
-    if (at.here) put4(o, at.r, at.block, codes, s);
+    if (at.here) put4<T>(o, at.r, at.piece, codes, s);
 }
 
 // scales [n][lds] into the layout of the tensor cores (tiles of `tile` rows; zeros behind the last row and block): a thread per row and group

@@ -65,15 +65,19 @@ static void arrange4(LaunchCtx& lc, const uint8_t* scale, int64_t lds, int64_t r
               (long long)rows, (int)blocks4(k), tiles, tile, (int)groups, (long long)slots);
 }
 
+// whether a product's rows are rounded inside its own launch (ops.py keeps the same rule, for the workspace)
+static bool token_fits4(int64_t rows, int64_t n, int64_t k) { return rows <= kL4TokenRows && rows * n * blocks4(k) <= kL4TokenWork && rows * blocks4(k) <= kL4TokenBlocks; }
 struct Linear4Room { size_t scale = 0, all = 0; };
-static Linear4Room linear4_room(int64_t rows, int64_t k, bool given) {
+static Linear4Room linear4_room(int64_t rows, int64_t n, int64_t k, bool given) {
     Linear4Room r;
+    if (!given && token_fits4(rows, n, k)) return r;
     r.scale = given ? 0 : up256((size_t)rows * blocks4(k) * 16);
     // the scales lie in tiles of as many rows as a product takes: 64 at least beyond 128 rows, padded to 128
     r.all = r.scale + (size_t)slots4(rows, rows > 128 ? 64 : 128) * groups4(k) * 4;
     return r;
 }
-size_t linear4_workspace(int64_t rows, int64_t k) { return linear4_room(rows, k, false).all; }
+constexpr int64_t kAnyN = kMaxRows;             // (no matrix needs more than a large one)
+size_t linear4_workspace(int64_t rows, int64_t k) { return linear4_room(rows, kAnyN, k, false).all; }
 
 // How a product of more than kL4FewRows rows goes over the pairs of SMs: the tile width whose waves cost least, by what a k block takes.
 constexpr int kL4FewRows = 128;
@@ -88,6 +92,8 @@ static L4Pair pair_plan4(int64_t rows, int64_t n, int64_t k, int clusters) {
         p.nk = (int)(groups4(k) / 2);
         p.mt = (int)((n + 255) / 256);
         p.nt = (int)((rows + f.bn - 1) / f.bn);
+        // weights come from memory once for as many activation tiles as stay in half of L2 (4096 x 3584 x 37888, 4, 8, 16 and 20 tiles: 230, 221, 215 and 208 us)
+        p.raster = (int)std::max<int64_t>(8, std::min<int64_t>(p.nt, ((int64_t)64 << 20) / (f.bn * blocks4(k) * 17)));
         p.stages = (int)std::min<uint32_t>(kL4PairMaxStages, kL4PairRing / l4_pair_stage(f.bn, f.parts));
         p.slots = std::min(l4_pair_slots(f.bn, f.parts), p.stages);
         const double block = std::max(1.38 * f.bn, l4_pair_stage(f.bn, f.parts) / 90.0), tail = f.parts == 2 ? 13.0 * f.bn : 0.0;      // ns; results that no product hides
@@ -125,14 +131,34 @@ static void launch_pair4(LaunchCtx& lc, uint64_t bytes, const uint8_t* x, int64_
     else atoms == 1 ? go(linear4_pair_kernel<2, 1>) : go(linear4_pair_kernel<2, 2>);
 }
 
+template <typename T, int R, bool kVec>
+static void launch_token4(LaunchCtx& lc, uint64_t bytes, const void* x, int64_t ldx, int64_t k, const uint8_t* w, int64_t ldw, const Linear4Args& g) {
+    const int per = kL4TokenThreads / 32;
+    launch_op(lc, "linear4", bytes, linear4_token_kernel<T, R, kVec>, dim3((unsigned)std::min<int64_t>(((int64_t)g.n + per - 1) / per, 4 * kNumSMs)), kL4TokenThreads, (size_t)R * g.blocks * 36, 1,
+              false, g, static_cast<const T*>(x), (long long)ldx, (int)k, w, (long long)ldw);
+}
+
 // x in 4 bits: lds its scales' row stride
 static void run_linear4(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, const uint8_t* x_scale, int64_t lds, const uint8_t* w, int64_t ldw, const uint8_t* w_tiles, const float* bias,
                         int64_t rows, int64_t n, int64_t k, void* y, int y_dtype, int64_t ldy, void* workspace, int* failed) {
     const bool given = x_dtype == FL_DTYPE_MX4, many = rows > kL4FewRows;
     FL_CHECK(!many || g_pair_clusters >= 1, FL_ERR_UNSUPPORTED, "linear4: no two SMs of this device form a pair");
-    const Linear4Room room = linear4_room(rows, k, given);
+    const Linear4Room room = linear4_room(rows, n, k, given);
     uint8_t *to = static_cast<uint8_t*>(workspace), *xs = to + room.scale;
     const int blocks = (int)blocks4(k), groups = (int)groups4(k);
+    if (n == 1) ldw = 16 * blocks;
+    const uint64_t bytes = (uint64_t)(n + rows) * blocks * 17 + rows * n * dtype_size(y_dtype);
+    if (!given && token_fits4(rows, n, k)) {
+        const Linear4Args a{(int)rows, (int)n, blocks, nullptr, w_tiles, groups, bias, y, ldy, y_dtype, failed, false};
+        by_type(x_dtype, [&](auto t) {
+            using T = decltype(t);
+            const bool vec = rows_on_16(x, rows, ldx, sizeof(T));
+            auto go = [&](auto one, auto two) { rows == 1 ? one(lc, bytes, x, ldx, k, w, ldw, a) : two(lc, bytes, x, ldx, k, w, ldw, a); };
+            if (vec) go(launch_token4<T, 1, true>, launch_token4<T, 2, true>);
+            else go(launch_token4<T, 1, false>, launch_token4<T, 2, false>);
+        });
+        return;
+    }
     const L4Pair p = many ? pair_plan4(rows, n, k, g_pair_clusters) : L4Pair{};
     const int tile = many ? p.bn / p.parts : 128;
     const uint8_t* q = to;
@@ -144,9 +170,7 @@ static void run_linear4(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
     } else {
         quantize4(lc, x, x_dtype, rows, k, ldx, Rows4Out{to, ldq, xs, 0, blocks, tile, groups});
     }
-    if (n == 1) ldw = 16 * blocks;
-    const Linear4Args a{(int)rows, (int)n, blocks, xs, w_tiles, groups, bias, y, ldy, y_dtype, failed};
-    const uint64_t bytes = (uint64_t)(n + rows) * blocks * 17 + rows * n * dtype_size(y_dtype);
+    const Linear4Args a{(int)rows, (int)n, blocks, xs, w_tiles, groups, bias, y, ldy, y_dtype, failed, y_dtype != FL_DTYPE_F32 && rows_on_16(y, rows, ldy, 2)};
     if (many) launch_pair4(lc, bytes, q, ldq, w, ldw, a, p);
     else if (rows <= 16) launch_few4<16>(lc, bytes, q, ldq, w, ldw, a);
     else if (rows <= 32) launch_few4<32>(lc, bytes, q, ldq, w, ldw, a);
@@ -171,6 +195,7 @@ static void set_up() {
             using T = decltype(t);
             load_kernels(quantize4_kernel<T, false>, quantize4_kernel<T, true>);
             load_kernels(dequantize4_kernel<T, false>, dequantize4_kernel<T, true>);
+            load_kernels(linear4_token_kernel<T, 1, false>, linear4_token_kernel<T, 1, true>, linear4_token_kernel<T, 2, false>, linear4_token_kernel<T, 2, true>);
             for (int act : {FL_ACT_SILU, FL_ACT_GELU_TANH, FL_ACT_RELU, FL_ACT_SWISH_CLAMP}) load_kernels(glu4_form<T, false>(act), glu4_form<T, true>(act));
         });
     load_kernels(arrange4_kernel);
@@ -292,7 +317,7 @@ FL_EXPORT int fl_linear4_workspace(int64_t rows, int64_t k, int x_dtype, size_t*
     FL_CHECK(bytes, FL_ERR_INVALID, "NULL argument");
     FL_CHECK(is_float(x_dtype) || x_dtype == FL_DTYPE_MX4, FL_ERR_INVALID, "linear4: activations are f32, bf16, f16 or 4-bit rows");
     FL_CHECK(rows >= 0 && rows <= kMaxRows && k >= 1 && k <= kMaxCols4, FL_ERR_INVALID, "linear4: rows from 0 to 2^30, k from 1 to 2^20");
-    *bytes = linear4_room(rows, k, x_dtype == FL_DTYPE_MX4).all;
+    *bytes = linear4_room(rows, kAnyN, k, x_dtype == FL_DTYPE_MX4).all;
     FL_API_END
 }
 
@@ -312,8 +337,8 @@ FL_EXPORT int fl_linear4(const void* x, int x_dtype, int64_t ldx, const uint8_t*
     if (given) check_rows4("linear4", x, ldx, x_scale, lds, rows, k);
     FL_CHECK((given || aligned(x, dtype_size(x_dtype))) && aligned(y, dtype_size(y_dtype)) && aligned(bias, 4), FL_ERR_INVALID, "linear4: a pointer is not aligned to its type");
     FL_CHECK(rows <= ((int64_t)1 << 40) / n && n <= kMaxNumbers4 / k && rows <= kMaxNumbers4 / k, FL_ERR_INVALID, "linear4: more than 2^40 results, or an operand of more than 2^39 numbers");
-    const Linear4Room room = linear4_room(rows, k, given);
-    FL_CHECK(workspace && aligned(workspace, 256) && workspace_bytes >= room.all, FL_ERR_INVALID,
+    const Linear4Room room = linear4_room(rows, n, k, given);
+    FL_CHECK(room.all == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= room.all), FL_ERR_INVALID,
              "linear4: the workspace is smaller than fl_linear4_workspace asks for, or not on a 256-byte border");
     DeviceScope dev;
     set_up();

@@ -19,6 +19,7 @@ struct Linear4Args {
     const float* bias;                                      // [n] or null
     void* y; long long ldy; int y_dtype;                    // fl_dtype
     int* failed;                                            // set when a wait ran out
+    bool wide;                                              // 16-bit results whose rows start on 16-byte borders
 };
 
 constexpr int kL4Row = 128;                                 // bytes of a row in a k block: one swizzle row
@@ -271,17 +272,143 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     }
 }
 
+// ---- a token or two -----------------------------------------------------------------------------------------------------------------
+// One or two rows, rounded inside the product's own launch: a warp per weight row, a block of 32 weights a lane and load.  2 e2m1 is a whole number of 8 bits, so a block's
+// products are summed exactly, four to an instruction, and its two scales are applied to the sum.  Every block of threads rounds the rows into its shared memory (from L2) while its
+// first weights are on their way.
+constexpr int kL4TokenRows = 2, kL4TokenBlocks = 1024, kL4TokenWork = 1 << 20, kL4TokenThreads = 256, kL4TokenAhead = 2;      // rows; most blocks of 32 of the rows, and over all products;
+                                                                                                                                // loads on their way a lane
+
+// codes of four columns in the low half (and what is above it), doubled, as four whole numbers of 8 bits
+__device__ __forceinline__ uint32_t e2m1_doubled(uint32_t w) {
+    const uint32_t at = w & 0x7777u, up = __byte_perm(0x03020100u, 0x0C080604u, at), down = __byte_perm(0xFDFEFF00u, 0xF4F8FAFCu, at);
+    uint32_t neg;                                               // bytes of the codes' signs (which __byte_perm's selector does not ask for)
+    asm("prmt.b32 %0, %1, %2, 0x9D8C;" : "=r"(neg) : "r"(w), "r"(w << 4));
+    return (up & ~neg) | (down & neg);
+}
+
+template <typename T, int R, bool kVec>
+__global__ void __launch_bounds__(kL4TokenThreads) linear4_token_kernel(const Linear4Args g, const T* __restrict__ x, const long long ldx, const int k, const uint8_t* __restrict__ w,
+                                                                        const long long ldw) {
+    constexpr int U = kL4TokenAhead, kWarps = kL4TokenThreads / 32;
+    extern __shared__ uint4 sx[];                               // [R][2 halves of a block][blocks] whole numbers, then [R][blocks] scales / 4
+    float* sscale = reinterpret_cast<float*>(sx + 2 * R * g.blocks);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, blocks = g.blocks;
+    const int steps = (blocks + 32 * U - 1) / (32 * U), stride = gridDim.x * kWarps;
+    struct Part { uint4 q; uint32_t s; };
+    // a step: U blocks a lane of one weight row
+    auto fetch = [&](int n, int step, Part (&to)[U]) {
+        const uint4* row = reinterpret_cast<const uint4*>(w + (long long)n * ldw);
+        const uint8_t* scales = g.ws + scale4_at(n, 0, 128, g.groups);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int b = (step * U + u) * 32 + lane;
+            to[u] = Part{make_uint4(0, 0, 0, 0), 0};
+            if (b < blocks) {
+                to[u].q = ldg_stream(row + b);
+                to[u].s = __ldg(scales + (long long)(b / 4) * 512 + b % 4);
+            }
+        }
+    };
+    int n = blockIdx.x * kWarps + warp, step = 0;
+    Part now[U], next[U];
+    if (n < g.n) fetch(n, 0, now);
+
+    for (int r = 0; r < R; ++r) {
+        const int per = blocks * kR4Lanes<T>;
+        for (int p0 = 0; p0 < per; p0 += kL4TokenThreads) {     // (whole warps: two threads of a block of 32-bit numbers meet)
+            const int piece = p0 + threadIdx.x, b = piece / kR4Lanes<T>;
+            uint32_t v[16] = {};
+            if (piece < per) load64<T, kVec>(x + r * ldx, piece * kR4Own<T>, k, v);
+            const uint32_t s = scale4(block_max<T>(most_of<T>(v)));
+            if (piece >= per) continue;
+            const float up = up4(s);
+            uint32_t out[8];
+#pragma unroll
+            for (int i = 0; i < kR4Own<T> / 8; ++i) {
+                float f[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f[j] = s == 255u ? 0.f : number_of<T>(v, 8 * i + j) * up;
+                const uint32_t c = e2m1x8(f);
+                out[2 * i] = e2m1_doubled(c);
+                out[2 * i + 1] = e2m1_doubled(c >> 16);
+            }
+            uint4* to = sx + 2 * r * blocks + b;
+            if constexpr (kR4Lanes<T> == 1) {
+                to[0] = make_uint4(out[0], out[1], out[2], out[3]);
+                to[blocks] = make_uint4(out[4], out[5], out[6], out[7]);
+            } else {
+                to[(piece & 1) * blocks] = make_uint4(out[0], out[1], out[2], out[3]);
+            }
+            if (piece % kR4Lanes<T> == 0) sscale[r * blocks + b] = 0.25f * down4(s);
+        }
+    }
+    __syncthreads();
+
+    float sum[R] = {};
+    while (n < g.n) {
+        const bool last = step + 1 == steps;
+        const int n1 = last ? n + stride : n, step1 = last ? 0 : step + 1;
+        if (n1 < g.n) fetch(n1, step1, next);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int b = (step * U + u) * 32 + lane;
+            if (b >= blocks) break;
+            const uint32_t q[4] = {now[u].q.x, now[u].q.y, now[u].q.z, now[u].q.w};
+            int dot[R] = {};
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t m[4];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    m[2 * i] = e2m1_doubled(q[2 * h + i]);
+                    m[2 * i + 1] = e2m1_doubled(q[2 * h + i] >> 16);
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const uint4 a = sx[(2 * r + h) * blocks + b];
+                    dot[r] = __dp4a((int)m[0], (int)a.x, dot[r]);
+                    dot[r] = __dp4a((int)m[1], (int)a.y, dot[r]);
+                    dot[r] = __dp4a((int)m[2], (int)a.z, dot[r]);
+                    dot[r] = __dp4a((int)m[3], (int)a.w, dot[r]);
+                }
+            }
+            const float d = down4(now[u].s);
+#pragma unroll
+            for (int r = 0; r < R; ++r) sum[r] = fmaf((float)dot[r], d * sscale[r * blocks + b], sum[r]);
+        }
+        if (last) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float v = warp_sum(sum[r]);
+                sum[r] = 0.f;
+                if (lane != r) continue;                        // (each row's result by a lane of its own)
+                if (g.bias != nullptr) v += __ldg(g.bias + n);
+                const long long at = (long long)r * g.ldy + n;
+                if (g.y_dtype == 0) reinterpret_cast<float*>(g.y)[at] = v;
+                else if (g.y_dtype == 1) reinterpret_cast<__nv_bfloat16*>(g.y)[at] = from_f32<__nv_bfloat16>(v);
+                else reinterpret_cast<__half*>(g.y)[at] = from_f32<__half>(v);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) now[u] = next[u];
+        n = n1;
+        step = step1;
+    }
+}
+
 // ---- many rows ----------------------------------------------------------------------------------------------------------------------
 // As linear8_pair_kernel: pairs of SMs on tiles of 256 weight rows x bn activation rows, each with its 128 weight rows and half of the activation tile, and the scales
 // of its weight rows and of all the tile's activation rows.
 constexpr int kL4PairEpi = 16, kL4PairThreads = 64 + 32 * kL4PairEpi, kL4PairMaxStages = 8;
-constexpr uint32_t kL4PairRing = 200 * 1024;
-constexpr size_t kL4PairSmem = kL4PairRing + 1024;
+constexpr uint32_t kL4PairRing = 200 * 1024, kL4PairOut = 16 * 256;            // the ring; 16 rows of 128 results on their way out, for each four warps
+constexpr size_t kL4PairSmem = kL4PairRing + kL4PairEpi / 4 * kL4PairOut + 1024;
 
 struct L4Pair {
     int bn;                     // activation rows of a tile
     int parts;                  // products of a tile, bn / parts rows each: 1, with two accumulators in turn, or 2
     int nk, mt, nt;             // k blocks; weight and activation tiles
+    int raster;                 // activation tiles that share a weight tile before the walk moves on
     int stages, slots;          // of the ring; k blocks whose scales tensor memory holds
 };
 inline int l4_pair_atoms(int pn) { return (pn + 127) / 128; }
@@ -300,6 +427,25 @@ __device__ __forceinline__ void tma_load_2d_pair_lead(uint32_t lead, uint32_t ds
         "@e cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n}\n" ::"r"(dst),
         "l"(tmap), "r"(c0), "r"(c1), "r"(mbar), "r"(lead)
         : "memory");
+}
+
+// 16 rows of the results of 128 weight rows from n0 on, by four warps through their shared memory: whole lines of a row at a time.  A warp alone writes 64 bytes of a row with
+// an instruction, and 416 rows took 5.3 us that no product hides.
+__device__ __forceinline__ void l4_store_wide(const Linear4Args& g, int r, int n0, int rows, float bn, const uint32_t (&sum)[16], uint8_t* out, int barrier) {
+    const int lane = threadIdx.x & 31, q = (threadIdx.x >> 5) & 3;
+    unsigned short* to = reinterpret_cast<unsigned short*>(out) + q * 32 + lane;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        const float v = g.bias != nullptr ? __uint_as_float(sum[j]) + bn : __uint_as_float(sum[j]);
+        to[j * 128] = g.y_dtype == 1 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+    }
+    asm volatile("bar.sync %0, 128;" ::"r"(barrier) : "memory");
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int j = 4 * q + 2 * i + (lane >> 4);
+        if (j < rows) *reinterpret_cast<uint4*>(reinterpret_cast<unsigned short*>(g.y) + (long long)(r + j) * g.ldy + n0 + (lane & 15) * 8) = *reinterpret_cast<const uint4*>(out + j * 256 + (lane & 15) * 16);
+    }
+    asm volatile("bar.sync %0, 128;" ::"r"(barrier) : "memory");
 }
 
 // kParts, kAtoms: L4Pair's parts and l4_pair_atoms of a part's rows
@@ -334,10 +480,8 @@ linear4_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = tmem_base_s;
-    // 8 activation tiles share a weight tile before the walk moves on (see kGemmRasterRows)
     auto place = [&](int tile, int& n, int& rt) {
-        constexpr int RM = kGemmRasterRows / 2;
-        const int per = RM * p.mt, first = tile / per * RM, local = tile % per, cnt = min(RM, p.nt - first);
+        const int per = p.raster * p.mt, first = tile / per * p.raster, local = tile % per, cnt = min(p.raster, p.nt - first);
         rt = first + local % cnt;
         n = local / cnt * 256 + (int)rank * 128;
     };
@@ -436,7 +580,9 @@ linear4_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
                 for (int c = cs * 16; ok && c < last_col; c += 64) {
                     uint32_t v[16];
                     tmem_ld16(at + (uint32_t)c, v);
-                    l4_store16(g, r0 + c, n, min(last_col - c, 16), bias, v);
+                    const int rows = min(last_col - c, 16);
+                    if (g.wide && n0 + 128 <= g.n) l4_store_wide(g, r0 + c, n0, rows, bias, v, gsm + kL4PairRing + cs * kL4PairOut, 1 + cs);
+                    else l4_store16(g, r0 + c, n, rows, bias, v);
                 }
                 tc_fence_before();
                 __syncwarp();

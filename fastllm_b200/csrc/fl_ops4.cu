@@ -65,19 +65,18 @@ static void arrange4(LaunchCtx& lc, const uint8_t* scale, int64_t lds, int64_t r
               (long long)rows, (int)blocks4(k), tiles, tile, (int)groups, (long long)slots);
 }
 
-// whether a product's rows are rounded inside its own launch (ops.py keeps the same rule, for the workspace)
-static bool token_fits4(int64_t rows, int64_t n, int64_t k) { return rows <= kL4TokenRows && rows * n * blocks4(k) <= kL4TokenWork && rows * blocks4(k) <= kL4TokenBlocks; }
+static bool token_fits4(int64_t rows, int64_t n, int64_t k) { return rows <= kL4TokenRows && rows * rows * n * blocks4(k) <= kL4TokenWork && rows * blocks4(k) <= kL4TokenBlocks; }
 struct Linear4Room { size_t scale = 0, all = 0; };
-static Linear4Room linear4_room(int64_t rows, int64_t n, int64_t k, bool given) {
+// (ops.py keeps the same rule)
+static Linear4Room linear4_room(int64_t rows, int64_t k, bool given) {
     Linear4Room r;
-    if (!given && token_fits4(rows, n, k)) return r;
+    if (!given && rows <= kL4SelfRows) return r;                // rounded inside the product's own launch
     r.scale = given ? 0 : up256((size_t)rows * blocks4(k) * 16);
     // the scales lie in tiles of as many rows as a product takes: 64 at least beyond 128 rows, padded to 128
     r.all = r.scale + (size_t)slots4(rows, rows > 128 ? 64 : 128) * groups4(k) * 4;
     return r;
 }
-constexpr int64_t kAnyN = kMaxRows;             // (no matrix needs more than a large one)
-size_t linear4_workspace(int64_t rows, int64_t k) { return linear4_room(rows, kAnyN, k, false).all; }
+size_t linear4_workspace(int64_t rows, int64_t k) { return linear4_room(rows, k, false).all; }
 
 // How a product of more than kL4FewRows rows goes over the pairs of SMs: the tile width whose waves cost least, by what a k block takes.
 constexpr int kL4FewRows = 128;
@@ -109,10 +108,11 @@ static FailedWord g_op4_failed;
 static int g_pair_clusters = 0;                 // pairs of SMs that can be resident at once
 bool products4_failed() { return g_op4_failed.take(); }
 
-// Blocks that share a 128-row weight tile (see few_slices of the 8-bit product).
+// Blocks that share a 128-row weight tile: one per SM at most, four k blocks each at least, and only where a block is spared twelve: the cluster's barriers and the exchange take as
+// long (S = 1, 2 and 4: 16 x 4096 x 4096 8.8, 8.9 and 8.1 us, 64 x 4096 x 4096 9.9, 9.7 and 8.7, 32 x 14336 x 4096 20.5, 14.6 and 11.9, 8 x 1024 x 4096 5.0, 6.7 and 6.5).
 static int few_slices4(int64_t tiles, int nk) {
     int S = 8;
-    while (S > 1 && (S * tiles > kNumSMs || nk < 8 * S || nk - nk / S < 24)) S /= 2;
+    while (S > 1 && (S * tiles > kNumSMs || nk < 4 * S || nk - nk / S < 12)) S /= 2;
     return S;
 }
 template <int BN>
@@ -120,6 +120,12 @@ static void launch_few4(LaunchCtx& lc, uint64_t bytes, const uint8_t* x, int64_t
     const int tiles = (g.n + 127) / 128, S = few_slices4(tiles, g.groups / 2);
     const CUtensorMap tw = make_tmap_i8(w, g.n, g.blocks * 16, ldw, 128), tx = make_tmap_i8(x, g.rows, g.blocks * 16, ldx, BN);
     launch_op(lc, "linear4", bytes, linear4_few_kernel<BN>, dim3((unsigned)(tiles * S)), L4Few<BN>::kThreads, L4Few<BN>::kSmem, S, true, tw, tx, g, S);
+}
+template <typename T, bool kVec>
+static void launch_self4(LaunchCtx& lc, uint64_t bytes, const void* x, int64_t ldx, int64_t k, const uint8_t* w, int64_t ldw, const Linear4Args& g) {
+    const int tiles = (g.n + 127) / 128, S = few_slices4(tiles, g.groups / 2);
+    const CUtensorMap tw = make_tmap_i8(w, g.n, g.blocks * 16, ldw, 128);
+    launch_op(lc, "linear4", bytes, linear4_self_kernel<T, kVec>, dim3((unsigned)(tiles * S)), L4Self::kThreads, L4Self::kSmem, S, false, tw, g, static_cast<const T*>(x), (long long)ldx, (int)k, S);
 }
 static void launch_pair4(LaunchCtx& lc, uint64_t bytes, const uint8_t* x, int64_t ldx, const uint8_t* w, int64_t ldw, const Linear4Args& g, const L4Pair& p) {
     const int pn = p.bn / p.parts, atoms = l4_pair_atoms(pn);
@@ -143,7 +149,7 @@ static void run_linear4(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
                         int64_t rows, int64_t n, int64_t k, void* y, int y_dtype, int64_t ldy, void* workspace, int* failed) {
     const bool given = x_dtype == FL_DTYPE_MX4, many = rows > kL4FewRows;
     FL_CHECK(!many || g_pair_clusters >= 1, FL_ERR_UNSUPPORTED, "linear4: no two SMs of this device form a pair");
-    const Linear4Room room = linear4_room(rows, n, k, given);
+    const Linear4Room room = linear4_room(rows, k, given);
     uint8_t *to = static_cast<uint8_t*>(workspace), *xs = to + room.scale;
     const int blocks = (int)blocks4(k), groups = (int)groups4(k);
     if (n == 1) ldw = 16 * blocks;
@@ -156,6 +162,14 @@ static void run_linear4(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
             auto go = [&](auto one, auto two) { rows == 1 ? one(lc, bytes, x, ldx, k, w, ldw, a) : two(lc, bytes, x, ldx, k, w, ldw, a); };
             if (vec) go(launch_token4<T, 1, true>, launch_token4<T, 2, true>);
             else go(launch_token4<T, 1, false>, launch_token4<T, 2, false>);
+        });
+        return;
+    }
+    if (!given && rows <= kL4SelfRows) {
+        const Linear4Args a{(int)rows, (int)n, blocks, nullptr, w_tiles, groups, bias, y, ldy, y_dtype, failed, false};
+        by_type(x_dtype, [&](auto t) {
+            using T = decltype(t);
+            rows_on_16(x, rows, ldx, sizeof(T)) ? launch_self4<T, true>(lc, bytes, x, ldx, k, w, ldw, a) : launch_self4<T, false>(lc, bytes, x, ldx, k, w, ldw, a);
         });
         return;
     }
@@ -178,6 +192,10 @@ static void run_linear4(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
     else launch_few4<128>(lc, bytes, q, ldq, w, ldw, a);
 }
 
+template <typename T>
+static void self_attr4() {
+    for (auto kern : {linear4_self_kernel<T, false>, linear4_self_kernel<T, true>}) FL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L4Self::kSmem));
+}
 template <int BN>
 static void few_attr4() {
     FL_CUDA(cudaFuncSetAttribute(linear4_few_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L4Few<BN>::kSmem));
@@ -195,6 +213,7 @@ static void set_up() {
             using T = decltype(t);
             load_kernels(quantize4_kernel<T, false>, quantize4_kernel<T, true>);
             load_kernels(dequantize4_kernel<T, false>, dequantize4_kernel<T, true>);
+            self_attr4<T>();
             load_kernels(linear4_token_kernel<T, 1, false>, linear4_token_kernel<T, 1, true>, linear4_token_kernel<T, 2, false>, linear4_token_kernel<T, 2, true>);
             for (int act : {FL_ACT_SILU, FL_ACT_GELU_TANH, FL_ACT_RELU, FL_ACT_SWISH_CLAMP}) load_kernels(glu4_form<T, false>(act), glu4_form<T, true>(act));
         });
@@ -317,7 +336,7 @@ FL_EXPORT int fl_linear4_workspace(int64_t rows, int64_t k, int x_dtype, size_t*
     FL_CHECK(bytes, FL_ERR_INVALID, "NULL argument");
     FL_CHECK(is_float(x_dtype) || x_dtype == FL_DTYPE_MX4, FL_ERR_INVALID, "linear4: activations are f32, bf16, f16 or 4-bit rows");
     FL_CHECK(rows >= 0 && rows <= kMaxRows && k >= 1 && k <= kMaxCols4, FL_ERR_INVALID, "linear4: rows from 0 to 2^30, k from 1 to 2^20");
-    *bytes = linear4_room(rows, kAnyN, k, x_dtype == FL_DTYPE_MX4).all;
+    *bytes = linear4_room(rows, k, x_dtype == FL_DTYPE_MX4).all;
     FL_API_END
 }
 
@@ -337,7 +356,7 @@ FL_EXPORT int fl_linear4(const void* x, int x_dtype, int64_t ldx, const uint8_t*
     if (given) check_rows4("linear4", x, ldx, x_scale, lds, rows, k);
     FL_CHECK((given || aligned(x, dtype_size(x_dtype))) && aligned(y, dtype_size(y_dtype)) && aligned(bias, 4), FL_ERR_INVALID, "linear4: a pointer is not aligned to its type");
     FL_CHECK(rows <= ((int64_t)1 << 40) / n && n <= kMaxNumbers4 / k && rows <= kMaxNumbers4 / k, FL_ERR_INVALID, "linear4: more than 2^40 results, or an operand of more than 2^39 numbers");
-    const Linear4Room room = linear4_room(rows, n, k, given);
+    const Linear4Room room = linear4_room(rows, k, given);
     FL_CHECK(room.all == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= room.all), FL_ERR_INVALID,
              "linear4: the workspace is smaller than fl_linear4_workspace asks for, or not on a 256-byte border");
     DeviceScope dev;

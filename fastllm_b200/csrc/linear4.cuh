@@ -272,11 +272,145 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     }
 }
 
+// ---- few rows, rounded on the way ------------------------------------------------------------------------------------------------------
+// Up to 16 rows that are not in 4 bits yet: the warps of the epilogue round a k block of all rows (a block of 32 a thread) while its weights are on their way, straight into the
+// ring.  Every block of threads rounds the rows anew, from L2; what that saves is a launch, and the wait for it between the first weights and the first product.
+constexpr int kL4SelfRows = 16;
+struct L4Self {
+    static constexpr int kRows = kL4SelfRows;
+    static constexpr uint32_t kX = kRows * kL4Row, kSW = kL4WBytes + kX, kStage = kSW + 2 * kL4Scales;
+    static constexpr int kPerSm = 2, kStages = 5, kThreads = 192, kRounders = 128;
+    static constexpr size_t kSmem = (size_t)kStages * kStage + 1024;
+    static constexpr uint32_t kTmem = 128;
+    static_assert(kRows + 16 * kStages <= (int)kTmem && kStages * kStage >= kRows * 512u, "accumulators and every stage's scales; the parts of a tile fit the ring");
+};
+
+template <typename T, bool kVec>
+__global__ void __launch_bounds__(L4Self::kThreads, L4Self::kPerSm)
+linear4_self_kernel(const __grid_constant__ CUtensorMap tmW, const Linear4Args g, const T* __restrict__ x, const long long ldx, const int k, const int S) {
+    using L = L4Self;
+    constexpr int kStages = L::kStages, BN = L::kRows, kPieces = BN * 8 * kR4Lanes<T> / L::kRounders;      // pieces of 64 bytes a thread and k block
+    extern __shared__ uint8_t gsm_raw[];
+    uint8_t* gsm = gsm_raw + ((1024u - (smem_u32(gsm_raw) & 1023u)) & 1023u);          // (the same offset in all blocks of a cluster)
+    __shared__ __align__(8) uint64_t full[kStages], empty[kStages], done;
+    __shared__ uint32_t tmem_base_s;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    const int s = S == 1 ? 0 : (int)cluster_rank();
+    const int tile = blockIdx.x / S, n0 = tile * 128;
+    const int nk = g.groups / 2, kb0 = (int)((long long)s * nk / S), kb1 = (int)((long long)(s + 1) * nk / S);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) { mbar_init(&full[i], 1 + L::kRounders / 32); mbar_init(&empty[i], 1); }
+        mbar_init(&done, 1);
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc(&tmem_base_s, L::kTmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_s;
+    bool ok = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int st = 0;
+            uint32_t ph = 1;
+            for (int kb = kb0; kb < kb1; ++kb) {
+                if (!(ok = mbar_wait_bounded(&empty[st], ph, kMbarTries))) break;
+                mbar_expect_tx(&full[st], kL4WBytes + kL4Scales);
+                tma_load_2d(gsm + st * L::kStage, &tmW, kb * kL4Row, n0, &full[st]);
+                bulk_g2s(gsm + st * L::kStage + L::kSW, g.ws + ((long long)tile * nk + kb) * kL4Scales, kL4Scales, &full[st]);
+                if (++st == kStages) { st = 0; ph ^= 1; }
+            }
+        }
+    } else if (warp == 1) {
+        const uint64_t base = umma_smem_desc_sw128(gsm), scales = umma_smem_desc_scales(gsm + L::kSW);
+        const uint32_t lead = elect_lead();
+        int st = 0;
+        uint32_t ph = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            if (ok) ok = mbar_wait_bounded(&full[st], ph, kMbarTries);
+            __syncwarp();
+            const uint64_t at = (uint64_t)(st * (L::kStage >> 4)), a = base + at, b = a + (kL4WBytes >> 4);
+            const uint32_t sa = tmem + BN + 16 * st, sb = sa + 8;
+            tmem_scales<1>(lead, sa, 4, scales + at, 512 >> 4);
+            tmem_scales<1>(lead, sb, 4, scales + at + (kL4Scales >> 4), 512 >> 4);
+            umma_mx4_block<1>(lead, tmem, a, b, umma_idesc_mx4(128, BN, 0), umma_idesc_mx4(128, BN, 1), sa, sb, 4, kb > kb0 ? 1u : 0u);
+            umma_commit_lead(lead, &empty[st]);
+            if (++st == kStages) { st = 0; ph ^= 1; }
+        }
+        umma_commit_lead(lead, &done);
+    } else {
+        const int t = threadIdx.x - 64;
+        // piece i of a thread: row and place among a k block's pieces of that row
+        auto row_of = [&](int i) { return (t + L::kRounders * i) / (8 * kR4Lanes<T>); };
+        auto place_of = [&](int i) { return (t + L::kRounders * i) % (8 * kR4Lanes<T>); };
+        uint32_t even[kPieces][16], odd[kPieces][16];           // two k blocks ahead: their way from L2 takes longer than a k block's weights
+        auto fetch = [&](int kb, uint32_t (&to)[kPieces][16]) {
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) to[i][j] = 0u;
+                if (kb < kb1 && row_of(i) < g.rows) load64<T, kVec>(x + row_of(i) * ldx, kb * 256 + place_of(i) * kR4Own<T>, k, to[i]);
+            }
+        };
+        int st = 0;
+        uint32_t ph = 1;
+        auto round = [&](int kb, uint32_t (&from)[kPieces][16]) {
+            uint32_t codes[kPieces][kR4Own<T> / 8], byte[kPieces];
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                byte[i] = scale4(block_max<T>(most_of<T>(from[i])));
+                const float up = up4(byte[i]);
+#pragma unroll
+                for (int h = 0; h < kR4Own<T> / 8; ++h) {
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = byte[i] == 255u ? 0.f : number_of<T>(from[i], 8 * h + j) * up;
+                    codes[i][h] = e2m1x8(v);
+                }
+            }
+            fetch(kb + 2, from);
+            if (ok) ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&empty[st], ph, kMbarTries));
+            uint8_t *to = gsm + st * L::kStage + kL4WBytes, *sc = gsm + st * L::kStage + L::kSW + kL4Scales;
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                const int r = row_of(i), b = place_of(i) / kR4Lanes<T>;                // the 16 bytes of block b lie at b ^ (r mod 8) of the row's 128 (the operands' swizzle)
+                uint8_t* at = to + r * kL4Row + ((b ^ (r & 7)) * 16);
+                if constexpr (kR4Lanes<T> == 1) *reinterpret_cast<uint4*>(at) = make_uint4(codes[i][0], codes[i][1], codes[i][2], codes[i][3]);
+                else *reinterpret_cast<uint2*>(at + 8 * (place_of(i) & 1)) = make_uint2(codes[i][0], codes[i][1]);
+                if (place_of(i) % kR4Lanes<T> == 0) sc[b / 4 * 512 + r * 16 + b % 4] = (uint8_t)byte[i];
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");               // written through the generic proxy, read by the products
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[st]);
+            if (++st == kStages) { st = 0; ph ^= 1; }
+        };
+        fetch(kb0, even);
+        fetch(kb0 + 1, odd);
+        for (int kb = kb0; kb < kb1; kb += 2) {
+            round(kb, even);
+            if (kb + 1 < kb1) round(kb + 1, odd);
+        }
+        if (ok) ok = __all_sync(0xFFFFFFFFu, mbar_wait_bounded(&done, 0, kMbarTries));
+        tc_fence_after();
+    }
+    l4_few_finish<BN>(g, S, s, n0, tmem, gsm, ok);
+    if (!ok) op_give_up(g.failed);
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, L::kTmem);
+    }
+}
+
 // ---- a token or two -----------------------------------------------------------------------------------------------------------------
 // One or two rows, rounded inside the product's own launch: a warp per weight row, a block of 32 weights a lane and load.  2 e2m1 is a whole number of 8 bits, so a block's
 // products are summed exactly, four to an instruction, and its two scales are applied to the sum.  Every block of threads rounds the rows into its shared memory (from L2) while its
 // first weights are on their way.
-constexpr int kL4TokenRows = 2, kL4TokenBlocks = 1024, kL4TokenWork = 1 << 20, kL4TokenThreads = 256, kL4TokenAhead = 2;      // rows; most blocks of 32 of the rows, and over all products;
+constexpr int kL4TokenRows = 2, kL4TokenBlocks = 1024, kL4TokenWork = 1 << 19, kL4TokenThreads = 256, kL4TokenAhead = 2;      // rows; most blocks of 32 of the rows, and over all products;
                                                                                                                                 // loads on their way a lane
 
 // codes of four columns in the low half (and what is above it), doubled, as four whole numbers of 8 bits

@@ -153,6 +153,10 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, b
 def _rows4(q: torch.Tensor, scale: torch.Tensor, dev: int, what: str, name: str):
     """4-bit rows [..., 16 blocks] and their scales [..., blocks] as matrices"""
     u8 = torch.uint8
+    if q.ndim == 2 == scale.ndim and q.dtype is u8 is scale.dtype and q.get_device() == dev == scale.get_device():       # (the usual call)
+        (rows, width), (lines, blocks) = q.shape, scale.shape
+        if rows == lines and width == 16 * blocks > 0 and q.stride(1) == 1 and (scale.stride(1) == 1 or blocks == 1):
+            return q, scale
     if q.dtype is not u8 or scale.dtype is not u8 or q.ndim == 0 or scale.ndim == 0 or q.shape[:-1] != scale.shape[:-1] or q.shape[-1] != 16 * scale.shape[-1]:
         _refuse(f"{what}: {name} are uint8 rows of 16 bytes per block with a uint8 scale per block, got {q.dtype} {tuple(q.shape)} and {scale.dtype} {tuple(scale.shape)}")
     if scale.shape[-1] == 0:
@@ -255,9 +259,9 @@ def weight4(q: torch.Tensor, scale: torch.Tensor) -> Weight4:
     return Weight4(q, tiles, scale)
 
 
-def _room4(rows: int, n: int, blocks: int, given: bool) -> int:
-    """what fl_linear4 needs of the workspace that fl_linear4_workspace tells of: a token or two through a small matrix need none"""
-    if not given and rows <= 2 and rows * n * blocks <= 1 << 20 and rows * blocks <= 1024:
+def _room4(rows: int, blocks: int, given: bool) -> int:
+    """fl_linear4_workspace's rule"""
+    if not given and rows <= 16:
         return 0
     return (0 if given else (rows * blocks * 16 + 255) // 256 * 256) + ((rows + 127) // 128 if rows <= 128 else (rows + 63) // 64) * ((blocks + 7) // 8) * 1024
 
@@ -315,7 +319,7 @@ def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = Non
     else:
         y2 = _rows(out, what)
         ldy = y2.stride(0)
-    room = _room4(rows, n, blocks, given)
+    room = _room4(rows, blocks, given)
     work = work_ptr = None
     if room:
         work = x.new_empty(room, dtype=torch.uint8)

@@ -85,8 +85,8 @@ def test_weight4_refuses(change, word):
     (dict(ldw=32), "row stride"), (dict(ldy=31), "row stride"), (dict(x=None), "NULL"), (dict(w=None), "NULL"), (dict(w_tiles=None), "NULL"), (dict(y=None), "NULL"),
     (dict(x_scale=P), "x_scale"), (dict(x_dtype=4, ldx=48), "x_scale"), (dict(w=P + 8), "16-byte"), (dict(ldw=56), "16-byte"), (dict(w_tiles=P + 8), "16-byte"),
     (dict(x_dtype=4, x_scale=P, lds=3, ldx=47), "row stride"), (dict(x_dtype=4, x_scale=P, lds=2, ldx=48), "row stride"), (dict(x_dtype=4, x_scale=P, lds=3, ldx=48, x=P + 4), "16-byte"),
-    (dict(x_dtype=4, x_scale=P, lds=3, ldx=56), "16-byte"), (dict(x=P + 1), "aligned"), (dict(y=P + 1), "aligned"), (dict(bias=P + 1), "aligned"), (dict(workspace=None), "workspace"),
-    (dict(workspace=P + 16), "workspace"), (dict(workspace_bytes=256 + 1024 - 1), "workspace"), (dict(rows=1 << 21, n=1 << 20, ldy=1 << 20), "2^40")])
+    (dict(x_dtype=4, x_scale=P, lds=3, ldx=56), "16-byte"), (dict(x=P + 1), "aligned"), (dict(y=P + 1), "aligned"), (dict(bias=P + 1), "aligned"), (dict(rows=17, workspace=None), "workspace"),
+    (dict(rows=17, workspace=P + 16), "workspace"), (dict(rows=17, workspace_bytes=1024 + 1024 - 1), "workspace"), (dict(x_dtype=4, x_scale=P, lds=3, ldx=48, workspace=None), "workspace"), (dict(rows=1 << 21, n=1 << 20, ldy=1 << 20), "2^40")])
 def test_linear4_refuses(change, word):
     _refused(_linear4(**change), word)
 
@@ -118,7 +118,7 @@ def test_workspace_of_fewer_rows_is_no_larger(k, dtype):
     n, most = C.c_size_t(), 0
     for rows in range(0, 700):
         assert _lib.load().fl_linear4_workspace(rows, k, dtype, C.byref(n)) == 0
-        assert n.value >= most and n.value == ops._room4(rows, 1 << 30, (k + 31) // 32, dtype == 4)
+        assert n.value >= most and n.value == ops._room4(rows, (k + 31) // 32, dtype == 4)
         most = n.value
 
 

@@ -66,38 +66,37 @@ static void arrange4(LaunchCtx& lc, const uint8_t* scale, int64_t lds, int64_t r
 }
 
 static bool token_fits4(int64_t rows, int64_t n, int64_t k) { return rows <= kL4TokenRows && rows * rows * n * blocks4(k) <= kL4TokenWork && rows * blocks4(k) <= kL4TokenBlocks; }
-struct Linear4Room { size_t scale = 0, all = 0; };
+struct Linear4Room { size_t scale = 0, all = 0; int64_t slots = 0; };
 // (ops.py keeps the same rule)
 static Linear4Room linear4_room(int64_t rows, int64_t k, bool given) {
     Linear4Room r;
     if (!given && rows <= kL4SelfRows) return r;                // rounded inside the product's own launch
     r.scale = given ? 0 : up256((size_t)rows * blocks4(k) * 16);
-    // the scales lie in tiles of as many rows as a product takes: 64 at least beyond 128 rows, padded to 128
-    r.all = r.scale + (size_t)slots4(rows, rows > 128 ? 64 : 128) * groups4(k) * 4;
+    // the scales lie in tiles of as many rows as a product takes, each padded to 128: beyond 128 rows 64 to 224, which is twice the rows at most and 256
+    r.slots = rows <= 128 ? (rows + 127) / 128 * 128 : (2 * rows + 127) / 128 * 128 + 256;
+    r.all = r.scale + (size_t)r.slots * groups4(k) * 4;
     return r;
 }
 size_t linear4_workspace(int64_t rows, int64_t k) { return linear4_room(rows, k, false).all; }
 
-// How a product of more than kL4FewRows rows goes over the pairs of SMs: the tile width whose waves cost least, by what a k block takes.
+// How a product of more than kL4FewRows rows goes over the pairs of SMs: the tile width whose waves cost least.  A k block takes 60 + 1.1 bn ns where its operands come from L2
+// (bn = 128, 160, 192, 208 and 224: 193, 228, 282, 257 to 290 and 287 to 307), and a tile no less than its results take, 1200 + 7 bn.
 constexpr int kL4FewRows = 128;
 static L4Pair pair_plan4(int64_t rows, int64_t n, int64_t k, int clusters) {
-    static constexpr struct { int bn, parts; } kForms[] = {{416, 2}, {384, 2}, {320, 2}, {256, 2}, {224, 1}, {208, 1}, {192, 1}, {160, 1}, {128, 1}, {96, 1}, {64, 1}};
     L4Pair best{};
     double cost = -1;
-    for (const auto& f : kForms) {
+    for (int bn = kL4PairMaxRows; bn >= kL4PairMinRows; bn -= 16) {
         L4Pair p{};
-        p.bn = f.bn;
-        p.parts = f.parts;
+        p.bn = bn;
         p.nk = (int)(groups4(k) / 2);
         p.mt = (int)((n + 255) / 256);
-        p.nt = (int)((rows + f.bn - 1) / f.bn);
+        p.nt = (int)((rows + bn - 1) / bn);
         // weights come from memory once for as many activation tiles as stay in half of L2 (4096 x 3584 x 37888, 4, 8, 16 and 20 tiles: 230, 221, 215 and 208 us)
-        p.raster = (int)std::max<int64_t>(8, std::min<int64_t>(p.nt, ((int64_t)64 << 20) / (f.bn * blocks4(k) * 17)));
-        p.stages = (int)std::min<uint32_t>(kL4PairMaxStages, kL4PairRing / l4_pair_stage(f.bn, f.parts));
-        p.slots = std::min(l4_pair_slots(f.bn, f.parts), p.stages);
-        const double block = std::max(1.38 * f.bn, l4_pair_stage(f.bn, f.parts) / 90.0), tail = f.parts == 2 ? 13.0 * f.bn : 0.0;      // ns; results that no product hides
+        p.raster = (int)std::max<int64_t>(8, std::min<int64_t>(p.nt, ((int64_t)64 << 20) / (bn * blocks4(k) * 17)));
+        p.stages = (int)std::min<uint32_t>(kL4PairMaxStages, kL4PairRing / l4_pair_stage(bn));
+        p.slots = std::min(l4_pair_slots(bn), p.stages);
         const double waves = (double)(((long long)p.mt * p.nt + clusters - 1) / clusters);
-        const double c = waves * (p.nk * block + tail);
+        const double c = waves * std::max(p.nk * (60 + 1.1 * bn), 1200.0 + 7.0 * bn);
         if (cost < 0 || c < cost) { cost = c; best = p; }
     }
     return best;
@@ -128,13 +127,12 @@ static void launch_self4(LaunchCtx& lc, uint64_t bytes, const void* x, int64_t l
     launch_op(lc, "linear4", bytes, linear4_self_kernel<T, kVec>, dim3((unsigned)(tiles * S)), L4Self::kThreads, L4Self::kSmem, S, false, tw, g, static_cast<const T*>(x), (long long)ldx, (int)k, S);
 }
 static void launch_pair4(LaunchCtx& lc, uint64_t bytes, const uint8_t* x, int64_t ldx, const uint8_t* w, int64_t ldw, const Linear4Args& g, const L4Pair& p) {
-    const int pn = p.bn / p.parts, atoms = l4_pair_atoms(pn);
-    const CUtensorMap tx = make_tmap_i8(x, g.rows, g.blocks * 16, ldx, pn / 2), tw = make_tmap_i8(w, g.n, g.blocks * 16, ldw, 128);
-    const CUtensorMap tws = make_tmap_scales(g.ws, (int64_t)((g.n + 127) / 128) * g.groups, 2), txs = make_tmap_scales(g.xs, (int64_t)((g.rows + pn - 1) / pn) * g.groups * atoms, 2 * atoms);
+    const int bn = p.bn, atoms = l4_pair_atoms(bn);
+    const CUtensorMap tx = make_tmap_i8(x, g.rows, g.blocks * 16, ldx, bn / 2), tw = make_tmap_i8(w, g.n, g.blocks * 16, ldw, 128);
+    const CUtensorMap tws = make_tmap_scales(g.ws, (int64_t)((g.n + 127) / 128) * g.groups, 2), txs = make_tmap_scales(g.xs, (int64_t)p.nt * g.groups * atoms, 2 * atoms);
     const long long clusters = std::min<long long>(g_pair_clusters, (long long)p.mt * p.nt);
     auto go = [&](auto kern) { launch_op(lc, "linear4", bytes, kern, dim3((unsigned)(2 * clusters)), kL4PairThreads, kL4PairSmem, 1, true, tw, tx, tws, txs, g, p); };
-    if (p.parts == 1) atoms == 1 ? go(linear4_pair_kernel<1, 1>) : go(linear4_pair_kernel<1, 2>);
-    else atoms == 1 ? go(linear4_pair_kernel<2, 1>) : go(linear4_pair_kernel<2, 2>);
+    atoms == 1 ? go(linear4_pair_kernel<1>) : go(linear4_pair_kernel<2>);
 }
 
 template <typename T, int R, bool kVec>
@@ -174,7 +172,8 @@ static void run_linear4(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
         return;
     }
     const L4Pair p = many ? pair_plan4(rows, n, k, g_pair_clusters) : L4Pair{};
-    const int tile = many ? p.bn / p.parts : 128;
+    const int tile = many ? p.bn : 128;
+    FL_CHECK(slots4(rows, tile) <= room.slots, FL_ERR_STATE, "linear4: the scales do not fit their workspace");
     const uint8_t* q = to;
     int64_t ldq = 16 * blocks;
     if (given) {
@@ -219,7 +218,7 @@ static void set_up() {
         });
     load_kernels(arrange4_kernel);
     few_attr4<16>(); few_attr4<32>(); few_attr4<64>(); few_attr4<128>();
-    for (auto kern : {linear4_pair_kernel<1, 1>, linear4_pair_kernel<1, 2>, linear4_pair_kernel<2, 1>, linear4_pair_kernel<2, 2>})
+    for (auto kern : {linear4_pair_kernel<1>, linear4_pair_kernel<2>})
         FL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL4PairSmem));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(kNumSMs); cfg.blockDim = dim3(kL4PairThreads); cfg.dynamicSmemBytes = kL4PairSmem;
@@ -228,7 +227,7 @@ static void set_up() {
     at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = 1;
     int pairs = 0;
-    FL_CUDA(cudaOccupancyMaxActiveClusters(&pairs, linear4_pair_kernel<2, 2>, &cfg));
+    FL_CUDA(cudaOccupancyMaxActiveClusters(&pairs, linear4_pair_kernel<2>, &cfg));
     g_pair_clusters = std::min(pairs, kNumSMs / 2);
     int* p = nullptr;
     FL_CUDA(cudaMallocHost(&p, sizeof(int)));

@@ -533,23 +533,23 @@ __global__ void __launch_bounds__(kL4TokenThreads) linear4_token_kernel(const Li
 
 // ---- many rows ----------------------------------------------------------------------------------------------------------------------
 // As linear8_pair_kernel: pairs of SMs on tiles of 256 weight rows x bn activation rows, each with its 128 weight rows and half of the activation tile, and the scales
-// of its weight rows and of all the tile's activation rows.
-constexpr int kL4PairEpi = 16, kL4PairThreads = 64 + 32 * kL4PairEpi, kL4PairMaxStages = 8;
+// of its weight rows and of all the tile's activation rows.  bn is at most 224: two accumulators and the scales of two k blocks fill tensor memory.  (Tiles of 256 to 416 rows
+// as two products, without a second accumulator, move a quarter less through L2, but nothing hides their results: 4096 x 3584 x 37888 251 us with 416 rows, 221 with 208.)
+constexpr int kL4PairEpi = 16, kL4PairThreads = 64 + 32 * kL4PairEpi, kL4PairMaxStages = 8, kL4PairMinRows = 64, kL4PairMaxRows = 224;
 constexpr uint32_t kL4PairRing = 200 * 1024, kL4PairOut = 16 * 256;            // the ring; 16 rows of 128 results on their way out, for each four warps
 constexpr size_t kL4PairSmem = kL4PairRing + kL4PairEpi / 4 * kL4PairOut + 1024;
 
 struct L4Pair {
-    int bn;                     // activation rows of a tile
-    int parts;                  // products of a tile, bn / parts rows each: 1, with two accumulators in turn, or 2
+    int bn;                     // activation rows of a tile, a multiple of 16
     int nk, mt, nt;             // k blocks; weight and activation tiles
     int raster;                 // activation tiles that share a weight tile before the walk moves on
     int stages, slots;          // of the ring; k blocks whose scales tensor memory holds
 };
-inline int l4_pair_atoms(int pn) { return (pn + 127) / 128; }
+inline int l4_pair_atoms(int bn) { return (bn + 127) / 128; }
 // bytes of a stage: weights | half of the activations | scales of the weights | of the activations
-inline uint32_t l4_pair_stage(int bn, int parts) { return kL4WBytes + (uint32_t)bn * (kL4Row / 2) + kL4Scales * (uint32_t)(1 + parts * l4_pair_atoms(bn / parts)); }
+inline uint32_t l4_pair_stage(int bn) { return kL4WBytes + (uint32_t)bn * (kL4Row / 2) + kL4Scales * (uint32_t)(1 + l4_pair_atoms(bn)); }
 // k blocks whose scales find a place in tensor memory beside two accumulators
-inline int l4_pair_slots(int bn, int parts) { return (512 - 2 * (bn / parts)) / (8 + 8 * parts * l4_pair_atoms(bn / parts)); }
+inline int l4_pair_slots(int bn) { return (512 - 2 * bn) / (8 + 8 * l4_pair_atoms(bn)); }
 
 __device__ __forceinline__ void expect_tx_lead(uint32_t lead, uint32_t bar, uint32_t bytes) {
     asm volatile("{\n.reg .pred e;\nsetp.ne.b32 e, %2, 0;\n@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}\n" ::"r"(bar), "r"(bytes), "r"(lead) : "memory");
@@ -562,9 +562,8 @@ __device__ __forceinline__ void tma_load_2d_pair_lead(uint32_t lead, uint32_t ds
         "l"(tmap), "r"(c0), "r"(c1), "r"(mbar), "r"(lead)
         : "memory");
 }
-
 // 16 rows of the results of 128 weight rows from n0 on, by four warps through their shared memory: whole lines of a row at a time.  A warp alone writes 64 bytes of a row with
-// an instruction, and 416 rows took 5.3 us that no product hides.
+// an instruction (4096 x 3584 x 37888 without this 224 us, with it 218).
 __device__ __forceinline__ void l4_store_wide(const Linear4Args& g, int r, int n0, int rows, float bn, const uint32_t (&sum)[16], uint8_t* out, int barrier) {
     const int lane = threadIdx.x & 31, q = (threadIdx.x >> 5) & 3;
     unsigned short* to = reinterpret_cast<unsigned short*>(out) + q * 32 + lane;
@@ -582,8 +581,8 @@ __device__ __forceinline__ void l4_store_wide(const Linear4Args& g, int r, int n
     asm volatile("bar.sync %0, 128;" ::"r"(barrier) : "memory");
 }
 
-// kParts, kAtoms: L4Pair's parts and l4_pair_atoms of a part's rows
-template <int kParts, int kAtoms>
+// kAtoms: l4_pair_atoms of a tile's rows
+template <int kAtoms>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kL4PairThreads, 1)
 linear4_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmWS, const __grid_constant__ CUtensorMap tmXS,
                     const Linear4Args g, const L4Pair p) {
@@ -593,8 +592,8 @@ linear4_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
     __shared__ uint32_t tmem_base_s;
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank();
-    const int cl = blockIdx.x >> 1, G = gridDim.x >> 1, nk = p.nk, T = p.mt * p.nt, bn = p.bn, pn = bn / kParts;
-    const uint32_t x_bytes = (uint32_t)bn * (kL4Row / 2), stage = kL4WBytes + x_bytes + kL4Scales * (uint32_t)(1 + kParts * kAtoms);
+    const int cl = blockIdx.x >> 1, G = gridDim.x >> 1, nk = p.nk, T = p.mt * p.nt, bn = p.bn;
+    const uint32_t x_bytes = (uint32_t)bn * (kL4Row / 2), stage = kL4WBytes + x_bytes + kL4Scales * (uint32_t)(1 + kAtoms);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < p.stages; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
@@ -627,30 +626,28 @@ linear4_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
         asm volatile("fence.proxy.async;" ::: "memory");
         int st = 0;
         uint32_t ph = 1;
-        const int w_last = (g.n + 127) / 128 - 1, x_last = (g.rows + pn - 1) / pn - 1;         // scales exist for tiles that hold a row
+        const int w_last = (g.n + 127) / 128 - 1;                                              // scales exist for tiles that hold a row
         for (int tile = cl; ok && tile < T; tile += G) {
             int n0, rt;
             place(tile, n0, rt);
-            const int r0 = rt * bn + (int)rank * (pn >> 1);
-            const int ws0 = min(n0 / 128, w_last) * nk * 2, xs0 = min(rt * kParts, x_last) * nk * 2 * kAtoms, xs1 = min(rt * kParts + 1, x_last) * nk * 2 * kAtoms;
+            const int r0 = rt * bn + (int)rank * (bn >> 1);
+            const int ws0 = min(n0 / 128, w_last) * nk * 2, xs0 = rt * nk * 2 * kAtoms;
             for (int kb = 0; kb < nk; ++kb) {
                 if (!(ok = mbar_wait_bounded(&empty[st], ph, kMbarTries))) break;
                 const uint32_t bar = mapa_u32(smem_u32(&full[st]), 0), sa = smem_u32(gsm) + st * stage, ss = sa + kL4WBytes + x_bytes;
                 if (rank == 0) expect_tx_lead(lead, smem_u32(&full[st]), 2 * stage);                           // both CTAs' loads complete on the first one's barrier
                 tma_load_2d_pair_lead(lead, sa, &tmW, kb * kL4Row, n0, bar);
                 tma_load_2d_pair_lead(lead, sa + kL4WBytes, &tmX, kb * kL4Row, r0, bar);
-                if (kParts == 2) tma_load_2d_pair_lead(lead, sa + kL4WBytes + (uint32_t)pn * (kL4Row / 2), &tmX, kb * kL4Row, r0 + pn, bar);
                 tma_load_2d_pair_lead(lead, ss, &tmWS, 0, ws0 + 2 * kb, bar);
                 tma_load_2d_pair_lead(lead, ss + kL4Scales, &tmXS, 0, xs0 + 2 * kAtoms * kb, bar);
-                if (kParts == 2) tma_load_2d_pair_lead(lead, ss + kL4Scales * (1 + kAtoms), &tmXS, 0, xs1 + 2 * kAtoms * kb, bar);
                 if (++st == p.stages) { st = 0; ph ^= 1; }
             }
         }
     } else if (warp == 1) {
         if (rank == 0) {
-            const uint32_t second = ((uint32_t)pn * (kL4Row / 2)) >> 4, id0 = umma_idesc_mx4(256, pn, 0), id1 = umma_idesc_mx4(256, pn, 1);
-            constexpr uint32_t kCols = 8 + 8 * kParts * kAtoms;
-            const uint32_t scale0 = tmem_base + 2 * pn, lead = elect_lead();
+            const uint32_t id0 = umma_idesc_mx4(256, bn, 0), id1 = umma_idesc_mx4(256, bn, 1);
+            constexpr uint32_t kCols = 8 + 8 * kAtoms;
+            const uint32_t scale0 = tmem_base + 2 * bn, lead = elect_lead();
             const uint64_t base = umma_smem_desc_sw128(gsm), scales = umma_smem_desc_scales(gsm + kL4WBytes + x_bytes);
             const bool look_back = p.slots < p.stages;
             int st = 0, back = 0, slot = 0, free = p.slots;                            // back: the stage of p.slots k blocks ago
@@ -663,9 +660,8 @@ linear4_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
                 tc_fence_after();
             };
             for (int tile = cl; tile < T; tile += G, ++seg) {
-                const uint32_t as = kParts == 2 ? 0 : seg & 1, uses = kParts == 2 ? seg : seg >> 1, tacc = tmem_base + as * pn;
-                wait(&acc_empty[as], (uses & 1) ^ 1);
-                if (kParts == 2) wait(&acc_empty[1], (uses & 1) ^ 1);
+                const uint32_t as = seg & 1, tacc = tmem_base + as * bn;
+                wait(&acc_empty[as], ((seg >> 1) & 1) ^ 1);
                 for (int kb = 0; kb < nk; ++kb) {
                     // (no fence behind these two: what they wait for are copies into shared memory and this thread's own products)
                     if (!here && ok) ok = mbar_wait_bounded(&full[st], ph, kMbarTries);
@@ -683,16 +679,14 @@ linear4_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
                     const uint64_t at = (uint64_t)(st0 * (stage >> 4)), a = base + at, b = a + (kL4WBytes >> 4), sd = scales + at;
                     const uint32_t sa = scale0 + slot * kCols, sb = sa + 8, more = kb > 0 ? 1u : 0u;
                     if (++slot == p.slots) slot = 0;
-                    // columns: weights' groups 0 and 1, then for each product and group the atoms of its rows
+                    // columns: weights' groups 0 and 1, then for each group the atoms of the activation rows
                     tmem_scales<2>(lead, sa, 4, sd, 512 >> 4);
 #pragma unroll
-                    for (int i = 0; i < kParts * kAtoms; ++i) tmem_scales<2>(lead, sb + 8 * i, 4, sd + (kL4Scales >> 4) * (1 + i), 512 >> 4);
+                    for (int i = 0; i < kAtoms; ++i) tmem_scales<2>(lead, sb + 8 * i, 4, sd + (kL4Scales >> 4) * (1 + i), 512 >> 4);
                     umma_mx4_block<2>(lead, tacc, a, b, id0, id1, sa, sb, 4 * kAtoms, more);
-                    if (kParts == 2) umma_mx4_block<2>(lead, tacc + pn, a, b + second, id0, id1, sa, sb + 8 * kAtoms, 4 * kAtoms, more);
                     umma_commit_pair_lead(lead, &empty[st0]);
                 }
                 umma_commit_pair_lead(lead, &acc_full[as]);
-                if (kParts == 2) umma_commit_pair_lead(lead, &acc_full[1]);
             }
         }
     } else {
@@ -704,24 +698,22 @@ linear4_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             place(tile, n0, rt);
             const int n = n0 + q * 32 + lane;
             const float bias = g.bias != nullptr && n < g.n ? __ldg(g.bias + n) : 0.f;
-            for (int h = 0; h < kParts; ++h) {
-                const uint32_t as = kParts == 2 ? (uint32_t)h : seg & 1, uses = kParts == 2 ? seg : seg >> 1;
-                const int r0 = rt * bn + h * pn, last_col = min(pn, g.rows - r0);
-                if (ok) ok = __all_sync(0xFFFFFFFFu, pair_wait(&acc_full[as], uses & 1));
-                tc_fence_after();
-                const uint32_t at = tmem_base + as * pn + ((uint32_t)(q * 32) << 16);
+            const uint32_t as = seg & 1;
+            const int r0 = rt * bn, last_col = min(bn, g.rows - r0);
+            if (ok) ok = __all_sync(0xFFFFFFFFu, pair_wait(&acc_full[as], (seg >> 1) & 1));
+            tc_fence_after();
+            const uint32_t at = tmem_base + as * bn + ((uint32_t)(q * 32) << 16);
 #pragma unroll 1
-                for (int c = cs * 16; ok && c < last_col; c += 64) {
-                    uint32_t v[16];
-                    tmem_ld16(at + (uint32_t)c, v);
-                    const int rows = min(last_col - c, 16);
-                    if (g.wide && n0 + 128 <= g.n) l4_store_wide(g, r0 + c, n0, rows, bias, v, gsm + kL4PairRing + cs * kL4PairOut, 1 + cs);
-                    else l4_store16(g, r0 + c, n, rows, bias, v);
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[as]), 0));
+            for (int c = cs * 16; ok && c < last_col; c += 64) {
+                uint32_t v[16];
+                tmem_ld16(at + (uint32_t)c, v);
+                const int rows = min(last_col - c, 16);
+                if (g.wide && n0 + 128 <= g.n) l4_store_wide(g, r0 + c, n0, rows, bias, v, gsm + kL4PairRing + cs * kL4PairOut, 1 + cs);
+                else l4_store16(g, r0 + c, n, rows, bias, v);
             }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[as]), 0));
         }
     }
     if (!ok) op_give_up(g.failed);

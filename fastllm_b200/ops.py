@@ -263,7 +263,7 @@ def _room4(rows: int, blocks: int, given: bool) -> int:
     """fl_linear4_workspace's rule"""
     if not given and rows <= 16:
         return 0
-    return (0 if given else (rows * blocks * 16 + 255) // 256 * 256) + ((rows + 127) // 128 if rows <= 128 else (rows + 63) // 64) * ((blocks + 7) // 8) * 1024
+    return (0 if given else (rows * blocks * 16 + 255) // 256 * 256) + ((rows + 127) // 128 if rows <= 128 else (2 * rows + 127) // 128 + 2) * ((blocks + 7) // 8) * 1024
 
 
 def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = None, *, x_scale: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,

@@ -26,6 +26,7 @@ _bound = [None]             # the device of the last call
 _FLOATS = {torch.float32: _lib.FL_DTYPE_F32, torch.bfloat16: _lib.FL_DTYPE_BF16, torch.float16: _lib.FL_DTYPE_F16}
 _TYPES = {**_FLOATS, torch.int8: _lib.FL_DTYPE_I8}
 _FLOATS4 = {**_FLOATS, torch.uint8: _lib.FL_DTYPE_MX4}
+_U8 = torch.uint8
 _TOKENS = {torch.int32: 4, torch.int64: 8}
 MAX_TOP = 32
 
@@ -152,12 +153,11 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, b
 
 def _rows4(q: torch.Tensor, scale: torch.Tensor, dev: int, what: str, name: str):
     """4-bit rows [..., 16 blocks] and their scales [..., blocks] as matrices"""
-    u8 = torch.uint8
-    if q.ndim == 2 == scale.ndim and q.dtype is u8 is scale.dtype and q.get_device() == dev == scale.get_device():       # (the usual call)
+    if q.ndim == 2 == scale.ndim and q.dtype is _U8 is scale.dtype and q.get_device() == dev == scale.get_device():       # (the usual call)
         (rows, width), (lines, blocks) = q.shape, scale.shape
-        if rows == lines and width == 16 * blocks > 0 and q.stride(1) == 1 and (scale.stride(1) == 1 or blocks == 1):
+        if rows == lines and width == 16 * blocks > 0 and q.stride()[1] == 1 and (blocks == 1 or scale.stride()[1] == 1):
             return q, scale
-    if q.dtype is not u8 or scale.dtype is not u8 or q.ndim == 0 or scale.ndim == 0 or q.shape[:-1] != scale.shape[:-1] or q.shape[-1] != 16 * scale.shape[-1]:
+    if q.dtype is not _U8 or scale.dtype is not _U8 or q.ndim == 0 or scale.ndim == 0 or q.shape[:-1] != scale.shape[:-1] or q.shape[-1] != 16 * scale.shape[-1]:
         _refuse(f"{what}: {name} are uint8 rows of 16 bytes per block with a uint8 scale per block, got {q.dtype} {tuple(q.shape)} and {scale.dtype} {tuple(scale.shape)}")
     if scale.shape[-1] == 0:
         _refuse(f"{what}: {name} have no columns")
@@ -178,11 +178,15 @@ def quantize4(x: torch.Tensor):
     dev = x.get_device()
     if dev != _bound[0]:
         _device(x, what)
-    x2 = x if x.ndim == 2 and x.stride(1) == 1 else _rows(x, what)
+    step = x.stride()
+    x2 = x
+    if len(step) != 2 or step[1] != 1:
+        x2 = _rows(x, what)
+        step = x2.stride()
     rows, cols = x2.shape
     blocks = (cols + 31) // 32
-    q, scale = x.new_empty((rows, 16 * blocks), dtype=torch.uint8), x.new_empty((rows, blocks), dtype=torch.uint8)
-    rc = _lib.load().fl_quantize4(x2.data_ptr(), kind, rows, cols, x2.stride(0), q.data_ptr(), 16 * blocks, scale.data_ptr(), blocks, _stream(dev))
+    q, scale = x.new_empty(rows, 16 * blocks, dtype=_U8), x.new_empty(rows, blocks, dtype=_U8)         # (sizes one by one: a tuple of them costs 0.4 us)
+    rc = _lib.load().fl_quantize4(x2.data_ptr(), kind, rows, cols, step[0], q.data_ptr(), 16 * blocks, scale.data_ptr(), blocks, _stream(dev))
     if rc:
         _lib.check(rc)
     return (q, scale) if x.ndim == 2 else (q.view(x.shape[:-1] + (16 * blocks,)), scale.view(x.shape[:-1] + (blocks,)))
@@ -203,8 +207,8 @@ def dequantize4(q: torch.Tensor, scale: torch.Tensor, cols: Optional[int] = None
         cols = 32 * blocks
     elif not 32 * blocks - 32 < cols <= 32 * blocks:
         _refuse(f"{what}: rows of {blocks} blocks have from {32 * blocks - 31} to {32 * blocks} columns, not {cols}")
-    y = q.new_empty((rows, cols), dtype=dtype)
-    rc = _lib.load().fl_dequantize4(q2.data_ptr(), q2.stride(0), s2.data_ptr(), s2.stride(0), rows, cols, y.data_ptr(), kind, cols, _stream(dev))
+    y = q.new_empty(rows, cols, dtype=dtype)
+    rc = _lib.load().fl_dequantize4(q2.data_ptr(), q2.stride()[0], s2.data_ptr(), s2.stride()[0], rows, cols, y.data_ptr(), kind, cols, _stream(dev))
     if rc:
         _lib.check(rc)
     return y if q.ndim == 2 else y.view(q.shape[:-1] + (cols,))
@@ -225,14 +229,18 @@ def glu4(x: torch.Tensor, act: str = "silu", *, limit: float = 7.0):
     dev = x.get_device()
     if dev != _bound[0]:
         _device(x, what)
-    x2 = x if x.ndim == 2 and x.stride(1) == 1 else _rows(x, what)
+    step = x.stride()
+    x2 = x
+    if len(step) != 2 or step[1] != 1:
+        x2 = _rows(x, what)
+        step = x2.stride()
     rows, both = x2.shape
     if both % 2:
         _refuse(f"{what}: a row holds as many gates as ups, got {both} numbers")
     cols = both // 2
     blocks = (cols + 31) // 32
-    q, scale = x.new_empty((rows, 16 * blocks), dtype=torch.uint8), x.new_empty((rows, blocks), dtype=torch.uint8)
-    rc = _lib.load().fl_glu4(x2.data_ptr(), kind, rows, cols, x2.stride(0), way, limit, q.data_ptr(), 16 * blocks, scale.data_ptr(), blocks, _stream(dev))
+    q, scale = x.new_empty(rows, 16 * blocks, dtype=_U8), x.new_empty(rows, blocks, dtype=_U8)         # (sizes one by one: a tuple of them costs 0.4 us)
+    rc = _lib.load().fl_glu4(x2.data_ptr(), kind, rows, cols, step[0], way, limit, q.data_ptr(), 16 * blocks, scale.data_ptr(), blocks, _stream(dev))
     if rc:
         _lib.check(rc)
     return (q, scale) if x.ndim == 2 else (q.view(x.shape[:-1] + (16 * blocks,)), scale.view(x.shape[:-1] + (blocks,)))
@@ -314,7 +322,7 @@ def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = Non
     if y_type is None:
         _refuse(f"{what}: results are f32, bf16 or f16, got {out_dtype}")
     if out is None:
-        y2 = x.new_empty((rows, n), dtype=out_dtype)
+        y2 = x.new_empty(rows, n, dtype=out_dtype)
         out, ldy = (y2 if x.ndim == 2 else y2.view(x.shape[:-1] + (n,))), n
     else:
         y2 = _rows(out, what)
@@ -322,7 +330,7 @@ def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = Non
     room = _room4(rows, blocks, given)
     work = work_ptr = None
     if room:
-        work = x.new_empty(room, dtype=torch.uint8)
+        work = x.new_empty(room, dtype=_U8)
         work_ptr = work.data_ptr()
     rc = _lib.load().fl_linear4(x2.data_ptr(), x_type, x2.stride(0), xs_ptr, lds, w.data_ptr(), w.stride(0), tiles.data_ptr(), bias_ptr, rows, n, k, y2.data_ptr(), y_type, ldy, work_ptr, room,
                                 _stream(dev))

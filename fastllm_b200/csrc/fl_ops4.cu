@@ -59,10 +59,10 @@ static void glu4(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t 
 }
 
 size_t weight4_bytes(int64_t n, int64_t k) { return (size_t)(slots4(n, 128) * groups4(k) * 4); }
-static void arrange4(LaunchCtx& lc, const uint8_t* scale, int64_t lds, int64_t rows, int64_t k, int tile, uint8_t* tiles, bool pdl) {
+static void arrange4(LaunchCtx& lc, const uint8_t* scale, int64_t lds, int64_t rows, int64_t k, int tile, uint8_t* tiles) {
     const int64_t slots = slots4(rows, tile), groups = groups4(k);
-    launch_op(lc, "arrange4", (uint64_t)(2 * slots * groups * 4), arrange4_kernel, dim3((unsigned)((slots + 127) / 128), (unsigned)groups), 128, 0, 1, pdl, scale, (long long)lds,
-              (long long)rows, (int)blocks4(k), tiles, tile, (int)groups, (long long)slots);
+    launch_op(lc, "arrange4", (uint64_t)(2 * slots * groups * 4), arrange4_kernel, dim3((unsigned)(slots / 128), (unsigned)((groups + kArrange - 1) / kArrange)), 128, 0, 1, false, scale,
+              (long long)lds, (long long)rows, (int)blocks4(k), tiles, tile, (int)groups, (tile + 127) / 128);
 }
 
 static bool token_fits4(int64_t rows, int64_t n, int64_t k) { return rows <= kL4TokenRows && rows * rows * n * blocks4(k) <= kL4TokenWork && rows * blocks4(k) <= kL4TokenBlocks; }
@@ -177,7 +177,7 @@ static void run_linear4(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
     const uint8_t* q = to;
     int64_t ldq = 16 * blocks;
     if (given) {
-        arrange4(lc, x_scale, lds, rows, k, tile, xs, false);
+        arrange4(lc, x_scale, lds, rows, k, tile, xs);
         q = static_cast<const uint8_t*>(x);
         if (rows > 1) ldq = ldx;
     } else {
@@ -326,7 +326,7 @@ FL_EXPORT int fl_weight4(const uint8_t* scale, int64_t lds, int64_t n, int64_t k
     DeviceScope dev;
     set_up();
     LaunchCtx lc = op_ctx(stream);
-    arrange4(lc, scale, lds, n, k, 128, static_cast<uint8_t*>(tiles), false);
+    arrange4(lc, scale, lds, n, k, 128, static_cast<uint8_t*>(tiles));
     FL_API_END
 }
 

@@ -388,22 +388,37 @@ __global__ void __launch_bounds__(kR4Threads) glu4_kernel(const T* __restrict__ 
     if (at.here) put4<T>(o, at.r, at.piece, codes, s);
 }
 
-// scales [n][lds] into the layout of the tensor cores (tiles of `tile` rows; zeros behind the last row and block): a thread per row and group
-__global__ void arrange4_kernel(const uint8_t* __restrict__ scale, long long lds, long long rows, int blocks, uint8_t* __restrict__ tiles, int tile, int groups, long long slots) {
-    const long long r = (long long)blockIdx.x * blockDim.x + threadIdx.x;       // counted in whole 128 rows of each tile
-    const int g = blockIdx.y;
+// Scales [rows][lds] into the layout of the tensor cores, in tiles of `tile` rows, zeros behind the last row and block.  A block of threads takes 128 rows (an atom of a tile) and
+// kArrange groups: a thread reads 32 neighbours of its row, and whole atoms of 512 bytes are written.
+constexpr int kArrange = 8;
+__global__ void __launch_bounds__(128) arrange4_kernel(const uint8_t* __restrict__ scale, long long lds, long long rows, int blocks, uint8_t* __restrict__ tiles, int tile, int groups, int atoms) {
+    __shared__ __align__(16) uint32_t part[kArrange][128];
+    const int t = threadIdx.x, g0 = blockIdx.y * kArrange;
+    const long long i = blockIdx.x / atoms;                     // the tile, and the atom's place in it
+    const int atom = (int)(blockIdx.x - i * atoms), in = atom * 128 + t;
+    const long long row = i * tile + in;
     pdl_launch_dependents();
-    if (r >= slots) return;
-    const int atoms = (tile + 127) / 128;
-    const long long t = r / (atoms * 128), in = r % (atoms * 128), row = t * tile + in;
-    uint32_t w = 0;
-    if (in < tile && row < rows) {
-        const uint8_t* from = scale + row * lds + 4 * g;
+    const uint8_t* from = scale + row * lds + 4 * g0;
+    const bool here = in < tile && row < rows, words = (reinterpret_cast<uintptr_t>(from) & 3u) == 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (4 * g + i < blocks) w |= (uint32_t)from[i] << (8 * i);
+    for (int g = 0; g < kArrange; ++g) {
+        const int left = here ? blocks - 4 * (g0 + g) : 0;
+        uint32_t w = 0;
+        if (words && left >= 4) {
+            w = __ldg(reinterpret_cast<const uint32_t*>(from) + g);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < left) w |= (uint32_t)from[4 * g + j] << (8 * j);
+        }
+        part[g][t % 32 * 4 + t / 32] = w;
     }
-    *reinterpret_cast<uint32_t*>(tiles + ((t * groups + g) * atoms + in / 128) * 512 + in % 32 * 16 + in % 128 / 32 * 4) = w;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kArrange / 4; ++j) {
+        const int g = 4 * j + t / 32;
+        if (g0 + g < groups) *reinterpret_cast<uint4*>(tiles + ((i * groups + g0 + g) * atoms + atom) * 512 + t % 32 * 16) = *reinterpret_cast<const uint4*>(&part[g][t % 32 * 4]);
+    }
 }
 
 }  // namespace fl

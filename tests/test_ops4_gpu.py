@@ -2,11 +2,14 @@
 
 Roundings to 4 bits are compared bit for bit; other tolerances count roundings: half = finfo(type).eps / 2 is half a step of the result's type."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
 
-from fastllm_b200 import ops
+from fastllm_b200 import _lib, ops
 from fastllm_b200._lib import FastllmError
 
 pytestmark = pytest.mark.gpu
@@ -164,6 +167,25 @@ def test_dequantize4(dtype, rows, cols):
                 ops.dequantize4(q, scale, bad)
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("cols, shift", [(96, 0), (70, 1), (33, 3), (1999, 2), (1, 5)])
+def test_rows_with_room_between_them(dtype, cols, shift):
+    """row strides on all sides, by the C ABI: what lies behind a row and behind the last row stays as it was"""
+    rows, blocks, kind = 9, (cols + 31) // 32, {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    lib, stream = _lib.load(), torch.cuda.current_stream().cuda_stream
+    x = (torch.randn(rows, cols + 7, device="cuda", generator=_gen(cols)) * 3).to(dtype)[:, shift:cols + shift]
+    q = torch.full((rows + 1, blocks * 16 + 48), 77, dtype=torch.uint8, device="cuda")
+    scale = torch.full((rows + 1, blocks + 5), 77, dtype=torch.uint8, device="cuda")
+    y = torch.full((rows + 1, cols + 9), 7.0, dtype=dtype, device="cuda")
+    assert lib.fl_quantize4(x.data_ptr(), kind, rows, cols, x.stride(0), q[:, 16:].data_ptr(), q.stride(0), scale[:, shift:].data_ptr(), scale.stride(0), stream) == 0
+    assert lib.fl_dequantize4(q[:, 16:].data_ptr(), q.stride(0), scale[:, shift:].data_ptr(), scale.stride(0), rows, cols, y[:, shift:].data_ptr(), kind, y.stride(0), stream) == 0
+    inner, s = q[:rows, 16:16 + blocks * 16], scale[:rows, shift:shift + blocks]
+    _check_rows(x, inner, s)
+    assert torch.equal(y[:rows, shift:shift + cols], _values(inner, s)[:, :cols].to(dtype))
+    inner.fill_(77), s.fill_(77), y[:rows, shift:shift + cols].fill_(7.0)
+    assert (q == 77).all() and (scale == 77).all() and (y == 7).all()
+
+
 # ---- the gated activation -----------------------------------------------------------------------------------------------------------
 def _activation(x, act, limit):
     g, u = x.double().chunk(2, -1)
@@ -290,6 +312,37 @@ def test_linear4(rows, n, k, dtype):
     y = ops.linear4(x, ops.weight4(q, scale), bias)
     assert y.dtype == dtype
     _check_product(y, _exact_x(x), _values(q, scale), bias)
+
+
+@pytest.mark.parametrize("rows", list(range(1, 20)) + [30, 63] + list(range(129, 260, 9)) + list(range(300, 1000, 67)))
+def test_linear4_row_counts(rows):
+    """every way to round the rows and to cut them into tiles, rows that start on odd elements, as many columns as no tile divides"""
+    n, k = 300, 545
+    x = (torch.randn(rows, k + 3, device="cuda", generator=_gen(rows)) * 2).to(FLOATS[rows % 3])[:, rows % 4:][:, :k]
+    q, scale = _rows4(n, k, 122, n)
+    xq, xs = ops.quantize4(x)
+    y = ops.linear4(x, ops.weight4(q, scale), out_dtype=torch.float32)
+    _check_product(y, _exact_x(x), _values(q, scale), None)
+    if rows > 2:                                # (a token or two are summed in another order)
+        assert torch.equal(y, ops.linear4(xq, ops.weight4(q, scale), x_scale=xs))
+
+
+@pytest.mark.parametrize("rows, n", [(1, 40), (2, 300), (7, 140), (40, 130), (100, 129), (150, 520)])
+def test_linear4_of_long_rows(rows, n):
+    """long sums: many k blocks of a cluster's part, more groups than a word of their count holds"""
+    k = 200003
+    x = torch.randn(rows, k, device="cuda", generator=_gen(rows)).bfloat16()
+    q, scale = _rows4(n, k, 118, n)
+    _check_product(ops.linear4(x, ops.weight4(q, scale), out_dtype=torch.float32), _exact_x(x), _values(q, scale), None)
+
+
+@pytest.mark.parametrize("rows, n", [(1, 70000), (3, 70000), (20, 40000), (300, 40000)])
+def test_linear4_of_wide_matrices(rows, n):
+    """more weight tiles than blocks that run at once"""
+    k = 96
+    x = torch.randn(rows, k, device="cuda", generator=_gen(rows)).half()
+    q, scale = _rows4(n, k, 122, n)
+    _check_product(ops.linear4(x, ops.weight4(q, scale)), _exact_x(x), _values(q, scale), None)
 
 
 @pytest.mark.parametrize("rows, n, k", SIZES)
@@ -490,3 +543,58 @@ def test_graphs(rows):
         for g, x, y, s in graphs:
             assert torch.equal(y, _feed_forward(x, w_in, w_out))
     ops.check()
+
+
+HEAD = """
+import threading
+import torch
+from fastllm_b200 import _lib, ops
+g = torch.Generator(device="cuda"); g.manual_seed(1)
+x = torch.randn(300, 200, device="cuda", generator=g).bfloat16()
+w = ops.Weight4(*[torch.randint(118, 124, s, dtype=torch.uint8, device="cuda", generator=g) for s in ((900, 112), (8 * 1024,), (900, 7))])
+calls = {"rows": lambda: ops.quantize4(x), "back": lambda: (ops.dequantize4(w.q, w.scale),), "glu": lambda: ops.glu4(x), "weight": lambda: ops.weight4(w.q, w.scale)[1:2],
+         "token": lambda: (ops.linear4(x[:1], w),), "self": lambda: (ops.linear4(x[:9], w),), "few": lambda: (ops.linear4(x[:60], w),), "pair": lambda: (ops.linear4(x, w),)}
+same = lambda a, b: all(torch.equal(u, v) for u, v in zip(a, b))
+_lib.init(0)                        # the process is bound, no operator has run
+"""
+
+
+def _run(code):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", HEAD + code], capture_output=True, text=True, timeout=300, cwd=root, env=dict(os.environ, PYTHONPATH=root))
+    assert r.returncode == 0 and r.stdout.strip() == "same", r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("name", ["rows", "back", "glu", "weight", "token", "self", "few", "pair"])
+def test_first_call_of_a_bound_process_inside_a_capture(name):
+    """set-up and loading do not break the capture"""
+    _run("""
+call = calls[%r]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = call()
+graph.replay()
+torch.cuda.synchronize()
+assert same(y, call())
+ops.check()
+print("same")
+""" % name)
+
+
+def test_first_calls_in_several_threads():
+    _run("""
+got = {}
+gate = threading.Barrier(16)
+def work(i, name):
+    gate.wait()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        got[i, name] = calls[name]()
+        torch.cuda.current_stream().synchronize()
+torch.cuda.synchronize()
+threads = [threading.Thread(target=work, args=(i, n)) for i in range(2) for n in calls]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert len(got) == 16 and all(same(y, calls[n]()) for (_, n), y in got.items())
+ops.check()
+print("same")
+""")

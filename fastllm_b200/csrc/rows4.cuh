@@ -151,6 +151,8 @@ __device__ __forceinline__ void load64(const T* row, int at, int cols, uint32_t 
             const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + at) + i);
             w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
         }
+    } else if (!kVec && at + kR4Own<T> <= cols) {
+        load_row(row, at, cols, w);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

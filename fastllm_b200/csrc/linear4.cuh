@@ -509,7 +509,10 @@ __global__ void __launch_bounds__(kL4TokenThreads) linear4_token_kernel(const Li
             }
             const float d = down4(now[u].s);
 #pragma unroll
-            for (int r = 0; r < R; ++r) sum[r] = fmaf((float)dot[r], d * sscale[r * blocks + b], sum[r]);
+            for (int r = 0; r < R; ++r) {
+                const float p = d * sscale[r * blocks + b];
+                sum[r] = fmaf((float)dot[r], dot[r] == 0 && p == INFINITY ? 0.f : p, sum[r]);     // (no products, whatever their scales)
+            }
         }
         if (last) {
 #pragma unroll
@@ -704,10 +707,10 @@ linear4_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_consta
             tc_fence_after();
             const uint32_t at = tmem_base + as * bn + ((uint32_t)(q * 32) << 16);
 #pragma unroll 1
-            for (int c = cs * 16; ok && c < last_col; c += 64) {
+            for (int c = cs * 16; c < last_col; c += 64) {
                 uint32_t v[16];
                 tmem_ld16(at + (uint32_t)c, v);
-                const int rows = min(last_col - c, 16);
+                const int rows = ok ? min(last_col - c, 16) : 0;                       // (the warps that store together go on together, whoever gave up)
                 if (g.wide && n0 + 128 <= g.n) l4_store_wide(g, r0 + c, n0, rows, bias, v, gsm + kL4PairRing + cs * kL4PairOut, 1 + cs);
                 else l4_store16(g, r0 + c, n, rows, bias, v);
             }

@@ -148,3 +148,12 @@ def test_every_way_to_an_operator_sets_up_first():
         body = source.split(f" {name}(", 1)[1].split("\n}\n", 1)[0]
         launch = re.search(r"\n    (?:run_linear4|quantize4|glu4|arrange4|by_type)\(", body)
         assert 0 <= body.index("set_up();") < launch.start(), name
+
+
+def test_waits_inside_the_products_end():
+    """every wait has a limit; a block that gave up goes through the same barriers as the others, reports it and leaves its copies time to land"""
+    source = (CSRC / "linear4.cuh").read_text()
+    assert re.search(r"\bmbar_wait\(", source) is None and source.count("if (!ok) op_give_up(g.failed);") == 3
+    wide = source.split("l4_store_wide(const Linear4Args& g", 1)[1].split("\n}\n", 1)[0]
+    assert wide.count("bar.sync") == 2 and " ok" not in wide
+    assert "for (int c = cs * 16; c < last_col; c += 64)" in source

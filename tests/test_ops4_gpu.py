@@ -394,6 +394,27 @@ def test_linear4_types_of_the_result(rows, out_dtype):
     _check_product(y, _exact_x(x), _values(q, scale), None)
 
 
+@pytest.mark.parametrize("rows", [1, 2, 9, 40, 200, 500])
+def test_linear4_of_far_scales(rows):
+    """scales from the least to the largest: their product may be anything as long as the results are numbers of f32, and zeros stay zeros at any scale"""
+    n, blocks = 130, 12
+    g = _gen(rows)
+    x = torch.randint(0, 256, (rows, 16 * blocks), dtype=torch.uint8, device="cuda", generator=g)
+    q = torch.randint(0, 256, (n, 16 * blocks), dtype=torch.uint8, device="cuda", generator=g)
+    xs = torch.tensor([0, 1, 40, 90, 127, 127, 180, 230, 253, 254, 120, 254], dtype=torch.uint8, device="cuda").repeat(rows, 1)
+    ws = torch.tensor([240, 230, 200, 164, 127, 120, 70, 20, 1, 0, 254, 254], dtype=torch.uint8, device="cuda").repeat(n, 1)
+    x[:, 16 * 10:16 * 11] = 0                   # zeros beside 2^120
+    q[:, 16 * 11:] = 0                          # zeros whose scales' product is no number of f32
+    y = ops.linear4(x, ops.weight4(q, ws), x_scale=xs)
+    _check_product(y, _values(x, xs), _values(q, ws), None)
+    v = _values(x, xs).float()                  # (the same numbers, rounded here; infinite ones would cost their rows)
+    v = torch.where(v.isinf(), 1e38, v)
+    w2, s2 = q.clone(), ws.clone()
+    w2[:, 16 * 9:16 * 10] = 0
+    s2[:, 9] = 254
+    _check_product(ops.linear4(v, ops.weight4(w2, s2)), _exact_x(v), _values(w2, s2), None)
+
+
 @pytest.mark.parametrize("rows", [3, 100, 300, 1111])
 def test_linear4_rows_without_a_scale(rows):
     """a row with a NaN or an infinity is NaN, a row of zeros the bias, the other rows are their own; likewise a weight row"""

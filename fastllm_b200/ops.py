@@ -340,7 +340,7 @@ def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = Non
 
 
 def check():
-    """Raises FastllmError when a product since the last check gave up on a wait inside its kernel, once (fl_operators_check; the next linear8 would raise it too).
+    """Raises FastllmError when a product since the last check gave up on a wait inside its kernel, once (fl_operators_check; the next linear8 or linear4 would raise its own too).
     To be asked after a synchronize, or after the replay of a graph has been waited for."""
     _lib.check(_lib.load().fl_operators_check())
 

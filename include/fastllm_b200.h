@@ -431,12 +431,13 @@ FL_EXPORT int fl_weight4(const uint8_t* scale, int64_t lds, int64_t n, int64_t k
 /* Matrix product of such rows:  y[r, i] = sum over j of x[r, j] * w[i, j] (+ bias[i]),  r < rows, i < n, j < k, the sum in f32, rounded once to y's type (f32, bf16, f16).
  * x: f32, bf16 or f16 rows, which the call rounds as fl_quantize4 does (x_scale NULL), or 4-bit rows (FL_DTYPE_MX4, ldx in bytes) with their x_scale [rows, lds].  w [n, k]
  * 4-bit rows (ldw in bytes), w_tiles fl_weight4 of its scales.  A row of x with a NaN or an infinity gives NaN.  Where one of x and w holds zeros, what the other's last
- * block has behind the row does not matter.  workspace: fl_linear4_workspace bytes on a 256-byte border, free again when the call's work on the stream is done. */
+ * block has behind the row does not matter.  Sums are taken in one order for a given call, but not in the same one for every number of rows.  workspace: fl_linear4_workspace
+ * bytes on a 256-byte border (the answer may be 0: none), free again when the call's work on the stream is done. */
 FL_EXPORT int fl_linear4_workspace(int64_t rows, int64_t k, int x_dtype, size_t* bytes);
 FL_EXPORT int fl_linear4(const void* x, int x_dtype, int64_t ldx, const uint8_t* x_scale, int64_t lds, const uint8_t* w, int64_t ldw, const void* w_tiles, const float* bias, int64_t rows,
                          int64_t n, int64_t k, void* y, int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
 /* Whether all products that have run are valid.  Waits inside their kernels have a limit; a product that gave up on one has returned FL_OK long before, and its
- * result is not valid.  FL_ERR_CUDA: one of those since the last check was such; told once, by this call or by the next fl_linear8, which then does nothing else,
+ * result is not valid.  FL_ERR_CUDA: one of those since the last check was such; told once, by this call or by the next fl_linear8 (of an 8-bit product) or fl_linear4 (of a 4-bit one), which then does nothing else,
  * to whichever thread asks first.  To be asked after waiting for the work in question, a replayed graph's too. */
 FL_EXPORT int fl_operators_check(void);
 /* Log probabilities over logits [rows, vocab] (f32, bf16, f16), z = logits / temperature:

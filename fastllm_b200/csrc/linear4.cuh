@@ -114,7 +114,8 @@ __device__ __forceinline__ void l4_store16(const Linear4Args& g, int r, int n, i
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------------------
 // As linear8_few_kernel: the weights are nearly all the traffic, BN activation rows the other operand; a cluster of S blocks cuts K of one tile, and its blocks add up
-// each other's parts in order through shared memory.
+// each other's parts in order through shared memory.  What bounds it: HBM behind 5 us of launch, rounding, first weights and last results (37 x 3584 x 152064 to f32 54 us, 5.6
+// TB/s of the measured 6.56; 64 x 4096 x 28672 15.6, 64 x 4096 x 4096 8.7).  Two blocks per SM hold 68 KB of weights on their way each.
 template <int BN> struct L4Few {
     static constexpr uint32_t kX = BN * kL4Row, kSW = kL4WBytes + kX, kStage = kSW + 2 * kL4Scales;     // weights | activations | their scales
     static constexpr int kPerSm = 2;                                                   // blocks that an SM holds
@@ -274,7 +275,9 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
 
 // ---- few rows, rounded on the way ------------------------------------------------------------------------------------------------------
 // Up to 16 rows that are not in 4 bits yet: the warps of the epilogue round a k block of all rows (a block of 32 a thread) while its weights are on their way, straight into the
-// ring.  Every block of threads rounds the rows anew, from L2; what that saves is a launch, and the wait for it between the first weights and the first product.
+// ring.  Every block of threads rounds the rows anew, from L2; what that saves is a launch, and the wait for it between the first weights and the first product.  What bounds it:
+// HBM for large matrices (1 x 3584 x 152064 50.8 us, 5.7 TB/s; with the rounding in a launch of its own 52.9; 16 rows 56.4 and 52.9), the way from launch to last result for
+// small ones (4 x 4096 x 4096 7.7).
 constexpr int kL4SelfRows = 16;
 struct L4Self {
     static constexpr int kRows = kL4SelfRows;
@@ -409,7 +412,8 @@ linear4_self_kernel(const __grid_constant__ CUtensorMap tmW, const Linear4Args g
 // ---- a token or two -----------------------------------------------------------------------------------------------------------------
 // One or two rows, rounded inside the product's own launch: a warp per weight row, a block of 32 weights a lane and load.  2 e2m1 is a whole number of 8 bits, so a block's
 // products are summed exactly, four to an instruction, and its two scales are applied to the sum.  Every block of threads rounds the rows into its shared memory (from L2) while its
-// first weights are on their way.
+// first weights are on their way.  What bounds it: trips to memory for small matrices (2048 x 2048 3.2 us, on the tensor cores 6.0; 4096 x 4096 6.3 and 7.8), the look-ups that make
+// e2m1 whole numbers for larger ones (28672 x 4096 23 and 13.6 us), which go the other way.
 constexpr int kL4TokenRows = 2, kL4TokenBlocks = 1024, kL4TokenWork = 1 << 19, kL4TokenThreads = 256, kL4TokenAhead = 2;      // rows; most blocks of 32 of the rows, and over all products;
                                                                                                                                 // loads on their way a lane
 
@@ -536,7 +540,8 @@ __global__ void __launch_bounds__(kL4TokenThreads) linear4_token_kernel(const Li
 
 // ---- many rows ----------------------------------------------------------------------------------------------------------------------
 // As linear8_pair_kernel: pairs of SMs on tiles of 256 weight rows x bn activation rows, each with its 128 weight rows and half of the activation tile, and the scales
-// of its weight rows and of all the tile's activation rows.  bn is at most 224: two accumulators and the scales of two k blocks fill tensor memory.  (Tiles of 256 to 416 rows
+// of its weight rows and of all the tile's activation rows.  What bounds it: the tensor cores and what feeds them (4096 x 3584 x 37888 204 us, 5.5 Pop/s and 75 % of the tensor
+// cores' cycles; 3000 x 8192 x 8192 71 us, 5.7 Pop/s), in long runs the power limit (256 us at 1.35 GHz).  bn is at most 224: two accumulators and the scales of two k blocks fill tensor memory.  (Tiles of 256 to 416 rows
 // as two products, without a second accumulator, move a quarter less through L2, but nothing hides their results: 4096 x 3584 x 37888 251 us with 416 rows, 221 with 208.)
 constexpr int kL4PairEpi = 16, kL4PairThreads = 64 + 32 * kL4PairEpi, kL4PairMaxStages = 8, kL4PairMinRows = 64, kL4PairMaxRows = 224;
 constexpr uint32_t kL4PairRing = 200 * 1024, kL4PairOut = 16 * 256;            // the ring; 16 rows of 128 results on their way out, for each four warps

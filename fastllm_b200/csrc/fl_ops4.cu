@@ -70,7 +70,7 @@ struct Linear4Room { size_t scale = 0, all = 0; int64_t slots = 0; };
 // (ops.py keeps the same rule)
 static Linear4Room linear4_room(int64_t rows, int64_t k, bool given) {
     Linear4Room r;
-    if (!given && rows <= kL4SelfRows) return r;                // rounded inside the product's own launch
+    if (rows <= kL4SelfRows) return r;                          // brought to the tensor cores inside the product's own launch
     r.scale = given ? 0 : up256((size_t)rows * blocks4(k) * 16);
     // the scales lie in tiles of as many rows as a product takes, each padded to 128: beyond 128 rows 64 to 224, which is twice the rows at most and 256
     r.slots = rows <= 128 ? (rows + 127) / 128 * 128 : (2 * rows + 127) / 128 * 128 + 256;
@@ -121,10 +121,11 @@ static void launch_few4(LaunchCtx& lc, uint64_t bytes, const uint8_t* x, int64_t
     launch_op(lc, "linear4", bytes, linear4_few_kernel<BN>, dim3((unsigned)(tiles * S)), L4Few<BN>::kThreads, L4Few<BN>::kSmem, S, true, tw, tx, g, S);
 }
 template <typename T, bool kVec>
-static void launch_self4(LaunchCtx& lc, uint64_t bytes, const void* x, int64_t ldx, int64_t k, const uint8_t* w, int64_t ldw, const Linear4Args& g) {
+static void launch_self4(LaunchCtx& lc, uint64_t bytes, const void* x, int64_t ldx, int64_t k, int64_t lds, const uint8_t* w, int64_t ldw, const Linear4Args& g) {
     const int tiles = (g.n + 127) / 128, S = few_slices4(tiles, g.groups / 2);
     const CUtensorMap tw = make_tmap_i8(w, g.n, g.blocks * 16, ldw, 128);
-    launch_op(lc, "linear4", bytes, linear4_self_kernel<T, kVec>, dim3((unsigned)(tiles * S)), L4Self::kThreads, L4Self::kSmem, S, false, tw, g, static_cast<const T*>(x), (long long)ldx, (int)k, S);
+    launch_op(lc, "linear4", bytes, linear4_self_kernel<T, kVec>, dim3((unsigned)(tiles * S)), L4Self::kThreads, L4Self::kSmem, S, false, tw, g, static_cast<const T*>(x), (long long)ldx, (int)k,
+              (long long)lds, S);
 }
 static void launch_pair4(LaunchCtx& lc, uint64_t bytes, const uint8_t* x, int64_t ldx, const uint8_t* w, int64_t ldw, const Linear4Args& g, const L4Pair& p) {
     const int bn = p.bn, atoms = l4_pair_atoms(bn);
@@ -163,11 +164,12 @@ static void run_linear4(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
         });
         return;
     }
-    if (!given && rows <= kL4SelfRows) {
-        const Linear4Args a{(int)rows, (int)n, blocks, nullptr, w_tiles, groups, bias, y, ldy, y_dtype, failed, false};
-        by_type(x_dtype, [&](auto t) {
+    if (rows <= kL4SelfRows) {
+        const Linear4Args a{(int)rows, (int)n, blocks, x_scale, w_tiles, groups, bias, y, ldy, y_dtype, failed, false};
+        if (given) launch_self4<uint8_t, true>(lc, bytes, x, ldx, k, lds, w, ldw, a);
+        else by_type(x_dtype, [&](auto t) {
             using T = decltype(t);
-            rows_on_16(x, rows, ldx, sizeof(T)) ? launch_self4<T, true>(lc, bytes, x, ldx, k, w, ldw, a) : launch_self4<T, false>(lc, bytes, x, ldx, k, w, ldw, a);
+            rows_on_16(x, rows, ldx, sizeof(T)) ? launch_self4<T, true>(lc, bytes, x, ldx, k, 0, w, ldw, a) : launch_self4<T, false>(lc, bytes, x, ldx, k, 0, w, ldw, a);
         });
         return;
     }
@@ -185,7 +187,6 @@ static void run_linear4(LaunchCtx& lc, const void* x, int x_dtype, int64_t ldx, 
     }
     const Linear4Args a{(int)rows, (int)n, blocks, xs, w_tiles, groups, bias, y, ldy, y_dtype, failed, y_dtype != FL_DTYPE_F32 && rows_on_16(y, rows, ldy, 2)};
     if (many) launch_pair4(lc, bytes, q, ldq, w, ldw, a, p);
-    else if (rows <= 16) launch_few4<16>(lc, bytes, q, ldq, w, ldw, a);
     else if (rows <= 32) launch_few4<32>(lc, bytes, q, ldq, w, ldw, a);
     else if (rows <= 64) launch_few4<64>(lc, bytes, q, ldq, w, ldw, a);
     else launch_few4<128>(lc, bytes, q, ldq, w, ldw, a);
@@ -217,7 +218,8 @@ static void set_up() {
             for (int act : {FL_ACT_SILU, FL_ACT_GELU_TANH, FL_ACT_RELU, FL_ACT_SWISH_CLAMP}) load_kernels(glu4_form<T, false>(act), glu4_form<T, true>(act));
         });
     load_kernels(arrange4_kernel);
-    few_attr4<16>(); few_attr4<32>(); few_attr4<64>(); few_attr4<128>();
+    FL_CUDA(cudaFuncSetAttribute(linear4_self_kernel<uint8_t, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L4Self::kSmem));
+    few_attr4<32>(); few_attr4<64>(); few_attr4<128>();
     for (auto kern : {linear4_pair_kernel<1>, linear4_pair_kernel<2>})
         FL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kL4PairSmem));
     cudaLaunchConfig_t cfg{};

@@ -273,9 +273,9 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
     }
 }
 
-// ---- few rows, rounded on the way ------------------------------------------------------------------------------------------------------
-// Up to 16 rows that are not in 4 bits yet: the warps of the epilogue round a k block of all rows (a block of 32 a thread) while its weights are on their way, straight into the
-// ring.  Every block of threads rounds the rows anew, from L2; what that saves is a launch, and the wait for it between the first weights and the first product.  What bounds it:
+// ---- up to 16 rows, brought to 4 bits on the way ---------------------------------------------------------------------------------------
+// The warps of the epilogue round a k block of all rows (a block of 32 a thread) while its weights are on their way, straight into the ring; rows that are in 4 bits already they
+// bring there with their scales.  Every block of threads does that anew, from L2; what it saves is a launch, and the wait for it between the first weights and the first product.  What bounds it:
 // HBM for large matrices (1 x 3584 x 152064 50.8 us, 5.7 TB/s; with the rounding in a launch of its own 52.9; 16 rows 56.4 and 52.9), the way from launch to last result for
 // small ones (4 x 4096 x 4096 7.7).
 constexpr int kL4SelfRows = 16;
@@ -288,11 +288,13 @@ struct L4Self {
     static_assert(kRows + 16 * kStages <= (int)kTmem && kStages * kStage >= kRows * 512u, "accumulators and every stage's scales; the parts of a tile fit the ring");
 };
 
+// T: the rows' type; uint8_t: 4-bit rows (ldx in bytes) with their scales g.xs [rows][lds]
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(L4Self::kThreads, L4Self::kPerSm)
-linear4_self_kernel(const __grid_constant__ CUtensorMap tmW, const Linear4Args g, const T* __restrict__ x, const long long ldx, const int k, const int S) {
+linear4_self_kernel(const __grid_constant__ CUtensorMap tmW, const Linear4Args g, const T* __restrict__ x, const long long ldx, const int k, const long long lds, const int S) {
     using L = L4Self;
-    constexpr int kStages = L::kStages, BN = L::kRows, kPieces = BN * 8 * kR4Lanes<T> / L::kRounders;      // pieces of 64 bytes a thread and k block
+    constexpr bool kGiven = std::is_same_v<T, uint8_t>;
+    constexpr int kStages = L::kStages, BN = L::kRows, kPieces = BN * 8 * kR4Lanes<T> / L::kRounders;      // pieces of 64 bytes (16 of 4-bit rows) a thread and k block
     extern __shared__ uint8_t gsm_raw[];
     uint8_t* gsm = gsm_raw + ((1024u - (smem_u32(gsm_raw) & 1023u)) & 1023u);          // (the same offset in all blocks of a cluster)
     __shared__ __align__(8) uint64_t full[kStages], empty[kStages], done;
@@ -348,29 +350,46 @@ linear4_self_kernel(const __grid_constant__ CUtensorMap tmW, const Linear4Args g
         // piece i of a thread: row and place among a k block's pieces of that row
         auto row_of = [&](int i) { return (t + L::kRounders * i) / (8 * kR4Lanes<T>); };
         auto place_of = [&](int i) { return (t + L::kRounders * i) % (8 * kR4Lanes<T>); };
-        uint32_t even[kPieces][16], odd[kPieces][16];           // two k blocks ahead: their way from L2 takes longer than a k block's weights
-        auto fetch = [&](int kb, uint32_t (&to)[kPieces][16]) {
+        constexpr int kWords = kGiven ? 5 : 16;
+        uint32_t even[kPieces][kWords], odd[kPieces][kWords];   // two k blocks ahead: their way from L2 takes longer than a k block's weights
+        auto fetch = [&](int kb, uint32_t (&to)[kPieces][kWords]) {
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) to[i][j] = 0u;
-                if (kb < kb1 && row_of(i) < g.rows) load64<T, kVec>(x + row_of(i) * ldx, kb * 256 + place_of(i) * kR4Own<T>, k, to[i]);
+                for (int j = 0; j < kWords; ++j) to[i][j] = 0u;
+                if (kb >= kb1 || row_of(i) >= g.rows) continue;
+                if constexpr (kGiven) {
+                    const int b = kb * 8 + place_of(i);
+                    if (b < g.blocks) {
+                        const uint4 q = __ldg(reinterpret_cast<const uint4*>(x + row_of(i) * ldx) + b);
+                        to[i][0] = q.x; to[i][1] = q.y; to[i][2] = q.z; to[i][3] = q.w;
+                        to[i][4] = __ldg(g.xs + row_of(i) * lds + b);
+                    }
+                } else {
+                    load64<T, kVec>(x + row_of(i) * ldx, kb * 256 + place_of(i) * kR4Own<T>, k, to[i]);
+                }
             }
         };
         int st = 0;
         uint32_t ph = 1;
-        auto round = [&](int kb, uint32_t (&from)[kPieces][16]) {
+        auto round = [&](int kb, uint32_t (&from)[kPieces][kWords]) {
             uint32_t codes[kPieces][kR4Own<T> / 8], byte[kPieces];
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
-                byte[i] = scale4(block_max<T>(most_of<T>(from[i])));
-                const float up = up4(byte[i]);
+                if constexpr (kGiven) {
 #pragma unroll
-                for (int h = 0; h < kR4Own<T> / 8; ++h) {
-                    float v[8];
+                    for (int h = 0; h < 4; ++h) codes[i][h] = from[i][h];
+                    byte[i] = from[i][4];
+                } else {
+                    byte[i] = scale4(block_max<T>(most_of<T>(from[i])));
+                    const float up = up4(byte[i]);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = byte[i] == 255u ? 0.f : number_of<T>(from[i], 8 * h + j) * up;
-                    codes[i][h] = e2m1x8(v);
+                    for (int h = 0; h < kR4Own<T> / 8; ++h) {
+                        float v[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] = byte[i] == 255u ? 0.f : number_of<T>(from[i], 8 * h + j) * up;
+                        codes[i][h] = e2m1x8(v);
+                    }
                 }
             }
             fetch(kb + 2, from);

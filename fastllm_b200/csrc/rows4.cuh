@@ -183,7 +183,7 @@ template <typename T>
 __device__ __forceinline__ uint32_t block_max(uint32_t m) { return kR4Lanes<T> == 1 ? m : max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1)); }
 
 // What a block costs once, its place and its scale, counts little beside the 32 numbers of a thread: with eight a thread the instructions were the bound, 19 a number.  What
-// bounds it: HBM (28672 x 4096 bf16 43 us, 6.9 TB/s read and written; 16384 x 4000 f32 55, 5.4 TB/s).
+// bounds it: HBM (28672 x 4096 bf16 there and back 99 us, 6.0 TB/s; 16384 x 4000 f32 55, 5.4 TB/s).
 template <typename T, bool kVec>
 __global__ void __launch_bounds__(kR4Threads) quantize4_kernel(const T* __restrict__ x, long long ldx, long long rows, int cols, int per, const Rows4Out o) {
     pdl_launch_dependents();
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(kR4Threads) quantize4_kernel(const T* __restri
 
 // Eight numbers a thread (of 32 bits: four), which it writes at once.  kShift: rows of results may start anywhere, some numbers behind a 16-byte border; a thread then takes the
 // columns between two borders, and its codes out of two words.  grid (rows, threads' pieces of a row): a division for eight numbers cost a fifth of the time.  What bounds it: HBM's
-// writes and the look-ups (28672 x 4096 bf16 52 us, 5.7 TB/s read and written).
+// writes and the look-ups (28672 x 4096 bf16 54 us, 5.5 TB/s).
 template <typename T, bool kShift>
 __global__ void __launch_bounds__(256) dequantize4_kernel(const uint8_t* __restrict__ q, long long ldq, const uint8_t* __restrict__ scale, long long lds, int cols, int words,
                                                                  T* __restrict__ y, long long ldy) {

@@ -269,7 +269,7 @@ def weight4(q: torch.Tensor, scale: torch.Tensor) -> Weight4:
 
 def _room4(rows: int, blocks: int, given: bool) -> int:
     """fl_linear4_workspace's rule"""
-    if not given and rows <= 16:
+    if rows <= 16:
         return 0
     return (0 if given else (rows * blocks * 16 + 255) // 256 * 256) + ((rows + 127) // 128 if rows <= 128 else (2 * rows + 127) // 128 + 2) * ((blocks + 7) // 8) * 1024
 

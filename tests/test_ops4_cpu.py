@@ -86,7 +86,7 @@ def test_weight4_refuses(change, word):
     (dict(x_scale=P), "x_scale"), (dict(x_dtype=4, ldx=48), "x_scale"), (dict(w=P + 8), "16-byte"), (dict(ldw=56), "16-byte"), (dict(w_tiles=P + 8), "16-byte"),
     (dict(x_dtype=4, x_scale=P, lds=3, ldx=47), "row stride"), (dict(x_dtype=4, x_scale=P, lds=2, ldx=48), "row stride"), (dict(x_dtype=4, x_scale=P, lds=3, ldx=48, x=P + 4), "16-byte"),
     (dict(x_dtype=4, x_scale=P, lds=3, ldx=56), "16-byte"), (dict(x=P + 1), "aligned"), (dict(y=P + 1), "aligned"), (dict(bias=P + 1), "aligned"), (dict(rows=17, workspace=None), "workspace"),
-    (dict(rows=17, workspace=P + 16), "workspace"), (dict(rows=17, workspace_bytes=1024 + 1024 - 1), "workspace"), (dict(x_dtype=4, x_scale=P, lds=3, ldx=48, workspace=None), "workspace"), (dict(rows=1 << 21, n=1 << 20, ldy=1 << 20), "2^40")])
+    (dict(rows=17, workspace=P + 16), "workspace"), (dict(rows=17, workspace_bytes=1024 + 1024 - 1), "workspace"), (dict(rows=17, x_dtype=4, x_scale=P, lds=3, ldx=48, workspace=None), "workspace"), (dict(rows=1 << 21, n=1 << 20, ldy=1 << 20), "2^40")])
 def test_linear4_refuses(change, word):
     _refused(_linear4(**change), word)
 

@@ -58,7 +58,7 @@ static void glu4(LaunchCtx& lc, const void* x, int dtype, int64_t rows, int64_t 
     });
 }
 
-size_t weight4_bytes(int64_t n, int64_t k) { return (size_t)(slots4(n, 128) * groups4(k) * 4); }
+static size_t weight4_bytes(int64_t n, int64_t k) { return (size_t)(slots4(n, 128) * groups4(k) * 4); }
 static void arrange4(LaunchCtx& lc, const uint8_t* scale, int64_t lds, int64_t rows, int64_t k, int tile, uint8_t* tiles) {
     const int64_t slots = slots4(rows, tile), groups = groups4(k);
     launch_op(lc, "arrange4", (uint64_t)(2 * slots * groups * 4), arrange4_kernel, dim3((unsigned)(slots / 128), (unsigned)((groups + kArrange - 1) / kArrange)), 128, 0, 1, false, scale,
@@ -77,7 +77,6 @@ static Linear4Room linear4_room(int64_t rows, int64_t k, bool given) {
     r.all = r.scale + (size_t)r.slots * groups4(k) * 4;
     return r;
 }
-size_t linear4_workspace(int64_t rows, int64_t k) { return linear4_room(rows, k, false).all; }
 
 // How a product of more than kL4FewRows rows goes over the pairs of SMs: the tile width whose waves cost least.  A k block takes 60 + 1.1 bn ns where its operands come from L2
 // (bn = 128, 160, 192, 208 and 224: 193, 228, 282, 257 to 290 and 287 to 307), and a tile no less than its results take, 1200 + 7 bn.

@@ -416,7 +416,7 @@ FL_EXPORT int fl_linear8(const void* x, int x_dtype, int64_t ldx, const float* x
  *
  * fl_quantize4: rows of f32, bf16 or f16 [rows, cols] as such rows: with a = max |x| of the block, s - 127 = max(floor(log2 a) - 2, -127) and e2m1 = x / 2^(s - 127) to
  * the nearest one, halves to the even mantissa, beyond 6 to 6.  A block of zeros has s = 0; one with a NaN or an infinity s = 255 and zeros.  What a row's last block
- * has behind the row is zero.  cols <= 2^20. */
+ * has behind the row is zero.  cols <= 2^20.  Rows of numbers may start anywhere (here and in the calls below): whole 16-byte pieces of memory that hold a part of a row are read. */
 FL_EXPORT int fl_quantize4(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, void* stream);
 /* The values that such rows stand for, rounded once to y's type (f32, bf16, f16), [rows, cols]. */
 FL_EXPORT int fl_dequantize4(const uint8_t* q, int64_t ldq, const uint8_t* scale, int64_t lds, int64_t rows, int64_t cols, void* y, int dtype, int64_t ldy, void* stream);

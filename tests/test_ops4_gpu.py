@@ -517,6 +517,24 @@ def test_feed_forward(rows, act):
     assert torch.equal(out, _feed_forward(x, w_in, w_out, act))
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("shift", [0, 1, 2, 3, 4, 5, 7])
+def test_what_lies_beside_the_rows_does_not_matter(dtype, shift):
+    """rows between numbers that are none, from every place within 16 bytes"""
+    rows, k = 24, 250
+    store = torch.full((rows, k + 11), math.nan, device="cuda").to(dtype)
+    x = store[:, shift:k + shift]
+    x.copy_(torch.randn(rows, k, device="cuda", generator=_gen(shift)) * 2)
+    dense = x.clone()
+    _check_rows(x, *ops.quantize4(x))
+    for a, b in zip(ops.glu4(x), ops.glu4(dense)):
+        assert torch.equal(a, b)
+    q, scale = _rows4(200, k, 122, 3)
+    w = ops.weight4(q, scale)
+    for r in (1, 2, 9, 24):
+        assert torch.equal(ops.linear4(x[:r], w), ops.linear4(dense[:r], w)) and not ops.linear4(x[:r], w).isnan().any()
+
+
 def test_same_bits_every_time():
     (_, w_in), (_, w_out) = _weights(640, 3000, 22)
     for rows in (1, 70, 400):

@@ -292,8 +292,13 @@ def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = Non
         _device(x, what)
     w, tiles, scale = weight
     n, blocks = scale.shape
-    if w.get_device() != dev:
+    ldw, w_step = w.stride()
+    # (its parts may have been put together by hand, and a kernel would read past the end of one that is too short)
+    if w.shape != (n, 16 * blocks) or w_step != 1 or tiles.numel() != (n + 127) // 128 * ((blocks + 7) // 8) * 1024 or not tiles.is_contiguous():
+        _refuse(f"{what}: the weight's parts do not belong together: {tuple(w.shape)}, {tuple(tiles.shape)} and {tuple(scale.shape)}")
+    if w.get_device() != dev or tiles.get_device() != dev:
         _same(dev, w, what, "the weight")
+        _same(dev, tiles, what, "the weight's scales")
     given = x_type == _lib.FL_DTYPE_MX4
     xs_ptr, lds = None, 0
     if given:
@@ -332,7 +337,7 @@ def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = Non
     if room:
         work = x.new_empty(room, dtype=_U8)
         work_ptr = work.data_ptr()
-    rc = _lib.load().fl_linear4(x2.data_ptr(), x_type, x2.stride(0), xs_ptr, lds, w.data_ptr(), w.stride(0), tiles.data_ptr(), bias_ptr, rows, n, k, y2.data_ptr(), y_type, ldy, work_ptr, room,
+    rc = _lib.load().fl_linear4(x2.data_ptr(), x_type, x2.stride(0), xs_ptr, lds, w.data_ptr(), ldw, tiles.data_ptr(), bias_ptr, rows, n, k, y2.data_ptr(), y_type, ldy, work_ptr, room,
                                 _stream(dev))
     if rc:
         _lib.check(rc)

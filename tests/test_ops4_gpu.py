@@ -517,6 +517,16 @@ def test_feed_forward(rows, act):
     assert torch.equal(out, _feed_forward(x, w_in, w_out, act))
 
 
+def test_parts_of_a_weight_that_do_not_belong_together():
+    """refused before a kernel is launched: it would read past their ends"""
+    x = torch.randn(3, 500, device="cuda")
+    w = ops.weight4(*_rows4(300, 500, 122, 3))
+    for bad in (w._replace(tiles=w.tiles[:-1024]), w._replace(q=w.q[:-1]), w._replace(q=w.q[:, :-16]), w._replace(scale=w.scale[:128]), w._replace(q=w.q.t().contiguous().t()),
+                w._replace(tiles=w.tiles[:1].expand(w.tiles.shape)), w._replace(tiles=w.tiles.cpu()), w._replace(q=w.q.cpu())):
+        with pytest.raises(FastllmError, match="belong together|lives on"):
+            ops.linear4(x, bad)
+
+
 @pytest.mark.parametrize("dtype", FLOATS)
 @pytest.mark.parametrize("shift", [0, 1, 2, 3, 4, 5, 7])
 def test_what_lies_beside_the_rows_does_not_matter(dtype, shift):

@@ -290,12 +290,13 @@ def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = Non
     dev = x.get_device()
     if dev != _bound[0]:
         _device(x, what)
-    w, tiles, scale = weight
-    n, blocks = scale.shape
+    w, tiles, _ = weight
+    n, width = w.shape
     ldw, w_step = w.stride()
+    blocks = width // 16
     # (its parts may have been put together by hand, and a kernel would read past the end of one that is too short)
-    if w.shape != (n, 16 * blocks) or w_step != 1 or tiles.numel() != (n + 127) // 128 * ((blocks + 7) // 8) * 1024 or not tiles.is_contiguous():
-        _refuse(f"{what}: the weight's parts do not belong together: {tuple(w.shape)}, {tuple(tiles.shape)} and {tuple(scale.shape)}")
+    if w_step != 1 or tiles.numel() != (n + 127) // 128 * ((blocks + 7) // 8) * 1024 or not tiles.is_contiguous():
+        _refuse(f"{what}: the weight's parts do not belong together: {tuple(w.shape)} and {tuple(tiles.shape)}")
     if w.get_device() != dev or tiles.get_device() != dev:
         _same(dev, w, what, "the weight")
         _same(dev, tiles, what, "the weight's scales")
@@ -312,7 +313,7 @@ def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = Non
             _refuse(f"{what}: x_scale comes with activations of 4 bits, and only with them")
         x2 = x if x.ndim == 2 and x.stride(1) == 1 else _rows(x, what)
         rows, k = x2.shape
-    if (k + 31) // 32 != blocks:
+    if (k + 31) // 32 * 16 != width:
         _refuse(f"{what}: the weight has {blocks} blocks of 32 columns, the activations have {k} columns")
     bias_ptr = None if bias is None else _vector(bias, n, dev, what, "bias")
     if out is not None:

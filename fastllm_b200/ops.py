@@ -294,9 +294,9 @@ def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = Non
     n, width = w.shape
     ldw, w_step = w.stride()
     blocks = width // 16
-    # (its parts may have been put together by hand, and a kernel would read past the end of one that is too short)
-    if w_step != 1 or tiles.numel() != (n + 127) // 128 * ((blocks + 7) // 8) * 1024 or not tiles.is_contiguous():
-        _refuse(f"{what}: the weight's parts do not belong together: {tuple(w.shape)} and {tuple(tiles.shape)}")
+    # (its parts may have been put together by hand, and a kernel would read past the end of one that is too short, or other bytes of one whose strides do not count bytes)
+    if w.dtype is not _U8 or tiles.dtype is not _U8 or w_step != 1 or tiles.numel() != (n + 127) // 128 * ((blocks + 7) // 8) * 1024 or not tiles.is_contiguous():
+        _refuse(f"{what}: the weight's parts do not belong together: {w.dtype} {tuple(w.shape)} and {tiles.dtype} {tuple(tiles.shape)}")
     if w.get_device() != dev or tiles.get_device() != dev:
         _same(dev, w, what, "the weight")
         _same(dev, tiles, what, "the weight's scales")

@@ -139,6 +139,22 @@ def test_types_are_refused():
             call()
 
 
+def _by_hand(monkeypatch, n=300, blocks=16):
+    """a weight's parts as weight4 makes them; tensors here pass for ones on the device, and a call that gets as far as the library fails"""
+    monkeypatch.setattr(ops, "_bound", [-1])
+    monkeypatch.setattr(_lib, "load", lambda: pytest.fail("not refused"))
+    return ops.Weight4(torch.zeros(n, 16 * blocks, dtype=torch.uint8), torch.zeros((n + 127) // 128 * ((blocks + 7) // 8) * 1024, dtype=torch.uint8), torch.zeros(n, blocks, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("part", ["q", "tiles"])
+@pytest.mark.parametrize("dtype", [torch.int8, torch.int32, torch.float32, torch.bfloat16])
+def test_a_weight_of_other_types_is_refused(monkeypatch, part, dtype):
+    """strides count elements and the kernel bytes: it would read other numbers"""
+    w = _by_hand(monkeypatch)
+    with pytest.raises(FastllmError, match="belong together"):
+        ops.linear4(torch.zeros(3, 512), w._replace(**{part: getattr(w, part).to(dtype)}))
+
+
 def test_every_way_to_an_operator_sets_up_first():
     source = (CSRC / "fl_ops4.cu").read_text()
     heads = re.findall(r"\n(?:FL_EXPORT int|void) ((?:fl|op)_\w+)\(", source)

@@ -248,8 +248,8 @@ def glu4(x: torch.Tensor, act: str = "silu", *, limit: float = 7.0):
 
 class Weight4(NamedTuple):
     q: torch.Tensor             # uint8 [n, 16 blocks], as given
-    tiles: torch.Tensor         # the scales in the order that linear4 takes them
-    scale: torch.Tensor         # uint8 [n, blocks], as given
+    tiles: torch.Tensor         # the scales in the order that linear4 takes them, uint8 [tiles of 128 rows, 256 columns, 1024] (or flat, as fl_weight4 writes them)
+    scale: torch.Tensor         # uint8 [n, blocks], as given; linear4 looks at its shape alone
 
 
 def weight4(q: torch.Tensor, scale: torch.Tensor) -> Weight4:
@@ -262,7 +262,7 @@ def weight4(q: torch.Tensor, scale: torch.Tensor) -> Weight4:
     n, blocks = s2.shape
     if n == 0:
         _refuse(f"{what}: the weight has no rows")
-    tiles = q.new_empty((n + 127) // 128 * ((blocks + 7) // 8) * 1024)
+    tiles = q.new_empty((n + 127) // 128, (blocks + 7) // 8, 1024)
     _lib.check(_lib.load().fl_weight4(s2.data_ptr(), s2.stride(0), n, 32 * blocks, tiles.data_ptr(), _stream(dev)))
     return Weight4(q, tiles, scale)
 
@@ -290,13 +290,14 @@ def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = Non
     dev = x.get_device()
     if dev != _bound[0]:
         _device(x, what)
-    w, tiles, _ = weight
-    n, width = w.shape
+    w, tiles, scale = weight
+    n, blocks = scale.shape
     ldw, w_step = w.stride()
-    blocks = width // 16
-    # (its parts may have been put together by hand, and a kernel would read past the end of one that is too short, or other bytes of one whose strides do not count bytes)
-    if w.dtype is not _U8 or tiles.dtype is not _U8 or w_step != 1 or tiles.numel() != (n + 127) // 128 * ((blocks + 7) // 8) * 1024 or not tiles.is_contiguous():
-        _refuse(f"{what}: the weight's parts do not belong together: {w.dtype} {tuple(w.shape)} and {tiles.dtype} {tuple(tiles.shape)}")
+    # (its parts may have been put together by hand: a kernel would read past the end of one that is too short, or other numbers)
+    shape = (n + 127) // 128, (blocks + 7) // 8, 1024
+    if (w.dtype is not _U8 or tiles.dtype is not _U8 or w.shape != (n, 16 * blocks) or w_step != 1 or tiles.shape != shape and tiles.shape != (shape[0] * shape[1] * 1024,)
+            or not tiles.is_contiguous()):
+        _refuse(f"{what}: the weight's parts do not belong together: {w.dtype} {tuple(w.shape)}, {tiles.dtype} {tuple(tiles.shape)} and scales {tuple(scale.shape)}")
     if w.get_device() != dev or tiles.get_device() != dev:
         _same(dev, w, what, "the weight")
         _same(dev, tiles, what, "the weight's scales")
@@ -313,7 +314,7 @@ def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = Non
             _refuse(f"{what}: x_scale comes with activations of 4 bits, and only with them")
         x2 = x if x.ndim == 2 and x.stride(1) == 1 else _rows(x, what)
         rows, k = x2.shape
-    if (k + 31) // 32 * 16 != width:
+    if (k + 31) // 32 != blocks:
         _refuse(f"{what}: the weight has {blocks} blocks of 32 columns, the activations have {k} columns")
     bias_ptr = None if bias is None else _vector(bias, n, dev, what, "bias")
     if out is not None:

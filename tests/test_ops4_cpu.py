@@ -155,6 +155,36 @@ def test_a_weight_of_other_types_is_refused(monkeypatch, part, dtype):
         ops.linear4(torch.zeros(3, 512), w._replace(**{part: getattr(w, part).to(dtype)}))
 
 
+@pytest.mark.parametrize("change", [
+    lambda w: dict(q=w.q[:-1]), lambda w: dict(scale=w.scale[:-1]), lambda w: dict(scale=w.scale[:128]), lambda w: dict(scale=w.scale[:, :-1]), lambda w: dict(q=w.q[:, :-16]),
+    lambda w: dict(q=w.q[:, :-1]), lambda w: dict(tiles=w.tiles[:2]), lambda w: dict(tiles=w.tiles.flatten()[:-1024]), lambda w: dict(tiles=w.tiles.view(2, 3, 1024)),
+    lambda w: dict(tiles=w.tiles.view(6, 1024)), lambda w: dict(tiles=w.tiles[:1].expand(3, 2, 1024))],
+    ids=["rows", "scales", "scales of fewer tiles", "scales of fewer blocks", "columns", "half a block", "tiles", "flat tiles", "tiles of another weight", "tiles of another shape", "tiles that repeat"])
+def test_parts_of_different_weights_are_refused(monkeypatch, change):
+    """also where no kernel would read out of bounds: 3 x 2 tiles are as many as 2 x 3, and other numbers"""
+    w = _by_hand(monkeypatch)
+    w = w._replace(tiles=w.tiles.view(3, 2, 1024))
+    with pytest.raises(FastllmError, match="belong together"):
+        ops.linear4(torch.zeros(3, 512), w._replace(**change(w)))
+
+
+def test_parts_of_one_weight_go_through(monkeypatch):
+    """tiles as weight4 shapes them, or the bytes that fl_weight4 wrote; rows with room between them"""
+    w = _by_hand(monkeypatch)
+
+    class Called(Exception):
+        pass
+
+    def load():
+        raise Called
+
+    monkeypatch.setattr(_lib, "load", load)
+    wide = torch.zeros(300, 512, dtype=torch.uint8)
+    for good in (w, w._replace(tiles=w.tiles.view(3, 2, 1024)), w._replace(q=wide[:, :256]), w._replace(scale=wide[:, 1:17])):
+        with pytest.raises(Called):
+            ops.linear4(torch.zeros(3, 512), good)
+
+
 def test_every_way_to_an_operator_sets_up_first():
     source = (CSRC / "fl_ops4.cu").read_text()
     heads = re.findall(r"\n(?:FL_EXPORT int|void) ((?:fl|op)_\w+)\(", source)

@@ -203,3 +203,16 @@ def test_waits_inside_the_products_end():
     wide = source.split("l4_store_wide(const Linear4Args& g", 1)[1].split("\n}\n", 1)[0]
     assert wide.count("bar.sync") == 2 and " ok" not in wide
     assert "for (int c = cs * 16; c < last_col; c += 64)" in source
+
+
+def test_a_product_that_gave_up_is_told_of():
+    """the word that the kernels set goes into every product, is asked for before the next one is launched, and by the check, which takes it whatever the 8-bit products' word says"""
+    source, ops8 = (CSRC / "fl_ops4.cu").read_text(), (CSRC / "fl_ops.cu").read_text()
+    assert source.count("g_op4_failed.take()") == 1 and "bool products4_failed() { return g_op4_failed.take(); }" in source
+    linear4 = source.split("FL_EXPORT int fl_linear4(", 1)[1].split("\n}\n", 1)[0]
+    told = linear4.index("FL_CHECK(!products4_failed(), FL_ERR_CUDA,")
+    assert linear4.index("set_up();") < told < linear4.index("run_linear4(") and linear4.split("run_linear4(", 1)[1].split(";", 1)[0].endswith("g_op4_failed.word)")
+    run = source.split("static void run_linear4(", 1)[1].split("\n}\n", 1)[0]
+    assert run.count("Linear4Args a{") == run.count(", failed, ") == 3
+    check = ops8.split("FL_EXPORT int fl_operators_check(", 1)[1].split("\n}\n", 1)[0]
+    assert check.index("= products4_failed();") < check.index("check_op_failed();") < check.index("FL_CHECK(!of4, FL_ERR_CUDA,")

@@ -489,6 +489,61 @@ def test_linear4_far_offsets():
     _check_product(y, _exact_x(x[:9]), _values(dense, scale), None)
 
 
+def _far(rows, cols, dtype):
+    """rows on 16-byte borders whose last one lies behind 2^31 elements"""
+    step = (1 << 31) // (rows - 1) // 16 * 16 + 16
+    return torch.empty((rows - 1) * step + cols, dtype=dtype, device="cuda").as_strided((rows, cols), (step, 1))
+
+
+@pytest.mark.parametrize("rows", [2, 9, 40, 140])
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_linear4_far_results(rows, out_dtype):
+    """every kernel's way of storing"""
+    n, k = 256, 320
+    x = torch.randn(rows, k, device="cuda", generator=_gen(rows)).bfloat16()
+    q, scale = _rows4(n, k, 122, 5)
+    out = _far(rows, n, out_dtype)
+    ops.linear4(x, ops.weight4(q, scale), out=out)
+    _check_product(out, _exact_x(x), _values(q, scale), None)
+
+
+@pytest.mark.parametrize("rows", [2, 9, 40, 140])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.uint8])
+def test_linear4_far_activations(rows, dtype):
+    """every kernel's way of loading; of rows in 4 bits already (uint8) their scales too"""
+    n, k = 200, 320
+    w = ops.weight4(*_rows4(n, k, 122, 6))
+    x = torch.randn(rows, k, device="cuda", generator=_gen(rows))
+    x, xs = ops.quantize4(x) if dtype == torch.uint8 else (x.to(dtype), None)
+    far, far_scale = _far(rows, x.shape[1], dtype), None
+    far.copy_(x)
+    if xs is not None:
+        far_scale = _far(rows, xs.shape[1], dtype)
+        far_scale.copy_(xs)
+    assert torch.equal(ops.linear4(far, w, x_scale=far_scale), ops.linear4(x, w, x_scale=xs))
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_far_rows_there_and_back(dtype):
+    x = torch.randn(3, 96, device="cuda", generator=_gen(7)).to(dtype)
+    far = _far(3, 96, dtype)
+    far.copy_(x)
+    for call in (ops.quantize4, ops.glu4):
+        for a, b in zip(call(far), call(x)):
+            assert torch.equal(a, b)
+    q, scale = ops.quantize4(x)
+    far_q, far_scale = _far(3, 48, torch.uint8), _far(3, 3, torch.uint8)
+    far_q.copy_(q), far_scale.copy_(scale)
+    assert torch.equal(ops.dequantize4(far_q, far_scale, dtype=dtype), ops.dequantize4(q, scale, dtype=dtype))
+    far.fill_(7)
+    kind, lib = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype], _lib.load()
+    assert lib.fl_dequantize4(q.data_ptr(), 48, scale.data_ptr(), 3, 3, 96, far.data_ptr(), kind, far.stride(0), torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(far, ops.dequantize4(q, scale, dtype=dtype))
+    far_q.fill_(77), far_scale.fill_(77)
+    assert lib.fl_quantize4(x.data_ptr(), kind, 3, 96, 96, far_q.data_ptr(), far_q.stride(0), far_scale.data_ptr(), far_scale.stride(0), torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(far_q, q) and torch.equal(far_scale, scale)
+
+
 # ---- together, on streams, in graphs ------------------------------------------------------------------------------------------------
 def _feed_forward(x, w_in, w_out, act="silu"):
     """a feed-forward with 4-bit weights: two products with the activation between them"""

@@ -444,6 +444,12 @@ __device__ __forceinline__ uint32_t e2m1_doubled(uint32_t w) {
     return (up & ~neg) | (down & neg);
 }
 
+// the smaller and the larger of two, NaN where one of them is
+__device__ __forceinline__ void in_order(float a, float b, float& lo, float& hi) {
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(lo) : "f"(a), "f"(b));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(hi) : "f"(a), "f"(b));
+}
+
 template <typename T, int R, bool kVec>
 __global__ void __launch_bounds__(kL4TokenThreads) linear4_token_kernel(const Linear4Args g, const T* __restrict__ x, const long long ldx, const int k, const uint8_t* __restrict__ w,
                                                                         const long long ldw) {
@@ -533,8 +539,10 @@ __global__ void __launch_bounds__(kL4TokenThreads) linear4_token_kernel(const Li
             const float d = down4(now[u].s);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const float p = d * sscale[r * blocks + b];
-                sum[r] = fmaf((float)dot[r], dot[r] == 0 && p == INFINITY ? 0.f : p, sum[r]);     // (no products, whatever their scales)
+                // times the smaller scale first, which is exact: the two scales' own product may be below f32's range, or above it beside a sum of zero
+                float lo, hi;
+                in_order(d, sscale[r * blocks + b], lo, hi);
+                sum[r] = fmaf((float)dot[r] * lo, hi, sum[r]);
             }
         }
         if (last) {

@@ -415,6 +415,24 @@ def test_linear4_of_far_scales(rows):
     _check_product(ops.linear4(v, ops.weight4(w2, s2)), _exact_x(v), _values(w2, s2), None)
 
 
+@pytest.mark.parametrize("rows", [1, 2, 3, 20, 200])
+@pytest.mark.parametrize("low", [-147, -140, -130])
+@pytest.mark.parametrize("of_x", [-127, -100, -60, -20])
+def test_linear4_of_numbers_below_the_smallest_normal_one(rows, low, of_x):
+    """scales whose product is below f32's range where the results are not: quarters of 2^low, up to 36 k of them, are all f32 numbers"""
+    n, k = 150, 320
+    of_w = low - of_x
+    q = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, device="cuda", generator=_gen(rows))
+    xq = torch.randint(0, 256, (rows, k // 2), dtype=torch.uint8, device="cuda", generator=_gen(rows + 1))
+    xq[:, ::16] = 0xF7                          # (a block's largest number is 6, so that rounding finds its scale again)
+    scale, xs = (torch.full((r, k // 32), 127 + e, dtype=torch.uint8, device="cuda") for r, e in ((n, of_w), (rows, of_x)))
+    w, xv = ops.weight4(q, scale), _values(xq, xs)
+    want = xv @ _values(q, scale).T
+    assert want.abs().max() < 2.0 ** -110 and torch.equal(want.float().double(), want)
+    assert torch.equal(ops.linear4(xv.float(), w).double(), want)
+    assert torch.equal(ops.linear4(xq, w, x_scale=xs).double(), want)
+
+
 @pytest.mark.parametrize("rows", [3, 100, 300, 1111])
 def test_linear4_rows_without_a_scale(rows):
     """a row with a NaN or an infinity is NaN, a row of zeros the bias, the other rows are their own; likewise a weight row"""

@@ -308,11 +308,16 @@ def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = Non
             _refuse(f"{what}: 4-bit rows come with their x_scale")
         x2, s2 = _rows4(x, x_scale, dev, what, "the activations")
         rows, k = s2.shape
-        xs_ptr, lds, k = s2.data_ptr(), s2.stride(0), 32 * k
+        ldx = x2.stride()[0]
+        xs_ptr, lds, k = s2.data_ptr(), s2.stride()[0], 32 * k
     else:
         if x_scale is not None:
             _refuse(f"{what}: x_scale comes with activations of 4 bits, and only with them")
-        x2 = x if x.ndim == 2 and x.stride(1) == 1 else _rows(x, what)
+        x2, step = x, x.stride()
+        if len(step) != 2 or step[1] != 1:
+            x2 = _rows(x, what)
+            step = x2.stride()
+        ldx = step[0]
         rows, k = x2.shape
     if (k + 31) // 32 != blocks:
         _refuse(f"{what}: the weight has {blocks} blocks of 32 columns, the activations have {k} columns")
@@ -339,7 +344,7 @@ def linear4(x: torch.Tensor, weight: Weight4, bias: Optional[torch.Tensor] = Non
     if room:
         work = x.new_empty(room, dtype=_U8)
         work_ptr = work.data_ptr()
-    rc = _lib.load().fl_linear4(x2.data_ptr(), x_type, x2.stride(0), xs_ptr, lds, w.data_ptr(), ldw, tiles.data_ptr(), bias_ptr, rows, n, k, y2.data_ptr(), y_type, ldy, work_ptr, room,
+    rc = _lib.load().fl_linear4(x2.data_ptr(), x_type, ldx, xs_ptr, lds, w.data_ptr(), ldw, tiles.data_ptr(), bias_ptr, rows, n, k, y2.data_ptr(), y_type, ldy, work_ptr, room,
                                 _stream(dev))
     if rc:
         _lib.check(rc)

@@ -454,6 +454,25 @@ def test_linear4_rows_without_a_scale(rows):
     assert torch.equal(y2[3:, keep], y[3:, keep]) and torch.equal(y2[0, keep], y[0, keep])
 
 
+@pytest.mark.parametrize("rows", [1, 2])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_linear4_of_a_token_without_a_scale(rows, bad):
+    """as rows among more: NaN for a row with a NaN or an infinity and for a weight row without a scale, also where the other side's block holds zeros"""
+    x = torch.randn(3, 200, device="cuda", generator=_gen(9)).bfloat16()
+    x[:, 128:160] = 0
+    x[rows - 1, 7] = bad
+    q, scale = _rows4(150, 200, 122, 10)
+    q, scale = q.clone(), scale.clone()
+    q[5, :16] = 0
+    scale[77, 4] = 255
+    w = ops.weight4(q, scale)
+    y, all_of_them = ops.linear4(x[:rows], w, out_dtype=torch.float32), ops.linear4(x, w, out_dtype=torch.float32)
+    assert y[rows - 1].isnan().all() and all_of_them[rows - 1].isnan().all() and y[:, 77].isnan().all() and all_of_them[:, 77].isnan().all()
+    keep = torch.arange(150, device="cuda") != 77
+    if rows == 2:
+        _check_product(y[:1, keep], _exact_x(x[:1]), _values(q, scale)[keep], None)
+
+
 @pytest.mark.parametrize("rows", [1, 6, 90, 200, 280, 1040])
 def test_linear4_writes_its_rows_and_nothing_else(rows):
     """strided input and result: rows behind the last one and columns behind the row stay as they were"""

@@ -79,7 +79,9 @@ static Linear4Room linear4_room(int64_t rows, int64_t k, bool given) {
 }
 
 // How a product of more than kL4FewRows rows goes over the pairs of SMs: the tile width whose waves cost least.  A k block takes 60 + 1.1 bn ns where its operands come from L2
-// (bn = 128, 160, 192, 208 and 224: 193, 228, 282, 257 to 290 and 287 to 307), and a tile no less than its results take, 1200 + 7 bn.
+// (bn = 128, 160, 192, 208 and 224: 193, 228, 282, 257 to 290 and 287 to 307), and a tile no less than its results take, 1200 + 7 bn.  It ranks widths and does not foretell a call: first
+// loads and last results are not in it, nor operands that come from memory (300 and 777 x 4096 x 28672 15 and 30 us by the rule, with the rounding's launch 26 and 45 measured; 3000 x 8192 x
+// 8192 61 by the rule, 71 alone).
 constexpr int kL4FewRows = 128;
 static L4Pair pair_plan4(int64_t rows, int64_t n, int64_t k, int clusters) {
     L4Pair best{};
@@ -107,7 +109,8 @@ static int g_pair_clusters = 0;                 // pairs of SMs that can be resi
 bool products4_failed() { return g_op4_failed.take(); }
 
 // Blocks that share a 128-row weight tile: one per SM at most, four k blocks each at least, and only where a block is spared twelve: the cluster's barriers and the exchange take as
-// long (S = 1, 2 and 4: 16 x 4096 x 4096 8.8, 8.9 and 8.1 us, 64 x 4096 x 4096 9.9, 9.7 and 8.7, 32 x 14336 x 4096 20.5, 14.6 and 11.9, 8 x 1024 x 4096 5.0, 6.7 and 6.5).
+// long (S = 1, 2 and 4: 16 x 4096 x 4096 8.8, 8.9 and 8.1 us, 64 x 4096 x 4096 9.9, 9.7 and 8.7, 32 x 14336 x 4096 20.5, 14.6 and 11.9, 8 x 1024 x 4096 5.0, 6.7 and 6.5; that is 16, 56 and 4 k blocks, and
+// no number between them was measured).
 static int few_slices4(int64_t tiles, int nk) {
     int S = 8;
     while (S > 1 && (S * tiles > kNumSMs || nk < 4 * S || nk - nk / S < 12)) S /= 2;

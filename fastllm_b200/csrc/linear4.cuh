@@ -276,8 +276,10 @@ linear4_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constan
 // ---- up to 16 rows, brought to 4 bits on the way ---------------------------------------------------------------------------------------
 // The warps of the epilogue round a k block of all rows (a block of 32 a thread) while its weights are on their way, straight into the ring; rows that are in 4 bits already they
 // bring there with their scales.  Every block of threads does that anew, from L2; what it saves is a launch, and the wait for it between the first weights and the first product.  What bounds it:
-// HBM for large matrices (1 x 3584 x 152064 50.8 us, 5.7 TB/s; with the rounding in a launch of its own 52.9; 16 rows 56.4 and 52.9), the way from launch to last result for
-// small ones (4 x 4096 x 4096 7.7).
+// HBM for one row of a large matrix (1 x 3584 x 152064 52 us, 5.6 TB/s), the rounding, done anew for every weight tile, for more rows of one, the way from launch to last result for
+// small ones.  The rule looks at the rows alone, so that a call of up to 16 is one launch without a workspace (9 us of the host's time, of two launches 15), and where that does not count it is the
+// slower form from three rows on: here 4, 8 and 16 rows, and 17 with the rounding in a launch of its own, take 60, 63, 66 and 53 us on the device; of 4096 x 28672 16.5, 17.2, 18.1 and
+// 16.0, of 4096 x 4096 7.5, 7.7, 8.1 and 7.5.
 constexpr int kL4SelfRows = 16;
 struct L4Self {
     static constexpr int kRows = kL4SelfRows;
@@ -432,7 +434,8 @@ linear4_self_kernel(const __grid_constant__ CUtensorMap tmW, const Linear4Args g
 // One or two rows, rounded inside the product's own launch: a warp per weight row, a block of 32 weights a lane and load.  2 e2m1 is a whole number of 8 bits, so a block's
 // products are summed exactly, four to an instruction, and its two scales are applied to the sum.  Every block of threads rounds the rows into its shared memory (from L2) while its
 // first weights are on their way.  What bounds it: trips to memory for small matrices (2048 x 2048 3.2 us, on the tensor cores 6.0; 4096 x 4096 6.3 and 7.8), the look-ups that make
-// e2m1 whole numbers for larger ones (28672 x 4096 23 and 13.6 us), which go the other way.
+// e2m1 whole numbers for larger ones (28672 x 4096 23 and 13.6 us), which go the other way.  The rule's border is the first of these two sizes; where they cross above it was not
+// measured (4096 x 4097, on the tensor cores, takes 7.4 us where 4096 x 4096 takes 6.4).
 constexpr int kL4TokenRows = 2, kL4TokenBlocks = 1024, kL4TokenWork = 1 << 19, kL4TokenThreads = 256, kL4TokenAhead = 2;      // rows; most blocks of 32 of the rows, and over all products;
                                                                                                                                 // loads on their way a lane
 
@@ -568,7 +571,8 @@ __global__ void __launch_bounds__(kL4TokenThreads) linear4_token_kernel(const Li
 // ---- many rows ----------------------------------------------------------------------------------------------------------------------
 // As linear8_pair_kernel: pairs of SMs on tiles of 256 weight rows x bn activation rows, each with its 128 weight rows and half of the activation tile, and the scales
 // of its weight rows and of all the tile's activation rows.  What bounds it: the tensor cores and what feeds them (4096 x 3584 x 37888 204 us, 5.5 Pop/s and 75 % of the tensor
-// cores' cycles; 3000 x 8192 x 8192 71 us, 5.7 Pop/s), in long runs the power limit (256 us at 1.35 GHz).  bn is at most 224: two accumulators and the scales of two k blocks fill tensor memory.  (Tiles of 256 to 416 rows
+// cores' cycles; 3000 x 8192 x 8192 71 us, 5.7 Pop/s), in long runs the power limit (256 us at 1.35 GHz); below some 800 rows the first loads, which wait for the rounding, and the last
+// results (300 x 4096 x 28672 26 us with the rounding's launch, 12.5 at the copy rate; the shares were not measured apart).  bn is at most 224: two accumulators and the scales of two k blocks fill tensor memory.  (Tiles of 256 to 416 rows
 // as two products, without a second accumulator, move a quarter less through L2, but nothing hides their results: 4096 x 3584 x 37888 251 us with 416 rows, 221 with 208.)
 constexpr int kL4PairEpi = 16, kL4PairThreads = 64 + 32 * kL4PairEpi, kL4PairMaxStages = 8, kL4PairMinRows = 64, kL4PairMaxRows = 224;
 constexpr uint32_t kL4PairRing = 200 * 1024, kL4PairOut = 16 * 256;            // the ring; 16 rows of 128 results on their way out, for each four warps
